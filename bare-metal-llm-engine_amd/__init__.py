@@ -130,6 +130,15 @@ SIGNATURES = {
     "eng_kv_cache_write_f16": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p],
     "eng_transpose_f16": [_p, _p, _i64, _i64, _p],
     "eng_transpose_f32": [_p, _p, _i64, _i64, _p],
+    "eng_mx4_quantize_f32": [_p, _p, _p, _i64, _i64, _p],
+    "eng_mx4_quantize_f16": [_p, _p, _p, _i64, _i64, _p],
+    "eng_mx4_dequantize_f32": [_p, _p, _p, _i64, _i64, _p],
+    "eng_mx4_dequantize_f16": [_p, _p, _p, _i64, _i64, _p],
+    "eng_linear_mx4w_nk": [_p, _p, _p, _p, _i64, _i64, _i64, _p],
+    "eng_rmsnorm_linear_mx4w_nk": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _f, _p],
+    "eng_kv_cache_write_q8": [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p],
+    "eng_attention_decode_q8": [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f,
+                                ctypes.c_int, _p],
     "eng_engref_open": [ctypes.c_char_p, _pp],
     "eng_engref_close": [_p],
     "eng_engref_count": [_p, ctypes.POINTER(ctypes.c_int32)],

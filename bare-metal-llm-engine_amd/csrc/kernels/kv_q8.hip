@@ -1,0 +1,604 @@
+// kv_q8.hip -- a KV cache held in 8 bits: the append and the decode attention
+// that reads it (the fp16 cache's are in attention.hip).
+//
+// Format: values are e4m3 (OCP FP8: 4 exponent bits, 3 of mantissa, largest
+// 448, no infinity), head-major like the fp16 caches, key j of KV head h of
+// sequence b at ((b n_kv_heads + h) kv_max_seq_len + j) D; each block of 32
+// tokens of a (sequence, KV head) has one fp32 scale for K and one for V, a
+// power of two, at (b n_kv_heads + h) ceil(kv_max_seq_len / 32) + j / 32. A
+// power of two keeps a code's value when a block's scale grows (only values that
+// fall below e4m3's normal range are rounded again), so a block filled token by
+// token is as exact as one written at once to within that rounding.
+#include "gemv_kernels.hpp"
+#include "launch.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace eng {
+namespace {
+
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+
+constexpr int kKvBlock = 32;  // tokens that share a scale
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ------------------------------------------------------------------- append
+
+constexpr int kWriteThreads = 256;
+
+// Four values as e4m3 bytes (nearest even; infinities and NaN become NaN).
+__device__ __forceinline__ unsigned fp8x4(float a, float b, float c, float d) {
+  int w = 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, w, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+#endif
+  return static_cast<unsigned>(w);
+}
+
+// One wave per (K or V, sequence, head, block of 32 tokens). A lane holds 8
+// consecutive dims of a token (16 bytes of the new rows, 8 of the cache), so a
+// wave load covers 64 / (D / 8) tokens and the block's new rows are in flight
+// together. The block's scale is the least power of two in [2^-15, 2^8] that
+// brings its largest finite new magnitude to 448 or less (2^-15 already holds
+// fp16's smallest steps), and no less than the scale of earlier tokens kept in
+// the block; if it grows, their codes are brought to it. Tokens at or past
+// kv_max_seq_len are dropped. Blocks belong to one wave each: no atomics.
+// Bound by the bytes of the new rows and their codes.
+template <int D>
+__global__ __launch_bounds__(kWriteThreads) void kv_write_q8_kernel(
+    const _Float16* __restrict__ k_new, const _Float16* __restrict__ v_new,
+    unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache,
+    float* __restrict__ k_scale, float* __restrict__ v_scale, const int* __restrict__ pos,
+    const int* __restrict__ n_new, long long units, long long s_new, long long n_kv_heads,
+    long long kv_max, int reach) {
+  constexpr int LPT = D / 8;         // lanes per token
+  constexpr int TPL = 64 / LPT;      // tokens per wave load
+  constexpr int LOADS = kKvBlock / TPL;
+  const int lane = threadIdx.x & 63;
+  const int sub = lane / LPT;
+  const int d0 = (lane % LPT) * 8;
+  // unit = ((b reach + block) heads + h) 2 + (K or V)
+  const long long unit = static_cast<long long>(blockIdx.x) * (kWriteThreads / 64) + (threadIdx.x >> 6);
+  if (unit >= units) return;
+  const bool is_v = (unit & 1) != 0;
+  const long long h = (unit >> 1) % n_kv_heads;
+  const long long rest = (unit >> 1) / n_kv_heads;
+  const long long b = rest / reach;
+  const long long p = pos[b];
+  const long long n = n_new != nullptr ? std::min<long long>(n_new[b], s_new) : s_new;
+  if (p < 0 || n <= 0) return;
+  const long long blk = p / kKvBlock + (rest - b * reach);
+  const long long first = blk * kKvBlock;
+  const long long lo = std::max(p, first);
+  const long long hi = std::min(std::min(p + n, kv_max), first + kKvBlock);
+  if (lo >= hi) return;
+
+  const _Float16* src = (is_v ? v_new : k_new) + ((b * s_new - p) * n_kv_heads + h) * D + d0;
+  unsigned char* dst = (is_v ? v_cache : k_cache) + ((b * n_kv_heads + h) * kv_max + first) * D + d0;
+  float* sp = (is_v ? v_scale : k_scale) + (b * n_kv_heads + h) * ((kv_max + kKvBlock - 1) / kKvBlock) + blk;
+
+  halfx8 x[LOADS];
+#pragma unroll
+  for (int r = 0; r < LOADS; ++r) {
+    const long long t = first + r * TPL + sub;
+    x[r] = halfx8{};
+    if (t >= lo && t < hi) x[r] = *reinterpret_cast<const halfx8*>(src + t * n_kv_heads * D);
+  }
+  const bool kept = lo > first;
+  const float s_old = kept ? *sp : 0.0f;
+  int top = 0;
+#pragma unroll
+  for (int r = 0; r < LOADS; ++r) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const _Float16 v = x[r][e];  // (bit-casting a vector's element in place reads element 0)
+      const int m = __builtin_bit_cast(unsigned short, v) & 0x7fff;
+      top = max(top, m < 0x7c00 ? m : 0);
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) top = max(top, __shfl_xor(top, off));
+  const float amax = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(top)));
+  // amax = 1.m 2^E: 448 = 1.75 2^8 holds it at 2^(E - 8) up to m = 0.75
+  const int bits = __float_as_int(amax);
+  int e = (bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
+  e = min(max(e, -15), 8);
+  const float s = fmaxf(__int_as_float((e + 127) << 23), s_old);
+  const float inv = 1.0f / s;
+#pragma unroll
+  for (int r = 0; r < LOADS; ++r) {
+    const int t = r * TPL + sub;
+    if (first + t >= lo && first + t < hi) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = static_cast<float>(x[r][q]) * inv;
+      *reinterpret_cast<uintx2*>(dst + t * D) =
+          uintx2{fp8x4(v[0], v[1], v[2], v[3]), fp8x4(v[4], v[5], v[6], v[7])};
+    }
+  }
+  if (kept && s > s_old) {
+    [[maybe_unused]] const float ratio = s_old * inv;
+#pragma unroll
+    for (int r = 0; r < LOADS; ++r) {
+      const int t = r * TPL + sub;
+      if (first + t < lo) {
+        [[maybe_unused]] const uintx2 c = *reinterpret_cast<const uintx2*>(dst + t * D);
+        uintx2 o = {0, 0};
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[q]), false);
+          const floatx2 z = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[q]), true);
+          o[q] = fp8x4(a[0] * ratio, a[1] * ratio, z[0] * ratio, z[1] * ratio);
+        }
+#endif
+        *reinterpret_cast<uintx2*>(dst + t * D) = o;
+      }
+    }
+  }
+  if (lane == 0 && s != s_old) *sp = s;
+}
+
+// ---------------------------------------------------------------- attention
+
+// 2^(a - b), 0 for a == -inf whatever b is; NaN stays NaN.
+__device__ __forceinline__ float weight2(float a, float b) {
+  const float w = __builtin_amdgcn_exp2f(a - b);
+  return a == kNegInf ? 0.0f : w;
+}
+
+struct AttnArgs {
+  const _Float16* q;
+  const unsigned char* k;
+  const unsigned char* v;
+  const float* ks;
+  const float* vs;
+  _Float16* out;
+  const int* lens;
+  long long n_heads, n_kv_heads, max_len, kv_max;
+  int group, tiles;   // query heads per KV head; 16-head tiles of it
+  int split_blocks;   // 32-token blocks per split
+  int nsplit;
+  float scale;
+};
+
+// One workgroup per (sequence, KV head, tile of up to 16 of its query heads,
+// split of `split_blocks` 32-token blocks), NW waves, block t of the split to
+// wave t % NW, P blocks in flight per wave. The matrix cores do both products:
+// scores S^T = K . Q^T with K as the A operand (the e4m3 bytes converted to
+// fp16, exact), O^T = V^T . P^T with the score accumulators, in place, as the B
+// operand: A row i is key (i / 4) + 4 (i % 4) of its 16, so accumulator element
+// r of lane group g is key g + 4 r, which is also the key that group loads of V.
+// K is 16-byte pieces of a key's row, V D / 16 bytes of a key for each lane.
+//
+// A block's K scale multiplies its scores. Its V scale joins the weights: with
+// s' = s + log2(v scale) the weight 2^(s' - m) multiplies the codes themselves
+// and 2^(s' - m) / (v scale) adds to l, so O needs no second accumulator. m runs
+// over s', is raised only when a score passes it by 8 or more, and the weights
+// carry 2^7 so that their fp16 high and low terms hold 22 bits down to 2^-10 of
+// the largest (as in the fp16 cache's kernel). Keys past a sequence's end read
+// its last key with weight 0. Sums, m and l are fp32.
+//
+// Bound by the cache's bytes.
+template <int D, int NW, int P, bool PARTIAL>
+__global__ __launch_bounds__(64 * NW) void decode_q8_kernel(AttnArgs a, float* __restrict__ part_o,
+                                                            float* __restrict__ part_ml) {
+  static_assert(D == 64 || D == 128, "head_dim 64 or 128");
+  constexpr int KS = D / 32;       // 32-dim steps of a score
+  constexpr int KL = D / 64;       // 16-byte loads of a key per lane
+  constexpr int VW = D / 16;       // dims of a value per lane: V words are VW / 4
+  constexpr int VD = VW / 4;
+  constexpr int WS = 16 * D + 32;  // floats of one wave's state in LDS
+  __shared__ __attribute__((aligned(16))) float s_state[NW > 1 ? NW * WS : 4];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15;
+  const int grp = lane >> 4;
+  const long long unit = blockIdx.x;
+  const int tile = static_cast<int>(unit % a.tiles);
+  const long long bh = unit / a.tiles;  // sequence and KV head
+  const long long b = bh / a.n_kv_heads;
+  const long long kvh = bh - b * a.n_kv_heads;
+  const int split = static_cast<int>(blockIdx.y);
+  const int gq = min(a.group - 16 * tile, 16);
+  const long long h0 = b * a.n_heads + kvh * a.group + 16 * tile;  // first (sequence, head)
+  const int len = static_cast<int>(std::min<long long>(max(a.lens[b], 0), a.max_len));
+  const int blocks = (len + kKvBlock - 1) / kKvBlock;
+  const long long t0 = static_cast<long long>(split) * a.split_blocks;
+  if (t0 >= blocks) {
+    // nothing here; a sequence without tokens gets zeros where no merge follows
+    if (!PARTIAL && blocks == 0) {
+      for (int i = tid; i < gq * D; i += 64 * NW) a.out[h0 * D + i] = static_cast<_Float16>(0.0f);
+    }
+    return;
+  }
+  const int nblocks = min(a.split_blocks, static_cast<int>(blocks - t0));
+  const int nkeys = min(nblocks * kKvBlock, static_cast<int>(len - t0 * kKvBlock));
+  const int nb = wave < nblocks ? (nblocks - wave + NW - 1) / NW : 0;  // this wave's blocks
+
+  // q^T as the score B operand: dims 64 (s / 2) + 16 grp + 8 (s % 2) + j of head col
+  halfx8 qb[KS];
+  const _Float16* qh = a.q + (h0 + min(col, gq - 1)) * D + 16 * grp;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) qb[s][j] = qh[64 * (s >> 1) + 8 * (s & 1) + j];
+  }
+  const float scale2 = a.scale * kLog2e;
+  const long long row0 = bh * a.kv_max + t0 * kKvBlock;
+  const unsigned char* kb = a.k + row0 * D + 16 * grp;
+  const unsigned char* vb = a.v + row0 * D + VW * col;
+  const long long sb = bh * ((a.kv_max + kKvBlock - 1) / kKvBlock) + t0;
+
+  typedef unsigned vword __attribute__((ext_vector_type(VD)));
+  struct Block {
+    uintx4 k[2][KL];
+    vword v[8];
+    float ks, vs;
+  };
+  auto load = [&](Block& x, int t) __attribute__((always_inline)) {
+    const int blk = min(wave + NW * t, nblocks - 1);
+    const int key0 = blk * kKvBlock;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long kk = min(key0 + 16 * h + (col >> 2) + 4 * (col & 3), nkeys - 1);
+#pragma unroll
+      for (int s = 0; s < KL; ++s)
+        x.k[h][s] = __builtin_nontemporal_load(reinterpret_cast<const uintx4*>(kb + kk * D + 64 * s));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const long long kk = min(key0 + 16 * (e >> 2) + grp + 4 * (e & 3), nkeys - 1);
+      x.v[e] = __builtin_nontemporal_load(reinterpret_cast<const vword*>(vb + kk * D));
+    }
+    x.ks = a.ks[sb + blk];
+    x.vs = a.vs[sb + blk];
+  };
+  auto group_max = [](float x) __attribute__((always_inline)) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+  };
+
+  constexpr float kLazy = 8.0f;
+  constexpr float kWeightShift = 7.0f;
+  float m = kNegInf;
+  float lsum = 0.0f;
+  floatx4 o[VW];
+#pragma unroll
+  for (int mb = 0; mb < VW; ++mb) o[mb] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // two e4m3 bytes (half H of a word) as fp16
+  auto two = [](unsigned w, auto half) __attribute__((always_inline)) {
+    halfx2 r = {};
+#if defined(__HIP_DEVICE_COMPILE__)
+    r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, decltype(half)::value);
+#endif
+    return r;
+  };
+  using Lo = std::false_type;
+  using Hi = std::true_type;
+  auto compute = [&](const Block& x, int t) __attribute__((always_inline)) {
+    floatx4 sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sc[h] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const unsigned w0 = x.k[h][s >> 1][2 * (s & 1)];
+        const unsigned w1 = x.k[h][s >> 1][2 * (s & 1) + 1];
+        const halfx2 c0 = two(w0, Lo{}), c1 = two(w0, Hi{}), c2 = two(w1, Lo{}), c3 = two(w1, Hi{});
+        [[maybe_unused]] const halfx8 ka = {c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
+#if defined(__HIP_DEVICE_COMPILE__)
+        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qb[s], sc[h], 0, 0, 0);
+#endif
+      }
+    }
+    const int kbase = (wave + NW * t) * kKvBlock + grp;
+    const float f = scale2 * x.ks;
+    const float lv = __builtin_amdgcn_logf(x.vs);  // log2
+    const float ivs = 1.0f / x.vs;
+    float sv[8];
+    float mx = kNegInf;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      sv[e] = kbase + 16 * (e >> 2) + 4 * (e & 3) < nkeys ? fmaf(sc[e >> 2][e & 3], f, lv) : kNegInf;
+      mx = fmaxf(mx, sv[e]);
+    }
+    mx = group_max(mx);
+    if (__any(mx > m + kLazy)) {
+      const float mn = fmaxf(m, mx);
+      const float alpha = weight2(m, mn);
+      m = mn;
+      lsum *= alpha;
+#pragma unroll
+      for (int mb = 0; mb < VW; ++mb) o[mb] *= alpha;
+    }
+    halfx8 ph, pl;
+    float ls = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float p = weight2(sv[e], m - kWeightShift);
+      ls += p;
+      ph[e] = static_cast<_Float16>(p);
+      pl[e] = static_cast<_Float16>(p - static_cast<float>(ph[e]));
+    }
+    lsum = fmaf(ls, ivs, lsum);
+#pragma unroll
+    for (int d = 0; d < VD; ++d) {
+      halfx8 av[4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const halfx2 c0 = two(x.v[e][d], Lo{}), c1 = two(x.v[e][d], Hi{});
+        av[0][e] = c0[0], av[1][e] = c0[1], av[2][e] = c1[0], av[3][e] = c1[1];
+      }
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        o[4 * d + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[u], pl, o[4 * d + u], 0, 0, 0);
+        o[4 * d + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[u], ph, o[4 * d + u], 0, 0, 0);
+      }
+#endif
+    }
+  };
+
+  Block buf[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) load(buf[i], i);
+  for (int t = 0; t < nb; t += P) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      if (t + i < nb) {
+        compute(buf[i], t + i);
+        if (t + i + P < nb) load(buf[i], t + i + P);
+      }
+    }
+  }
+
+  // Lane (col, grp) holds dims VW (4 grp + r) + mb of head col in o[mb][r].
+  float lt = lsum + __shfl_xor(lsum, 16);
+  lt += __shfl_xor(lt, 32);
+  if constexpr (NW == 1) {
+    if (col < gq) {
+      const long long h = h0 + col;
+      const long long slot = h * a.nsplit + split;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int mb = 0; mb < VW; ++mb) {
+          const int d = VW * (4 * grp + r) + mb;
+          if constexpr (PARTIAL) part_o[slot * D + d] = o[mb][r];
+          else a.out[h * D + d] = static_cast<_Float16>(o[mb][r] / lt);
+        }
+      }
+      if (PARTIAL && grp == 0) {
+        part_ml[2 * slot] = m;
+        part_ml[2 * slot + 1] = lt;
+      }
+    }
+    return;
+  }
+  float* const ws = s_state + wave * WS;
+  if (col < gq) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+      for (int c = 0; c < VW; c += 4)
+        *reinterpret_cast<floatx4*>(ws + col * D + VW * (4 * grp + r) + c) =
+            floatx4{o[c][r], o[c + 1][r], o[c + 2][r], o[c + 3][r]};
+    }
+    if (grp == 0) {
+      ws[16 * D + col] = m;
+      ws[16 * D + 16 + col] = lt;
+    }
+  }
+  __syncthreads();
+  const int live = min(NW, nblocks);  // waves with a block
+  for (int idx = tid; idx < gq * D; idx += 64 * NW) {
+    const int gh = idx / D;
+    const int d = idx - gh * D;
+    float mb = kNegInf;
+    for (int w = 0; w < live; ++w) mb = fmaxf(mb, s_state[w * WS + 16 * D + gh]);
+    float lb = 0.0f, ob = 0.0f;
+    for (int w = 0; w < live; ++w) {
+      const float wt = weight2(s_state[w * WS + 16 * D + gh], mb);
+      lb = fmaf(s_state[w * WS + 16 * D + 16 + gh], wt, lb);
+      ob = fmaf(s_state[w * WS + gh * D + d], wt, ob);
+    }
+    const long long h = h0 + gh;
+    if constexpr (PARTIAL) {
+      const long long slot = h * a.nsplit + split;
+      part_o[slot * D + d] = ob;
+      if (d == 0) {
+        part_ml[2 * slot] = mb;
+        part_ml[2 * slot + 1] = lb;
+      }
+    } else {
+      a.out[h * D + d] = static_cast<_Float16>(ob / lb);
+    }
+  }
+}
+
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the splits that the
+// sequence's length reaches, one workgroup of D threads per (sequence, head), in
+// split order.
+template <int D>
+__global__ __launch_bounds__(D) void merge_q8_kernel(const float* __restrict__ part_o,
+                                                     const float* __restrict__ part_ml,
+                                                     const int* __restrict__ lens,
+                                                     _Float16* __restrict__ out, long long n_heads,
+                                                     long long max_len, int split_blocks,
+                                                     int nsplit) {
+  const long long h = blockIdx.x;
+  const int d = threadIdx.x;
+  const int len = static_cast<int>(std::min<long long>(max(lens[h / n_heads], 0), max_len));
+  const int blocks = (len + kKvBlock - 1) / kKvBlock;
+  const int ns = (blocks + split_blocks - 1) / split_blocks;
+  const long long base = h * nsplit;
+  float mx = kNegInf;
+  for (int s = 0; s < ns; ++s) mx = fmaxf(mx, part_ml[2 * (base + s)]);
+  float l = 0.0f, o = 0.0f;
+  for (int s = 0; s < ns; ++s) {
+    const float w = weight2(part_ml[2 * (base + s)], mx);
+    l = fmaf(part_ml[2 * (base + s) + 1], w, l);
+    o = fmaf(part_o[(base + s) * D + d], w, o);
+  }
+  out[h * D + d] = static_cast<_Float16>(ns == 0 ? 0.0f : o / l);
+}
+
+// Splits when the caller passes split_kv = 0: about two workgroups per CU over
+// all (sequence, head) units, at least two blocks per split.
+int auto_splits(long long blocks, long long units) {
+  const long long cus = device_cu_count();
+  const long long wanted = (2 * cus + units - 1) / units;
+  return static_cast<int>(std::max(1ll, std::min({wanted, blocks / 2, 256ll})));
+}
+
+template <int D, bool PARTIAL>
+void launch_decode(const AttnArgs& a, float* part_o, float* part_ml, dim3 grid, hipStream_t s) {
+  auto go = [&](auto kernel, int waves) {
+    kernel<<<grid, 64 * waves, 0, s>>>(a, part_o, part_ml);
+  };
+  if (a.split_blocks <= 1) go(decode_q8_kernel<D, 1, 1, PARTIAL>, 1);
+  else if (a.split_blocks <= 2) go(decode_q8_kernel<D, 2, 1, PARTIAL>, 2);
+  else if (a.split_blocks <= 4) go(decode_q8_kernel<D, 4, 1, PARTIAL>, 4);
+  else if (a.split_blocks <= 8) go(decode_q8_kernel<D, 8, 1, PARTIAL>, 8);
+  else go(decode_q8_kernel<D, 8, 2, PARTIAL>, 8);
+  ENG_LAUNCH_CHECK();
+}
+
+template <int D>
+void run_decode(AttnArgs a, long long batch, hipStream_t s) {
+  const long long units = batch * a.n_kv_heads * a.tiles;
+  const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(a.nsplit));
+  if (a.nsplit == 1) {
+    launch_decode<D, false>(a, nullptr, nullptr, grid, s);
+    return;
+  }
+  const std::size_t slots = static_cast<std::size_t>(batch) * a.n_heads * a.nsplit;
+  StreamScratch scratch(s, slots * (D + 2) * sizeof(float));
+  float* part_o = static_cast<float*>(scratch.get());
+  float* part_ml = part_o + slots * D;
+  launch_decode<D, true>(a, part_o, part_ml, grid, s);
+  merge_q8_kernel<D><<<static_cast<unsigned>(batch * a.n_heads), D, 0, s>>>(
+      part_o, part_ml, a.lens, a.out, a.n_heads, a.max_len, a.split_blocks, a.nsplit);
+  ENG_LAUNCH_CHECK();
+}
+
+constexpr long long kMaxLen = 0x7fffffffLL - kKvBlock;  // positions are 32-bit on the device
+
+}  // namespace
+}  // namespace eng
+
+using eng::guarded;
+
+extern "C" {
+
+int eng_kv_cache_write_q8(const eng_half* k_new, const eng_half* v_new, uint8_t* k_cache,
+                          uint8_t* v_cache, float* k_scale, float* v_scale, const int32_t* pos,
+                          const int32_t* n_new, int64_t batch, int64_t s_new, int64_t n_kv_heads,
+                          int64_t head_dim, int64_t kv_max_seq_len, eng_stream stream) {
+  return guarded([&] {
+    ENG_CHECK(batch >= 0, "kv_cache_write_q8: batch must be non-negative");
+    ENG_CHECK(s_new >= 0, "kv_cache_write_q8: s_new must be non-negative");
+    ENG_CHECK(n_kv_heads > 0, "kv_cache_write_q8: n_kv_heads must be positive");
+    ENG_CHECK(head_dim == 64 || head_dim == 128, "kv_cache_write_q8: head_dim must be 64 or 128");
+    ENG_CHECK(kv_max_seq_len >= 0 && kv_max_seq_len <= eng::kMaxLen,
+              "kv_cache_write_q8: kv_max_seq_len must be non-negative and below 2^31 - 32");
+    ENG_CHECK(s_new <= kv_max_seq_len, "kv_cache_write_q8: kv_max_seq_len < s_new");
+    if (batch == 0 || s_new == 0) return;
+    ENG_CHECK(k_new != nullptr && v_new != nullptr, "kv_cache_write_q8: k_new/v_new is null");
+    ENG_CHECK(k_cache != nullptr && v_cache != nullptr, "kv_cache_write_q8: k_cache/v_cache is null");
+    ENG_CHECK(k_scale != nullptr && v_scale != nullptr, "kv_cache_write_q8: k_scale/v_scale is null");
+    ENG_CHECK(pos != nullptr, "kv_cache_write_q8: pos is null");
+    ENG_CHECK(eng::aligned_to(k_new, 16) && eng::aligned_to(v_new, 16) &&
+                  eng::aligned_to(k_cache, 16) && eng::aligned_to(v_cache, 16),
+              "kv_cache_write_q8: k_new, v_new and the caches must be 16-byte aligned");
+    const int reach = static_cast<int>((s_new + eng::kKvBlock - 2) / eng::kKvBlock + 1);
+    ENG_CHECK(batch <= 0x7fffffffLL && n_kv_heads <= 0x7fffffffLL &&
+                  batch * n_kv_heads <= 0x7fffffffLL / reach,
+              "kv_cache_write_q8: too many (sequence, head, block) units for one launch");
+    const long long units = 2 * batch * n_kv_heads * reach;
+    const unsigned grid = static_cast<unsigned>((units + 3) / 4);
+    auto go = [&](auto kernel) {
+      kernel<<<grid, eng::kWriteThreads, 0, eng::as_stream(stream)>>>(
+          reinterpret_cast<const _Float16*>(k_new), reinterpret_cast<const _Float16*>(v_new),
+          k_cache, v_cache, k_scale, v_scale, pos, n_new, units, s_new, n_kv_heads, kv_max_seq_len,
+          reach);
+    };
+    if (head_dim == 64) go(eng::kv_write_q8_kernel<64>);
+    else go(eng::kv_write_q8_kernel<128>);
+    ENG_LAUNCH_CHECK();
+  });
+}
+
+int eng_attention_decode_q8(const eng_half* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                            const float* k_scale, const float* v_scale, eng_half* out,
+                            const int32_t* kv_len, int64_t batch, int64_t n_heads,
+                            int64_t n_kv_heads, int64_t head_dim, int64_t max_kv_len,
+                            int64_t kv_max_seq_len, float scale, int split_kv, eng_stream stream) {
+  return guarded([&] {
+    ENG_CHECK(q != nullptr, "attention_decode_q8: q is null");
+    ENG_CHECK(k_cache != nullptr, "attention_decode_q8: k_cache is null");
+    ENG_CHECK(v_cache != nullptr, "attention_decode_q8: v_cache is null");
+    ENG_CHECK(k_scale != nullptr && v_scale != nullptr, "attention_decode_q8: k_scale/v_scale is null");
+    ENG_CHECK(out != nullptr, "attention_decode_q8: out is null");
+    ENG_CHECK(kv_len != nullptr, "attention_decode_q8: kv_len is null");
+    ENG_CHECK(batch >= 0, "attention_decode_q8: batch must be non-negative");
+    ENG_CHECK(n_heads > 0, "attention_decode_q8: n_heads must be positive");
+    ENG_CHECK(n_kv_heads > 0, "attention_decode_q8: n_kv_heads must be positive");
+    ENG_CHECK(n_heads % n_kv_heads == 0,
+              "attention_decode_q8: n_heads must be divisible by n_kv_heads");
+    ENG_CHECK(head_dim == 64 || head_dim == 128, "attention_decode_q8: head_dim must be 64 or 128");
+    ENG_CHECK(max_kv_len >= 0, "attention_decode_q8: max_kv_len must be non-negative");
+    ENG_CHECK(kv_max_seq_len >= max_kv_len, "attention_decode_q8: kv_max_seq_len < max_kv_len");
+    ENG_CHECK(kv_max_seq_len <= eng::kMaxLen,
+              "attention_decode_q8: kv_max_seq_len must be below 2^31 - 32");
+    ENG_CHECK(std::isfinite(scale), "attention_decode_q8: scale must be finite");
+    ENG_CHECK(split_kv >= 0, "attention_decode_q8: split_kv must be non-negative");
+    ENG_CHECK(eng::aligned_to(k_cache, 16) && eng::aligned_to(v_cache, 16),
+              "attention_decode_q8: the caches must be 16-byte aligned");
+    if (batch == 0) return;
+    ENG_CHECK(batch <= 0x7fffffffLL && n_heads <= 0x7fffffffLL && batch * n_heads <= 0x7fffffffLL,
+              "attention_decode_q8: too many (sequence, head) pairs for one launch");
+    hipStream_t s = eng::as_stream(stream);
+    if (max_kv_len == 0) {
+      eng::fill_zero_async(out, static_cast<std::size_t>(batch * n_heads * head_dim) * sizeof(eng_half), s);
+      return;
+    }
+    eng::AttnArgs a;
+    a.q = reinterpret_cast<const _Float16*>(q);
+    a.k = k_cache;
+    a.v = v_cache;
+    a.ks = k_scale;
+    a.vs = v_scale;
+    a.out = reinterpret_cast<_Float16*>(out);
+    a.lens = kv_len;
+    a.n_heads = n_heads;
+    a.n_kv_heads = n_kv_heads;
+    a.max_len = max_kv_len;
+    a.kv_max = kv_max_seq_len;
+    a.group = static_cast<int>(n_heads / n_kv_heads);
+    a.tiles = (a.group + 15) / 16;
+    a.scale = scale;
+    const long long blocks = (max_kv_len + eng::kKvBlock - 1) / eng::kKvBlock;
+    const long long want = split_kv == 0
+                               ? eng::auto_splits(blocks, batch * n_kv_heads * a.tiles)
+                               : std::min<long long>({split_kv, blocks, 256});
+    a.split_blocks = static_cast<int>((blocks + want - 1) / want);
+    a.nsplit = static_cast<int>((blocks + a.split_blocks - 1) / a.split_blocks);
+    if (head_dim == 64) eng::run_decode<64>(a, batch, s);
+    else eng::run_decode<128>(a, batch, s);
+  });
+}
+
+}  // extern "C"

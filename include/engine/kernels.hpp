@@ -125,6 +125,41 @@ inline void rmsnorm_linear_nk(const float* in, const float* rms_weight, const fl
   ENGINE_ABI_CHECK(eng_rmsnorm_linear_f32_nk(in, rms_weight, W, out, M, N, K, eps, stream));
 }
 
+/// Weights in microscaled 4-bit floating point (additive): src [rows x cols] to
+/// codes [rows x 16 ceil(cols / 32)] and scale bytes [rows x ceil(cols / 32)],
+/// and the values back. The format is described in engine_hip.h.
+inline void mx4_quantize(const float* src, std::uint8_t* codes, std::uint8_t* scales,
+                         std::int64_t rows, std::int64_t cols, hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_mx4_quantize_f32(src, codes, scales, rows, cols, stream));
+}
+inline void mx4_quantize(const half* src, std::uint8_t* codes, std::uint8_t* scales,
+                         std::int64_t rows, std::int64_t cols, hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_mx4_quantize_f16(detail::bits(src), codes, scales, rows, cols, stream));
+}
+inline void mx4_dequantize(const std::uint8_t* codes, const std::uint8_t* scales, float* dst,
+                           std::int64_t rows, std::int64_t cols, hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_mx4_dequantize_f32(codes, scales, dst, rows, cols, stream));
+}
+inline void mx4_dequantize(const std::uint8_t* codes, const std::uint8_t* scales, half* dst,
+                           std::int64_t rows, std::int64_t cols, hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_mx4_dequantize_f16(codes, scales, detail::bits(dst), rows, cols, stream));
+}
+
+/// Output-major 4-bit weights W [N x K]: y[M x N] = x[M x K] * W^T, any M.
+inline void linear_nk(const float* x, const std::uint8_t* codes, const std::uint8_t* scales,
+                      float* y, std::int64_t M, std::int64_t N, std::int64_t K,
+                      hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_linear_mx4w_nk(x, codes, scales, y, M, N, K, stream));
+}
+/// out[M x N] = RMSNorm(in[M x K], rms_weight, eps) * W^T with the same weights.
+inline void rmsnorm_linear_nk(const float* in, const float* rms_weight, const std::uint8_t* codes,
+                              const std::uint8_t* scales, float* out, std::int64_t M,
+                              std::int64_t N, std::int64_t K, float eps,
+                              hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(
+      eng_rmsnorm_linear_mx4w_nk(in, rms_weight, codes, scales, out, M, N, K, eps, stream));
+}
+
 /// out[i] = a[i] + b[i], bit-exact (reference kernels.hpp:47-50).
 inline void vector_add(const float* a, const float* b, float* out, std::int64_t n,
                        hipStream_t stream = nullptr) {
@@ -228,6 +263,34 @@ inline void attention_decode(const half* q, const half* k, const half* v, half* 
   ENGINE_ABI_CHECK(eng_attention_decode_f16(detail::bits(q), detail::bits(k), detail::bits(v),
                                             detail::bits(out), kv_len, n_heads, n_kv_heads,
                                             head_dim, kv_head_stride, scale, split_kv, stream));
+}
+
+/// New K / V rows of a batch of sequences into 8-bit (e4m3) caches with one scale
+/// for each 32 tokens of a head, at device positions pos[b] (additive).
+inline void kv_cache_write_q8(const half* k_new, const half* v_new, std::uint8_t* k_cache,
+                              std::uint8_t* v_cache, float* k_scale, float* v_scale,
+                              const std::int32_t* pos, const std::int32_t* n_new,
+                              std::int64_t batch, std::int64_t s_new, std::int64_t n_kv_heads,
+                              std::int64_t head_dim, std::int64_t kv_max_seq_len,
+                              hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_kv_cache_write_q8(detail::bits(k_new), detail::bits(v_new), k_cache, v_cache,
+                                         k_scale, v_scale, pos, n_new, batch, s_new, n_kv_heads,
+                                         head_dim, kv_max_seq_len, stream));
+}
+
+/// Single-token decode attention of a batch over such caches, lengths kv_len[b]
+/// on the device and at most max_kv_len (additive).
+inline void attention_decode_q8(const half* q, const std::uint8_t* k_cache,
+                                const std::uint8_t* v_cache, const float* k_scale,
+                                const float* v_scale, half* out, const std::int32_t* kv_len,
+                                std::int64_t batch, std::int64_t n_heads, std::int64_t n_kv_heads,
+                                std::int64_t head_dim, std::int64_t max_kv_len,
+                                std::int64_t kv_max_seq_len, float scale, int split_kv = 0,
+                                hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_attention_decode_q8(detail::bits(q), k_cache, v_cache, k_scale, v_scale,
+                                           detail::bits(out), kv_len, batch, n_heads, n_kv_heads,
+                                           head_dim, max_kv_len, kv_max_seq_len, scale, split_kv,
+                                           stream));
 }
 
 }  // namespace hip

@@ -437,6 +437,97 @@ int eng_transpose_f32(const float* src, float* dst, int64_t rows, int64_t cols,
                       eng_stream stream);
 
 /* ------------------------------------------------------------------------
+ * Weights in microscaled 4-bit floating point (MXFP4 of the OCP Microscaling
+ * Formats specification v1.0; additive, no reference counterpart).
+ *
+ * A matrix [rows x cols] is two buffers. Each run of 32 values along a row (a
+ * block; the last one of a row is filled with zeros) shares a scale 2^(s - 127)
+ * held as the byte s, 255 standing for NaN; a value is a 4-bit code: sign and
+ * one of 0, 0.5, 1, 1.5, 2, 3, 4, 6. With nb = ceil(cols / 32):
+ *   codes   rows * nb * 16 bytes, 16-byte aligned: row r's at r * nb * 16, two
+ *           values a byte, the even one in the low four bits
+ *   scales  rows * nb bytes: row r's at r * nb
+ *
+ * eng_mx4_quantize_*: the scale's exponent is floor(log2(largest magnitude of
+ * the block)) - 2, at least -127 (s = 0, also for a block of zeros); values are
+ * divided by the scale and rounded to the nearest code, ties to the even one,
+ * magnitudes above 6 to 6. A block that holds a NaN or an infinity gets s = 255
+ * and zero codes. Output-major weights [N x K] (eng_transpose_* makes them) are
+ * quantised along K, as the products below take them.
+ * eng_mx4_dequantize_*: the values again, rounded to nearest even where fp16
+ * does not hold them (infinity past its range).
+ * rows == 0 or cols == 0 is a no-op. src / dst need no more than their type's
+ * alignment; at 16 bytes and rows of whole 16 bytes they move in 16-byte pieces.
+ *
+ * eng_linear_mx4w_nk: y[M x N] = x[M x K] . W^T, fp32 x and y, W [N x K] as
+ * above, for any M (M == 1 is the decode GEMV). K == 0 zero-fills y.
+ * eng_rmsnorm_linear_mx4w_nk: out = RMSNorm(in, rms_weight, eps) . W^T, rms_weight
+ * may be NULL; as for eng_rmsnorm_linear_* any zero dimension is a no-op.
+ * Products are exact and sums fp32, as for fp16 weights: every fp32 activation
+ * enters the matrix cores as three bf16 terms that add up to it. K is at most
+ * 2^31 - 256. The same call gives the same bits; the kernel, and with it the
+ * order of the sums, depends on M, N, K and the alignment of x.
+ * ---------------------------------------------------------------------- */
+int eng_mx4_quantize_f32(const float* src, uint8_t* codes, uint8_t* scales, int64_t rows,
+                         int64_t cols, eng_stream stream);
+int eng_mx4_quantize_f16(const eng_half* src, uint8_t* codes, uint8_t* scales, int64_t rows,
+                         int64_t cols, eng_stream stream);
+int eng_mx4_dequantize_f32(const uint8_t* codes, const uint8_t* scales, float* dst, int64_t rows,
+                           int64_t cols, eng_stream stream);
+int eng_mx4_dequantize_f16(const uint8_t* codes, const uint8_t* scales, eng_half* dst,
+                           int64_t rows, int64_t cols, eng_stream stream);
+int eng_linear_mx4w_nk(const float* x, const uint8_t* codes, const uint8_t* scales, float* y,
+                       int64_t M, int64_t N, int64_t K, eng_stream stream);
+int eng_rmsnorm_linear_mx4w_nk(const float* in, const float* rms_weight, const uint8_t* codes,
+                               const uint8_t* scales, float* out, int64_t M, int64_t N, int64_t K,
+                               float eps, eng_stream stream);
+
+/* ------------------------------------------------------------------------
+ * A KV cache in 8 bits for batches of sequences (additive; the fp16 cache of one
+ * sequence is eng_kv_cache_write_f16 / eng_attention_decode_f16).
+ *
+ * Caches are e4m3 bytes (OCP FP8: no infinity, largest value 448), head-major,
+ * [batch, n_kv_heads, kv_max_seq_len, head_dim], 16-byte aligned; every block of
+ * ENG_KV_Q8_BLOCK tokens of a (sequence, KV head) has one fp32 scale for K and
+ * one for V, [batch, n_kv_heads, ceil(kv_max_seq_len / ENG_KV_Q8_BLOCK)]. The
+ * value of a code is its e4m3 value times its block's scale. head_dim is 64 or
+ * 128. Positions and lengths are read on the device (int32 arrays of `batch`), so
+ * a captured decode step is replayed for every token.
+ *
+ * eng_kv_cache_write_q8: rows k_new / v_new [batch, s_new, n_kv_heads, head_dim]
+ * (16-byte aligned) become tokens pos[b] .. of sequence b; the first n_new[b] of
+ * its s_new rows where n_new is given, all of them where it is NULL. A block's
+ * scale is the least power of two from 2^-15 to 2^8 that brings its largest
+ * finite new magnitude to 448 or below, or its present scale if that is larger
+ * and the block holds tokens before pos[b]; if the scale grows, the codes of
+ * those tokens are rounded to it. Values are rounded to nearest even; infinities
+ * and NaN become NaN codes and do not count for the scale. Tokens at or past
+ * kv_max_seq_len are dropped, and a sequence with pos[b] < 0 or n_new[b] <= 0 is
+ * left as it is. What a block holds behind the last new token is no longer
+ * defined: those tokens are not part of the sequence. s_new <= kv_max_seq_len.
+ *
+ * eng_attention_decode_q8: for each sequence b and query head h,
+ *   out[b][h] = softmax(scale q[b][h] . K[b][h / (n_heads / n_kv_heads)]^T) . V
+ * over its first kv_len[b] tokens, q and out fp16 [batch, n_heads, head_dim]; a
+ * sequence without tokens (kv_len[b] <= 0) gets zeros. max_kv_len is the caller's
+ * bound on kv_len: it chooses the launch, lengths above it are taken as
+ * max_kv_len. split_kv = 0 chooses the number of splits of a sequence; a
+ * positive value asks for as many (at most 256, and at least one block each).
+ * Blocks that a sequence's length reaches must have been written. Scores, softmax
+ * and sums are fp32. More than one split uses the stream's scratch arena.
+ * ---------------------------------------------------------------------- */
+#define ENG_KV_Q8_BLOCK 32
+int eng_kv_cache_write_q8(const eng_half* k_new, const eng_half* v_new, uint8_t* k_cache,
+                          uint8_t* v_cache, float* k_scale, float* v_scale, const int32_t* pos,
+                          const int32_t* n_new, int64_t batch, int64_t s_new, int64_t n_kv_heads,
+                          int64_t head_dim, int64_t kv_max_seq_len, eng_stream stream);
+int eng_attention_decode_q8(const eng_half* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                            const float* k_scale, const float* v_scale, eng_half* out,
+                            const int32_t* kv_len, int64_t batch, int64_t n_heads,
+                            int64_t n_kv_heads, int64_t head_dim, int64_t max_kv_len,
+                            int64_t kv_max_seq_len, float scale, int split_kv, eng_stream stream);
+
+/* ------------------------------------------------------------------------
  * ENGREF01 tensor files and device weight slabs.
  *
  * The container is the reference's golden format (tools/gen_reference.py:
