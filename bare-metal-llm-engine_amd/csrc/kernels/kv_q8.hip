@@ -28,6 +28,8 @@ typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 constexpr int kKvBlock = 32;  // tokens that share a scale
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
+[[maybe_unused]] constexpr int kRsrcWord3 = 0x00020000;  // buffer descriptor: raw, 32-bit elements
+[[maybe_unused]] constexpr int kNonTemporal = 2;  // a buffer load's cache policy
 
 // ------------------------------------------------------------------- append
 
@@ -172,7 +174,8 @@ struct AttnArgs {
 
 // One workgroup per (sequence, KV head, tile of up to 16 of its query heads,
 // split of `split_blocks` 32-token blocks), NW waves, block t of the split to
-// wave t % NW, P blocks in flight per wave. The matrix cores do both products:
+// wave t % NW, P blocks in flight per wave (RING: more than P of them, the loads of
+// one P blocks on following each compute). The matrix cores do both products:
 // scores S^T = K . Q^T with K as the A operand (the e4m3 bytes converted to
 // fp16, exact), O^T = V^T . P^T with the score accumulators, in place, as the B
 // operand: A row i is key (i / 4) + 4 (i % 4) of its 16, so accumulator element
@@ -184,20 +187,26 @@ struct AttnArgs {
 // and 2^(s' - m) / (v scale) adds to l, so O needs no second accumulator. m runs
 // over s', is raised only when a score passes it by 8 or more, and the weights
 // carry 2^7 so that their fp16 high and low terms hold 22 bits down to 2^-10 of
-// the largest (as in the fp16 cache's kernel). Keys past a sequence's end read
-// its last key with weight 0. Sums, m and l are fp32.
+// the largest (as in the fp16 cache's kernel). Sums, m and l are fp32.
 //
-// Bound by the cache's bytes.
-template <int D, int NW, int P, bool PARTIAL>
-__global__ __launch_bounds__(64 * NW) void decode_q8_kernel(AttnArgs a, float* __restrict__ part_o,
+// Bound by the cache's bytes: 131072 tokens of 32 / 8 heads, D = 128 (270 MB) in 46
+// us with the merge, 5.9 TB/s. Workgroups of 4 waves, three to a CU, cover the
+// latency of a split's start and end (16 unlike sequences of up to 8192 tokens: 29
+// us, 35 on 8 waves). K's 64-byte pieces stay cacheable, since two loads share a
+// line; V's whole rows are read past the caches (16 sequences 29 us, 32 with V
+// cached, 33 with K uncached as well).
+template <int D, int NW, int P, bool RING, bool PARTIAL>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 3 : 1) void decode_q8_kernel(AttnArgs a, float* __restrict__ part_o,
                                                             float* __restrict__ part_ml) {
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");
   constexpr int KS = D / 32;       // 32-dim steps of a score
   constexpr int KL = D / 64;       // 16-byte loads of a key per lane
   constexpr int VW = D / 16;       // dims of a value per lane: V words are VW / 4
   constexpr int VD = VW / 4;
-  constexpr int WS = 16 * D + 32;  // floats of one wave's state in LDS
-  __shared__ __attribute__((aligned(16))) float s_state[NW > 1 ? NW * WS : 4];
+  // One wave's state in LDS, for the heads that the tile has: o [heads][D], m, l.
+  extern __shared__ __attribute__((aligned(16))) float s_state[];
+  const int heads = min(a.group, 16);
+  const int WS = heads * (D + 2);
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -229,15 +238,30 @@ __global__ __launch_bounds__(64 * NW) void decode_q8_kernel(AttnArgs a, float* _
   // q^T as the score B operand: dims 64 (s / 2) + 16 grp + 8 (s % 2) + j of head col
   halfx8 qb[KS];
   const _Float16* qh = a.q + (h0 + min(col, gq - 1)) * D + 16 * grp;
+  if ((reinterpret_cast<std::uintptr_t>(a.q) & 15) == 0) {
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
+    for (int s = 0; s < KS; ++s)
+      qb[s] = *reinterpret_cast<const halfx8*>(qh + 64 * (s >> 1) + 8 * (s & 1));
+  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) qb[s][j] = qh[64 * (s >> 1) + 8 * (s & 1) + j];
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) qb[s][j] = qh[64 * (s >> 1) + 8 * (s & 1) + j];
+    }
   }
   const float scale2 = a.scale * kLog2e;
-  const long long row0 = bh * a.kv_max + t0 * kKvBlock;
-  const unsigned char* kb = a.k + row0 * D + 16 * grp;
-  const unsigned char* vb = a.v + row0 * D + VW * col;
+  // The split's part of each cache through a buffer descriptor that ends with its
+  // last token: rows past it read as zeros (weight 0, and no stale code can reach a
+  // product), and a block's loads need one address each for K and V.
+  [[maybe_unused]] const long long row0 = (bh * a.kv_max + t0 * kKvBlock) * D;
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.k + row0), 0,
+                                                    nkeys * D, kRsrcWord3);
+  const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.v + row0), 0,
+                                                    nkeys * D, kRsrcWord3);
+#endif
+  [[maybe_unused]] const int koff = ((col >> 2) + 4 * (col & 3)) * D + 16 * grp;
+  [[maybe_unused]] const int voff = grp * D + VW * col;
   const long long sb = bh * ((a.kv_max + kKvBlock - 1) / kKvBlock) + t0;
 
   typedef unsigned vword __attribute__((ext_vector_type(VD)));
@@ -246,27 +270,44 @@ __global__ __launch_bounds__(64 * NW) void decode_q8_kernel(AttnArgs a, float* _
     vword v[8];
     float ks, vs;
   };
+  // Every call issues the same loads, whether or not the wave has a block t (past
+  // the last one they return zeros without a memory access), so that the waits
+  // count exactly the blocks in flight behind the one a compute needs.
   auto load = [&](Block& x, int t) __attribute__((always_inline)) {
-    const int blk = min(wave + NW * t, nblocks - 1);
-    const int key0 = blk * kKvBlock;
+    const int blk = wave + NW * t;
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int at = blk * (kKvBlock * D);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const long long kk = min(key0 + 16 * h + (col >> 2) + 4 * (col & 3), nkeys - 1);
 #pragma unroll
       for (int s = 0; s < KL; ++s)
-        x.k[h][s] = __builtin_nontemporal_load(reinterpret_cast<const uintx4*>(kb + kk * D + 64 * s));
+        x.k[h][s] = __builtin_amdgcn_raw_buffer_load_b128(rk, at + koff + 16 * h * D + 64 * s, 0, 0);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const long long kk = min(key0 + 16 * (e >> 2) + grp + 4 * (e & 3), nkeys - 1);
-      x.v[e] = __builtin_nontemporal_load(reinterpret_cast<const vword*>(vb + kk * D));
+      const int o = at + voff + (16 * (e >> 2) + 4 * (e & 3)) * D;
+      if constexpr (VD == 2) x.v[e] = __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, kNonTemporal);
+      else x.v[e][0] = __builtin_amdgcn_raw_buffer_load_b32(rv, o, 0, kNonTemporal);
     }
-    x.ks = a.ks[sb + blk];
-    x.vs = a.vs[sb + blk];
+#endif
+    const int sblk = min(blk, nblocks - 1);
+    x.ks = a.ks[sb + sblk];
+    x.vs = a.vs[sb + sblk];
   };
+  // Largest of x over the four lanes of a head (each swap leaves this lane's value
+  // and its partner's in the two results, copied to scalars before they are cast).
   auto group_max = [](float x) __attribute__((always_inline)) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+#if defined(__HIP_DEVICE_COMPILE__)
+    const unsigned u = __float_as_uint(x);
+    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned p0 = p[0], p1 = p[1];
+    x = fmaxf(__uint_as_float(p0), __uint_as_float(p1));
+    const unsigned w = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    x = fmaxf(__uint_as_float(r0), __uint_as_float(r1));
+#endif
+    return x;
   };
 
   constexpr float kLazy = 8.0f;
@@ -303,17 +344,20 @@ __global__ __launch_bounds__(64 * NW) void decode_q8_kernel(AttnArgs a, float* _
 #endif
       }
     }
-    const int kbase = (wave + NW * t) * kKvBlock + grp;
+    const int left = nkeys - (wave + NW * t) * kKvBlock;  // keys from the block's first one on
     const float f = scale2 * x.ks;
     const float lv = __builtin_amdgcn_logf(x.vs);  // log2
-    const float ivs = 1.0f / x.vs;
+    const float ivs = __builtin_amdgcn_rcpf(x.vs);
     float sv[8];
-    float mx = kNegInf;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      sv[e] = kbase + 16 * (e >> 2) + 4 * (e & 3) < nkeys ? fmaf(sc[e >> 2][e & 3], f, lv) : kNegInf;
-      mx = fmaxf(mx, sv[e]);
+    for (int e = 0; e < 8; ++e) sv[e] = fmaf(sc[e >> 2][e & 3], f, lv);
+    if (left < kKvBlock) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (grp + 16 * (e >> 2) + 4 * (e & 3) >= left) sv[e] = kNegInf;
     }
+    float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])),
+                     fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
     mx = group_max(mx);
     if (__any(mx > m + kLazy)) {
       const float mn = fmaxf(m, mx);
@@ -323,14 +367,22 @@ __global__ __launch_bounds__(64 * NW) void decode_q8_kernel(AttnArgs a, float* _
 #pragma unroll
       for (int mb = 0; mb < VW; ++mb) o[mb] *= alpha;
     }
-    halfx8 ph, pl;
+    // (while every score so far is -inf, against 0: weights 0, not NaN)
+    const float ref = m == kNegInf ? 0.0f : m - kWeightShift;
+    [[maybe_unused]] halfx8 ph, pl;
     float ls = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float p = weight2(sv[e], m - kWeightShift);
-      ls += p;
-      ph[e] = static_cast<_Float16>(p);
-      pl[e] = static_cast<_Float16>(p - static_cast<float>(ph[e]));
+    for (int e = 0; e < 8; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(sv[e] - ref);
+      const float p1 = __builtin_amdgcn_exp2f(sv[e + 1] - ref);
+      ls += p0 + p1;
+#if defined(__HIP_DEVICE_COMPILE__)
+      const halfx2 hi = __builtin_bit_cast(halfx2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+      const halfx2 lo = __builtin_bit_cast(
+          halfx2, __builtin_amdgcn_cvt_pkrtz(p0 - static_cast<float>(hi[0]), p1 - static_cast<float>(hi[1])));
+      ph[e] = hi[0], ph[e + 1] = hi[1];
+      pl[e] = lo[0], pl[e + 1] = lo[1];
+#endif
     }
     lsum = fmaf(ls, ivs, lsum);
 #pragma unroll
@@ -353,13 +405,22 @@ __global__ __launch_bounds__(64 * NW) void decode_q8_kernel(AttnArgs a, float* _
 
   Block buf[P];
 #pragma unroll
-  for (int i = 0; i < P; ++i) load(buf[i], i);
-  for (int t = 0; t < nb; t += P) {
+  for (int i = 0; i < P; ++i) {
+    load(buf[i], i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if constexpr (!RING) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      if (t + i < nb) {
-        compute(buf[i], t + i);
-        if (t + i + P < nb) load(buf[i], t + i + P);
+    for (int i = 0; i < P; ++i)
+      if (i < nb) compute(buf[i], i);
+  } else {
+    for (int t = 0; t < nb; t += P) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        if (t + i < nb) compute(buf[i], t + i);
+        __builtin_amdgcn_sched_barrier(0);
+        load(buf[i], t + i + P);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -392,13 +453,13 @@ __global__ __launch_bounds__(64 * NW) void decode_q8_kernel(AttnArgs a, float* _
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
 #pragma unroll
-      for (int c = 0; c < VW; c += 4)
-        *reinterpret_cast<floatx4*>(ws + col * D + VW * (4 * grp + r) + c) =
-            floatx4{o[c][r], o[c + 1][r], o[c + 2][r], o[c + 3][r]};
+      for (int c = 0; c < VW; c += 2)  // (a state's start is 8-byte aligned)
+        *reinterpret_cast<floatx2*>(ws + col * D + VW * (4 * grp + r) + c) =
+            floatx2{o[c][r], o[c + 1][r]};
     }
     if (grp == 0) {
-      ws[16 * D + col] = m;
-      ws[16 * D + 16 + col] = lt;
+      ws[heads * D + col] = m;
+      ws[heads * (D + 1) + col] = lt;
     }
   }
   __syncthreads();
@@ -407,11 +468,11 @@ __global__ __launch_bounds__(64 * NW) void decode_q8_kernel(AttnArgs a, float* _
     const int gh = idx / D;
     const int d = idx - gh * D;
     float mb = kNegInf;
-    for (int w = 0; w < live; ++w) mb = fmaxf(mb, s_state[w * WS + 16 * D + gh]);
+    for (int w = 0; w < live; ++w) mb = fmaxf(mb, s_state[w * WS + heads * D + gh]);
     float lb = 0.0f, ob = 0.0f;
     for (int w = 0; w < live; ++w) {
-      const float wt = weight2(s_state[w * WS + 16 * D + gh], mb);
-      lb = fmaf(s_state[w * WS + 16 * D + 16 + gh], wt, lb);
+      const float wt = weight2(s_state[w * WS + heads * D + gh], mb);
+      lb = fmaf(s_state[w * WS + heads * (D + 1) + gh], wt, lb);
       ob = fmaf(s_state[w * WS + gh * D + d], wt, ob);
     }
     const long long h = h0 + gh;
@@ -429,50 +490,99 @@ __global__ __launch_bounds__(64 * NW) void decode_q8_kernel(AttnArgs a, float* _
 }
 
 // out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the splits that the
-// sequence's length reaches, one workgroup of D threads per (sequence, head), in
-// split order.
-template <int D>
-__global__ __launch_bounds__(D) void merge_q8_kernel(const float* __restrict__ part_o,
-                                                     const float* __restrict__ part_ml,
-                                                     const int* __restrict__ lens,
-                                                     _Float16* __restrict__ out, long long n_heads,
-                                                     long long max_len, int split_blocks,
-                                                     int nsplit) {
+// sequence's length reaches: one wave per (sequence, head), in split order. Lane s
+// holds state s's (m, l), every lane its D / 64 dims of all states, C states at a
+// time and their loads issued together, so up to C splits cost one round trip;
+// the weight of state s is read from lane s.
+template <int D, int C>
+__global__ __launch_bounds__(64) void merge_q8_kernel(const float* __restrict__ part_o,
+                                                      const float* __restrict__ part_ml,
+                                                      const int* __restrict__ lens,
+                                                      _Float16* __restrict__ out, long long n_heads,
+                                                      long long max_len, int split_blocks,
+                                                      int nsplit) {
+  static_assert(C <= 64, "a lane per state");
+  constexpr int DPL = D / 64;
+  const int lane = threadIdx.x;
   const long long h = blockIdx.x;
-  const int d = threadIdx.x;
   const int len = static_cast<int>(std::min<long long>(max(lens[h / n_heads], 0), max_len));
   const int blocks = (len + kKvBlock - 1) / kKvBlock;
   const int ns = (blocks + split_blocks - 1) / split_blocks;
   const long long base = h * nsplit;
-  float mx = kNegInf;
-  for (int s = 0; s < ns; ++s) mx = fmaxf(mx, part_ml[2 * (base + s)]);
-  float l = 0.0f, o = 0.0f;
-  for (int s = 0; s < ns; ++s) {
-    const float w = weight2(part_ml[2 * (base + s)], mx);
-    l = fmaf(part_ml[2 * (base + s) + 1], w, l);
-    o = fmaf(part_o[(base + s) * D + d], w, o);
+  float m = kNegInf, l = 0.0f;
+  float o[DPL];
+#pragma unroll
+  for (int j = 0; j < DPL; ++j) o[j] = 0.0f;
+  for (int s0 = 0; s0 < ns; s0 += C) {
+    // states past the last one are read as the last one, with weight 0
+    const long long sl = base + min(s0 + min(lane, C - 1), ns - 1);
+    const float ms = part_ml[2 * sl];
+    const float ls = part_ml[2 * sl + 1];
+    float os[C][DPL];
+#pragma unroll
+    for (int s = 0; s < C; ++s) {
+      const long long slot = base + min(s0 + s, ns - 1);
+#pragma unroll
+      for (int j = 0; j < DPL; ++j) os[s][j] = part_o[slot * D + lane + 64 * j];
+    }
+    const bool live = lane < C && s0 + lane < ns;
+    float mx = live ? ms : kNegInf;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+    const float mn = fmaxf(m, mx);
+    const float was = weight2(m, mn);
+    m = mn;
+    const float w = live ? weight2(ms, mn) : 0.0f;
+    l = l * was + gemv::wave_sum(live ? w * ls : 0.0f);
+#pragma unroll
+    for (int j = 0; j < DPL; ++j) o[j] *= was;
+#pragma unroll
+    for (int s = 0; s < C; ++s) {
+      const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s));
+#pragma unroll
+      for (int j = 0; j < DPL; ++j) o[j] = s0 + s < ns ? fmaf(ws, os[s][j], o[j]) : o[j];
+    }
   }
-  out[h * D + d] = static_cast<_Float16>(ns == 0 ? 0.0f : o / l);
+#pragma unroll
+  for (int j = 0; j < DPL; ++j)
+    out[h * D + lane + 64 * j] = static_cast<_Float16>(ns == 0 ? 0.0f : o[j] / l);
 }
 
-// Splits when the caller passes split_kv = 0: about two workgroups per CU over
-// all (sequence, head) units, at least two blocks per split.
+// Splits when the caller passes split_kv = 0: the largest power of two that keeps
+// one workgroup per CU or fewer over all (sequence, KV head) units (splits of
+// unlike lengths, as a division that does not come out even makes, were 5-25%
+// slower), and at least four blocks per split, one per wave, past 32 blocks. A
+// sweep of 1 to 64 splits over 18 shapes put it at the best count or within 6%:
+// 32 / 32 heads, D = 128, 8192 tokens 8 splits 15.4 us (16: 16.7, 4: 18.1); 32 / 8
+// heads, 131072 tokens 32 splits 46 us (16: 59, 64: 49); 32 sequences of 32 / 8
+// heads, 4096 tokens 1 split 43 us (2: 47.5, 8: 54.6); 1000 tokens, 32 / 8 heads 32
+// splits 6.3 us (8: 7.3).
 int auto_splits(long long blocks, long long units) {
   const long long cus = device_cu_count();
-  const long long wanted = (2 * cus + units - 1) / units;
-  return static_cast<int>(std::max(1ll, std::min({wanted, blocks / 2, 256ll})));
+  const long long most = std::min(256ll, blocks <= 32 ? blocks : blocks / 4);
+  long long s = 1;
+  while (2 * s <= most && 2 * s * units <= cus) s *= 2;
+  return static_cast<int>(s);
 }
+
+// A split's cache bytes stay below 2^31: buffer offsets are 32-bit.
+constexpr long long kMaxSplitBlocks = (1ll << 30) / (128 * kKvBlock);
 
 template <int D, bool PARTIAL>
 void launch_decode(const AttnArgs& a, float* part_o, float* part_ml, dim3 grid, hipStream_t s) {
   auto go = [&](auto kernel, int waves) {
-    kernel<<<grid, 64 * waves, 0, s>>>(a, part_o, part_ml);
+    const std::size_t lds =
+        waves == 1 ? 0 : static_cast<std::size_t>(waves) * std::min(a.group, 16) * (D + 2) * 4;
+    static std::atomic<bool> done[64];
+    allow_staged_lds(reinterpret_cast<const void*>(kernel), done, lds);
+    kernel<<<grid, 64 * waves, lds, s>>>(a, part_o, part_ml);
   };
-  if (a.split_blocks <= 1) go(decode_q8_kernel<D, 1, 1, PARTIAL>, 1);
-  else if (a.split_blocks <= 2) go(decode_q8_kernel<D, 2, 1, PARTIAL>, 2);
-  else if (a.split_blocks <= 4) go(decode_q8_kernel<D, 4, 1, PARTIAL>, 4);
-  else if (a.split_blocks <= 8) go(decode_q8_kernel<D, 8, 1, PARTIAL>, 8);
-  else go(decode_q8_kernel<D, 8, 2, PARTIAL>, 8);
+  constexpr int W = 4;
+  if (a.split_blocks <= 1) go(decode_q8_kernel<D, 1, 1, false, PARTIAL>, 1);
+  else if (a.split_blocks <= 2) go(decode_q8_kernel<D, 2, 1, false, PARTIAL>, 2);
+  else if (a.split_blocks <= W) go(decode_q8_kernel<D, W, 1, false, PARTIAL>, W);
+  else if (a.split_blocks <= 2 * W) go(decode_q8_kernel<D, W, 2, false, PARTIAL>, W);
+  else go(decode_q8_kernel<D, W, 2, true, PARTIAL>, W);
   ENG_LAUNCH_CHECK();
 }
 
@@ -489,8 +599,13 @@ void run_decode(AttnArgs a, long long batch, hipStream_t s) {
   float* part_o = static_cast<float*>(scratch.get());
   float* part_ml = part_o + slots * D;
   launch_decode<D, true>(a, part_o, part_ml, grid, s);
-  merge_q8_kernel<D><<<static_cast<unsigned>(batch * a.n_heads), D, 0, s>>>(
-      part_o, part_ml, a.lens, a.out, a.n_heads, a.max_len, a.split_blocks, a.nsplit);
+  auto merge = [&](auto kernel) {
+    kernel<<<static_cast<unsigned>(batch * a.n_heads), 64, 0, s>>>(
+        part_o, part_ml, a.lens, a.out, a.n_heads, a.max_len, a.split_blocks, a.nsplit);
+  };
+  if (a.nsplit <= 8) merge(merge_q8_kernel<D, 8>);
+  else if (a.nsplit <= 16) merge(merge_q8_kernel<D, 16>);
+  else merge(merge_q8_kernel<D, 32>);
   ENG_LAUNCH_CHECK();
 }
 
@@ -594,7 +709,8 @@ int eng_attention_decode_q8(const eng_half* q, const uint8_t* k_cache, const uin
     const long long want = split_kv == 0
                                ? eng::auto_splits(blocks, batch * n_kv_heads * a.tiles)
                                : std::min<long long>({split_kv, blocks, 256});
-    a.split_blocks = static_cast<int>((blocks + want - 1) / want);
+    a.split_blocks =
+        static_cast<int>(std::min((blocks + want - 1) / want, eng::kMaxSplitBlocks));
     a.nsplit = static_cast<int>((blocks + a.split_blocks - 1) / a.split_blocks);
     if (head_dim == 64) eng::run_decode<64>(a, batch, s);
     else eng::run_decode<128>(a, batch, s);
