@@ -37,6 +37,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
+[[maybe_unused]] constexpr int kRsrcWord3 = 0x00020000;  // buffer descriptor: raw, 32-bit elements
 constexpr int kChunk = 128;  // k of a chunk: one 16-byte weight load per lane
 
 struct Mx4Args {
@@ -443,6 +444,335 @@ void run_rows(const Mx4Args& a, hipStream_t stream) {
   ENG_LAUNCH_CHECK();
 }
 
+// -------------------------------------------------------------- 33 rows and up
+//
+// X split into planes first: 16 rows x 32 k of one term is a fragment, 1 KiB in the
+// order the matrix instruction's lanes take it (lane (i, g): row i, the eight k of
+// step j in its group's 32-block), fragments [M / 16][chunk][step j][term]. A tile's
+// planes are then runs of whole KiB for the direct loads, and a fragment is one
+// conflict-free 16-byte LDS read per lane. Rows past M and k past K are zeros.
+// Beside them the sums of squares of each row over kPlaneK columns at a time.
+constexpr int kPlaneK = 512;  // columns of a workgroup: a chunk per wave
+
+template <bool RMS, bool VEC>
+__global__ __launch_bounds__(256) void mx4_planes_kernel(const float* __restrict__ x,
+                                                         const float* __restrict__ gamma,
+                                                         unsigned short* __restrict__ planes,
+                                                         float* __restrict__ part, long long M,
+                                                         int K, int chunks) {
+  __shared__ float red[4][16];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15;
+  const int g = lane >> 4;
+  const long long row = 16ll * blockIdx.x + i;
+  const int c = blockIdx.y * (kPlaneK / kChunk) + wave;
+  float ss = 0.0f;
+  if (c < chunks) {
+    const float* xr = x + (row < M ? row : 0) * K;
+    auto load4 = [&](const float* p, int k) {
+      floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (VEC) {
+        if (k < K) v = *reinterpret_cast<const floatx4*>(p + k);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = k + e < K ? p[k + e] : 0.0f;
+      }
+      return v;
+    };
+    floatx4 v[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = c * kChunk + 32 * g + 8 * j;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        v[j][h] = load4(xr, k + 4 * h);
+        if (row >= M) v[j][h] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (RMS) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ss = fmaf(v[j][h][e], v[j][h][e], ss);
+          if (gamma != nullptr) {
+            const floatx4 gm = load4(gamma, k + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j][h][e] *= gm[e];
+          }
+        }
+      }
+    }
+    uintx4* dst = reinterpret_cast<uintx4*>(planes) +
+                  ((static_cast<long long>(blockIdx.x) * chunks + c) * 12) * 64 + lane;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float t[8][3];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = v[j][e >> 2][e & 3];
+        split3(f, t[e]);
+      }
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        dst[(3 * j + p) * 64] = uintx4{pack_hi(t[0][p], t[1][p]), pack_hi(t[2][p], t[3][p]),
+                                       pack_hi(t[4][p], t[5][p]), pack_hi(t[6][p], t[7][p])};
+    }
+  }
+  if constexpr (RMS) {
+    ss += __shfl_xor(ss, 16);
+    ss += __shfl_xor(ss, 32);
+    if (g == 0) red[wave][i] = ss;
+    __syncthreads();
+    if (tid < 16 && row < M)
+      part[row * gridDim.y + blockIdx.y] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+  }
+}
+
+// C tiles of 16 BMB x 64 NT on BMB waves: BMB / 4 of them along M, 4 along N, each 64
+// rows x 16 NT columns. A step is one j of a chunk (32 k): its 3 BMB plane fragments
+// sit in one of four LDS stages, loaded three steps ahead by direct loads (three a
+// wave); the weights of a chunk, which only one row of waves uses, come straight
+// into registers a chunk ahead (4-bit: 16 NT bytes a lane and chunk) and are
+// converted as their step begins.
+template <int BMB, int NT, bool RMS>
+__global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
+    const unsigned short* __restrict__ planes, const float* __restrict__ part,
+    const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
+    float* __restrict__ y, long long M, long long N, int K, int nb, int tiles_m, int mblocks,
+    int groups, float eps) {
+  static_assert(BMB == 8 || BMB == 4, "64- or 128-row tiles");
+  constexpr int STAGE = BMB * 3 * 512;  // bf16 of a stage
+  __shared__ __attribute__((aligned(1024))) unsigned short st0[STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned short st1[STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned short st2[STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned short st3[STAGE];
+  __shared__ float row_scale[16 * BMB];
+  auto stage = [&](auto j) -> unsigned short* {
+    if constexpr (decltype(j)::value == 0) return st0;
+    else if constexpr (decltype(j)::value == 1) return st1;
+    else if constexpr (decltype(j)::value == 2) return st2;
+    else return st3;
+  };
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15;
+  const int g = lane >> 4;
+  const int wm = wave >> 2;
+  const int wn = wave & 3;
+  const long long logical = gemv::xcd_contiguous(blockIdx.x, gridDim.x);
+  const int tm = static_cast<int>(logical % tiles_m);
+  const long long n0 = (logical / tiles_m) * (64 * NT);
+  const long long m0 = 16ll * BMB * tm;
+  const int chunks = (K + kChunk - 1) / kChunk;
+
+  if constexpr (RMS) {
+    if (tid < 16 * BMB) {
+      const long long row = std::min(m0 + tid, M - 1);
+      float t = 0.0f;
+      for (int q = 0; q < groups; ++q) t += part[row * groups + q];
+      row_scale[tid] = 1.0f / sqrtf(t / static_cast<float>(K) + eps);
+    }
+  }
+
+  // This wave stages the three planes of m-block `wave` (the last one again past
+  // the matrix): 3 KiB a step, contiguous over all steps.
+  const long long mb_src = std::min<long long>(static_cast<long long>(BMB) * tm + wave, mblocks - 1);
+  [[maybe_unused]] const unsigned short* a_src = planes + mb_src * chunks * (12 * 512);
+  // Weight rows of this wave; rows past N read as zeros.
+  const long long nw = n0 + 16 * NT * wn;  // (uniform)
+  [[maybe_unused]] const long long rows_left = std::max(std::min<long long>(N - nw, 16 * NT), 0ll);
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned short*>(a_src), 0,
+                                                    chunks * 12 * 1024, kRsrcWord3);
+  const auto rc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<unsigned char*>(codes + (rows_left > 0 ? nw : 0) * 16 * nb), 0,
+      static_cast<int>(rows_left * 16 * nb), kRsrcWord3);
+  const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<unsigned char*>(scales + (rows_left > 0 ? nw : 0) * nb), 0,
+      static_cast<int>(rows_left * nb), kRsrcWord3);
+#endif
+  [[maybe_unused]] const int steps = 4 * chunks;
+  auto fetch_a = [&](unsigned short* dst, int step) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int so = min(step, steps - 1) * 3072;
+    unsigned short* d = dst + wave * (3 * 512);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, d, 16, lane * 16, so, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, d + 512, 16, lane * 16, so + 1024, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, d + 1024, 16, lane * 16, so + 2048, 0, 0);
+#endif
+  };
+  struct W {
+    uintx4 w[NT];
+    unsigned s[NT];
+  };
+  auto load_w = [&](W& x, int c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int b = min(4 * min(c, chunks - 1) + g, nb - 1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      x.w[t] = __builtin_amdgcn_raw_buffer_load_b128(rc, ((16 * t + i) * nb + b) * 16, 0, 0);
+      x.s[t] = __builtin_amdgcn_raw_buffer_load_b8(rs, (16 * t + i) * nb + b, 0, 0);
+    }
+#endif
+  };
+
+  floatx4 acc[4][NT];
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[mb][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // Step (c, j): its planes have landed and every wave is past the step before;
+  // the weights of the next chunk (at j == 0), then the planes three steps on go
+  // out, into the stage read last. Younger loads that the wait leaves in flight:
+  // two steps' planes (6), and the next chunk's weights where step 0 was one of
+  // the two. LAST: the chunk after which nothing reads weights; it loads none (the
+  // compiler would drop loads that nothing reads, and the count be too high).
+  auto step = [&](auto jt, int c, const W& w, W& next, auto last) __attribute__((always_inline)) {
+    constexpr int J = decltype(jt)::value;
+    constexpr bool LAST = decltype(last)::value;
+    using Prev = std::integral_constant<int, (J + 3) & 3>;
+    [[maybe_unused]] constexpr int YOUNGER = 6 + (!LAST && (J == 1 || J == 2) ? 2 * NT : 0);
+    __builtin_amdgcn_sched_barrier(0);
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_s_waitcnt(vmcnt_le(YOUNGER) & lgkmcnt_zero());
+#endif
+    barrier_no_fence();
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (J == 0 && !LAST) load_w(next, c + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_a(stage(Prev{}), 4 * c + J + 3);
+    __builtin_amdgcn_sched_barrier(0);
+    const unsigned short* as = stage(jt) + (wm * 4) * (3 * 512) + 8 * lane;
+    bf16x8 b[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) b[t] = weights8(w.w[t][J], scale_of(w.s[t]));
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb) {
+#pragma unroll
+      for (int p = 2; p >= 0; --p) {
+        const bf16x8 a = *reinterpret_cast<const bf16x8*>(as + (mb * 3 + p) * 512);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[mb][t] = mfma(a, b[t], acc[mb][t]);
+      }
+    }
+  };
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I3 = std::integral_constant<int, 3>;
+  W w0, w1;
+  auto chunk = [&](int c, const W& w, W& next, auto last) __attribute__((always_inline)) {
+    step(I0{}, c, w, next, last);
+    step(I1{}, c, w, next, last);
+    step(I2{}, c, w, next, last);
+    step(I3{}, c, w, next, last);
+  };
+  load_w(w0, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  fetch_a(st0, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  fetch_a(st1, 1);
+  __builtin_amdgcn_sched_barrier(0);
+  fetch_a(st2, 2);
+  int c = 0;
+  for (; c + 1 < chunks; c += 2) {
+    chunk(c, w0, w1, std::false_type{});
+    chunk(c + 1, w1, w0, std::false_type{});
+  }
+  if (c < chunks) chunk(c, w0, w1, std::true_type{});
+  // no direct load may be in flight when the workgroup gives its LDS back
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_s_waitcnt(0);
+#endif
+
+  // lane (i, g): element r of acc is row 4 g + r, column i
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int rt = 16 * (4 * wm + mb) + 4 * g + r;
+      const long long row = m0 + rt;
+      const float sc = RMS ? row_scale[rt] : 1.0f;
+      if (row < M) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const long long col = nw + 16 * t + i;
+          if (col < N) y[row * N + col] = acc[mb][t][r] * sc;
+        }
+      }
+    }
+  }
+}
+
+struct Mx4Planes {
+  unsigned short* planes;
+  float* part;
+};
+
+template <int BMB, int NT>
+void run_gemm(const Mx4Args& a, const Mx4Planes& p, hipStream_t stream) {
+  const int K = static_cast<int>(a.K);
+  const int nb = (K + 31) / 32;
+  const int mblocks = static_cast<int>((a.M + 15) / 16);
+  const int tiles_m = (mblocks + BMB - 1) / BMB;
+  const long long tiles = tiles_m * ((a.N + 64 * NT - 1) / (64 * NT));
+  ENG_CHECK(tiles <= 0x7fffffffLL, "linear_mx4w: too many tiles for one launch");
+  const int groups = (K + kPlaneK - 1) / kPlaneK;
+  auto go = [&](auto rms) {
+    mx4_gemm_kernel<BMB, NT, decltype(rms)::value>
+        <<<static_cast<unsigned>(tiles), 64 * BMB, 0, stream>>>(
+            p.planes, p.part, a.codes, a.scales, a.y, a.M, a.N, K, nb, tiles_m, mblocks, groups,
+            a.eps);
+  };
+  if (a.rms) go(std::true_type{});
+  else go(std::false_type{});
+  ENG_LAUNCH_CHECK();
+}
+
+// Buffer offsets are 32-bit: a tile's weight rows (256) and an m-block's planes
+// stay below 2^31 bytes.
+constexpr long long kGemmMaxK = 1ll << 23;
+
+void launch_mx4_gemm(const Mx4Args& a, hipStream_t stream) {
+  const int K = static_cast<int>(a.K);
+  const int chunks = (K + kChunk - 1) / kChunk;
+  const int groups = (K + kPlaneK - 1) / kPlaneK;
+  const long long mblocks = (a.M + 15) / 16;
+  const std::size_t plane_bytes = static_cast<std::size_t>(mblocks) * chunks * 12 * 1024;
+  StreamScratch ws(stream, plane_bytes + static_cast<std::size_t>(a.M) * groups * sizeof(float));
+  Mx4Planes p;
+  p.planes = static_cast<unsigned short*>(ws.get());
+  p.part = reinterpret_cast<float*>(static_cast<char*>(ws.get()) + plane_bytes);
+  const bool vec = a.K % 4 == 0 && aligned_to(a.x, 16) && aligned_to(a.gamma, 16);
+  auto split = [&](auto rms, auto v) {
+    mx4_planes_kernel<decltype(rms)::value, decltype(v)::value>
+        <<<dim3(static_cast<unsigned>(mblocks), static_cast<unsigned>(groups)), 256, 0, stream>>>(
+            a.x, a.gamma, p.planes, p.part, a.M, K, chunks);
+  };
+  using T = std::true_type;
+  using F = std::false_type;
+  if (a.rms) vec ? split(T{}, T{}) : split(T{}, F{});
+  else vec ? split(F{}, T{}) : split(F{}, F{});
+  ENG_LAUNCH_CHECK();
+  if (a.M <= 64) {
+    run_gemm<4, 2>(a, p, stream);
+    return;
+  }
+  // the width whose tiles take the least time in whole rounds of one per CU
+  const long long cus = device_cu_count();
+  long long best = 0;
+  int nt = 0;
+  for (int cand : {4, 3, 2}) {
+    const long long tiles = (mblocks + 7) / 8 * ((a.N + 64 * cand - 1) / (64 * cand));
+    const long long cost = (tiles + cus - 1) / cus * (16 * cand + 6);
+    if (nt == 0 || cost < best) best = cost, nt = cand;
+  }
+  if (nt == 4) run_gemm<8, 4>(a, p, stream);
+  else if (nt == 3) run_gemm<8, 3>(a, p, stream);
+  else run_gemm<8, 2>(a, p, stream);
+}
+
 // Up to 32 rows at a.x, a.y.
 void launch_few(const Mx4Args& a, hipStream_t stream) {
   switch (a.M) {
@@ -456,13 +786,18 @@ void launch_few(const Mx4Args& a, hipStream_t stream) {
   else run_rows<2, 2>(a, stream);
 }
 
+// Rows in passes whose planes take at most 256 MiB of the stream's arena.
 void linear_mx4w(const Mx4Args& a, hipStream_t stream) {
-  for (long long m = 0; m < a.M; m += 32) {
+  const bool gemm = a.M > 32 && a.K <= kGemmMaxK;
+  const long long row_bytes = (a.K + kChunk - 1) / kChunk * kChunk * 6;
+  const long long pass = gemm ? std::max(128ll, (256ll << 20) / row_bytes / 128 * 128) : 32;
+  for (long long m = 0; m < a.M; m += pass) {
     Mx4Args p = a;
-    p.M = std::min(32ll, a.M - m);
+    p.M = std::min(pass, a.M - m);
     p.x = a.x + m * a.K;
     p.y = a.y + m * a.N;
-    launch_few(p, stream);
+    if (gemm && p.M > 32) launch_mx4_gemm(p, stream);
+    else launch_few(p, stream);
   }
 }
 
