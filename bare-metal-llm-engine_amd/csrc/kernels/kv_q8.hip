@@ -571,10 +571,8 @@ constexpr long long kMaxSplitBlocks = (1ll << 30) / (128 * kKvBlock);
 template <int D, bool PARTIAL>
 void launch_decode(const AttnArgs& a, float* part_o, float* part_ml, dim3 grid, hipStream_t s) {
   auto go = [&](auto kernel, int waves) {
-    const std::size_t lds =
+    const std::size_t lds =  // at most 33 KiB
         waves == 1 ? 0 : static_cast<std::size_t>(waves) * std::min(a.group, 16) * (D + 2) * 4;
-    static std::atomic<bool> done[64];
-    allow_staged_lds(reinterpret_cast<const void*>(kernel), done, lds);
     kernel<<<grid, 64 * waves, lds, s>>>(a, part_o, part_ml);
   };
   constexpr int W = 4;

@@ -18,9 +18,8 @@
 //
 //   M <= 4            mx4_decode_kernel: the three terms of row m are rows 4 m ..
 //                     4 m + 2 of one A operand, split once per workgroup into LDS
-//   5 <= M <= 32      mx4_rows_kernel: a workgroup's waves split K, X split in
-//                     registers
-//   M > 32            mx4_gemm_kernel on planes made by mx4_planes_kernel
+//   M <= 64           mx4_slice_kernel: workgroups split K, then a reduce
+//   M > 64            mx4_planes_kernel, then mx4_gemm_kernel: tiles of C
 #include "device_sync.hpp"
 #include "gemv_kernels.hpp"
 #include "launch.hpp"
@@ -92,232 +91,79 @@ __device__ __forceinline__ floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) {
   return c;
 }
 
+// A unit of weights: 256 k of NT tiles of 16 rows, two chunks, so that the pieces of a
+// 128-byte line are asked for together (64-byte pieces asked for one by one made the
+// caches fetch lines twice). Lane (i, g) holds blocks 8 u + g and 8 u + 4 + g of row
+// i; their scale bytes come out of one 8-byte load where rows of scales are whole
+// eights of bytes (SV), else as two bytes. Blocks past the row read its last one.
+constexpr int kUnit = 2 * kChunk;
+
+template <int NT, bool SV>
+struct Unit {
+  uintx4 w[2][NT];
+  uintx2 s[NT];
+  __device__ __forceinline__ void load(int t, const unsigned char* crow, const unsigned char* srow,
+                                       int u, int g, int nb) {
+    const int b0 = min(8 * u + g, nb - 1);
+    const int b1 = min(8 * u + 4 + g, nb - 1);
+    w[0][t] = *reinterpret_cast<const uintx4*>(crow + 16ll * b0);
+    w[1][t] = *reinterpret_cast<const uintx4*>(crow + 16ll * b1);
+    if constexpr (SV) s[t] = *reinterpret_cast<const uintx2*>(srow + 8 * u);
+    else s[t] = uintx2{srow[b0], srow[b1]};
+  }
+  // the scale of half h
+  __device__ __forceinline__ float scale(int t, int h, int g) const {
+    const unsigned v = s[t][h];
+    return scale_of(SV ? (v >> (8 * g)) & 255u : v);
+  }
+};
+
 // ---------------------------------------------------------------- 1 to 4 rows
 //
-// A workgroup of 8 waves owns 16 weight rows; the waves split K by chunks. X is
-// split into LDS once per workgroup (MR rows x 3 terms, a segment of `seg` k at
-// a time); the first four chunks of weights are already on their way while it
-// is. Terms sit 16 bytes apart modulo the banks' 256, so the reads of a step
-// (3 MR rows x 4 groups) spread over the banks.
-constexpr int kDecodeWaves = 8;
-constexpr int kDecodeRing = 4;  // chunks of weights in flight per wave
+// One workgroup of 16 waves per CU. X is split into LDS once (MR rows x 3 terms x K);
+// then the workgroup goes through its tiles of 16 weight rows, p, p + G, ..., the
+// waves splitting K by units. A wave's weights come P units ahead, across the
+// tiles, so the stream does not stop where a tile ends: there the waves leave their
+// sums in LDS (two buffers in turn, one barrier a tile that waits for no load) and
+// one wave, another for each tile, adds and writes them. Rows 4 m + p of the A
+// operand are term p of row m; rows that are no term's read some other term (no
+// output comes from them). Terms sit 16 bytes apart modulo the banks' 256, so the
+// reads of a step (3 MR rows x 4 groups) spread over the banks.
+constexpr int kDecodeWaves = 16;
 constexpr int kDecodeLds = 120 * 1024;
 
-template <int MR, bool RMS, bool VEC>
+constexpr int decode_pitch(int K) { return (K + kUnit - 1) / kUnit * kUnit + 8; }
+// Whether M rows of X fit the decode kernel's LDS.
+bool decode_applies(long long M, long long K) {
+  return M <= 4 && K <= kDecodeLds && 6 * M * decode_pitch(static_cast<int>(K)) <= kDecodeLds;
+}
+
+template <int MR, bool RMS, bool VEC, bool SV>
 __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
     const float* __restrict__ x, const float* __restrict__ gamma,
     const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-    float* __restrict__ y, long long N, int K, int nb, int seg, float eps) {
+    float* __restrict__ y, long long N, int K, int nb, float eps) {
   constexpr int THREADS = 64 * kDecodeWaves;
-  extern __shared__ __attribute__((aligned(16))) unsigned short planes[];  // [MR][3][seg + 8]
-  __shared__ float red[kDecodeWaves][MR][16];
+  constexpr int PX = MR == 1 ? 3 : MR == 2 ? 2 : 1;  // X loads ahead of the weights'
+  constexpr int P = 2;                               // units of weights in flight
+  extern __shared__ __attribute__((aligned(16))) unsigned short planes[];  // [MR][3][pitch]
+  __shared__ float red[2][kDecodeWaves][MR][16];
   __shared__ float red_ss[kDecodeWaves][MR];
-  const int pitch = seg + 8;
+  const int pitch = decode_pitch(K);
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15;
   const int g = lane >> 4;
-  const long long n0 = 16ll * blockIdx.x;
-  const long long n = std::min(n0 + i, N - 1);
-  const unsigned char* crow = codes + n * (16ll * nb);
-  const unsigned char* srow = scales + n * nb;
-  // A row 4 m + p: term p of x row m; p == 3 and m >= MR are zero
-  const int am = i >> 2;
-  const int ap = i & 3;
-  const bool a_on = am < MR && ap < 3;
-  const unsigned short* abase = planes + (a_on ? (am * 3 + ap) * pitch : 0) + 32 * g;
+  const int units = (K + kUnit - 1) / kUnit;
+  const int staged = units * kUnit;  // whole units: zeros past K
+  const int u0 = units * wave / kDecodeWaves;
+  const int u1 = units * (wave + 1) / kDecodeWaves;
+  const long long tiles = (N + 15) / 16;
+  const int mine = static_cast<int>((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
 
-  floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  float ss[MR];
-#pragma unroll
-  for (int m = 0; m < MR; ++m) ss[m] = 0.0f;
-
-  for (int k0 = 0; k0 < K; k0 += seg) {
-    const int klen = min(seg, K - k0);
-    const int chunks = (klen + kChunk - 1) / kChunk;
-    const int c0 = chunks * wave / kDecodeWaves;
-    const int c1 = chunks * (wave + 1) / kDecodeWaves;
-    const int b0 = k0 / 32 + g;
-    uintx4 w[kDecodeRing];
-    unsigned s[kDecodeRing];
-    auto load = [&](int r, int c) {
-      const int b = min(b0 + 4 * min(c, chunks - 1), nb - 1);
-      w[r] = __builtin_nontemporal_load(reinterpret_cast<const uintx4*>(crow + 16ll * b));
-      s[r] = srow[b];
-    };
-#pragma unroll
-    for (int r = 0; r < kDecodeRing; ++r) load(r, c0 + r);
-
-    if (k0 > 0) __syncthreads();  // the last segment's planes have been read
-    // whole chunks are staged: zeros past K
-    for (int q = 4 * tid; q < chunks * kChunk; q += 4 * THREADS) {
-      const int k = k0 + q;
-      float gm[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-      if constexpr (RMS) {
-        if (gamma != nullptr) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) gm[e] = gamma[min(k + e, K - 1)];
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < MR; ++m) {
-        float v[4];
-        const float* xp = x + static_cast<long long>(m) * K + k;
-        if constexpr (VEC) {
-          floatx4 t = {0.0f, 0.0f, 0.0f, 0.0f};
-          if (k < K) t = *reinterpret_cast<const floatx4*>(xp);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = t[e];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = k + e < K ? xp[e] : 0.0f;
-        }
-        float t[4][3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (RMS) {
-            ss[m] = fmaf(v[e], v[e], ss[m]);
-            v[e] = k + e < K ? v[e] * gm[e] : 0.0f;
-          }
-          split3(v[e], t[e]);
-        }
-#pragma unroll
-        for (int p = 0; p < 3; ++p)
-          *reinterpret_cast<uintx2*>(planes + (m * 3 + p) * pitch + q) =
-              uintx2{pack_hi(t[0][p], t[1][p]), pack_hi(t[2][p], t[3][p])};
-      }
-    }
-    __syncthreads();
-
-    for (int c = c0; c < c1; c += kDecodeRing) {
-#pragma unroll
-      for (int r = 0; r < kDecodeRing; ++r) {
-        if (c + r < c1) {
-          const float sc = scale_of(s[r]);
-          const unsigned short* ap0 = abase + (c + r) * kChunk;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            bf16x8 a = *reinterpret_cast<const bf16x8*>(ap0 + 8 * j);
-            if (!a_on) a = bf16x8{};
-            acc = mfma(a, weights8(w[r][j], sc), acc);
-          }
-          if (c + r + kDecodeRing < c1) load(r, c + r + kDecodeRing);
-        }
-      }
-    }
-  }
-
-  // lane (i, g): element r of acc is A row 4 g + r, weight row i
-  if (g < MR) red[wave][g][i] = (acc[0] + acc[1]) + acc[2];
-  if constexpr (RMS) {
-#pragma unroll
-    for (int m = 0; m < MR; ++m) {
-      const float t = gemv::wave_sum(ss[m]);
-      if (lane == 0) red_ss[wave][m] = t;
-    }
-  }
-  __syncthreads();
-  if (tid < 16 * MR) {
-    const int m = tid >> 4;
-    const int col = tid & 15;
-    float v = red[0][m][col];
-#pragma unroll
-    for (int q = 1; q < kDecodeWaves; ++q) v += red[q][m][col];
-    if constexpr (RMS) {
-      float t = red_ss[0][m];
-#pragma unroll
-      for (int q = 1; q < kDecodeWaves; ++q) t += red_ss[q][m];
-      v *= 1.0f / sqrtf(t / static_cast<float>(K) + eps);
-    }
-    if (n0 + col < N) y[m * N + n0 + col] = v;
-  }
-}
-
-template <int MR>
-void run_decode(const Mx4Args& a, hipStream_t stream) {
-  const long long grid = (a.N + 15) / 16;
-  ENG_CHECK(grid <= 0x7fffffffLL, "linear_mx4w: grid too large for one launch");
-  const int K = static_cast<int>(a.K);
-  const int nb = (K + 31) / 32;
-  const bool vec = a.K % 4 == 0 && aligned_to(a.x, 16);
-  const int cap = (kDecodeLds / (6 * MR) - 8) / kChunk * kChunk;
-  const int seg = std::min((K + kChunk - 1) / kChunk * kChunk, cap);
-  const std::size_t lds = static_cast<std::size_t>(6) * MR * (seg + 8);
-  auto go = [&](auto rms, auto v) {
-    constexpr bool R = decltype(rms)::value;
-    constexpr bool V = decltype(v)::value;
-    static std::atomic<bool> done[64];
-    allow_staged_lds(reinterpret_cast<const void*>(mx4_decode_kernel<MR, R, V>), done, lds);
-    mx4_decode_kernel<MR, R, V><<<static_cast<unsigned>(grid), 64 * kDecodeWaves, lds, stream>>>(
-        a.x, a.gamma, a.codes, a.scales, a.y, a.N, K, nb, seg, a.eps);
-  };
-  using T = std::true_type;
-  using F = std::false_type;
-  if (a.rms) vec ? go(T{}, T{}) : go(T{}, F{});
-  else vec ? go(F{}, T{}) : go(F{}, F{});
-  ENG_LAUNCH_CHECK();
-}
-
-// --------------------------------------------------------------- 5 to 32 rows
-//
-// A workgroup of 8 waves owns 16 NT weight rows and all of K, which the waves
-// split by chunks. Each wave loads its own part of X (as fp32, straight into the
-// operand's lanes) and splits it in registers, MB blocks of 16 rows.
-constexpr int kRowsWaves = 8;
-
-template <int MB, int NT, bool RMS, bool VEC>
-__global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows_kernel(
-    const float* __restrict__ x, const float* __restrict__ gamma,
-    const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-    float* __restrict__ y, int M, long long N, int K, int nb, float eps) {
-  __shared__ float red[kRowsWaves][MB * NT][256];
-  __shared__ float red_ss[kRowsWaves][16 * MB];
-  __shared__ float row_scale[16 * MB];
-
-  const int tid = threadIdx.x;
-  const int lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i = lane & 15;
-  const int g = lane >> 4;
-  const long long n0 = 16ll * NT * blockIdx.x;
-  const unsigned char* crow[NT];
-  const unsigned char* srow[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const long long n = std::min(n0 + 16 * t + i, N - 1);
-    crow[t] = codes + n * (16ll * nb);
-    srow[t] = scales + n * nb;
-  }
-  const float* xrow[MB];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
-    xrow[mb] = x + static_cast<long long>(min(16 * mb + i, M - 1)) * K;
-  const int chunks = (K + kChunk - 1) / kChunk;
-  const int c0 = chunks * wave / kRowsWaves;
-  const int c1 = chunks * (wave + 1) / kRowsWaves;
-
-  floatx4 acc[MB][NT];
-  float ss[MB];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    ss[mb] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[mb][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
-  uintx4 w[2][NT];
-  unsigned s[2][NT];
-  auto load_w = [&](auto r, int c) {
-    constexpr int R = decltype(r)::value;
-    const int b = min(4 * c + g, nb - 1);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      w[R][t] = __builtin_nontemporal_load(reinterpret_cast<const uintx4*>(crow[t] + 16ll * b));
-      s[R][t] = srow[t][b];
-    }
-  };
+  // four values of a row at k, zeros from K on
   auto load4 = [&](const float* p, int k) {
     floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     if constexpr (VEC) {
@@ -328,206 +174,576 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows_kernel(
     }
     return v;
   };
-  auto compute = [&](auto r, int c) {
-    constexpr int R = decltype(r)::value;
-    floatx4 xv[4][MB][2];
-    floatx4 gv[RMS ? 4 : 1][2];
+  struct X {
+    floatx4 v[MR];
+    floatx4 gm;
+  };
+  auto load_x = [&](X& r, int k) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = c * kChunk + 32 * g + 8 * j;
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        xv[j][mb][0] = load4(xrow[mb], k);
-        xv[j][mb][1] = load4(xrow[mb], k + 4);
-      }
-      if constexpr (RMS) {
-        if (gamma != nullptr) {
-          gv[j][0] = load4(gamma, k);
-          gv[j][1] = load4(gamma, k + 4);
-        } else {
-          gv[j][0] = gv[j][1] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bf16x8 b[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) b[t] = weights8(w[R][t][j], scale_of(s[R][t]));
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        float t3[8][3];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float v = xv[j][mb][e >> 2][e & 3];
-          if constexpr (RMS) {
-            ss[mb] = fmaf(v, v, ss[mb]);
-            v *= gv[j][e >> 2][e & 3];
-          }
-          split3(v, t3[e]);
-        }
-#pragma unroll
-        for (int p = 2; p >= 0; --p) {
-          const uintx4 u = {pack_hi(t3[0][p], t3[1][p]), pack_hi(t3[2][p], t3[3][p]),
-                            pack_hi(t3[4][p], t3[5][p]), pack_hi(t3[6][p], t3[7][p])};
-          const bf16x8 av = __builtin_bit_cast(bf16x8, u);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) acc[mb][t] = mfma(av, b[t], acc[mb][t]);
-        }
-      }
+    for (int m = 0; m < MR; ++m) r.v[m] = load4(x + static_cast<long long>(m) * K, k);
+    r.gm = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
+    if constexpr (RMS) {
+      if (gamma != nullptr) r.gm = load4(gamma, k);
     }
   };
-  using I0 = std::integral_constant<int, 0>;
-  using I1 = std::integral_constant<int, 1>;
-  if (c0 < c1) load_w(I0{}, c0);
-  for (int c = c0; c < c1; c += 2) {
-    if (c + 1 < c1) load_w(I1{}, c + 1);
-    compute(I0{}, c);
-    if (c + 1 < c1) {
-      if (c + 2 < c1) load_w(I0{}, c + 2);
-      compute(I1{}, c + 1);
+  float ss[MR];
+#pragma unroll
+  for (int m = 0; m < MR; ++m) ss[m] = 0.0f;
+  auto put_x = [&](const X& r, int q) {
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      float t[4][3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = r.v[m][e];
+        if constexpr (RMS) {
+          ss[m] = fmaf(v, v, ss[m]);
+          v *= r.gm[e];
+        }
+        split3(v, t[e]);
+      }
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        *reinterpret_cast<uintx2*>(planes + (m * 3 + p) * pitch + q) =
+            uintx2{pack_hi(t[0][p], t[1][p]), pack_hi(t[2][p], t[3][p])};
     }
-  }
+  };
+
+  X xr[PX];
+#pragma unroll
+  for (int u = 0; u < PX; ++u)
+    if (4 * (tid + u * THREADS) < staged) load_x(xr[u], 4 * (tid + u * THREADS));
+  __builtin_amdgcn_sched_barrier(0);
+
+  // The next weights to ask for: unit fu of this workgroup's tile ft. Past the last
+  // tile every lane asks for the same first bytes (the waits count loads, so some
+  // have to go out; no one uses them).
+  Unit<1, SV> w[P];
+  int ft = 0, fu = u0;
+  const unsigned char* crow;
+  const unsigned char* srow;
+  auto seek = [&] {
+    const long long t = blockIdx.x + static_cast<long long>(ft) * gridDim.x;
+    const long long n = ft < mine ? std::min(16 * t + i, N - 1) : 0;
+    crow = codes + n * (16ll * nb);
+    srow = scales + n * nb;
+  };
+  auto load_w = [&](int r) {
+    const bool live = ft < mine;
+    w[r].load(0, crow, srow, live ? fu : 0, live ? g : 0, nb);
+    if (++fu >= u1) {
+      fu = u0;
+      ++ft;
+      seek();
+    }
+  };
+  seek();
+#pragma unroll
+  for (int r = 0; r < P; ++r) load_w(r);
+  __builtin_amdgcn_sched_barrier(0);
 
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
+  for (int u = 0; u < PX; ++u)
+    if (4 * (tid + u * THREADS) < staged) put_x(xr[u], 4 * (tid + u * THREADS));
+  for (int q = 4 * (tid + PX * THREADS); q < staged; q += 4 * THREADS) {
+    load_x(xr[0], q);
+    put_x(xr[0], q);
+  }
+  if constexpr (RMS) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) red[wave][mb * NT + t][(4 * g + r) * 16 + i] = acc[mb][t][r];
-    if constexpr (RMS) {
-      float v = ss[mb];
-      v += __shfl_xor(v, 16);
-      v += __shfl_xor(v, 32);
-      if (g == 0) red_ss[wave][16 * mb + i] = v;
+    for (int m = 0; m < MR; ++m) {
+      const float t = gemv::wave_sum(ss[m]);
+      if (lane == 0) red_ss[wave][m] = t;
     }
   }
-  __syncthreads();
-  if (tid < 16 * MB) {
-    float sc = 1.0f;
-    if constexpr (RMS) {
-      float t = red_ss[0][tid];
+  lds_barrier();
+  [[maybe_unused]] float row_scale = 1.0f;  // of row lane / 16
+  if constexpr (RMS) {
+    float t = 0.0f;
 #pragma unroll
-      for (int q = 1; q < kRowsWaves; ++q) t += red_ss[q][tid];
-      sc = 1.0f / sqrtf(t / static_cast<float>(K) + eps);
-    }
-    row_scale[tid] = sc;
+    for (int q = 0; q < kDecodeWaves; ++q) t += red_ss[q][min(g, MR - 1)];
+    row_scale = 1.0f / sqrtf(t / static_cast<float>(K) + eps);
   }
-  __syncthreads();
-  for (int q = tid; q < MB * NT * 256; q += 64 * kRowsWaves) {
-    const int blk = q >> 8;
-    const int row = 16 * (blk / NT) + ((q & 255) >> 4);
-    const long long col = n0 + 16 * (blk % NT) + (q & 15);
-    float v = red[0][blk][q & 255];
+
+  const unsigned short* abase =
+      planes + (min(i >> 2, MR - 1) * 3 + min(i & 3, 2)) * pitch + 32 * g;
+  floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  int tile = 0;
+  // lane (i, g): element r of acc is A row 4 g + r, weight row i
+  auto finish = [&] {
+    float (*rb)[MR][16] = red[tile & 1];
+    if (g < MR) rb[wave][g][i] = (acc[0] + acc[1]) + acc[2];
+    acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    lds_barrier();
+    if (wave == (tile & (kDecodeWaves - 1)) && g < MR) {
+      float v = rb[0][g][i];
 #pragma unroll
-    for (int u = 1; u < kRowsWaves; ++u) v += red[u][blk][q & 255];
-    if (row < M && col < N) y[row * N + col] = v * row_scale[row];
+      for (int q = 1; q < kDecodeWaves; ++q) v += rb[q][g][i];
+      const long long n = 16 * (blockIdx.x + static_cast<long long>(tile) * gridDim.x) + i;
+      if (n < N) y[g * N + n] = v * row_scale;
+    }
+    ++tile;
+  };
+  if (u0 == u1) {  // fewer units than waves: this one only joins the barriers
+    while (tile < mine) finish();
+    return;
+  }
+  int u = u0;
+  while (true) {
+#pragma unroll
+    for (int r = 0; r < P; ++r) {
+      const unsigned short* ap = abase + u * kUnit;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float sc = w[r].scale(0, h, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc = mfma(*reinterpret_cast<const bf16x8*>(ap + h * kChunk + 8 * j),
+                     weights8(w[r].w[h][0][j], sc), acc);
+      }
+      if (++u == u1) {
+        u = u0;
+        finish();
+        if (tile == mine) return;
+      }
+      load_w(r);
+    }
   }
 }
 
-template <int MB, int NT>
-void run_rows(const Mx4Args& a, hipStream_t stream) {
-  const long long grid = (a.N + 16 * NT - 1) / (16 * NT);
-  ENG_CHECK(grid <= 0x7fffffffLL, "linear_mx4w: grid too large for one launch");
+// Whether every row's scale bytes are whole aligned eights (Unit's SV).
+bool scales_by_8(const Mx4Args& a) {
+  return (a.K + 31) / 32 % 8 == 0 && aligned_to(a.scales, 8);
+}
+
+template <int MR>
+void run_decode(const Mx4Args& a, hipStream_t stream) {
   const int K = static_cast<int>(a.K);
   const int nb = (K + 31) / 32;
   const bool vec = a.K % 4 == 0 && aligned_to(a.x, 16) && aligned_to(a.gamma, 16);
-  auto go = [&](auto rms, auto v) {
-    mx4_rows_kernel<MB, NT, decltype(rms)::value, decltype(v)::value>
-        <<<static_cast<unsigned>(grid), 64 * kRowsWaves, 0, stream>>>(
-            a.x, a.gamma, a.codes, a.scales, a.y, static_cast<int>(a.M), a.N, K, nb, a.eps);
+  const std::size_t lds = static_cast<std::size_t>(6) * MR * decode_pitch(K);
+  const unsigned grid =
+      static_cast<unsigned>(std::min<long long>((a.N + 15) / 16, device_cu_count()));
+  auto go = [&](auto rms, auto v, auto sv) {
+    constexpr bool R = decltype(rms)::value;
+    constexpr bool V = decltype(v)::value;
+    constexpr bool SV = decltype(sv)::value;
+    static std::atomic<bool> done[64];
+    allow_staged_lds(reinterpret_cast<const void*>(mx4_decode_kernel<MR, R, V, SV>), done, lds);
+    mx4_decode_kernel<MR, R, V, SV><<<grid, 64 * kDecodeWaves, lds, stream>>>(
+        a.x, a.gamma, a.codes, a.scales, a.y, a.N, K, nb, a.eps);
   };
   using T = std::true_type;
   using F = std::false_type;
-  if (a.rms) vec ? go(T{}, T{}) : go(T{}, F{});
-  else vec ? go(F{}, T{}) : go(F{}, F{});
+  auto pick = [&](auto rms) {
+    if (!vec) go(rms, F{}, F{});
+    else if (!scales_by_8(a)) go(rms, T{}, F{});
+    else go(rms, T{}, T{});
+  };
+  if (a.rms) pick(T{});
+  else pick(F{});
   ENG_LAUNCH_CHECK();
 }
 
-// -------------------------------------------------------------- 33 rows and up
+// ------------------------------------------------------------- planes of X
 //
-// X split into planes first: 16 rows x 32 k of one term is a fragment, 1 KiB in the
-// order the matrix instruction's lanes take it (lane (i, g): row i, the eight k of
-// step j in its group's 32-block), fragments [M / 16][chunk][step j][term]. A tile's
-// planes are then runs of whole KiB for the direct loads, and a fragment is one
-// conflict-free 16-byte LDS read per lane. Rows past M and k past K are zeros.
-// Beside them the sums of squares of each row over kPlaneK columns at a time.
-constexpr int kPlaneK = 512;  // columns of a workgroup: a chunk per wave
-
+// For the GEMM X is split into planes first: 16 rows x 32 k of one term is a fragment,
+// 1 KiB in the order the matrix instruction's lanes take it (lane (i, g): row i, the
+// eight k of step j in its group's 32-block), fragments [M / 16][chunk][step j][term].
+// A wave's load of a fragment is then 1 KiB in one piece, and one of X as it stands 64
+// pieces of 16 bytes. Rows past M and k past K are zeros. Beside them the sums of
+// squares of each row's chunks.
 template <bool RMS, bool VEC>
 __global__ __launch_bounds__(256) void mx4_planes_kernel(const float* __restrict__ x,
                                                          const float* __restrict__ gamma,
                                                          unsigned short* __restrict__ planes,
                                                          float* __restrict__ part, long long M,
                                                          int K, int chunks) {
-  __shared__ float red[4][16];
+  // thread (row i of 16, eighth of 16 of the chunk): 8 values, one lane's of a step
+  const int i = threadIdx.x >> 4;
+  const int e8 = threadIdx.x & 15;
+  const int c = blockIdx.x;
+  const long long mb = blockIdx.y;
+  const long long row = 16 * mb + i;
+  const int k = c * kChunk + 8 * e8;
+  float v[8];
+  float ss = 0.0f;
+  const float* xr = x + (row < M ? row : 0) * K;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    floatx4 f = {0.0f, 0.0f, 0.0f, 0.0f};
+    floatx4 gm = {1.0f, 1.0f, 1.0f, 1.0f};
+    const int kh = k + 4 * h;
+    if constexpr (VEC) {
+      if (row < M && kh < K) {
+        f = *reinterpret_cast<const floatx4*>(xr + kh);
+        if (RMS && gamma != nullptr) gm = *reinterpret_cast<const floatx4*>(gamma + kh);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (row < M && kh + e < K) {
+          f[e] = xr[kh + e];
+          if (RMS && gamma != nullptr) gm[e] = gamma[kh + e];
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[4 * h + e] = f[e];
+      if constexpr (RMS) {
+        ss = fmaf(f[e], f[e], ss);
+        v[4 * h + e] = f[e] * gm[e];
+      }
+    }
+  }
+  float t[8][3];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) split3(v[e], t[e]);
+  uintx4* dst = reinterpret_cast<uintx4*>(planes) + ((mb * chunks + c) * 12 + 3 * (e8 & 3)) * 64 +
+                (i + 16 * (e8 >> 2));
+#pragma unroll
+  for (int p = 0; p < 3; ++p)
+    dst[p * 64] = uintx4{pack_hi(t[0][p], t[1][p]), pack_hi(t[2][p], t[3][p]),
+                         pack_hi(t[4][p], t[5][p]), pack_hi(t[6][p], t[7][p])};
+  if constexpr (RMS) {
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) ss += __shfl_xor(ss, off);
+    if (e8 == 0 && row < M) part[row * chunks + c] = ss;
+  }
+}
+
+struct Mx4Planes {
+  unsigned short* planes;
+  float* part;
+};
+
+std::size_t plane_bytes(long long M, long long K) {
+  return static_cast<std::size_t>((M + 15) / 16) * ((K + kChunk - 1) / kChunk) * 12 * 1024;
+}
+std::size_t planes_scratch(const Mx4Args& a) {
+  return plane_bytes(a.M, a.K) +
+         static_cast<std::size_t>(a.M) * ((a.K + kChunk - 1) / kChunk) * sizeof(float);
+}
+
+Mx4Planes launch_planes(const Mx4Args& a, void* scratch, hipStream_t stream) {
+  Mx4Planes p;
+  p.planes = static_cast<unsigned short*>(scratch);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(scratch) + plane_bytes(a.M, a.K));
+  const int K = static_cast<int>(a.K);
+  const int chunks = (K + kChunk - 1) / kChunk;
+  const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>((a.M + 15) / 16));
+  const bool vec = a.K % 4 == 0 && aligned_to(a.x, 16) && aligned_to(a.gamma, 16);
+  auto go = [&](auto rms, auto v) {
+    mx4_planes_kernel<decltype(rms)::value, decltype(v)::value><<<grid, 256, 0, stream>>>(
+        a.x, a.gamma, p.planes, p.part, a.M, K, chunks);
+  };
+  using T = std::true_type;
+  using F = std::false_type;
+  if (a.rms) vec ? go(T{}, T{}) : go(T{}, F{});
+  else vec ? go(F{}, T{}) : go(F{}, F{});
+  ENG_LAUNCH_CHECK();
+  return p;
+}
+
+// s_m of rows m0 .. m0 + ROWS - 1 (row M - 1's past the matrix) into LDS, by all
+// THREADS of the workgroup: THREADS / ROWS of them share a row's partial sums.
+template <int ROWS, int THREADS>
+__device__ __forceinline__ void row_scales(const float* __restrict__ part, long long m0, long long M,
+                                           int K, int chunks, float eps, float* row_scale) {
+  constexpr int S = THREADS / ROWS;
+  static_assert(S >= 1 && S <= 64 && (S & (S - 1)) == 0, "a power of two of neighbouring lanes");
+  const int r = threadIdx.x / S;
+  const float* p = part + std::min(m0 + r, M - 1) * chunks;
+  float t = 0.0f;
+#pragma unroll 4
+  for (int q = threadIdx.x % S; q < chunks; q += S) t += p[q];
+#pragma unroll
+  for (int off = 1; off < S; off <<= 1) t += __shfl_xor(t, off);
+  if (threadIdx.x % S == 0) row_scale[r] = 1.0f / sqrtf(t / static_cast<float>(K) + eps);
+}
+
+// --------------------------------------------------------------- 5 to 64 rows
+//
+// A workgroup of 8 waves owns 128 NT weight rows (16 NT a wave) and a slice of K, at
+// most KU units of it: it splits its slice of X into LDS once, as the fragments of
+// the matrix instruction (16 rows x 32 k of one term, 1 KiB in the order the lanes
+// take it), and every wave multiplies them by its own weights, all of which are on
+// their way before X is split. The slices' sums go to scratch and
+// mx4_slice_reduce_kernel adds them in slice order and applies the rows' scales (from
+// the sums of squares that the first column of workgroups leaves).
+// Slices, because X outweighs the weights otherwise: 16 rows are 96 bytes per k
+// in three terms against 8 of a 16-row tile of weights, and with all of K in every
+// workgroup their way from L2 set the time (16 x 11008 x 4096: 114 MB, 15 us).
+constexpr int kSliceWaves = 8;
+
+template <int MB>
+constexpr int slice_units() { return MB == 1 ? 2 : 1; }  // 48 KiB of fragments, 96 at 64 rows
+
+__device__ __forceinline__ int frag_slot(int i, int g) { return 16 * g + ((i + 4 * g) & 15); }
+
+template <int MB, int NT, bool RMS, bool VEC, bool SV>
+__global__ __launch_bounds__(64 * kSliceWaves, MB == 4 ? 2 : 4) void mx4_slice_kernel(
+    const float* __restrict__ x, const float* __restrict__ gamma,
+    const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
+    float* __restrict__ sums, float* __restrict__ squares, int M, long long N, int K, int nb) {
+  constexpr int KU = slice_units<MB>();
+  constexpr int PX = MB * KU;  // pieces of 8 values a thread splits
+  __shared__ __attribute__((aligned(1024))) unsigned short frag[MB * KU * 24 * 512];
+
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15;
   const int g = lane >> 4;
-  const long long row = 16ll * blockIdx.x + i;
-  const int c = blockIdx.y * (kPlaneK / kChunk) + wave;
-  float ss = 0.0f;
-  if (c < chunks) {
-    const float* xr = x + (row < M ? row : 0) * K;
-    auto load4 = [&](const float* p, int k) {
-      floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-      if constexpr (VEC) {
-        if (k < K) v = *reinterpret_cast<const floatx4*>(p + k);
-      } else {
+  const int units = (K + kUnit - 1) / kUnit;
+  const int slices = gridDim.y;
+  const int slice = blockIdx.y;
+  const int u0 = static_cast<int>(static_cast<long long>(units) * slice / slices);
+  const int n_units = static_cast<int>(static_cast<long long>(units) * (slice + 1) / slices) - u0;
+
+  // X: piece q of a thread is row 16 mb + r, values 8 e .. + 7 of chunk c of the
+  // slice, (mb, c) = (q / KU, 2 (q % KU) + tid / 256).
+  const int r = (tid >> 4) & 15;
+  const int e8 = tid & 15;
+  floatx4 xv[PX][2], gv[RMS ? PX : 1][2];
+  auto load4 = [&](const float* p, int k, float fill) {
+    floatx4 v = {fill, fill, fill, fill};
+    if constexpr (VEC) {
+      if (k < K) v = *reinterpret_cast<const floatx4*>(p + k);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = k + e < K ? p[k + e] : 0.0f;
+      for (int e = 0; e < 4; ++e)
+        if (k + e < K) v[e] = p[k + e];
+    }
+    return v;
+  };
+#pragma unroll
+  for (int q = 0; q < PX; ++q) {
+    const int row = 16 * (q / KU) + r;
+    const int k = u0 * kUnit + (2 * (q % KU) + (tid >> 8)) * kChunk + 8 * e8;
+    const float* xr = x + static_cast<long long>(min(row, M - 1)) * K;
+    // rows past M count as past K
+    const int kk = row < M ? k : K;
+    if (q % KU >= n_units) continue;  // (uniform)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      xv[q][h] = load4(xr, kk + 4 * h, 0.0f);
+      if constexpr (RMS) {
+        gv[q][h] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
+        if (gamma != nullptr) gv[q][h] = load4(gamma, kk + 4 * h, 0.0f);
       }
-      return v;
-    };
-    floatx4 v[4][2];
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  const long long n0 = (static_cast<long long>(blockIdx.x) * kSliceWaves + wave) * (16 * NT);
+  Unit<NT, SV> w[KU];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = c * kChunk + 32 * g + 8 * j;
+  for (int t = 0; t < NT; ++t) {
+    const long long n = std::min(n0 + 16 * t + i, N - 1);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        v[j][h] = load4(xr, k + 4 * h);
-        if (row >= M) v[j][h] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        if constexpr (RMS) {
+    for (int q = 0; q < KU; ++q)
+      if (q < n_units) w[q].load(t, codes + n * (16ll * nb), scales + n * nb, u0 + q, g, nb);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+
+  float ss[MB];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) ss = fmaf(v[j][h][e], v[j][h][e], ss);
-          if (gamma != nullptr) {
-            const floatx4 gm = load4(gamma, k + 4 * h);
+  for (int mb = 0; mb < MB; ++mb) ss[mb] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[j][h][e] *= gm[e];
+  for (int q = 0; q < PX; ++q) {
+    if (q % KU >= n_units) continue;  // (uniform)
+    float t[8][3];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float v = xv[q][e >> 2][e & 3];
+      if constexpr (RMS) {
+        ss[q / KU] = fmaf(v, v, ss[q / KU]);
+        v *= gv[q][e >> 2][e & 3];
+      }
+      split3(v, t[e]);
+    }
+    const int c = 2 * (q % KU) + (tid >> 8);
+    // fragments [chunk][step][m-block][term]; this thread's is lane (r, group e8 / 4)
+    // of step e8 % 4. Lane (i, g)'s 16 bytes sit at 16 g + (i + 4 g) % 16, so that
+    // these stores (4 rows of every group and step) and the reads (whole fragments)
+    // both spread over the banks.
+    uintx4* dst = reinterpret_cast<uintx4*>(frag) +
+                  (((c * 4 + (e8 & 3)) * MB + q / KU) * 3) * 64 + frag_slot(r, e8 >> 2);
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      dst[p * 64] = uintx4{pack_hi(t[0][p], t[1][p]), pack_hi(t[2][p], t[3][p]),
+                           pack_hi(t[4][p], t[5][p]), pack_hi(t[6][p], t[7][p])};
+  }
+  lds_barrier();
+
+  floatx4 acc[MB][NT];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[mb][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int q = 0; q < KU; ++q) {
+    if (q >= n_units) break;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned short* f = frag + ((8 * q + 4 * h + j) * MB * 3) * 512 + 8 * frag_slot(i, g);
+        bf16x8 b[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) b[t] = weights8(w[q].w[h][t][j], w[q].scale(t, h, g));
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+          for (int p = 2; p >= 0; --p) {
+            const bf16x8 av = *reinterpret_cast<const bf16x8*>(f + (mb * 3 + p) * 512);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[mb][t] = mfma(av, b[t], acc[mb][t]);
           }
         }
       }
     }
-    uintx4* dst = reinterpret_cast<uintx4*>(planes) +
-                  ((static_cast<long long>(blockIdx.x) * chunks + c) * 12) * 64 + lane;
+  }
+
+  // lane (i, g): element v of acc is row 4 g + v, column i
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float t[8][3];
+  for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = v[j][e >> 2][e & 3];
-        split3(f, t[e]);
+    for (int v = 0; v < 4; ++v) {
+      const int row = 16 * mb + 4 * g + v;
+      if (row < M) {
+        float* dst = sums + (static_cast<long long>(slice) * M + row) * N;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const long long n = n0 + 16 * t + i;
+          if (n < N) dst[n] = acc[mb][t][v];
+        }
       }
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        dst[(3 * j + p) * 64] = uintx4{pack_hi(t[0][p], t[1][p]), pack_hi(t[2][p], t[3][p]),
-                                       pack_hi(t[4][p], t[5][p]), pack_hi(t[6][p], t[7][p])};
     }
   }
   if constexpr (RMS) {
-    ss += __shfl_xor(ss, 16);
-    ss += __shfl_xor(ss, 32);
-    if (g == 0) red[wave][i] = ss;
-    __syncthreads();
-    if (tid < 16 && row < M)
-      part[row * gridDim.y + blockIdx.y] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+    if (blockIdx.x == 0) {  // (uniform)
+      __syncthreads();      // the fragments have been read
+      float* red = reinterpret_cast<float*>(frag);  // [2][16 MB]: the two halves of the threads
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) ss[mb] += __shfl_xor(ss[mb], off);
+        if (e8 == 0) red[(tid >> 8) * 16 * MB + 16 * mb + r] = ss[mb];
+      }
+      __syncthreads();
+      if (tid < 16 * MB && tid < M)
+        squares[static_cast<long long>(tid) * slices + slice] = red[tid] + red[16 * MB + tid];
+    }
   }
 }
 
-// C tiles of 16 BMB x 64 NT on BMB waves: BMB / 4 of them along M, 4 along N, each 64
-// rows x 16 NT columns. A step is one j of a chunk (32 k): its 3 BMB plane fragments
+// y[m][n] = s_m times the sum over the slices, in their order. blockIdx.y: a row, whose
+// sum of squares is in `parts` parts.
+template <bool RMS, bool VEC>
+__global__ __launch_bounds__(256) void mx4_slice_reduce_kernel(const float* __restrict__ sums,
+                                                               const float* __restrict__ squares,
+                                                               float* __restrict__ y, long long M,
+                                                               long long N, int K, int slices,
+                                                               int parts, float eps) {
+  const long long row = blockIdx.y;
+  const long long stride = M * N;
+  float sc = 1.0f;
+  if constexpr (RMS) {
+    float t = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) t += squares[row * parts + s];
+    sc = 1.0f / sqrtf(t / static_cast<float>(K) + eps);
+  }
+  if constexpr (VEC) {
+    const long long n = 4 * (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x);
+    if (n >= N) return;
+    const float* p = sums + row * N + n;
+    floatx4 v = *reinterpret_cast<const floatx4*>(p);
+#pragma unroll 4
+    for (int s = 1; s < slices; ++s) {
+      const floatx4 a = *reinterpret_cast<const floatx4*>(p + s * stride);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += a[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[row * N + n + e] = v[e] * sc;
+  } else {
+    const long long n = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    if (n >= N) return;
+    const float* p = sums + row * N + n;
+    float v = *p;
+#pragma unroll 4
+    for (int s = 1; s < slices; ++s) v += p[s * stride];
+    y[row * N + n] = v * sc;
+  }
+}
+
+void launch_reduce(const Mx4Args& a, const float* sums, const float* squares, int slices, int parts,
+                   hipStream_t stream) {
+  const bool wide = a.N % 4 == 0;
+  const long long per = wide ? 1024 : 256;
+  ENG_CHECK(a.M <= 65535, "linear_mx4w: too many rows in a pass");
+  const dim3 grid(static_cast<unsigned>((a.N + per - 1) / per), static_cast<unsigned>(a.M));
+  auto go = [&](auto rms, auto v) {
+    mx4_slice_reduce_kernel<decltype(rms)::value, decltype(v)::value><<<grid, 256, 0, stream>>>(
+        sums, squares, a.y, a.M, a.N, static_cast<int>(a.K), slices, parts, a.eps);
+  };
+  using T = std::true_type;
+  using F = std::false_type;
+  if (a.rms) wide ? go(T{}, T{}) : go(T{}, F{});
+  else wide ? go(F{}, T{}) : go(F{}, F{});
+  ENG_LAUNCH_CHECK();
+}
+
+// Slices of K: enough that a slice's units fit the kernel, and more while the
+// workgroups do not fill the CUs.
+template <int MB>
+int slice_count(long long N, long long K, int nt) {
+  const long long units = (K + kUnit - 1) / kUnit;
+  const long long groups = (N + 128 * nt - 1) / (128 * nt);
+  const long long fit = (units + slice_units<MB>() - 1) / slice_units<MB>();
+  const long long fill = std::max(1ll, device_cu_count() / groups);
+  return static_cast<int>(std::min(units, std::max(fit, fill)));
+}
+
+template <int MB, int NT>
+void run_slices(const Mx4Args& a, hipStream_t stream) {
+  const int K = static_cast<int>(a.K);
+  const int M = static_cast<int>(a.M);
+  const int nb = (K + 31) / 32;
+  const int slices = slice_count<MB>(a.N, a.K, NT);
+  const long long groups = (a.N + 128 * NT - 1) / (128 * NT);
+  ENG_CHECK(groups <= 0x7fffffffLL && slices <= 65535, "linear_mx4w: grid too large for one launch");
+  const std::size_t sum_bytes = (static_cast<std::size_t>(slices) * M * a.N + 3) / 4 * 16;
+  StreamScratch ws(stream, sum_bytes + static_cast<std::size_t>(M) * slices * sizeof(float));
+  float* sums = static_cast<float*>(ws.get());
+  float* squares = reinterpret_cast<float*>(static_cast<char*>(ws.get()) + sum_bytes);
+  const bool vec = a.K % 4 == 0 && aligned_to(a.x, 16) && aligned_to(a.gamma, 16);
+  const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(slices));
+  using T = std::true_type;
+  using F = std::false_type;
+  auto go = [&](auto rms, auto v, auto sv) {
+    mx4_slice_kernel<MB, NT, decltype(rms)::value, decltype(v)::value, decltype(sv)::value>
+        <<<grid, 64 * kSliceWaves, 0, stream>>>(a.x, a.gamma, a.codes, a.scales, sums, squares, M, a.N,
+                                                K, nb);
+  };
+  auto pick = [&](auto rms) {
+    if (!vec) go(rms, F{}, F{});
+    else if (!scales_by_8(a)) go(rms, T{}, F{});
+    else go(rms, T{}, T{});
+  };
+  if (a.rms) pick(T{});
+  else pick(F{});
+  ENG_LAUNCH_CHECK();
+  launch_reduce(a, sums, squares, slices, slices, stream);
+}
+
+// -------------------------------------------------------------- 65 rows and up
+//
+// C tiles of 128 x 64 NT on 8 waves: 2 of them along M, 4 along N, each 64 rows x 16
+// NT columns. A step is one j of a chunk (32 k): its 3 BMB plane fragments
 // sit in one of four LDS stages, loaded three steps ahead by direct loads (three a
 // wave); the weights of a chunk, which only one row of waves uses, come straight
 // into registers a chunk ahead (4-bit: 16 NT bytes a lane and chunk) and are
@@ -536,9 +752,9 @@ template <int BMB, int NT, bool RMS>
 __global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
     const unsigned short* __restrict__ planes, const float* __restrict__ part,
     const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-    float* __restrict__ y, long long M, long long N, int K, int nb, int tiles_m, int mblocks,
-    int groups, float eps) {
-  static_assert(BMB == 8 || BMB == 4, "64- or 128-row tiles");
+    float* __restrict__ y, float* __restrict__ sums, long long M, long long N, int K, int nb,
+    int tiles_m, int mblocks, float eps) {
+  static_assert(BMB == 8, "128-row tiles on 8 waves");
   constexpr int STAGE = BMB * 3 * 512;  // bf16 of a stage
   __shared__ __attribute__((aligned(1024))) unsigned short st0[STAGE];
   __shared__ __attribute__((aligned(1024))) unsigned short st1[STAGE];
@@ -565,14 +781,12 @@ __global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
   const long long m0 = 16ll * BMB * tm;
   const int chunks = (K + kChunk - 1) / kChunk;
 
-  if constexpr (RMS) {
-    if (tid < 16 * BMB) {
-      const long long row = std::min(m0 + tid, M - 1);
-      float t = 0.0f;
-      for (int q = 0; q < groups; ++q) t += part[row * groups + q];
-      row_scale[tid] = 1.0f / sqrtf(t / static_cast<float>(K) + eps);
-    }
-  }
+  // This slice's chunks. One slice writes scaled rows of y, several their sums.
+  const int slices = gridDim.y;
+  const int cb = static_cast<int>(static_cast<long long>(chunks) * blockIdx.y / slices);
+  const int ce = static_cast<int>(static_cast<long long>(chunks) * (blockIdx.y + 1) / slices);
+  const bool scaled = RMS && slices == 1;  // (uniform)
+  if (scaled) row_scales<16 * BMB, 64 * BMB>(part, m0, M, K, chunks, eps, row_scale);
 
   // This wave stages the three planes of m-block `wave` (the last one again past
   // the matrix): 3 KiB a step, contiguous over all steps.
@@ -591,7 +805,7 @@ __global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
       const_cast<unsigned char*>(scales + (rows_left > 0 ? nw : 0) * nb), 0,
       static_cast<int>(rows_left * nb), kRsrcWord3);
 #endif
-  [[maybe_unused]] const int steps = 4 * chunks;
+  [[maybe_unused]] const int steps = 4 * ce;
   auto fetch_a = [&](unsigned short* dst, int step) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const int so = min(step, steps - 1) * 3072;
@@ -607,7 +821,7 @@ __global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
   };
   auto load_w = [&](W& x, int c) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int b = min(4 * min(c, chunks - 1) + g, nb - 1);
+    const int b = min(4 * min(c, ce - 1) + g, nb - 1);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       x.w[t] = __builtin_amdgcn_raw_buffer_load_b128(rc, ((16 * t + i) * nb + b) * 16, 0, 0);
@@ -668,19 +882,19 @@ __global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
     step(I2{}, c, w, next, last);
     step(I3{}, c, w, next, last);
   };
-  load_w(w0, 0);
+  load_w(w0, cb);
   __builtin_amdgcn_sched_barrier(0);
-  fetch_a(st0, 0);
+  fetch_a(st0, 4 * cb);
   __builtin_amdgcn_sched_barrier(0);
-  fetch_a(st1, 1);
+  fetch_a(st1, 4 * cb + 1);
   __builtin_amdgcn_sched_barrier(0);
-  fetch_a(st2, 2);
-  int c = 0;
-  for (; c + 1 < chunks; c += 2) {
+  fetch_a(st2, 4 * cb + 2);
+  int c = cb;
+  for (; c + 1 < ce; c += 2) {
     chunk(c, w0, w1, std::false_type{});
     chunk(c + 1, w1, w0, std::false_type{});
   }
-  if (c < chunks) chunk(c, w0, w1, std::true_type{});
+  if (c < ce) chunk(c, w0, w1, std::true_type{});
   // no direct load may be in flight when the workgroup gives its LDS back
 #if defined(__HIP_DEVICE_COMPILE__)
   __builtin_amdgcn_s_waitcnt(0);
@@ -693,37 +907,32 @@ __global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
     for (int r = 0; r < 4; ++r) {
       const int rt = 16 * (4 * wm + mb) + 4 * g + r;
       const long long row = m0 + rt;
-      const float sc = RMS ? row_scale[rt] : 1.0f;
+      const float sc = scaled ? row_scale[rt] : 1.0f;
       if (row < M) {
+        float* dst = slices == 1 ? y + row * N : sums + (blockIdx.y * M + row) * N;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const long long col = nw + 16 * t + i;
-          if (col < N) y[row * N + col] = acc[mb][t][r] * sc;
+          if (col < N) dst[col] = acc[mb][t][r] * sc;
         }
       }
     }
   }
 }
 
-struct Mx4Planes {
-  unsigned short* planes;
-  float* part;
-};
-
-template <int BMB, int NT>
-void run_gemm(const Mx4Args& a, const Mx4Planes& p, hipStream_t stream) {
+template <int NT>
+void run_gemm(const Mx4Args& a, const Mx4Planes& p, float* sums, int slices, hipStream_t stream) {
+  constexpr int BMB = 8;
   const int K = static_cast<int>(a.K);
   const int nb = (K + 31) / 32;
   const int mblocks = static_cast<int>((a.M + 15) / 16);
   const int tiles_m = (mblocks + BMB - 1) / BMB;
   const long long tiles = tiles_m * ((a.N + 64 * NT - 1) / (64 * NT));
   ENG_CHECK(tiles <= 0x7fffffffLL, "linear_mx4w: too many tiles for one launch");
-  const int groups = (K + kPlaneK - 1) / kPlaneK;
+  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(slices));
   auto go = [&](auto rms) {
-    mx4_gemm_kernel<BMB, NT, decltype(rms)::value>
-        <<<static_cast<unsigned>(tiles), 64 * BMB, 0, stream>>>(
-            p.planes, p.part, a.codes, a.scales, a.y, a.M, a.N, K, nb, tiles_m, mblocks, groups,
-            a.eps);
+    mx4_gemm_kernel<BMB, NT, decltype(rms)::value><<<grid, 64 * BMB, 0, stream>>>(
+        p.planes, p.part, a.codes, a.scales, a.y, sums, a.M, a.N, K, nb, tiles_m, mblocks, a.eps);
   };
   if (a.rms) go(std::true_type{});
   else go(std::false_type{});
@@ -734,70 +943,73 @@ void run_gemm(const Mx4Args& a, const Mx4Planes& p, hipStream_t stream) {
 // stay below 2^31 bytes.
 constexpr long long kGemmMaxK = 1ll << 23;
 
-void launch_mx4_gemm(const Mx4Args& a, hipStream_t stream) {
-  const int K = static_cast<int>(a.K);
-  const int chunks = (K + kChunk - 1) / kChunk;
-  const int groups = (K + kPlaneK - 1) / kPlaneK;
-  const long long mblocks = (a.M + 15) / 16;
-  const std::size_t plane_bytes = static_cast<std::size_t>(mblocks) * chunks * 12 * 1024;
-  StreamScratch ws(stream, plane_bytes + static_cast<std::size_t>(a.M) * groups * sizeof(float));
-  Mx4Planes p;
-  p.planes = static_cast<unsigned short*>(ws.get());
-  p.part = reinterpret_cast<float*>(static_cast<char*>(ws.get()) + plane_bytes);
-  const bool vec = a.K % 4 == 0 && aligned_to(a.x, 16) && aligned_to(a.gamma, 16);
-  auto split = [&](auto rms, auto v) {
-    mx4_planes_kernel<decltype(rms)::value, decltype(v)::value>
-        <<<dim3(static_cast<unsigned>(mblocks), static_cast<unsigned>(groups)), 256, 0, stream>>>(
-            a.x, a.gamma, p.planes, p.part, a.M, K, chunks);
-  };
-  using T = std::true_type;
-  using F = std::false_type;
-  if (a.rms) vec ? split(T{}, T{}) : split(T{}, F{});
-  else vec ? split(F{}, T{}) : split(F{}, F{});
-  ENG_LAUNCH_CHECK();
-  if (a.M <= 64) {
-    run_gemm<4, 2>(a, p, stream);
-    return;
-  }
-  // the width whose tiles take the least time in whole rounds of one per CU
+// Tile width and slices of K: the least estimate, in microseconds, of whole rounds of
+// one workgroup per CU (a chunk of a 128 x 64 NT tile: its 192 NT matrix
+// instructions on four SIMDs and about a quarter of a microsecond; the fill and the
+// end of a tile about 2) and, past one slice, the sums' way out and back and the
+// reduce launch.
+void gemm_shape(const Mx4Args& a, int& nt, int& slices) {
   const long long cus = device_cu_count();
-  long long best = 0;
-  int nt = 0;
+  const long long chunks = (a.K + kChunk - 1) / kChunk;
+  double best = 0.0;
+  nt = 0;
   for (int cand : {4, 3, 2}) {
-    const long long tiles = (mblocks + 7) / 8 * ((a.N + 64 * cand - 1) / (64 * cand));
-    const long long cost = (tiles + cus - 1) / cus * (16 * cand + 6);
-    if (nt == 0 || cost < best) best = cost, nt = cand;
+    const long long tiles = (a.M + 127) / 128 * ((a.N + 64 * cand - 1) / (64 * cand));
+    for (int s : {1, 2, 4, 8, 16}) {
+      if (s > 1 && (2 * s > chunks || tiles * s > 2 * cus)) break;
+      const double rounds = static_cast<double>((tiles * s + cus - 1) / cus);
+      double us = rounds * (static_cast<double>((chunks + s - 1) / s) * (0.64 * cand + 0.25) + 2.0);
+      if (s > 1) us += 4.0 + 8.0e-6 * s * a.M * a.N / 4.0;
+      if (nt == 0 || us < best) best = us, nt = cand, slices = s;
+    }
   }
-  if (nt == 4) run_gemm<8, 4>(a, p, stream);
-  else if (nt == 3) run_gemm<8, 3>(a, p, stream);
-  else run_gemm<8, 2>(a, p, stream);
 }
 
-// Up to 32 rows at a.x, a.y.
-void launch_few(const Mx4Args& a, hipStream_t stream) {
-  switch (a.M) {
-    case 1: run_decode<1>(a, stream); return;
-    case 2: run_decode<2>(a, stream); return;
-    case 3: run_decode<3>(a, stream); return;
-    case 4: run_decode<4>(a, stream); return;
-    default: break;
+void launch_mx4_gemm(const Mx4Args& a, hipStream_t stream) {
+  int nt = 0, slices = 1;
+  gemm_shape(a, nt, slices);
+  const std::size_t planes = (planes_scratch(a) + 15) / 16 * 16;
+  const std::size_t sum_bytes =
+      slices > 1 ? static_cast<std::size_t>(slices) * a.M * a.N * sizeof(float) : 0;
+  StreamScratch ws(stream, planes + sum_bytes);
+  float* sums = reinterpret_cast<float*>(static_cast<char*>(ws.get()) + planes);
+  const Mx4Planes p = launch_planes(a, ws.get(), stream);
+  if (nt == 4) run_gemm<4>(a, p, sums, slices, stream);
+  else if (nt == 3) run_gemm<3>(a, p, sums, slices, stream);
+  else run_gemm<2>(a, p, sums, slices, stream);
+  if (slices > 1)
+    launch_reduce(a, sums, p.part, slices, static_cast<int>((a.K + kChunk - 1) / kChunk), stream);
+}
+
+// One pass of rows at a.x, a.y.
+void launch_pass(const Mx4Args& a, hipStream_t stream) {
+  if (decode_applies(a.M, a.K)) {
+    switch (a.M) {
+      case 1: run_decode<1>(a, stream); break;
+      case 2: run_decode<2>(a, stream); break;
+      case 3: run_decode<3>(a, stream); break;
+      default: run_decode<4>(a, stream); break;
+    }
+    return;
   }
-  if (a.M <= 16) run_rows<1, 2>(a, stream);
-  else run_rows<2, 2>(a, stream);
+  if (a.M <= 16) run_slices<1, 2>(a, stream);
+  else if (a.M <= 32) run_slices<2, 2>(a, stream);
+  else if (a.M <= 64) run_slices<4, 3>(a, stream);
+  else launch_mx4_gemm(a, stream);
 }
 
 // Rows in passes whose planes take at most 256 MiB of the stream's arena.
 void linear_mx4w(const Mx4Args& a, hipStream_t stream) {
-  const bool gemm = a.M > 32 && a.K <= kGemmMaxK;
   const long long row_bytes = (a.K + kChunk - 1) / kChunk * kChunk * 6;
-  const long long pass = gemm ? std::max(128ll, (256ll << 20) / row_bytes / 128 * 128) : 32;
+  const long long pass = a.K <= kGemmMaxK
+                             ? std::clamp((256ll << 20) / row_bytes / 128 * 128, 128ll, 32768ll)
+                             : 64;
   for (long long m = 0; m < a.M; m += pass) {
     Mx4Args p = a;
     p.M = std::min(pass, a.M - m);
     p.x = a.x + m * a.K;
     p.y = a.y + m * a.N;
-    if (gemm && p.M > 32) launch_mx4_gemm(p, stream);
-    else launch_few(p, stream);
+    launch_pass(p, stream);
   }
 }
 
