@@ -744,7 +744,7 @@ void run_slices(const Mx4Args& a, hipStream_t stream) {
 //
 // C tiles of 128 x 64 NT on 8 waves: 2 of them along M, 4 along N, each 64 rows x 16
 // NT columns. A step is one j of a chunk (32 k): its 3 BMB plane fragments
-// sit in one of four LDS stages, loaded three steps ahead by direct loads (three a
+// sit in one of four LDS stages, loaded four steps ahead by direct loads (three a
 // wave); the weights of a chunk, which only one row of waves uses, come straight
 // into registers a chunk ahead (4-bit: 16 NT bytes a lane and chunk) and are
 // converted as their step begins.
@@ -836,17 +836,46 @@ __global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[mb][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // Step (c, j): its planes have landed and every wave is past the step before;
-  // the weights of the next chunk (at j == 0), then the planes three steps on go
-  // out, into the stage read last. Younger loads that the wait leaves in flight:
-  // two steps' planes (6), and the next chunk's weights where step 0 was one of
-  // the two. LAST: the chunk after which nothing reads weights; it loads none (the
-  // compiler would drop loads that nothing reads, and the count be too high).
+  // Fragments of m-blocks 2 h and 2 h + 1 of the wave.
+  struct A {
+    bf16x8 a[2][3];
+  };
+  auto read_a = [&](A& f, const unsigned short* st, int h) __attribute__((always_inline)) {
+    const unsigned short* as = st + (wm * 4 + 2 * h) * (3 * 512) + 8 * lane;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        f.a[mb][p] = *reinterpret_cast<const bf16x8*>(as + (mb * 3 + p) * 512);
+  };
+  auto mma = [&](const A& f, int h, const bf16x8 (&b)[NT]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int p = 2; p >= 0; --p)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[2 * h + mb][t] = mfma(f.a[mb][p], b[t], acc[2 * h + mb][t]);
+  };
+  // Step (c, j), x holding its first two m-blocks: the other two are read while those
+  // are multiplied, then the hand-over (the next step's planes have landed, and every
+  // wave has read all of this one's): the next chunk's weights (at j == 0) and the
+  // planes four steps on go out, into the stage just read, and the next step's first
+  // two m-blocks are read while the second two are multiplied. Younger loads that the
+  // wait leaves in flight: two steps' planes (6), and the next chunk's weights where
+  // step 0 was one of the two before. LAST: the chunk after which nothing reads
+  // weights; it loads none (the compiler would drop loads that nothing reads, and the
+  // count be too high).
+  A x, z;
   auto step = [&](auto jt, int c, const W& w, W& next, auto last) __attribute__((always_inline)) {
     constexpr int J = decltype(jt)::value;
     constexpr bool LAST = decltype(last)::value;
-    using Prev = std::integral_constant<int, (J + 3) & 3>;
+    using Next = std::integral_constant<int, (J + 1) & 3>;
     [[maybe_unused]] constexpr int YOUNGER = 6 + (!LAST && (J == 1 || J == 2) ? 2 * NT : 0);
+    bf16x8 b[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) b[t] = weights8(w.w[t][J], scale_of(w.s[t]));
+    read_a(z, stage(jt), 1);
+    mma(x, 0, b);
     __builtin_amdgcn_sched_barrier(0);
 #if defined(__HIP_DEVICE_COMPILE__)
     __builtin_amdgcn_s_waitcnt(vmcnt_le(YOUNGER) & lgkmcnt_zero());
@@ -855,21 +884,11 @@ __global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (J == 0 && !LAST) load_w(next, c + 1);
     __builtin_amdgcn_sched_barrier(0);
-    fetch_a(stage(Prev{}), 4 * c + J + 3);
+    fetch_a(stage(jt), 4 * c + J + 4);
     __builtin_amdgcn_sched_barrier(0);
-    const unsigned short* as = stage(jt) + (wm * 4) * (3 * 512) + 8 * lane;
-    bf16x8 b[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) b[t] = weights8(w.w[t][J], scale_of(w.s[t]));
-#pragma unroll
-    for (int mb = 0; mb < 4; ++mb) {
-#pragma unroll
-      for (int p = 2; p >= 0; --p) {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>(as + (mb * 3 + p) * 512);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[mb][t] = mfma(a, b[t], acc[mb][t]);
-      }
-    }
+    read_a(x, stage(Next{}), 0);
+    mma(z, 1, b);
+    __builtin_amdgcn_sched_barrier(0);
   };
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
@@ -889,6 +908,15 @@ __global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
   fetch_a(st1, 4 * cb + 1);
   __builtin_amdgcn_sched_barrier(0);
   fetch_a(st2, 4 * cb + 2);
+  __builtin_amdgcn_sched_barrier(0);
+  fetch_a(st3, 4 * cb + 3);
+  __builtin_amdgcn_sched_barrier(0);
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_s_waitcnt(vmcnt_le(9));  // the first step's have landed
+#endif
+  lds_barrier();
+  read_a(x, st0, 0);
+  __builtin_amdgcn_sched_barrier(0);
   int c = cb;
   for (; c + 1 < ce; c += 2) {
     chunk(c, w0, w1, std::false_type{});
