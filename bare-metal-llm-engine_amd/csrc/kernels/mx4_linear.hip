@@ -33,6 +33,8 @@ namespace {
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+// four floats at any float's address (the hardware's loads need no more)
+typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
@@ -66,6 +68,19 @@ __device__ __forceinline__ void split3(float v, float (&t)[3]) {
   t[0] = v != v ? __uint_as_float(b | 0x00400000u) : h;
   t[1] = m;
   t[2] = r - m;
+}
+
+// Four values of a row of K at k, zeros from K on.
+__device__ __forceinline__ floatx4 load4(const float* __restrict__ row, int k, int K) {
+  floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (k + 4 <= K) {
+    v = *reinterpret_cast<const floatx4u*>(row + k);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (k + e < K) v[e] = row[k + e];
+  }
+  return v;
 }
 
 // The eight bf16 weights of one code word.
@@ -131,6 +146,7 @@ struct Unit {
 // reads of a step (3 MR rows x 4 groups) spread over the banks.
 constexpr int kDecodeWaves = 16;
 constexpr int kDecodeLds = 120 * 1024;
+constexpr int kDecodeTiles = 48;  // most tiles of a workgroup
 
 constexpr int decode_pitch(int K) { return (K + kUnit - 1) / kUnit * kUnit + 8; }
 // Whether M rows of X fit the decode kernel's LDS.
@@ -138,7 +154,7 @@ bool decode_applies(long long M, long long K) {
   return M <= 4 && K <= kDecodeLds && 6 * M * decode_pitch(static_cast<int>(K)) <= kDecodeLds;
 }
 
-template <int MR, bool RMS, bool VEC, bool SV>
+template <int MR, bool RMS, bool SV>
 __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
     const float* __restrict__ x, const float* __restrict__ gamma,
     const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
@@ -149,6 +165,7 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
   extern __shared__ __attribute__((aligned(16))) unsigned short planes[];  // [MR][3][pitch]
   __shared__ float red[2][kDecodeWaves][MR][16];
   __shared__ float red_ss[kDecodeWaves][MR];
+  __shared__ float out[kDecodeTiles][MR][16];
   const int pitch = decode_pitch(K);
 
   const int tid = threadIdx.x;
@@ -163,27 +180,16 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
   const long long tiles = (N + 15) / 16;
   const int mine = static_cast<int>((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
 
-  // four values of a row at k, zeros from K on
-  auto load4 = [&](const float* p, int k) {
-    floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (VEC) {
-      if (k < K) v = *reinterpret_cast<const floatx4*>(p + k);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = k + e < K ? p[k + e] : 0.0f;
-    }
-    return v;
-  };
   struct X {
     floatx4 v[MR];
     floatx4 gm;
   };
   auto load_x = [&](X& r, int k) {
 #pragma unroll
-    for (int m = 0; m < MR; ++m) r.v[m] = load4(x + static_cast<long long>(m) * K, k);
+    for (int m = 0; m < MR; ++m) r.v[m] = load4(x + static_cast<long long>(m) * K, k, K);
     r.gm = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
     if constexpr (RMS) {
-      if (gamma != nullptr) r.gm = load4(gamma, k);
+      if (gamma != nullptr) r.gm = load4(gamma, k, K);
     }
   };
   float ss[MR];
@@ -269,7 +275,9 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
       planes + (min(i >> 2, MR - 1) * 3 + min(i & 3, 2)) * pitch + 32 * g;
   floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   int tile = 0;
-  // lane (i, g): element r of acc is A row 4 g + r, weight row i
+  // lane (i, g): element r of acc is A row 4 g + r, weight row i. The rows of y stay
+  // in LDS until the end: a store among the loads would make every later wait one
+  // for all of them.
   auto finish = [&] {
     float (*rb)[MR][16] = red[tile & 1];
     if (g < MR) rb[wave][g][i] = (acc[0] + acc[1]) + acc[2];
@@ -279,36 +287,56 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
       float v = rb[0][g][i];
 #pragma unroll
       for (int q = 1; q < kDecodeWaves; ++q) v += rb[q][g][i];
-      const long long n = 16 * (blockIdx.x + static_cast<long long>(tile) * gridDim.x) + i;
-      if (n < N) y[g * N + n] = v * row_scale;
+      out[tile][g][i] = v * row_scale;
     }
     ++tile;
   };
-  if (u0 == u1) {  // fewer units than waves: this one only joins the barriers
-    while (tile < mine) finish();
-    return;
-  }
   int u = u0;
-  while (true) {
+  auto compute = [&](const Unit<1, SV>& x) __attribute__((always_inline)) {
+    const unsigned short* ap = abase + u * kUnit;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float sc = x.scale(0, h, g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc = mfma(*reinterpret_cast<const bf16x8*>(ap + h * kChunk + 8 * j),
+                   weights8(x.w[h][0][j], sc), acc);
+    }
+    if (++u == u1) {
+      u = u0;
+      finish();
+    }
+  };
+  // (a wave without units, where K has fewer than waves, only joins the barriers)
+  const int items = mine * (u1 - u0);
+  int it = 0;
+  for (; it + P < items; it += P) {
 #pragma unroll
     for (int r = 0; r < P; ++r) {
-      const unsigned short* ap = abase + u * kUnit;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float sc = w[r].scale(0, h, g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc = mfma(*reinterpret_cast<const bf16x8*>(ap + h * kChunk + 8 * j),
-                     weights8(w[r].w[h][0][j], sc), acc);
-      }
-      if (++u == u1) {
-        u = u0;
-        finish();
-        if (tile == mine) return;
-      }
+      compute(w[r]);
       load_w(r);
     }
   }
+#pragma unroll
+  for (int r = 0; r < P; ++r)
+    if (it + r < items) compute(w[r]);
+  while (tile < mine) finish();
+  lds_barrier();
+  for (int q = tid; q < 16 * MR * mine; q += THREADS) {
+    const int t = q / (16 * MR);
+    const int m = q / 16 % MR;
+    const long long n = 16 * (blockIdx.x + static_cast<long long>(t) * gridDim.x) + q % 16;
+    if (n < N) y[m * N + n] = out[t][m][q % 16];
+  }
+}
+
+// f with both truth values as types.
+template <class F>
+void with_flags(bool a, bool b, F&& f) {
+  using T = std::true_type;
+  using N = std::false_type;
+  if (a) b ? f(T{}, T{}) : f(T{}, N{});
+  else b ? f(N{}, T{}) : f(N{}, N{});
 }
 
 // Whether every row's scale bytes are whole aligned eights (Unit's SV).
@@ -320,28 +348,21 @@ template <int MR>
 void run_decode(const Mx4Args& a, hipStream_t stream) {
   const int K = static_cast<int>(a.K);
   const int nb = (K + 31) / 32;
-  const bool vec = a.K % 4 == 0 && aligned_to(a.x, 16) && aligned_to(a.gamma, 16);
   const std::size_t lds = static_cast<std::size_t>(6) * MR * decode_pitch(K);
-  const unsigned grid =
-      static_cast<unsigned>(std::min<long long>((a.N + 15) / 16, device_cu_count()));
-  auto go = [&](auto rms, auto v, auto sv) {
+  const long long tiles = (a.N + 15) / 16;
+  const long long wgs = std::min<long long>(
+      tiles, std::max<long long>(device_cu_count(), (tiles + kDecodeTiles - 1) / kDecodeTiles));
+  ENG_CHECK(wgs <= 0x7fffffffLL, "linear_mx4w: grid too large for one launch");
+  const unsigned grid = static_cast<unsigned>(wgs);
+  auto go = [&](auto rms, auto sv) {
     constexpr bool R = decltype(rms)::value;
-    constexpr bool V = decltype(v)::value;
     constexpr bool SV = decltype(sv)::value;
     static std::atomic<bool> done[64];
-    allow_staged_lds(reinterpret_cast<const void*>(mx4_decode_kernel<MR, R, V, SV>), done, lds);
-    mx4_decode_kernel<MR, R, V, SV><<<grid, 64 * kDecodeWaves, lds, stream>>>(
+    allow_staged_lds(reinterpret_cast<const void*>(mx4_decode_kernel<MR, R, SV>), done, lds);
+    mx4_decode_kernel<MR, R, SV><<<grid, 64 * kDecodeWaves, lds, stream>>>(
         a.x, a.gamma, a.codes, a.scales, a.y, a.N, K, nb, a.eps);
   };
-  using T = std::true_type;
-  using F = std::false_type;
-  auto pick = [&](auto rms) {
-    if (!vec) go(rms, F{}, F{});
-    else if (!scales_by_8(a)) go(rms, T{}, F{});
-    else go(rms, T{}, T{});
-  };
-  if (a.rms) pick(T{});
-  else pick(F{});
+  with_flags(a.rms, scales_by_8(a), go);
   ENG_LAUNCH_CHECK();
 }
 
@@ -353,7 +374,7 @@ void run_decode(const Mx4Args& a, hipStream_t stream) {
 // A wave's load of a fragment is then 1 KiB in one piece, and one of X as it stands 64
 // pieces of 16 bytes. Rows past M and k past K are zeros. Beside them the sums of
 // squares of each row's chunks.
-template <bool RMS, bool VEC>
+template <bool RMS>
 __global__ __launch_bounds__(256) void mx4_planes_kernel(const float* __restrict__ x,
                                                          const float* __restrict__ gamma,
                                                          unsigned short* __restrict__ planes,
@@ -366,28 +387,15 @@ __global__ __launch_bounds__(256) void mx4_planes_kernel(const float* __restrict
   const long long mb = blockIdx.y;
   const long long row = 16 * mb + i;
   const int k = c * kChunk + 8 * e8;
+  const int kr = row < M ? k : K;  // rows past M count as past K
   float v[8];
   float ss = 0.0f;
   const float* xr = x + (row < M ? row : 0) * K;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    floatx4 f = {0.0f, 0.0f, 0.0f, 0.0f};
+    const floatx4 f = load4(xr, kr + 4 * h, K);
     floatx4 gm = {1.0f, 1.0f, 1.0f, 1.0f};
-    const int kh = k + 4 * h;
-    if constexpr (VEC) {
-      if (row < M && kh < K) {
-        f = *reinterpret_cast<const floatx4*>(xr + kh);
-        if (RMS && gamma != nullptr) gm = *reinterpret_cast<const floatx4*>(gamma + kh);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (row < M && kh + e < K) {
-          f[e] = xr[kh + e];
-          if (RMS && gamma != nullptr) gm[e] = gamma[kh + e];
-        }
-      }
-    }
+    if (RMS && gamma != nullptr) gm = load4(gamma, kr + 4 * h, K);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[4 * h + e] = f[e];
@@ -433,15 +441,11 @@ Mx4Planes launch_planes(const Mx4Args& a, void* scratch, hipStream_t stream) {
   const int K = static_cast<int>(a.K);
   const int chunks = (K + kChunk - 1) / kChunk;
   const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>((a.M + 15) / 16));
-  const bool vec = a.K % 4 == 0 && aligned_to(a.x, 16) && aligned_to(a.gamma, 16);
-  auto go = [&](auto rms, auto v) {
-    mx4_planes_kernel<decltype(rms)::value, decltype(v)::value><<<grid, 256, 0, stream>>>(
-        a.x, a.gamma, p.planes, p.part, a.M, K, chunks);
+  auto go = [&](auto kernel) {
+    kernel<<<grid, 256, 0, stream>>>(a.x, a.gamma, p.planes, p.part, a.M, K, chunks);
   };
-  using T = std::true_type;
-  using F = std::false_type;
-  if (a.rms) vec ? go(T{}, T{}) : go(T{}, F{});
-  else vec ? go(F{}, T{}) : go(F{}, F{});
+  if (a.rms) go(mx4_planes_kernel<true>);
+  else go(mx4_planes_kernel<false>);
   ENG_LAUNCH_CHECK();
   return p;
 }
@@ -482,7 +486,7 @@ constexpr int slice_units() { return MB == 1 ? 2 : 1; }  // 48 KiB of fragments,
 
 __device__ __forceinline__ int frag_slot(int i, int g) { return 16 * g + ((i + 4 * g) & 15); }
 
-template <int MB, int NT, bool RMS, bool VEC, bool SV>
+template <int MB, int NT, bool RMS, bool SV>
 __global__ __launch_bounds__(64 * kSliceWaves, MB == 4 ? 2 : 4) void mx4_slice_kernel(
     const float* __restrict__ x, const float* __restrict__ gamma,
     const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
@@ -507,17 +511,6 @@ __global__ __launch_bounds__(64 * kSliceWaves, MB == 4 ? 2 : 4) void mx4_slice_k
   const int r = (tid >> 4) & 15;
   const int e8 = tid & 15;
   floatx4 xv[PX][2], gv[RMS ? PX : 1][2];
-  auto load4 = [&](const float* p, int k, float fill) {
-    floatx4 v = {fill, fill, fill, fill};
-    if constexpr (VEC) {
-      if (k < K) v = *reinterpret_cast<const floatx4*>(p + k);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (k + e < K) v[e] = p[k + e];
-    }
-    return v;
-  };
 #pragma unroll
   for (int q = 0; q < PX; ++q) {
     const int row = 16 * (q / KU) + r;
@@ -528,10 +521,10 @@ __global__ __launch_bounds__(64 * kSliceWaves, MB == 4 ? 2 : 4) void mx4_slice_k
     if (q % KU >= n_units) continue;  // (uniform)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      xv[q][h] = load4(xr, kk + 4 * h, 0.0f);
+      xv[q][h] = load4(xr, kk + 4 * h, K);
       if constexpr (RMS) {
         gv[q][h] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
-        if (gamma != nullptr) gv[q][h] = load4(gamma, kk + 4 * h, 0.0f);
+        if (gamma != nullptr) gv[q][h] = load4(gamma, kk + 4 * h, K);
       }
     }
   }
@@ -641,7 +634,7 @@ __global__ __launch_bounds__(64 * kSliceWaves, MB == 4 ? 2 : 4) void mx4_slice_k
 
 // y[m][n] = s_m times the sum over the slices, in their order. blockIdx.y: a row, whose
 // sum of squares is in `parts` parts.
-template <bool RMS, bool VEC>
+template <bool RMS>
 __global__ __launch_bounds__(256) void mx4_slice_reduce_kernel(const float* __restrict__ sums,
                                                                const float* __restrict__ squares,
                                                                float* __restrict__ y, long long M,
@@ -656,44 +649,40 @@ __global__ __launch_bounds__(256) void mx4_slice_reduce_kernel(const float* __re
     for (int s = 0; s < parts; ++s) t += squares[row * parts + s];
     sc = 1.0f / sqrtf(t / static_cast<float>(K) + eps);
   }
-  if constexpr (VEC) {
-    const long long n = 4 * (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x);
-    if (n >= N) return;
-    const float* p = sums + row * N + n;
-    floatx4 v = *reinterpret_cast<const floatx4*>(p);
+  const long long n = 4 * (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x);
+  if (n >= N) return;
+  const float* p = sums + row * N + n;
+  float* out = y + row * N + n;
+  if (n + 4 <= N) {
+    floatx4 v = *reinterpret_cast<const floatx4u*>(p);
 #pragma unroll 4
     for (int s = 1; s < slices; ++s) {
-      const floatx4 a = *reinterpret_cast<const floatx4*>(p + s * stride);
+      const floatx4 a = *reinterpret_cast<const floatx4u*>(p + s * stride);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += a[e];
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[row * N + n + e] = v[e] * sc;
+    for (int e = 0; e < 4; ++e) v[e] *= sc;
+    *reinterpret_cast<floatx4u*>(out) = v;
   } else {
-    const long long n = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    if (n >= N) return;
-    const float* p = sums + row * N + n;
-    float v = *p;
-#pragma unroll 4
-    for (int s = 1; s < slices; ++s) v += p[s * stride];
-    y[row * N + n] = v * sc;
+    for (int e = 0; e < N - n; ++e) {
+      float v = p[e];
+      for (int s = 1; s < slices; ++s) v += p[s * stride + e];
+      out[e] = v * sc;
+    }
   }
 }
 
 void launch_reduce(const Mx4Args& a, const float* sums, const float* squares, int slices, int parts,
                    hipStream_t stream) {
-  const bool wide = a.N % 4 == 0;
-  const long long per = wide ? 1024 : 256;
   ENG_CHECK(a.M <= 65535, "linear_mx4w: too many rows in a pass");
-  const dim3 grid(static_cast<unsigned>((a.N + per - 1) / per), static_cast<unsigned>(a.M));
-  auto go = [&](auto rms, auto v) {
-    mx4_slice_reduce_kernel<decltype(rms)::value, decltype(v)::value><<<grid, 256, 0, stream>>>(
-        sums, squares, a.y, a.M, a.N, static_cast<int>(a.K), slices, parts, a.eps);
+  const dim3 grid(static_cast<unsigned>((a.N + 1023) / 1024), static_cast<unsigned>(a.M));
+  auto go = [&](auto kernel) {
+    kernel<<<grid, 256, 0, stream>>>(sums, squares, a.y, a.M, a.N, static_cast<int>(a.K), slices, parts,
+                                     a.eps);
   };
-  using T = std::true_type;
-  using F = std::false_type;
-  if (a.rms) wide ? go(T{}, T{}) : go(T{}, F{});
-  else wide ? go(F{}, T{}) : go(F{}, F{});
+  if (a.rms) go(mx4_slice_reduce_kernel<true>);
+  else go(mx4_slice_reduce_kernel<false>);
   ENG_LAUNCH_CHECK();
 }
 
@@ -708,6 +697,16 @@ int slice_count(long long N, long long K, int nt) {
   return static_cast<int>(std::min(units, std::max(fit, fill)));
 }
 
+// Whether slices of one unit of K by 128 nt columns are at least `wgs_per_cu`
+// workgroups a CU: wider ones otherwise leave CUs idle, and narrow ones split X more
+// often (16 x 4096 x 4096 10.8 us at nt = 1, 11.7 at 2; 16 x 11008 x 4096 23.4 and
+// 18.4; 64 x 4096 x 4096 26.3, 23.9 and at 3 24.4; 64 x 11008 x 4096 61, 48 and 43).
+bool slice_fills(const Mx4Args& a, int nt, double wgs_per_cu) {
+  const long long units = (a.K + kUnit - 1) / kUnit;
+  const long long groups = (a.N + 128 * nt - 1) / (128 * nt);
+  return static_cast<double>(units * groups) >= wgs_per_cu * device_cu_count();
+}
+
 template <int MB, int NT>
 void run_slices(const Mx4Args& a, hipStream_t stream) {
   const int K = static_cast<int>(a.K);
@@ -720,22 +719,13 @@ void run_slices(const Mx4Args& a, hipStream_t stream) {
   StreamScratch ws(stream, sum_bytes + static_cast<std::size_t>(M) * slices * sizeof(float));
   float* sums = static_cast<float*>(ws.get());
   float* squares = reinterpret_cast<float*>(static_cast<char*>(ws.get()) + sum_bytes);
-  const bool vec = a.K % 4 == 0 && aligned_to(a.x, 16) && aligned_to(a.gamma, 16);
   const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(slices));
-  using T = std::true_type;
-  using F = std::false_type;
-  auto go = [&](auto rms, auto v, auto sv) {
-    mx4_slice_kernel<MB, NT, decltype(rms)::value, decltype(v)::value, decltype(sv)::value>
+  auto go = [&](auto rms, auto sv) {
+    mx4_slice_kernel<MB, NT, decltype(rms)::value, decltype(sv)::value>
         <<<grid, 64 * kSliceWaves, 0, stream>>>(a.x, a.gamma, a.codes, a.scales, sums, squares, M, a.N,
                                                 K, nb);
   };
-  auto pick = [&](auto rms) {
-    if (!vec) go(rms, F{}, F{});
-    else if (!scales_by_8(a)) go(rms, T{}, F{});
-    else go(rms, T{}, T{});
-  };
-  if (a.rms) pick(T{});
-  else pick(F{});
+  with_flags(a.rms, scales_by_8(a), go);
   ENG_LAUNCH_CHECK();
   launch_reduce(a, sums, squares, slices, slices, stream);
 }
@@ -1020,10 +1010,19 @@ void launch_pass(const Mx4Args& a, hipStream_t stream) {
     }
     return;
   }
-  if (a.M <= 16) run_slices<1, 2>(a, stream);
-  else if (a.M <= 32) run_slices<2, 2>(a, stream);
-  else if (a.M <= 64) run_slices<4, 3>(a, stream);
-  else launch_mx4_gemm(a, stream);
+  if (a.M <= 16) {
+    if (slice_fills(a, 2, 1.5)) run_slices<1, 2>(a, stream);
+    else run_slices<1, 1>(a, stream);
+  } else if (a.M <= 32) {
+    if (slice_fills(a, 2, 1.5)) run_slices<2, 2>(a, stream);
+    else run_slices<2, 1>(a, stream);
+  } else if (a.M <= 64) {
+    if (slice_fills(a, 3, 1.0)) run_slices<4, 3>(a, stream);
+    else if (slice_fills(a, 2, 1.0)) run_slices<4, 2>(a, stream);
+    else run_slices<4, 1>(a, stream);
+  } else {
+    launch_mx4_gemm(a, stream);
+  }
 }
 
 // Rows in passes whose planes take at most 256 MiB of the stream's arena.
