@@ -346,8 +346,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 3 : 1) void decode_q8_kernel(Att
     }
     const int left = nkeys - (wave + NW * t) * kKvBlock;  // keys from the block's first one on
     const float f = scale2 * x.ks;
-    const float lv = __builtin_amdgcn_logf(x.vs);  // log2
-    const float ivs = __builtin_amdgcn_rcpf(x.vs);
+    // a V scale of zero (a block of zeros in a cache written elsewhere): the keys
+    // count, their values are zero
+    const bool no_v = x.vs == 0.0f;  // (uniform)
+    const float lv = no_v ? 0.0f : __builtin_amdgcn_logf(x.vs);  // log2
+    const float ivs = no_v ? 1.0f : __builtin_amdgcn_rcpf(x.vs);
     float sv[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sv[e] = fmaf(sc[e >> 2][e & 3], f, lv);
@@ -385,6 +388,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 3 : 1) void decode_q8_kernel(Att
 #endif
     }
     lsum = fmaf(ls, ivs, lsum);
+    if (no_v) return;
 #pragma unroll
     for (int d = 0; d < VD; ++d) {
       halfx8 av[4];

@@ -469,13 +469,14 @@ __device__ __forceinline__ void row_scales(const float* __restrict__ part, long 
 
 // --------------------------------------------------------------- 5 to 64 rows
 //
-// A workgroup of 8 waves owns 128 NT weight rows (16 NT a wave) and a slice of K, at
-// most KU units of it: it splits its slice of X into LDS once, as the fragments of
+// A workgroup of 8 waves owns 128 NT weight rows (16 NT a wave) and a slice of K, which
+// it takes KU units at a time: it splits its piece of X into LDS, as the fragments of
 // the matrix instruction (16 rows x 32 k of one term, 1 KiB in the order the lanes
-// take it), and every wave multiplies them by its own weights, all of which are on
-// their way before X is split. The slices' sums go to scratch and
-// mx4_slice_reduce_kernel adds them in slice order and applies the rows' scales (from
-// the sums of squares that the first column of workgroups leaves).
+// take it), and every wave multiplies them by its own weights; X and weights of the
+// next piece are on their way meanwhile. With several slices the sums go to scratch
+// and mx4_slice_reduce_kernel adds them in slice order and applies the rows' scales
+// (from the sums of squares that the first column of workgroups leaves); with one the
+// workgroup scales and writes its rows of y itself.
 // Slices, because X outweighs the weights otherwise: 16 rows are 96 bytes per k
 // in three terms against 8 of a 16-row tile of weights, and with all of K in every
 // workgroup their way from L2 set the time (16 x 11008 x 4096: 114 MB, 15 us).
@@ -487,10 +488,11 @@ constexpr int slice_units() { return MB == 1 ? 2 : 1; }  // 48 KiB of fragments,
 __device__ __forceinline__ int frag_slot(int i, int g) { return 16 * g + ((i + 4 * g) & 15); }
 
 template <int MB, int NT, bool RMS, bool SV>
-__global__ __launch_bounds__(64 * kSliceWaves, MB == 4 ? 2 : 4) void mx4_slice_kernel(
+__global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
     const float* __restrict__ x, const float* __restrict__ gamma,
     const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-    float* __restrict__ sums, float* __restrict__ squares, int M, long long N, int K, int nb) {
+    float* __restrict__ y, float* __restrict__ sums, float* __restrict__ squares, int M, long long N,
+    int K, int nb, float eps) {
   constexpr int KU = slice_units<MB>();
   constexpr int PX = MB * KU;  // pieces of 8 values a thread splits
   __shared__ __attribute__((aligned(1024))) unsigned short frag[MB * KU * 24 * 512];
@@ -504,130 +506,165 @@ __global__ __launch_bounds__(64 * kSliceWaves, MB == 4 ? 2 : 4) void mx4_slice_k
   const int slices = gridDim.y;
   const int slice = blockIdx.y;
   const int u0 = static_cast<int>(static_cast<long long>(units) * slice / slices);
-  const int n_units = static_cast<int>(static_cast<long long>(units) * (slice + 1) / slices) - u0;
+  const int u1 = static_cast<int>(static_cast<long long>(units) * (slice + 1) / slices);
 
-  // X: piece q of a thread is row 16 mb + r, values 8 e .. + 7 of chunk c of the
-  // slice, (mb, c) = (q / KU, 2 (q % KU) + tid / 256).
+  // X: piece q of a thread is row 16 mb + r, values 8 e8 .. + 7 of chunk c of the
+  // KU units, (mb, c) = (q / KU, 2 (q % KU) + tid / 256).
   const int r = (tid >> 4) & 15;
   const int e8 = tid & 15;
-  floatx4 xv[PX][2], gv[RMS ? PX : 1][2];
+  struct X {
+    floatx4 v[PX][2];
+    floatx4 gm[RMS ? KU : 1][2];
+  };
+  auto load_x = [&](X& f, int ub) __attribute__((always_inline)) {
 #pragma unroll
-  for (int q = 0; q < PX; ++q) {
-    const int row = 16 * (q / KU) + r;
-    const int k = u0 * kUnit + (2 * (q % KU) + (tid >> 8)) * kChunk + 8 * e8;
-    const float* xr = x + static_cast<long long>(min(row, M - 1)) * K;
-    // rows past M count as past K
-    const int kk = row < M ? k : K;
-    if (q % KU >= n_units) continue;  // (uniform)
+    for (int q = 0; q < PX; ++q) {
+      const int row = 16 * (q / KU) + r;
+      const int k = (ub + q % KU) * kUnit + (tid >> 8) * kChunk + 8 * e8;
+      const float* xr = x + static_cast<long long>(min(row, M - 1)) * K;
+      // rows past M, and units past the slice, count as past K
+      const int kk = row < M && ub + q % KU < u1 ? k : K;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      xv[q][h] = load4(xr, kk + 4 * h, K);
-      if constexpr (RMS) {
-        gv[q][h] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
-        if (gamma != nullptr) gv[q][h] = load4(gamma, kk + 4 * h, K);
+      for (int h = 0; h < 2; ++h) {
+        f.v[q][h] = load4(xr, kk + 4 * h, K);
+        if (RMS && q < KU) {
+          f.gm[q][h] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
+          if (gamma != nullptr) f.gm[q][h] = load4(gamma, ub + q < u1 ? k + 4 * h : K, K);
+        }
       }
     }
-  }
-  __builtin_amdgcn_sched_barrier(0);
-  const long long n0 = (static_cast<long long>(blockIdx.x) * kSliceWaves + wave) * (16 * NT);
-  Unit<NT, SV> w[KU];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const long long n = std::min(n0 + 16 * t + i, N - 1);
-#pragma unroll
-    for (int q = 0; q < KU; ++q)
-      if (q < n_units) w[q].load(t, codes + n * (16ll * nb), scales + n * nb, u0 + q, g, nb);
-  }
-  __builtin_amdgcn_sched_barrier(0);
-
+  };
   float ss[MB];
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) ss[mb] = 0.0f;
+  auto put_x = [&](const X& f, int ub) __attribute__((always_inline)) {
 #pragma unroll
-  for (int q = 0; q < PX; ++q) {
-    if (q % KU >= n_units) continue;  // (uniform)
-    float t[8][3];
+    for (int q = 0; q < PX; ++q) {
+      if (ub + q % KU >= u1) continue;  // (uniform)
+      float t[8][3];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float v = xv[q][e >> 2][e & 3];
-      if constexpr (RMS) {
-        ss[q / KU] = fmaf(v, v, ss[q / KU]);
-        v *= gv[q][e >> 2][e & 3];
+      for (int e = 0; e < 8; ++e) {
+        float v = f.v[q][e >> 2][e & 3];
+        if constexpr (RMS) {
+          ss[q / KU] = fmaf(v, v, ss[q / KU]);
+          v *= f.gm[q % KU][e >> 2][e & 3];
+        }
+        split3(v, t[e]);
       }
-      split3(v, t[e]);
-    }
-    const int c = 2 * (q % KU) + (tid >> 8);
-    // fragments [chunk][step][m-block][term]; this thread's is lane (r, group e8 / 4)
-    // of step e8 % 4. Lane (i, g)'s 16 bytes sit at 16 g + (i + 4 g) % 16, so that
-    // these stores (4 rows of every group and step) and the reads (whole fragments)
-    // both spread over the banks.
-    uintx4* dst = reinterpret_cast<uintx4*>(frag) +
-                  (((c * 4 + (e8 & 3)) * MB + q / KU) * 3) * 64 + frag_slot(r, e8 >> 2);
+      const int c = 2 * (q % KU) + (tid >> 8);
+      // fragments [chunk][step][m-block][term]; this thread's is lane (r, group e8 / 4)
+      // of step e8 % 4. Lane (i, g)'s 16 bytes sit at 16 g + (i + 4 g) % 16, so that
+      // these stores (4 rows of every group and step) and the reads (whole fragments)
+      // both spread over the banks.
+      uintx4* dst = reinterpret_cast<uintx4*>(frag) +
+                    (((c * 4 + (e8 & 3)) * MB + q / KU) * 3) * 64 + frag_slot(r, e8 >> 2);
 #pragma unroll
-    for (int p = 0; p < 3; ++p)
-      dst[p * 64] = uintx4{pack_hi(t[0][p], t[1][p]), pack_hi(t[2][p], t[3][p]),
-                           pack_hi(t[4][p], t[5][p]), pack_hi(t[6][p], t[7][p])};
-  }
-  lds_barrier();
-
+      for (int p = 0; p < 3; ++p)
+        dst[p * 64] = uintx4{pack_hi(t[0][p], t[1][p]), pack_hi(t[2][p], t[3][p]),
+                             pack_hi(t[4][p], t[5][p]), pack_hi(t[6][p], t[7][p])};
+    }
+  };
+  const long long n0 = (static_cast<long long>(blockIdx.x) * kSliceWaves + wave) * (16 * NT);
+  struct W {
+    Unit<NT, SV> u[KU];
+  };
+  auto load_w = [&](W& w, int ub) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const long long n = std::min(n0 + 16 * t + i, N - 1);
+#pragma unroll
+      for (int q = 0; q < KU; ++q)
+        w.u[q].load(t, codes + n * (16ll * nb), scales + n * nb, min(ub + q, u1 - 1), g, nb);
+    }
+  };
   floatx4 acc[MB][NT];
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[mb][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto compute = [&](const W& w, int ub) __attribute__((always_inline)) {
 #pragma unroll
-  for (int q = 0; q < KU; ++q) {
-    if (q >= n_units) break;
+    for (int q = 0; q < KU; ++q) {
+      if (ub + q >= u1) break;  // (uniform)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned short* f = frag + ((8 * q + 4 * h + j) * MB * 3) * 512 + 8 * frag_slot(i, g);
-        bf16x8 b[NT];
+        for (int j = 0; j < 4; ++j) {
+          const unsigned short* f =
+              frag + ((8 * q + 4 * h + j) * MB * 3) * 512 + 8 * frag_slot(i, g);
+          bf16x8 b[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) b[t] = weights8(w[q].w[h][t][j], w[q].scale(t, h, g));
+          for (int t = 0; t < NT; ++t) b[t] = weights8(w.u[q].w[h][t][j], w.u[q].scale(t, h, g));
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
+          for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
-          for (int p = 2; p >= 0; --p) {
-            const bf16x8 av = *reinterpret_cast<const bf16x8*>(f + (mb * 3 + p) * 512);
+            for (int p = 2; p >= 0; --p) {
+              const bf16x8 av = *reinterpret_cast<const bf16x8*>(f + (mb * 3 + p) * 512);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[mb][t] = mfma(av, b[t], acc[mb][t]);
+              for (int t = 0; t < NT; ++t) acc[mb][t] = mfma(av, b[t], acc[mb][t]);
+            }
           }
         }
       }
     }
+  };
+
+  X xr;
+  W w0, w1;
+  load_x(xr, u0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_w(w0, u0);
+  __builtin_amdgcn_sched_barrier(0);
+  auto piece = [&](const W& w, W& next, int ub) __attribute__((always_inline)) {
+    put_x(xr, ub);
+    lds_barrier();
+    if (ub + KU < u1) {  // (uniform)
+      load_x(xr, ub + KU);
+      load_w(next, ub + KU);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    compute(w, ub);
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();  // the fragments have been read
+  };
+  for (int ub = u0; ub < u1; ub += 2 * KU) {
+    piece(w0, w1, ub);
+    if (ub + KU < u1) piece(w1, w0, ub + KU);
   }
 
-  // lane (i, g): element v of acc is row 4 g + v, column i
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int row = 16 * mb + 4 * g + v;
-      if (row < M) {
-        float* dst = sums + (static_cast<long long>(slice) * M + row) * N;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const long long n = n0 + 16 * t + i;
-          if (n < N) dst[n] = acc[mb][t][v];
-        }
-      }
-    }
-  }
+  // The rows' sums of squares over the slice, in LDS (the fragments have been read).
+  float* red = reinterpret_cast<float*>(frag);  // [2][16 MB]: the two halves of the threads
   if constexpr (RMS) {
-    if (blockIdx.x == 0) {  // (uniform)
-      __syncthreads();      // the fragments have been read
-      float* red = reinterpret_cast<float*>(frag);  // [2][16 MB]: the two halves of the threads
+    if (slices == 1 || blockIdx.x == 0) {  // (uniform)
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
         for (int off = 1; off < 16; off <<= 1) ss[mb] += __shfl_xor(ss[mb], off);
         if (e8 == 0) red[(tid >> 8) * 16 * MB + 16 * mb + r] = ss[mb];
       }
-      __syncthreads();
-      if (tid < 16 * MB && tid < M)
+      lds_barrier();
+      if (slices > 1 && tid < 16 * MB && tid < M)
         squares[static_cast<long long>(tid) * slices + slice] = red[tid] + red[16 * MB + tid];
+    }
+  }
+  // lane (i, g): element v of acc is row 4 g + v, column i
+  float* out = slices == 1 ? y : sums + static_cast<long long>(slice) * M * N;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int row = 16 * mb + 4 * g + v;
+      if (row < M) {
+        float sc = 1.0f;
+        if (RMS && slices == 1)
+          sc = 1.0f / sqrtf((red[row] + red[16 * MB + row]) / static_cast<float>(K) + eps);
+        float* dst = out + row * N;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const long long n = n0 + 16 * t + i;
+          if (n < N) dst[n] = acc[mb][t][v] * sc;
+        }
+      }
     }
   }
 }
@@ -686,15 +723,24 @@ void launch_reduce(const Mx4Args& a, const float* sums, const float* squares, in
   ENG_LAUNCH_CHECK();
 }
 
-// Slices of K: enough that a slice's units fit the kernel, and more while the
-// workgroups do not fill the CUs.
-template <int MB>
-int slice_count(long long N, long long K, int nt) {
+// Slices of K: the least estimate, in microseconds, of whole rounds of one workgroup
+// per CU (a unit of K takes 3 us at 16 rows by 256 columns, 5 at 32, 10 at 64 rows by
+// 384: measured where the units follow one another) and, past one slice, the sums'
+// way out and back and the reduce launch.
+int slice_count(long long M, long long N, long long K, int mb, int nt) {
+  const long long cus = device_cu_count();
   const long long units = (K + kUnit - 1) / kUnit;
   const long long groups = (N + 128 * nt - 1) / (128 * nt);
-  const long long fit = (units + slice_units<MB>() - 1) / slice_units<MB>();
-  const long long fill = std::max(1ll, device_cu_count() / groups);
-  return static_cast<int>(std::min(units, std::max(fit, fill)));
+  const double unit_us = 1.0 + 0.5 * mb + (0.25 + 0.375 * mb) * nt;
+  double best = 0.0;
+  long long count = 1;
+  for (long long s = 1; s <= std::min(units, 32ll); ++s) {
+    double us = static_cast<double>((groups * s + cus - 1) / cus) *
+                (static_cast<double>((units + s - 1) / s) * unit_us + 3.0);
+    if (s > 1) us += 4.0 + 8.0e-6 * static_cast<double>(s * M * N) / 4.0;
+    if (s == 1 || us < best) best = us, count = s;
+  }
+  return static_cast<int>(count);
 }
 
 // Whether slices of one unit of K by 128 nt columns are at least `wgs_per_cu`
@@ -712,21 +758,27 @@ void run_slices(const Mx4Args& a, hipStream_t stream) {
   const int K = static_cast<int>(a.K);
   const int M = static_cast<int>(a.M);
   const int nb = (K + 31) / 32;
-  const int slices = slice_count<MB>(a.N, a.K, NT);
+  const int slices = slice_count(a.M, a.N, a.K, MB, NT);
   const long long groups = (a.N + 128 * NT - 1) / (128 * NT);
-  ENG_CHECK(groups <= 0x7fffffffLL && slices <= 65535, "linear_mx4w: grid too large for one launch");
+  ENG_CHECK(groups <= 0x7fffffffLL, "linear_mx4w: grid too large for one launch");
+  const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(slices));
+  auto launch = [&](float* sums, float* squares) {
+    with_flags(a.rms, scales_by_8(a), [&](auto rms, auto sv) {
+      mx4_slice_kernel<MB, NT, decltype(rms)::value, decltype(sv)::value>
+          <<<grid, 64 * kSliceWaves, 0, stream>>>(a.x, a.gamma, a.codes, a.scales, a.y, sums, squares, M,
+                                                  a.N, K, nb, a.eps);
+    });
+    ENG_LAUNCH_CHECK();
+  };
+  if (slices == 1) {
+    launch(nullptr, nullptr);
+    return;
+  }
   const std::size_t sum_bytes = (static_cast<std::size_t>(slices) * M * a.N + 3) / 4 * 16;
   StreamScratch ws(stream, sum_bytes + static_cast<std::size_t>(M) * slices * sizeof(float));
   float* sums = static_cast<float*>(ws.get());
   float* squares = reinterpret_cast<float*>(static_cast<char*>(ws.get()) + sum_bytes);
-  const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(slices));
-  auto go = [&](auto rms, auto sv) {
-    mx4_slice_kernel<MB, NT, decltype(rms)::value, decltype(sv)::value>
-        <<<grid, 64 * kSliceWaves, 0, stream>>>(a.x, a.gamma, a.codes, a.scales, sums, squares, M, a.N,
-                                                K, nb);
-  };
-  with_flags(a.rms, scales_by_8(a), go);
-  ENG_LAUNCH_CHECK();
+  launch(sums, squares);
   launch_reduce(a, sums, squares, slices, slices, stream);
 }
 
@@ -957,10 +1009,6 @@ void run_gemm(const Mx4Args& a, const Mx4Planes& p, float* sums, int slices, hip
   ENG_LAUNCH_CHECK();
 }
 
-// Buffer offsets are 32-bit: a tile's weight rows (256) and an m-block's planes
-// stay below 2^31 bytes.
-constexpr long long kGemmMaxK = 1ll << 23;
-
 // Tile width and slices of K: the least estimate, in microseconds, of whole rounds of
 // one workgroup per CU (a chunk of a 128 x 64 NT tile: its 192 NT matrix
 // instructions on four SIMDs and about a quarter of a microsecond; the fill and the
@@ -1028,9 +1076,7 @@ void launch_pass(const Mx4Args& a, hipStream_t stream) {
 // Rows in passes whose planes take at most 256 MiB of the stream's arena.
 void linear_mx4w(const Mx4Args& a, hipStream_t stream) {
   const long long row_bytes = (a.K + kChunk - 1) / kChunk * kChunk * 6;
-  const long long pass = a.K <= kGemmMaxK
-                             ? std::clamp((256ll << 20) / row_bytes / 128 * 128, 128ll, 32768ll)
-                             : 64;
+  const long long pass = std::clamp((256ll << 20) / row_bytes / 128 * 128, 128ll, 32768ll);
   for (long long m = 0; m < a.M; m += pass) {
     Mx4Args p = a;
     p.M = std::min(pass, a.M - m);
@@ -1046,7 +1092,9 @@ void check_linear(const std::string& name, const void* x, const void* codes, con
   ENG_CHECK(x != nullptr && codes != nullptr && scales != nullptr && y != nullptr,
             name + ": null device pointer");
   ENG_CHECK(aligned_to(codes, 16), name + ": codes must be 16-byte aligned");
-  ENG_CHECK(K <= 0x7fffff00LL, name + ": K too large");
+  // buffer offsets are 32-bit: a GEMM tile's weight rows and an m-block's planes stay
+  // below 2^31 bytes
+  ENG_CHECK(K <= (1ll << 23), name + ": K too large (at most 2^23)");
 }
 
 }  // namespace

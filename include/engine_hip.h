@@ -465,8 +465,9 @@ int eng_transpose_f32(const float* src, float* dst, int64_t rows, int64_t cols,
  * may be NULL; as for eng_rmsnorm_linear_* any zero dimension is a no-op.
  * Products are exact and sums fp32, as for fp16 weights: every fp32 activation
  * enters the matrix cores as three bf16 terms that add up to it. K is at most
- * 2^31 - 256. The same call gives the same bits; the kernel, and with it the
- * order of the sums, depends on M, N, K and the alignment of x.
+ * 2^23. The same call gives the same bits; the kernel, and with it the order of
+ * the sums, depends on M, N and K. From 5 rows (below that, where X does not fit
+ * the LDS: M K past 20000 or so) the stream's scratch arena is used.
  * ---------------------------------------------------------------------- */
 int eng_mx4_quantize_f32(const float* src, uint8_t* codes, uint8_t* scales, int64_t rows,
                          int64_t cols, eng_stream stream);
@@ -490,7 +491,8 @@ int eng_rmsnorm_linear_mx4w_nk(const float* in, const float* rms_weight, const u
  * [batch, n_kv_heads, kv_max_seq_len, head_dim], 16-byte aligned; every block of
  * ENG_KV_Q8_BLOCK tokens of a (sequence, KV head) has one fp32 scale for K and
  * one for V, [batch, n_kv_heads, ceil(kv_max_seq_len / ENG_KV_Q8_BLOCK)]. The
- * value of a code is its e4m3 value times its block's scale. head_dim is 64 or
+ * value of a code is its e4m3 value times its block's scale (a cache written by
+ * other means may have any finite scales of zero or more). head_dim is 64 or
  * 128. Positions and lengths are read on the device (int32 arrays of `batch`), so
  * a captured decode step is replayed for every token.
  *

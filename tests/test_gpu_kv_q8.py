@@ -234,6 +234,24 @@ def test_attention_unlike_block_scales(gpu):
         check_attend(gpu, c, q, [L], L, split=split)
 
 
+def test_attention_over_a_cache_written_elsewhere(gpu):
+    """Scales that are no powers of two, and zero for blocks of K, of V and of both."""
+    rng = np.random.default_rng(17)
+    B, H, G, D, L = 2, 6, 2, 64, 300
+    c = Cache(gpu, rng, B, G, L, D)
+    finite = lambda: (rng.integers(0, 2, (B, G, L, D)) * 128 + rng.integers(0, 127, (B, G, L, D))).astype(np.uint8)  # noqa: E731
+    c.k, c.v = finite(), finite()
+    c.ks = (0.002 * rng.random(c.ks.shape)).astype(np.float32)
+    c.vs = (0.01 * rng.random(c.vs.shape)).astype(np.float32)
+    c.ks[0, 0, 2:4] = 0
+    c.vs[0, 0, 3:5] = 0
+    c.vs[1, 1, :] = 0
+    c.dev = [gpu.upload(a) for a in (c.k, c.v, c.ks, c.vs)]
+    q = (0.3 * rng.standard_normal((B, H, D))).astype(np.float16)
+    for split in (0, 1, 3):
+        check_attend(gpu, c, q, [L, 217], L, split=split)
+
+
 @pytest.mark.parametrize("skew", [1, 4])
 def test_attention_unaligned_q_and_out(gpu, skew):
     rng = np.random.default_rng(14)
