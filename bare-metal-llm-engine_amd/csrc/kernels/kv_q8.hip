@@ -555,13 +555,17 @@ __global__ __launch_bounds__(64) void merge_q8_kernel(const float* __restrict__ 
 // Splits when the caller passes split_kv = 0: the largest power of two that keeps
 // one workgroup per CU or fewer over all (sequence, KV head) units (splits of
 // unlike lengths, as a division that does not come out even makes, were 5-25%
-// slower), and at least four blocks per split, one per wave, past 32 blocks. A
+// slower), at least four blocks per split, one per wave, past 32 blocks, and one
+// split, without the merge's launch, up to 12 blocks at D = 128 or 24 at D = 64
+// (300 tokens, 32 / 4 heads of 64 5.3 us, 6.5 in 8 splits; 600 tokens, 32 / 8 heads
+// of 128 7.8 us, 7.1 in 16). A
 // sweep of 1 to 64 splits over 18 shapes put it at the best count or within 6%:
 // 32 / 32 heads, D = 128, 8192 tokens 8 splits 15.4 us (16: 16.7, 4: 18.1); 32 / 8
 // heads, 131072 tokens 32 splits 46 us (16: 59, 64: 49); 32 sequences of 32 / 8
 // heads, 4096 tokens 1 split 43 us (2: 47.5, 8: 54.6); 1000 tokens, 32 / 8 heads 32
-// splits 6.3 us (8: 7.3).
-int auto_splits(long long blocks, long long units) {
+// splits 6.3 us (8: 7.3, 1: 9.5).
+int auto_splits(long long blocks, long long units, long long head_dim) {
+  if (blocks * head_dim <= 12 * 128) return 1;
   const long long cus = device_cu_count();
   const long long most = std::min(256ll, blocks <= 32 ? blocks : blocks / 4);
   long long s = 1;
@@ -709,7 +713,7 @@ int eng_attention_decode_q8(const eng_half* q, const uint8_t* k_cache, const uin
     a.scale = scale;
     const long long blocks = (max_kv_len + eng::kKvBlock - 1) / eng::kKvBlock;
     const long long want = split_kv == 0
-                               ? eng::auto_splits(blocks, batch * n_kv_heads * a.tiles)
+                               ? eng::auto_splits(blocks, batch * n_kv_heads * a.tiles, head_dim)
                                : std::min<long long>({split_kv, blocks, 256});
     a.split_blocks =
         static_cast<int>(std::min((blocks + want - 1) / want, eng::kMaxSplitBlocks));
