@@ -470,20 +470,21 @@ __device__ __forceinline__ void row_scales(const float* __restrict__ part, long 
 // --------------------------------------------------------------- 5 to 64 rows
 //
 // A workgroup of 8 waves owns 128 NT weight rows (16 NT a wave) and a slice of K, which
-// it takes KU units at a time: it splits its piece of X into LDS, as the fragments of
+// it takes a unit at a time: it splits its unit of X into LDS, as the fragments of
 // the matrix instruction (16 rows x 32 k of one term, 1 KiB in the order the lanes
-// take it), and every wave multiplies them by its own weights; X and weights of the
-// next piece are on their way meanwhile. With several slices the sums go to scratch
+// take it), and every wave multiplies them by its own weights. The next unit of X is
+// on its way meanwhile, the next weights from there to the end of its split. With several slices the sums go to scratch
 // and mx4_slice_reduce_kernel adds them in slice order and applies the rows' scales
 // (from the sums of squares that the first column of workgroups leaves); with one the
 // workgroup scales and writes its rows of y itself.
 // Slices, because X outweighs the weights otherwise: 16 rows are 96 bytes per k
 // in three terms against 8 of a 16-row tile of weights, and with all of K in every
 // workgroup their way from L2 set the time (16 x 11008 x 4096: 114 MB, 15 us).
+// What bounds it: with a few units to a workgroup, the latencies of one pass and the
+// instructions' own way in (a third of the wave's time there); two units at a
+// time, or their weights in a second set of registers, cost more in code than they
+// hide (16 x 152064 x 4096 115 us, 138 with either; 16 x 11008 x 4096 17.1, 18.1, 17.2).
 constexpr int kSliceWaves = 8;
-
-template <int MB>
-constexpr int slice_units() { return MB == 1 ? 2 : 1; }  // 48 KiB of fragments, 96 at 64 rows
 
 __device__ __forceinline__ int frag_slot(int i, int g) { return 16 * g + ((i + 4 * g) & 15); }
 
@@ -493,9 +494,7 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
     const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
     float* __restrict__ y, float* __restrict__ sums, float* __restrict__ squares, int M, long long N,
     int K, int nb, float eps) {
-  constexpr int KU = slice_units<MB>();
-  constexpr int PX = MB * KU;  // pieces of 8 values a thread splits
-  __shared__ __attribute__((aligned(1024))) unsigned short frag[MB * KU * 24 * 512];
+  __shared__ __attribute__((aligned(1024))) unsigned short frag[MB * 24 * 512];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -508,56 +507,54 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
   const int u0 = static_cast<int>(static_cast<long long>(units) * slice / slices);
   const int u1 = static_cast<int>(static_cast<long long>(units) * (slice + 1) / slices);
 
-  // X: piece q of a thread is row 16 mb + r, values 8 e8 .. + 7 of chunk c of the
-  // KU units, (mb, c) = (q / KU, 2 (q % KU) + tid / 256).
+  // X: a thread splits values 8 e8 .. + 7 of chunk tid / 256 of the unit, of rows
+  // 16 mb + r.
   const int r = (tid >> 4) & 15;
   const int e8 = tid & 15;
   struct X {
-    floatx4 v[PX][2];
-    floatx4 gm[RMS ? KU : 1][2];
+    floatx4 v[MB][2];
+    floatx4 gm[2];
   };
-  auto load_x = [&](X& f, int ub) __attribute__((always_inline)) {
+  auto load_x = [&](X& f, int u) __attribute__((always_inline)) {
+    const int k = u * kUnit + (tid >> 8) * kChunk + 8 * e8;
 #pragma unroll
-    for (int q = 0; q < PX; ++q) {
-      const int row = 16 * (q / KU) + r;
-      const int k = (ub + q % KU) * kUnit + (tid >> 8) * kChunk + 8 * e8;
+    for (int mb = 0; mb < MB; ++mb) {
+      const int row = 16 * mb + r;
       const float* xr = x + static_cast<long long>(min(row, M - 1)) * K;
-      // rows past M, and units past the slice, count as past K
-      const int kk = row < M && ub + q % KU < u1 ? k : K;
+      const int kk = row < M ? k : K;  // rows past M count as past K
+#pragma unroll
+      for (int h = 0; h < 2; ++h) f.v[mb][h] = load4(xr, kk + 4 * h, K);
+    }
+    if constexpr (RMS) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        f.v[q][h] = load4(xr, kk + 4 * h, K);
-        if (RMS && q < KU) {
-          f.gm[q][h] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
-          if (gamma != nullptr) f.gm[q][h] = load4(gamma, ub + q < u1 ? k + 4 * h : K, K);
-        }
+        f.gm[h] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
+        if (gamma != nullptr) f.gm[h] = load4(gamma, k + 4 * h, K);
       }
     }
   };
   float ss[MB];
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) ss[mb] = 0.0f;
-  auto put_x = [&](const X& f, int ub) __attribute__((always_inline)) {
+  auto put_x = [&](const X& f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int q = 0; q < PX; ++q) {
-      if (ub + q % KU >= u1) continue;  // (uniform)
+    for (int mb = 0; mb < MB; ++mb) {
       float t[8][3];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float v = f.v[q][e >> 2][e & 3];
+        float v = f.v[mb][e >> 2][e & 3];
         if constexpr (RMS) {
-          ss[q / KU] = fmaf(v, v, ss[q / KU]);
-          v *= f.gm[q % KU][e >> 2][e & 3];
+          ss[mb] = fmaf(v, v, ss[mb]);
+          v *= f.gm[e >> 2][e & 3];
         }
         split3(v, t[e]);
       }
-      const int c = 2 * (q % KU) + (tid >> 8);
       // fragments [chunk][step][m-block][term]; this thread's is lane (r, group e8 / 4)
       // of step e8 % 4. Lane (i, g)'s 16 bytes sit at 16 g + (i + 4 g) % 16, so that
       // these stores (4 rows of every group and step) and the reads (whole fragments)
       // both spread over the banks.
       uintx4* dst = reinterpret_cast<uintx4*>(frag) +
-                    (((c * 4 + (e8 & 3)) * MB + q / KU) * 3) * 64 + frag_slot(r, e8 >> 2);
+                    ((((tid >> 8) * 4 + (e8 & 3)) * MB + mb) * 3) * 64 + frag_slot(r, e8 >> 2);
 #pragma unroll
       for (int p = 0; p < 3; ++p)
         dst[p * 64] = uintx4{pack_hi(t[0][p], t[1][p]), pack_hi(t[2][p], t[3][p]),
@@ -565,16 +562,12 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
     }
   };
   const long long n0 = (static_cast<long long>(blockIdx.x) * kSliceWaves + wave) * (16 * NT);
-  struct W {
-    Unit<NT, SV> u[KU];
-  };
-  auto load_w = [&](W& w, int ub) __attribute__((always_inline)) {
+  Unit<NT, SV> w;
+  auto load_w = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const long long n = std::min(n0 + 16 * t + i, N - 1);
-#pragma unroll
-      for (int q = 0; q < KU; ++q)
-        w.u[q].load(t, codes + n * (16ll * nb), scales + n * nb, min(ub + q, u1 - 1), g, nb);
+      w.load(t, codes + n * (16ll * nb), scales + n * nb, u, g, nb);
     }
   };
   floatx4 acc[MB][NT];
@@ -582,27 +575,22 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
   for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[mb][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  auto compute = [&](const W& w, int ub) __attribute__((always_inline)) {
+  auto compute = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int q = 0; q < KU; ++q) {
-      if (ub + q >= u1) break;  // (uniform)
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int j = 0; j < 4; ++j) {
+        const unsigned short* f = frag + ((4 * h + j) * MB * 3) * 512 + 8 * frag_slot(i, g);
+        bf16x8 b[NT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const unsigned short* f =
-              frag + ((8 * q + 4 * h + j) * MB * 3) * 512 + 8 * frag_slot(i, g);
-          bf16x8 b[NT];
+        for (int t = 0; t < NT; ++t) b[t] = weights8(w.w[h][t][j], w.scale(t, h, g));
 #pragma unroll
-          for (int t = 0; t < NT; ++t) b[t] = weights8(w.u[q].w[h][t][j], w.u[q].scale(t, h, g));
+        for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
-          for (int mb = 0; mb < MB; ++mb) {
+          for (int p = 2; p >= 0; --p) {
+            const bf16x8 av = *reinterpret_cast<const bf16x8*>(f + (mb * 3 + p) * 512);
 #pragma unroll
-            for (int p = 2; p >= 0; --p) {
-              const bf16x8 av = *reinterpret_cast<const bf16x8*>(f + (mb * 3 + p) * 512);
-#pragma unroll
-              for (int t = 0; t < NT; ++t) acc[mb][t] = mfma(av, b[t], acc[mb][t]);
-            }
+            for (int t = 0; t < NT; ++t) acc[mb][t] = mfma(av, b[t], acc[mb][t]);
           }
         }
       }
@@ -610,26 +598,20 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
   };
 
   X xr;
-  W w0, w1;
   load_x(xr, u0);
   __builtin_amdgcn_sched_barrier(0);
-  load_w(w0, u0);
+  load_w(u0);
   __builtin_amdgcn_sched_barrier(0);
-  auto piece = [&](const W& w, W& next, int ub) __attribute__((always_inline)) {
-    put_x(xr, ub);
+  for (int u = u0; u < u1; ++u) {
+    put_x(xr);
     lds_barrier();
-    if (ub + KU < u1) {  // (uniform)
-      load_x(xr, ub + KU);
-      load_w(next, ub + KU);
-    }
+    if (u + 1 < u1) load_x(xr, u + 1);  // (uniform)
     __builtin_amdgcn_sched_barrier(0);
-    compute(w, ub);
+    compute();
+    __builtin_amdgcn_sched_barrier(0);
+    if (u + 1 < u1) load_w(u + 1);
     __builtin_amdgcn_sched_barrier(0);
     lds_barrier();  // the fragments have been read
-  };
-  for (int ub = u0; ub < u1; ub += 2 * KU) {
-    piece(w0, w1, ub);
-    if (ub + KU < u1) piece(w1, w0, ub + KU);
   }
 
   // The rows' sums of squares over the slice, in LDS (the fragments have been read).
