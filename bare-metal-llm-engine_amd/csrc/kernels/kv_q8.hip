@@ -59,7 +59,7 @@ __global__ __launch_bounds__(kWriteThreads) void kv_write_q8_kernel(
     const _Float16* __restrict__ k_new, const _Float16* __restrict__ v_new,
     unsigned char* __restrict__ k_cache, unsigned char* __restrict__ v_cache,
     float* __restrict__ k_scale, float* __restrict__ v_scale, const int* __restrict__ pos,
-    const int* __restrict__ n_new, long long units, long long s_new, long long n_kv_heads,
+    const int* __restrict__ n_new, unsigned units, long long s_new, long long n_kv_heads,
     long long kv_max, int reach) {
   constexpr int LPT = D / 8;         // lanes per token
   constexpr int TPL = 64 / LPT;      // tokens per wave load
@@ -68,16 +68,18 @@ __global__ __launch_bounds__(kWriteThreads) void kv_write_q8_kernel(
   const int sub = lane / LPT;
   const int d0 = (lane % LPT) * 8;
   // unit = ((b reach + block) heads + h) 2 + (K or V)
-  const long long unit = static_cast<long long>(blockIdx.x) * (kWriteThreads / 64) + (threadIdx.x >> 6);
+  const unsigned unit = blockIdx.x * (kWriteThreads / 64) +
+                        __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (unit >= units) return;
   const bool is_v = (unit & 1) != 0;
-  const long long h = (unit >> 1) % n_kv_heads;
-  const long long rest = (unit >> 1) / n_kv_heads;
-  const long long b = rest / reach;
+  const unsigned heads = static_cast<unsigned>(n_kv_heads);
+  const unsigned rest = (unit >> 1) / heads;
+  const long long h = (unit >> 1) - rest * heads;
+  const long long b = rest / static_cast<unsigned>(reach);
   const long long p = pos[b];
   const long long n = n_new != nullptr ? std::min<long long>(n_new[b], s_new) : s_new;
   if (p < 0 || n <= 0) return;
-  const long long blk = p / kKvBlock + (rest - b * reach);
+  const long long blk = p / kKvBlock + (rest - b * reach);  // (p >= 0)
   const long long first = blk * kKvBlock;
   const long long lo = std::max(p, first);
   const long long hi = std::min(std::min(p + n, kv_max), first + kKvBlock);
@@ -213,10 +215,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 3 : 1) void decode_q8_kernel(Att
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15;
   const int grp = lane >> 4;
-  const long long unit = blockIdx.x;
-  const int tile = static_cast<int>(unit % a.tiles);
-  const long long bh = unit / a.tiles;  // sequence and KV head
-  const long long b = bh / a.n_kv_heads;
+  const unsigned n_kv = static_cast<unsigned>(a.n_kv_heads);  // 32-bit division: below 2^31
+  const unsigned bh32 = blockIdx.x / static_cast<unsigned>(a.tiles);
+  const int tile = static_cast<int>(blockIdx.x - bh32 * static_cast<unsigned>(a.tiles));
+  const long long bh = bh32;  // sequence and KV head
+  const long long b = bh32 / n_kv;
   const long long kvh = bh - b * a.n_kv_heads;
   const int split = static_cast<int>(blockIdx.y);
   const int gq = min(a.group - 16 * tile, 16);
@@ -648,8 +651,8 @@ int eng_kv_cache_write_q8(const eng_half* k_new, const eng_half* v_new, uint8_t*
     ENG_CHECK(batch <= 0x7fffffffLL && n_kv_heads <= 0x7fffffffLL &&
                   batch * n_kv_heads <= 0x7fffffffLL / reach,
               "kv_cache_write_q8: too many (sequence, head, block) units for one launch");
-    const long long units = 2 * batch * n_kv_heads * reach;
-    const unsigned grid = static_cast<unsigned>((units + 3) / 4);
+    const unsigned units = 2u * static_cast<unsigned>(batch * n_kv_heads * reach);
+    const unsigned grid = static_cast<unsigned>((units + 3ull) / 4);
     auto go = [&](auto kernel) {
       kernel<<<grid, eng::kWriteThreads, 0, eng::as_stream(stream)>>>(
           reinterpret_cast<const _Float16*>(k_new), reinterpret_cast<const _Float16*>(v_new),

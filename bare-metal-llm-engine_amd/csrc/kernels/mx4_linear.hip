@@ -144,6 +144,11 @@ struct Unit {
 // operand are term p of row m; rows that are no term's read some other term (no
 // output comes from them). Terms sit 16 bytes apart modulo the banks' 256, so the
 // reads of a step (3 MR rows x 4 groups) spread over the banks.
+// Bound by the weights' bytes once they are many (1 x 152064 x 4096, 331 MB: 59 us,
+// 5.6 TB/s; 1 x 11008 x 4096, 24 MB: 8.8 us), below that by the latencies of one pass
+// (X, its split, one unit of weights, the sum: 4.2 us at 1 x 2051 x 1023). Two units in
+// flight: three or four make the last ones, which nothing needs, cost more (1 x 4096 x
+// 4096 5.2 us, 5.8 and 6.2).
 constexpr int kDecodeWaves = 16;
 constexpr int kDecodeLds = 120 * 1024;
 constexpr int kDecodeTiles = 48;  // most tiles of a workgroup
@@ -473,10 +478,11 @@ __device__ __forceinline__ void row_scales(const float* __restrict__ part, long 
 // it takes a unit at a time: it splits its unit of X into LDS, as the fragments of
 // the matrix instruction (16 rows x 32 k of one term, 1 KiB in the order the lanes
 // take it), and every wave multiplies them by its own weights. The next unit of X is
-// on its way meanwhile, the next weights from there to the end of its split. With several slices the sums go to scratch
-// and mx4_slice_reduce_kernel adds them in slice order and applies the rows' scales
-// (from the sums of squares that the first column of workgroups leaves); with one the
-// workgroup scales and writes its rows of y itself.
+// on its way meanwhile, the next weights from there to the end of its split. With
+// several slices the sums go to scratch, and mx4_slice_reduce_kernel adds them in
+// slice order and applies the rows' scales (from the sums of squares that the first
+// column of workgroups leaves); with one the workgroup scales and writes its rows of
+// y itself.
 // Slices, because X outweighs the weights otherwise: 16 rows are 96 bytes per k
 // in three terms against 8 of a 16-row tile of weights, and with all of K in every
 // workgroup their way from L2 set the time (16 x 11008 x 4096: 114 MB, 15 us).
@@ -767,18 +773,23 @@ void run_slices(const Mx4Args& a, hipStream_t stream) {
 // -------------------------------------------------------------- 65 rows and up
 //
 // C tiles of 128 x 64 NT on 8 waves: 2 of them along M, 4 along N, each 64 rows x 16
-// NT columns. A step is one j of a chunk (32 k): its 3 BMB plane fragments
-// sit in one of four LDS stages, loaded four steps ahead by direct loads (three a
-// wave); the weights of a chunk, which only one row of waves uses, come straight
-// into registers a chunk ahead (4-bit: 16 NT bytes a lane and chunk) and are
-// converted as their step begins.
-template <int BMB, int NT, bool RMS>
-__global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
+// NT columns. A step is one j of a chunk (32 k): its 24 plane fragments sit in one of
+// four LDS stages, loaded four steps ahead by direct loads (three a wave); the
+// weights of a chunk come straight into registers a chunk ahead (4-bit: 16 NT bytes a
+// lane and chunk) and are converted as their step begins. Tiles with K split among
+// gridDim.y slices leave their sums for mx4_slice_reduce_kernel.
+// Bound by the matrix cores: 2048 x 4096 x 4096 196 us with the planes' pass, 1051
+// TFLOP/s of bf16 products (three per weight), where a plain bf16 product of 8192^3
+// runs at 1198 through the library on the same card.
+constexpr int kGemmBlocks = 8;  // m-blocks of a tile, and waves
+
+template <int NT, bool RMS>
+__global__ __launch_bounds__(64 * kGemmBlocks, 2) void mx4_gemm_kernel(
     const unsigned short* __restrict__ planes, const float* __restrict__ part,
     const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
     float* __restrict__ y, float* __restrict__ sums, long long M, long long N, int K, int nb,
     int tiles_m, int mblocks, float eps) {
-  static_assert(BMB == 8, "128-row tiles on 8 waves");
+  constexpr int BMB = kGemmBlocks;
   constexpr int STAGE = BMB * 3 * 512;  // bf16 of a stage
   __shared__ __attribute__((aligned(1024))) unsigned short st0[STAGE];
   __shared__ __attribute__((aligned(1024))) unsigned short st1[STAGE];
@@ -974,7 +985,7 @@ __global__ __launch_bounds__(64 * BMB, 2) void mx4_gemm_kernel(
 
 template <int NT>
 void run_gemm(const Mx4Args& a, const Mx4Planes& p, float* sums, int slices, hipStream_t stream) {
-  constexpr int BMB = 8;
+  constexpr int BMB = kGemmBlocks;
   const int K = static_cast<int>(a.K);
   const int nb = (K + 31) / 32;
   const int mblocks = static_cast<int>((a.M + 15) / 16);
@@ -983,7 +994,7 @@ void run_gemm(const Mx4Args& a, const Mx4Planes& p, float* sums, int slices, hip
   ENG_CHECK(tiles <= 0x7fffffffLL, "linear_mx4w: too many tiles for one launch");
   const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(slices));
   auto go = [&](auto rms) {
-    mx4_gemm_kernel<BMB, NT, decltype(rms)::value><<<grid, 64 * BMB, 0, stream>>>(
+    mx4_gemm_kernel<NT, decltype(rms)::value><<<grid, 64 * BMB, 0, stream>>>(
         p.planes, p.part, a.codes, a.scales, a.y, sums, a.M, a.N, K, nb, tiles_m, mblocks, a.eps);
   };
   if (a.rms) go(std::true_type{});
