@@ -489,7 +489,8 @@ __device__ __forceinline__ void row_scales(const float* __restrict__ part, long 
 // What bounds it: with a few units to a workgroup, the latencies of one pass and the
 // instructions' own way in (a third of the wave's time there); two units at a
 // time, or their weights in a second set of registers, cost more in code than they
-// hide (16 x 152064 x 4096 115 us, 138 with either; 16 x 11008 x 4096 17.1, 18.1, 17.2).
+// hide (16 x 152064 x 4096 115 us, 138 with either; 16 x 11008 x 4096 at 256 columns
+// and 4 slices 17.1, 18.1, 17.2).
 constexpr int kSliceWaves = 8;
 
 __device__ __forceinline__ int frag_slot(int i, int g) { return 16 * g + ((i + 4 * g) & 15); }
@@ -711,42 +712,36 @@ void launch_reduce(const Mx4Args& a, const float* sums, const float* squares, in
   ENG_LAUNCH_CHECK();
 }
 
-// Slices of K: the least estimate, in microseconds, of whole rounds of one workgroup
-// per CU (a unit of K takes 3 us at 16 rows by 256 columns, 5 at 32, 10 at 64 rows by
-// 384: measured where the units follow one another) and, past one slice, the sums'
-// way out and back and the reduce launch.
-int slice_count(long long M, long long N, long long K, int mb, int nt) {
+// Width (128 nt columns) and slices of K: the least estimate, in microseconds, of whole
+// rounds of one workgroup per CU (a unit of K takes 0.7 mb + (0.3 + 0.2 mb) nt, a
+// workgroup's start and end 1.5) and, past one slice, the reduce launch and the sums'
+// way out and back. Fitted to every width and 1 to 32 slices at 8 to 64 rows of eight
+// matrices, 1024 x 4096 to 28672 x 8192: what it picks takes 0.5 % (geometric mean) more
+// than the fastest of them. One width for all loses at one end: 16 x 4096 x 4096 10.2
+// us at nt = 1, 11.0 at 2 and 11.9 at 3 (X is split more often, CUs idle), 16 x
+// 11008 x 4096 17.3, 16.8 and 15.9, 64 x 11008 x 4096 49, 36 and 31.
+void slice_shape(const Mx4Args& a, int mb, int& nt, int& slices) {
   const long long cus = device_cu_count();
-  const long long units = (K + kUnit - 1) / kUnit;
-  const long long groups = (N + 128 * nt - 1) / (128 * nt);
-  const double unit_us = 1.0 + 0.5 * mb + (0.25 + 0.375 * mb) * nt;
-  double best = 0.0;
-  long long count = 1;
-  for (long long s = 1; s <= std::min(units, 32ll); ++s) {
-    double us = static_cast<double>((groups * s + cus - 1) / cus) *
-                (static_cast<double>((units + s - 1) / s) * unit_us + 3.0);
-    if (s > 1) us += 4.0 + 8.0e-6 * static_cast<double>(s * M * N) / 4.0;
-    if (s == 1 || us < best) best = us, count = s;
-  }
-  return static_cast<int>(count);
-}
-
-// Whether slices of one unit of K by 128 nt columns are at least `wgs_per_cu`
-// workgroups a CU: wider ones otherwise leave CUs idle, and narrow ones split X more
-// often (16 x 4096 x 4096 10.8 us at nt = 1, 11.7 at 2; 16 x 11008 x 4096 23.4 and
-// 18.4; 64 x 4096 x 4096 26.3, 23.9 and at 3 24.4; 64 x 11008 x 4096 61, 48 and 43).
-bool slice_fills(const Mx4Args& a, int nt, double wgs_per_cu) {
   const long long units = (a.K + kUnit - 1) / kUnit;
-  const long long groups = (a.N + 128 * nt - 1) / (128 * nt);
-  return static_cast<double>(units * groups) >= wgs_per_cu * device_cu_count();
+  double best = 0.0;
+  nt = 0;
+  for (int cand : {1, 2, 3}) {
+    const long long groups = (a.N + 128 * cand - 1) / (128 * cand);
+    const double unit_us = 0.7 * mb + (0.3 + 0.2 * mb) * cand;
+    for (long long s = 1; s <= std::min(units, 32ll); ++s) {
+      double us = static_cast<double>((groups * s + cus - 1) / cus) *
+                  (static_cast<double>((units + s - 1) / s) * unit_us + 1.5);
+      if (s > 1) us += 3.0 + 0.1 * static_cast<double>(s) + 1.2e-6 * static_cast<double>(s * a.M * a.N);
+      if (nt == 0 || us < best) best = us, nt = cand, slices = static_cast<int>(s);
+    }
+  }
 }
 
 template <int MB, int NT>
-void run_slices(const Mx4Args& a, hipStream_t stream) {
+void run_slices(const Mx4Args& a, int slices, hipStream_t stream) {
   const int K = static_cast<int>(a.K);
   const int M = static_cast<int>(a.M);
   const int nb = (K + 31) / 32;
-  const int slices = slice_count(a.M, a.N, a.K, MB, NT);
   const long long groups = (a.N + 128 * NT - 1) / (128 * NT);
   ENG_CHECK(groups <= 0x7fffffffLL, "linear_mx4w: grid too large for one launch");
   const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(slices));
@@ -768,6 +763,15 @@ void run_slices(const Mx4Args& a, hipStream_t stream) {
   float* squares = reinterpret_cast<float*>(static_cast<char*>(ws.get()) + sum_bytes);
   launch(sums, squares);
   launch_reduce(a, sums, squares, slices, slices, stream);
+}
+
+template <int MB>
+void launch_slices(const Mx4Args& a, hipStream_t stream) {
+  int nt = 0, slices = 1;
+  slice_shape(a, MB, nt, slices);
+  if (nt == 1) run_slices<MB, 1>(a, slices, stream);
+  else if (nt == 2) run_slices<MB, 2>(a, slices, stream);
+  else run_slices<MB, 3>(a, slices, stream);
 }
 
 // -------------------------------------------------------------- 65 rows and up
@@ -1052,15 +1056,11 @@ void launch_pass(const Mx4Args& a, hipStream_t stream) {
     return;
   }
   if (a.M <= 16) {
-    if (slice_fills(a, 2, 1.5)) run_slices<1, 2>(a, stream);
-    else run_slices<1, 1>(a, stream);
+    launch_slices<1>(a, stream);
   } else if (a.M <= 32) {
-    if (slice_fills(a, 2, 1.5)) run_slices<2, 2>(a, stream);
-    else run_slices<2, 1>(a, stream);
+    launch_slices<2>(a, stream);
   } else if (a.M <= 64) {
-    if (slice_fills(a, 3, 1.0)) run_slices<4, 3>(a, stream);
-    else if (slice_fills(a, 2, 1.0)) run_slices<4, 2>(a, stream);
-    else run_slices<4, 1>(a, stream);
+    launch_slices<4>(a, stream);
   } else {
     launch_mx4_gemm(a, stream);
   }
