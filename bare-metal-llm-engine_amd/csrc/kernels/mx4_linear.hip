@@ -712,14 +712,14 @@ void launch_reduce(const Mx4Args& a, const float* sums, const float* squares, in
   ENG_LAUNCH_CHECK();
 }
 
-// Width (128 nt columns) and slices of K: the least estimate, in microseconds, of whole
-// rounds of one workgroup per CU (a unit of K takes 0.7 mb + (0.3 + 0.2 mb) nt, a
-// workgroup's start and end 1.5) and, past one slice, the reduce launch and the sums'
-// way out and back. Fitted to every width and 1 to 32 slices at 8 to 64 rows of eight
-// matrices, 1024 x 4096 to 28672 x 8192: what it picks takes 0.5 % (geometric mean) more
-// than the fastest of them. One width for all loses at one end: 16 x 4096 x 4096 10.2
-// us at nt = 1, 11.0 at 2 and 11.9 at 3 (X is split more often, CUs idle), 16 x
-// 11008 x 4096 17.3, 16.8 and 15.9, 64 x 11008 x 4096 49, 36 and 31.
+// Width (128 nt columns) and slices of K: the least estimate, in units of about half a
+// microsecond, of whole rounds of one workgroup per CU (mb + 3 nt for a unit of K, 1.5
+// beside the units) and, past one slice, the reduce launch and the sums' way out and
+// back. Fitted to every width and 1 to 32 slices at 5 to 64 rows of sixteen matrices,
+// 1024 x 4096 to 128256 x 8192: what it picks takes 0.9 % (geometric mean) more than
+// the fastest of them, 7 % at most. One width for all loses at one end: 16 x 4096 x 4096 10.2 us
+// at nt = 1, 11.0 at 2 and 11.9 at 3 (X is split more often, CUs idle), 16 x 11008 x
+// 4096 17.3, 16.8 and 15.9, 64 x 11008 x 4096 49, 36 and 31.
 void slice_shape(const Mx4Args& a, int mb, int& nt, int& slices) {
   const long long cus = device_cu_count();
   const long long units = (a.K + kUnit - 1) / kUnit;
@@ -727,12 +727,11 @@ void slice_shape(const Mx4Args& a, int mb, int& nt, int& slices) {
   nt = 0;
   for (int cand : {1, 2, 3}) {
     const long long groups = (a.N + 128 * cand - 1) / (128 * cand);
-    const double unit_us = 0.7 * mb + (0.3 + 0.2 * mb) * cand;
     for (long long s = 1; s <= std::min(units, 32ll); ++s) {
-      double us = static_cast<double>((groups * s + cus - 1) / cus) *
-                  (static_cast<double>((units + s - 1) / s) * unit_us + 1.5);
-      if (s > 1) us += 3.0 + 0.1 * static_cast<double>(s) + 1.2e-6 * static_cast<double>(s * a.M * a.N);
-      if (nt == 0 || us < best) best = us, nt = cand, slices = static_cast<int>(s);
+      double time = static_cast<double>((groups * s + cus - 1) / cus) *
+                    (static_cast<double>((units + s - 1) / s * (mb + 3 * cand)) + 1.5);
+      if (s > 1) time += 2.0 + 0.13 * static_cast<double>(s) + 1.8e-6 * static_cast<double>(s * a.M * a.N);
+      if (nt == 0 || time < best) best = time, nt = cand, slices = static_cast<int>(s);
     }
   }
 }
