@@ -493,7 +493,11 @@ __device__ __forceinline__ void row_scales(const float* __restrict__ part, long 
 // and 4 slices 17.1, 18.1, 17.2).
 constexpr int kSliceWaves = 8;
 
-__device__ __forceinline__ int frag_slot(int i, int g) { return 16 * g + ((i + 4 * g) & 15); }
+// Where lane (i, g)'s 16 bytes of step j sit in their fragment. A read is served in
+// passes of 16 lanes, half of a lane group and the other half of its neighbour, a store
+// in passes of eight consecutive lanes (of a row: two lane groups, four steps); with
+// these bits changed both hit every bank once (no conflicts by the counter).
+__device__ __forceinline__ int frag_slot(int i, int g, int j) { return 16 * g + (i ^ j ^ (-g & 3) << 2); }
 
 template <int MB, int NT, bool RMS, bool SV>
 __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
@@ -522,19 +526,31 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
     floatx4 v[MB][2];
     floatx4 gm[2];
   };
+  // Rows past M repeat the last one: nothing comes of them.
+  const float* xr[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+    xr[mb] = x + static_cast<long long>(min(16 * mb + r, M - 1)) * K;
   auto load_x = [&](X& f, int u) __attribute__((always_inline)) {
     const int k = u * kUnit + (tid >> 8) * kChunk + 8 * e8;
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      const int row = 16 * mb + r;
-      const float* xr = x + static_cast<long long>(min(row, M - 1)) * K;
-      const int kk = row < M ? k : K;  // rows past M count as past K
-#pragma unroll
-      for (int h = 0; h < 2; ++h) f.v[mb][h] = load4(xr, kk + 4 * h, K);
-    }
-    if constexpr (RMS) {
+    if ((u + 1) * kUnit <= K) {  // (uniform) a whole unit needs no bounds
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+          f.v[mb][h] = *reinterpret_cast<const floatx4u*>(xr[mb] + k + 4 * h);
+        if constexpr (RMS) {
+          f.gm[h] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
+          if (gamma != nullptr) f.gm[h] = *reinterpret_cast<const floatx4u*>(gamma + k + 4 * h);
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) f.v[mb][h] = load4(xr[mb], k + 4 * h, K);
+      if constexpr (RMS) {
         f.gm[h] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
         if (gamma != nullptr) f.gm[h] = load4(gamma, k + 4 * h, K);
       }
@@ -557,11 +573,9 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
         split3(v, t[e]);
       }
       // fragments [chunk][step][m-block][term]; this thread's is lane (r, group e8 / 4)
-      // of step e8 % 4. Lane (i, g)'s 16 bytes sit at 16 g + (i + 4 g) % 16, so that
-      // these stores (4 rows of every group and step) and the reads (whole fragments)
-      // both spread over the banks.
+      // of step e8 % 4.
       uintx4* dst = reinterpret_cast<uintx4*>(frag) +
-                    ((((tid >> 8) * 4 + (e8 & 3)) * MB + mb) * 3) * 64 + frag_slot(r, e8 >> 2);
+                    ((((tid >> 8) * 4 + (e8 & 3)) * MB + mb) * 3) * 64 + frag_slot(r, e8 >> 2, e8 & 3);
 #pragma unroll
       for (int p = 0; p < 3; ++p)
         dst[p * 64] = uintx4{pack_hi(t[0][p], t[1][p]), pack_hi(t[2][p], t[3][p]),
@@ -587,7 +601,7 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const unsigned short* f = frag + ((4 * h + j) * MB * 3) * 512 + 8 * frag_slot(i, g);
+        const unsigned short* f = frag + ((4 * h + j) * MB * 3) * 512 + 8 * frag_slot(i, g, j);
         bf16x8 b[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) b[t] = weights8(w.w[h][t][j], w.scale(t, h, g));
@@ -604,15 +618,15 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
     }
   };
 
-  X xr;
-  load_x(xr, u0);
+  X xv;
+  load_x(xv, u0);
   __builtin_amdgcn_sched_barrier(0);
   load_w(u0);
   __builtin_amdgcn_sched_barrier(0);
   for (int u = u0; u < u1; ++u) {
-    put_x(xr);
+    put_x(xv);
     lds_barrier();
-    if (u + 1 < u1) load_x(xr, u + 1);  // (uniform)
+    if (u + 1 < u1) load_x(xv, u + 1);  // (uniform)
     __builtin_amdgcn_sched_barrier(0);
     compute();
     __builtin_amdgcn_sched_barrier(0);
