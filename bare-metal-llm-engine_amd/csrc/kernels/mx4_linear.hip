@@ -57,15 +57,14 @@ __device__ __forceinline__ unsigned pack_hi(float a, float b) {
   return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 
-// v as three bf16 terms, left in the top halves of t[0..2]. An infinity is its
-// own first term with zeros after it; a NaN stays a NaN.
+// v as three bf16 terms, left in the top halves of t[0..2]. An infinity is its own
+// first term with zeros after it; a NaN's difference, and so the second term, is a
+// NaN with its top bit set, which the first need not be (payloads in the low bits).
 __device__ __forceinline__ void split3(float v, float (&t)[3]) {
-  const unsigned b = __float_as_uint(v);
-  const bool fin = (b & 0x7f800000u) != 0x7f800000u;
-  const float h = __uint_as_float(b & 0xffff0000u);
-  const float r = fin ? v - h : 0.0f;
+  const float h = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+  const float r = __builtin_isinf(v) ? 0.0f : v - h;
   const float m = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-  t[0] = v != v ? __uint_as_float(b | 0x00400000u) : h;
+  t[0] = h;
   t[1] = m;
   t[2] = r - m;
 }
@@ -527,33 +526,78 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
     floatx4 gm[2];
   };
   // Rows past M repeat the last one: nothing comes of them.
-  const float* xr[MB];
+  int row_at[MB];  // the row's first byte (x is at most 2^31 of them)
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb)
-    xr[mb] = x + static_cast<long long>(min(16 * mb + r, M - 1)) * K;
-  auto load_x = [&](X& f, int u) __attribute__((always_inline)) {
-    const int k = u * kUnit + (tid >> 8) * kChunk + 8 * e8;
-    if ((u + 1) * kUnit <= K) {  // (uniform) a whole unit needs no bounds
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
-          f.v[mb][h] = *reinterpret_cast<const floatx4u*>(xr[mb] + k + 4 * h);
-        if constexpr (RMS) {
-          f.gm[h] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
-          if (gamma != nullptr) f.gm[h] = *reinterpret_cast<const floatx4u*>(gamma + k + 4 * h);
-        }
-      }
-      return;
-    }
+    row_at[mb] = static_cast<int>(4u * static_cast<unsigned>(min(16 * mb + r, M - 1)) *
+                                  static_cast<unsigned>(K));
+  // The weight rows of this wave; those past N read as zeros.
+  const long long nw = (static_cast<long long>(blockIdx.x) * kSliceWaves + wave) * (16 * NT);
+  [[maybe_unused]] const long long rows_left = std::max(std::min<long long>(N - nw, 16 * NT), 0ll);
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(x), 0,
+                                                    static_cast<int>(4u * static_cast<unsigned>(M) *
+                                                                     static_cast<unsigned>(K)),
+                                                    kRsrcWord3);
+  const auto rg = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(gamma), 0,
+                                                    gamma != nullptr ? 4 * K : 0, kRsrcWord3);
+  const auto rc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<unsigned char*>(codes + (rows_left > 0 ? nw : 0) * 16 * nb), 0,
+      static_cast<int>(rows_left * 16 * nb), kRsrcWord3);
+  const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<unsigned char*>(scales + (rows_left > 0 ? nw : 0) * nb), 0,
+      static_cast<int>(rows_left * nb), kRsrcWord3);
+#endif
+  // Unit u's loads, the same ones every time, so that the waits between them are exact;
+  // without `live` all are out of their buffers' range, and move nothing. Values past K - 4
+  // are loaded at K - 4 and moved by align_x.
+  const int k_thread = (tid >> 8) * kChunk + 8 * e8;
+  auto load_x = [&](X& f, int u, bool live) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int dead = live ? -4 : 1 << 29;  // (uniform)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      const int k = max(min(u * kUnit + k_thread + 4 * h, K - 4), dead);
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) f.v[mb][h] = load4(xr[mb], k + 4 * h, K);
+      for (int mb = 0; mb < MB; ++mb)
+        f.v[mb][h] = __builtin_bit_cast(
+            floatx4, __builtin_amdgcn_raw_buffer_load_b128(rx, row_at[mb] + 4 * k, 0, 0));
+      if constexpr (RMS)
+        f.gm[h] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rg, 4 * k, 0, 0));
+    }
+#endif
+  };
+  // A first unit that is not whole: value by value (K may be below 4).
+  auto load_x_tail = [&](X& f, int u) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = u * kUnit + k_thread + 4 * h;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+        f.v[mb][h] = load4(x + static_cast<long long>(min(16 * mb + r, M - 1)) * K, k, K);
       if constexpr (RMS) {
-        f.gm[h] = floatx4{1.0f, 1.0f, 1.0f, 1.0f};
-        if (gamma != nullptr) f.gm[h] = load4(gamma, k + 4 * h, K);
+        f.gm[h] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (gamma != nullptr) f.gm[h] = load4(gamma, k, K);
       }
+    }
+  };
+  auto align_x = [&](X& f, int u) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int past = u * kUnit + k_thread + 4 * h - (K - 4);
+      auto move = [&](floatx4& v) __attribute__((always_inline)) {
+        const floatx4 w = v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float t = past <= 0 ? w[e] : 0.0f;
+#pragma unroll
+          for (int d = 1; e + d < 4; ++d) t = past == d ? w[e + d] : t;
+          v[e] = t;
+        }
+      };
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) move(f.v[mb][h]);
+      if constexpr (RMS) move(f.gm[h]);
     }
   };
   float ss[MB];
@@ -568,7 +612,7 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
         float v = f.v[mb][e >> 2][e & 3];
         if constexpr (RMS) {
           ss[mb] = fmaf(v, v, ss[mb]);
-          v *= f.gm[e >> 2][e & 3];
+          v *= gamma != nullptr ? f.gm[e >> 2][e & 3] : 1.0f;
         }
         split3(v, t[e]);
       }
@@ -582,14 +626,25 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
                              pack_hi(t[4][p], t[5][p]), pack_hi(t[6][p], t[7][p])};
     }
   };
-  const long long n0 = (static_cast<long long>(blockIdx.x) * kSliceWaves + wave) * (16 * NT);
   Unit<NT, SV> w;
-  auto load_w = [&](int u) __attribute__((always_inline)) {
+  auto load_w = [&](int u, bool live) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int dead = live ? 0 : 1 << 27;  // (uniform) a block past any row's last
+    const int b0 = max(min(8 * u + g, nb - 1), dead);
+    const int b1 = max(min(8 * u + 4 + g, nb - 1), dead);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const long long n = std::min(n0 + 16 * t + i, N - 1);
-      w.load(t, codes + n * (16ll * nb), scales + n * nb, u, g, nb);
+      const int row = (16 * t + i) * nb;
+      w.w[0][t] = __builtin_amdgcn_raw_buffer_load_b128(rc, static_cast<int>(16u * (row + b0)), 0, 0);
+      w.w[1][t] = __builtin_amdgcn_raw_buffer_load_b128(rc, static_cast<int>(16u * (row + b1)), 0, 0);
+      if constexpr (SV) {
+        w.s[t] = __builtin_amdgcn_raw_buffer_load_b64(rs, row + max(8 * u, dead), 0, 0);
+      } else {
+        w.s[t][0] = __builtin_amdgcn_raw_buffer_load_b8(rs, row + b0, 0, 0);
+        w.s[t][1] = __builtin_amdgcn_raw_buffer_load_b8(rs, row + b1, 0, 0);
+      }
     }
+#endif
   };
   floatx4 acc[MB][NT];
 #pragma unroll
@@ -619,18 +674,21 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
   };
 
   X xv;
-  load_x(xv, u0);
+  if ((u0 + 1) * kUnit <= K) load_x(xv, u0, true);  // (uniform)
+  else load_x_tail(xv, u0);
   __builtin_amdgcn_sched_barrier(0);
-  load_w(u0);
+  load_w(u0, true);
   __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
   for (int u = u0; u < u1; ++u) {
+    if (u > u0 && (u + 1) * kUnit > K) align_x(xv, u);  // (uniform)
     put_x(xv);
     lds_barrier();
-    if (u + 1 < u1) load_x(xv, u + 1);  // (uniform)
+    load_x(xv, u + 1, u + 1 < u1);
     __builtin_amdgcn_sched_barrier(0);
     compute();
     __builtin_amdgcn_sched_barrier(0);
-    if (u + 1 < u1) load_w(u + 1);
+    load_w(u + 1, u + 1 < u1);
     __builtin_amdgcn_sched_barrier(0);
     lds_barrier();  // the fragments have been read
   }
@@ -664,7 +722,7 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
         float* dst = out + row * N;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const long long n = n0 + 16 * t + i;
+          const long long n = nw + 16 * t + i;
           if (n < N) dst[n] = acc[mb][t][v] * sc;
         }
       }
