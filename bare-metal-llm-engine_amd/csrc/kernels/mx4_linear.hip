@@ -486,10 +486,11 @@ __device__ __forceinline__ void row_scales(const float* __restrict__ part, long 
 // in three terms against 8 of a 16-row tile of weights, and with all of K in every
 // workgroup their way from L2 set the time (16 x 11008 x 4096: 114 MB, 15 us).
 // What bounds it: with a few units to a workgroup, the latencies of one pass and the
-// instructions' own way in (a third of the wave's time there); two units at a
-// time, or their weights in a second set of registers, cost more in code than they
-// hide (16 x 152064 x 4096 115 us, 138 with either; 16 x 11008 x 4096 at 256 columns
-// and 4 slices 17.1, 18.1, 17.2).
+// instructions' own way in (a third of the wave's time at 16 x 11008 x 4096, 15.1 us
+// with the reduce); with many, the sum of a unit's parts, which barriers keep from
+// overlapping within a workgroup (16 x 57344 x 8192 86 us; its weights alone 48 at a
+// large copy's rate). Weights a unit ahead in a second set of registers cost more than
+// they hide: 16 x 152064 x 4096 107 us, 115 so.
 constexpr int kSliceWaves = 8;
 
 // Where lane (i, g)'s 16 bytes of step j sit in their fragment. A read is served in
@@ -784,14 +785,14 @@ void launch_reduce(const Mx4Args& a, const float* sums, const float* squares, in
   ENG_LAUNCH_CHECK();
 }
 
-// Width (128 nt columns) and slices of K: the least estimate, in units of about half a
-// microsecond, of whole rounds of one workgroup per CU (mb + 3 nt for a unit of K, 1.5
-// beside the units) and, past one slice, the reduce launch and the sums' way out and
-// back. Fitted to every width and 1 to 32 slices at 5 to 64 rows of sixteen matrices,
-// 1024 x 4096 to 128256 x 8192: what it picks takes 0.9 % (geometric mean) more than
-// the fastest of them, 7 % at most. One width for all loses at one end: 16 x 4096 x 4096 10.2 us
-// at nt = 1, 11.0 at 2 and 11.9 at 3 (X is split more often, CUs idle), 16 x 11008 x
-// 4096 17.3, 16.8 and 15.9, 64 x 11008 x 4096 49, 36 and 31.
+// Width (128 nt columns) and slices of K: the least estimate, in microseconds or so, of
+// whole rounds of one workgroup per CU (mb + 1.7 nt for a unit of K, 1.25 beside the
+// units) and, past one slice, the reduce launch and the sums' way out and back.
+// Fitted to every width and 1 to 32 slices at 5 to 64 rows of eighteen matrices, 1024 x
+// 4096 to 128256 x 8192: what it picks takes 0.4 % (geometric mean) more than the
+// fastest of them, 7 % at most. One width for all loses at one end: 16 x 4096 x 4096
+// 9.9, 11.1 and 12.2 us at its best slices with nt = 1, 2 and 3 (X is split more often,
+// CUs idle), 64 x 11008 x 4096 38, 34 and 30.
 void slice_shape(const Mx4Args& a, int mb, int& nt, int& slices) {
   const long long cus = device_cu_count();
   const long long units = (a.K + kUnit - 1) / kUnit;
@@ -801,8 +802,8 @@ void slice_shape(const Mx4Args& a, int mb, int& nt, int& slices) {
     const long long groups = (a.N + 128 * cand - 1) / (128 * cand);
     for (long long s = 1; s <= std::min(units, 32ll); ++s) {
       double time = static_cast<double>((groups * s + cus - 1) / cus) *
-                    (static_cast<double>((units + s - 1) / s * (mb + 3 * cand)) + 1.5);
-      if (s > 1) time += 2.0 + 0.13 * static_cast<double>(s) + 1.8e-6 * static_cast<double>(s * a.M * a.N);
+                    (static_cast<double>((units + s - 1) / s) * (mb + 1.7 * cand) + 1.25);
+      if (s > 1) time += 0.5 + 0.25 * static_cast<double>(s) + 1.7e-6 * static_cast<double>(s * a.M * a.N);
       if (nt == 0 || time < best) best = time, nt = cand, slices = static_cast<int>(s);
     }
   }
