@@ -162,7 +162,7 @@ template <int MR, bool RMS, bool SV>
 __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
     const float* __restrict__ x, const float* __restrict__ gamma,
     const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-    float* __restrict__ y, long long N, int K, int nb, float eps) {
+    float* __restrict__ y, long long N, int K, int nb, int tiles_each, unsigned more, float eps) {
   constexpr int THREADS = 64 * kDecodeWaves;
   constexpr int PX = MR == 1 ? 3 : MR == 2 ? 2 : 1;  // X loads ahead of the weights'
   constexpr int P = 2;                               // units of weights in flight
@@ -181,8 +181,8 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
   const int staged = units * kUnit;  // whole units: zeros past K
   const int u0 = units * wave / kDecodeWaves;
   const int u1 = units * (wave + 1) / kDecodeWaves;
-  const long long tiles = (N + 15) / 16;
-  const int mine = static_cast<int>((tiles - blockIdx.x + gridDim.x - 1) / gridDim.x);
+  // its tiles: `tiles_each`, and one more for the first `more` workgroups
+  const int mine = tiles_each + (blockIdx.x < more ? 1 : 0);
 
   struct X {
     floatx4 v[MR];
@@ -364,7 +364,8 @@ void run_decode(const Mx4Args& a, hipStream_t stream) {
     static std::atomic<bool> done[64];
     allow_staged_lds(reinterpret_cast<const void*>(mx4_decode_kernel<MR, R, SV>), done, lds);
     mx4_decode_kernel<MR, R, SV><<<grid, 64 * kDecodeWaves, lds, stream>>>(
-        a.x, a.gamma, a.codes, a.scales, a.y, a.N, K, nb, a.eps);
+        a.x, a.gamma, a.codes, a.scales, a.y, a.N, K, nb, static_cast<int>(tiles / wgs),
+        static_cast<unsigned>(tiles % wgs), a.eps);
   };
   with_flags(a.rms, scales_by_8(a), go);
   ENG_LAUNCH_CHECK();
@@ -515,8 +516,8 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
   const int units = (K + kUnit - 1) / kUnit;
   const int slices = gridDim.y;
   const int slice = blockIdx.y;
-  const int u0 = static_cast<int>(static_cast<long long>(units) * slice / slices);
-  const int u1 = static_cast<int>(static_cast<long long>(units) * (slice + 1) / slices);
+  const int u0 = units * slice / slices;  // (units <= 2^15, slices <= 32)
+  const int u1 = units * (slice + 1) / slices;
 
   // X: a thread splits values 8 e8 .. + 7 of chunk tid / 256 of the unit, of rows
   // 16 mb + r.
@@ -886,16 +887,17 @@ __global__ __launch_bounds__(64 * kGemmBlocks, 2) void mx4_gemm_kernel(
   const int g = lane >> 4;
   const int wm = wave >> 2;
   const int wn = wave & 3;
-  const long long logical = gemv::xcd_contiguous(blockIdx.x, gridDim.x);
-  const int tm = static_cast<int>(logical % tiles_m);
-  const long long n0 = (logical / tiles_m) * (64 * NT);
+  const unsigned logical = static_cast<unsigned>(gemv::xcd_contiguous(blockIdx.x, gridDim.x));
+  const unsigned tn = logical / static_cast<unsigned>(tiles_m);
+  const int tm = static_cast<int>(logical - tn * static_cast<unsigned>(tiles_m));
+  const long long n0 = static_cast<long long>(tn) * (64 * NT);
   const long long m0 = 16ll * BMB * tm;
   const int chunks = (K + kChunk - 1) / kChunk;
 
   // This slice's chunks. One slice writes scaled rows of y, several their sums.
   const int slices = gridDim.y;
-  const int cb = static_cast<int>(static_cast<long long>(chunks) * blockIdx.y / slices);
-  const int ce = static_cast<int>(static_cast<long long>(chunks) * (blockIdx.y + 1) / slices);
+  const int cb = chunks * static_cast<int>(blockIdx.y) / slices;  // (chunks <= 2^16, slices <= 16)
+  const int ce = chunks * (static_cast<int>(blockIdx.y) + 1) / slices;
   const bool scaled = RMS && slices == 1;  // (uniform)
   if (scaled) row_scales<16 * BMB, 64 * BMB>(part, m0, M, K, chunks, eps, row_scale);
 
