@@ -512,7 +512,8 @@ __global__ __launch_bounds__(64) void merge_q8_kernel(const float* __restrict__ 
   constexpr int DPL = D / 64;
   const int lane = threadIdx.x;
   const long long h = blockIdx.x;
-  const int len = static_cast<int>(std::min<long long>(max(lens[h / n_heads], 0), max_len));
+  const unsigned b = blockIdx.x / static_cast<unsigned>(n_heads);
+  const int len = static_cast<int>(std::min<long long>(max(lens[b], 0), max_len));
   const int blocks = (len + kKvBlock - 1) / kKvBlock;
   const int ns = (blocks + split_blocks - 1) / split_blocks;
   const long long base = h * nsplit;

@@ -9,7 +9,7 @@ import pytest
 
 import helpers
 import narrow
-from test_gpu_kv_q8 import Cache, check_attend, rows
+from test_gpu_kv_q8 import Cache, attend, check_attend, rows
 from test_gpu_mx4 import EPS, check_linear, linear, weights
 
 pytestmark = pytest.mark.gpu
@@ -91,6 +91,23 @@ def test_many_sequences(gpu):
     lens[rng.integers(0, B, 20)] = 0
     check_attend(gpu, c, q, lens, L)
     check_attend(gpu, c, q, lens, L, split=3)
+
+
+def test_splits_that_a_sequence_does_not_reach(gpu):
+    """The merge reads the scratch of splits past a sequence's end, whatever an earlier
+    call left there: NaN and infinities (of q), then lengths that leave splits, or all of
+    them, unused."""
+    rng = np.random.default_rng(9)
+    B, H, G, D, L = 5, 8, 2, 128, 640
+    c = Cache(gpu, rng, B, G, L, D)
+    c.write(rows(rng, B, L, G, D), rows(rng, B, L, G, D), np.zeros(B, int), None)
+    q = rng.standard_normal((B, H, D)).astype(np.float16)
+    for split in (0, 4, 12, 20):
+        bad = q.copy()
+        bad[:, ::2] = np.nan
+        bad[:, 1::2, 3] = np.inf
+        attend(gpu, c, bad, np.full(B, L), L, 0.1, split)
+        check_attend(gpu, c, q, np.array([0, 1, 33, 320, 640]), L, split=split)
 
 
 def test_rmsnorm_of_zero_and_of_large_rows(gpu):
