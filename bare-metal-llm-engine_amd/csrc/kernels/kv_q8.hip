@@ -53,7 +53,9 @@ __device__ __forceinline__ unsigned fp8x4(float a, float b, float c, float d) {
 // fp16's smallest steps), and no less than the scale of earlier tokens kept in
 // the block; if it grows, their codes are brought to it. Tokens at or past
 // kv_max_seq_len are dropped. Blocks belong to one wave each: no atomics.
-// Bound by the bytes of the new rows and their codes.
+// Bound by the bytes of the new rows and their codes, and for a token each by the round
+// trips of position, old codes and scale (4 prompts of up to 1000 tokens, 8 heads of 128:
+// 6.8 us; one token each of 32 sequences of 32 heads 4.6).
 template <int D>
 __global__ __launch_bounds__(kWriteThreads) void kv_write_q8_kernel(
     const _Float16* __restrict__ k_new, const _Float16* __restrict__ v_new,
@@ -500,7 +502,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 3 : 1) void decode_q8_kernel(Att
 // sequence's length reaches: one wave per (sequence, head), in split order. Lane s
 // holds state s's (m, l), every lane its D / 64 dims of all states, C states at a
 // time and their loads issued together, so up to C splits cost one round trip;
-// the weight of state s is read from lane s.
+// the weight of state s is read from lane s. Bound by the round trips of length and
+// states: 2.9 us at 32 heads and 16 splits.
 template <int D, int C>
 __global__ __launch_bounds__(64) void merge_q8_kernel(const float* __restrict__ part_o,
                                                       const float* __restrict__ part_ml,
@@ -562,8 +565,7 @@ __global__ __launch_bounds__(64) void merge_q8_kernel(const float* __restrict__ 
 // slower), at least four blocks per split, one per wave, past 32 blocks, and one
 // split, without the merge's launch, up to 12 blocks at D = 128 or 24 at D = 64
 // (300 tokens, 32 / 4 heads of 64 5.3 us, 6.5 in 8 splits; 600 tokens, 32 / 8 heads
-// of 128 7.8 us, 7.1 in 16). A
-// sweep of 1 to 64 splits over 18 shapes put it at the best count or within 6%:
+// of 128 7.8 us, 7.1 in 16). A sweep of 1 to 64 splits over 18 shapes put it at the best count or within 6%:
 // 32 / 32 heads, D = 128, 8192 tokens 8 splits 15.4 us (16: 16.7, 4: 18.1); 32 / 8
 // heads, 131072 tokens 32 splits 46 us (16: 59, 64: 49); 32 sequences of 32 / 8
 // heads, 4096 tokens 1 split 43 us (2: 47.5, 8: 54.6); 1000 tokens, 32 / 8 heads 32

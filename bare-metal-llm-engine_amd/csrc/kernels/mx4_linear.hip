@@ -144,10 +144,10 @@ struct Unit {
 // output comes from them). Terms sit 16 bytes apart modulo the banks' 256, so the
 // reads of a step (3 MR rows x 4 groups) spread over the banks.
 // Bound by the weights' bytes once they are many (1 x 152064 x 4096, 331 MB: 59 us,
-// 5.6 TB/s; 1 x 11008 x 4096, 24 MB: 8.8 us), below that by the latencies of one pass
-// (X, its split, one unit of weights, the sum: 4.2 us at 1 x 2051 x 1023). Two units in
-// flight: three or four make the last ones, which nothing needs, cost more (1 x 4096 x
-// 4096 5.2 us, 5.8 and 6.2).
+// 5.6 TB/s; 1 x 11008 x 4096, 24 MB: 7.7 us), below that by the latencies of one pass
+// (X, its split, one unit of weights, the sum: 4.0 us at 1 x 2051 x 1023). Two units in
+// flight: with three or four the last ones, which nothing needs, cost more (1 x 4096 x
+// 4096, 4.4 us, 0.6 and 1.0 us).
 constexpr int kDecodeWaves = 16;
 constexpr int kDecodeLds = 120 * 1024;
 constexpr int kDecodeTiles = 48;  // most tiles of a workgroup
@@ -378,7 +378,8 @@ void run_decode(const Mx4Args& a, hipStream_t stream) {
 // eight k of step j in its group's 32-block), fragments [M / 16][chunk][step j][term].
 // A wave's load of a fragment is then 1 KiB in one piece, and one of X as it stands 64
 // pieces of 16 bytes. Rows past M and k past K are zeros. Beside them the sums of
-// squares of each row's chunks.
+// squares of each row's chunks. Bound by its bytes and one round trip (512 x 4096, 21
+// MB: 7.8 us).
 template <bool RMS>
 __global__ __launch_bounds__(256) void mx4_planes_kernel(const float* __restrict__ x,
                                                          const float* __restrict__ gamma,
@@ -733,7 +734,8 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
 }
 
 // y[m][n] = s_m times the sum over the slices, in their order. blockIdx.y: a row, whose
-// sum of squares is in `parts` parts.
+// sum of squares is in `parts` parts. The sums are read from L2 mostly; what it costs is a
+// launch and two round trips (16 x 11008, 8 slices, 6.3 MB: 4 us).
 template <bool RMS>
 __global__ __launch_bounds__(256) void mx4_slice_reduce_kernel(const float* __restrict__ sums,
                                                                const float* __restrict__ squares,
@@ -855,7 +857,7 @@ void launch_slices(const Mx4Args& a, hipStream_t stream) {
 // weights of a chunk come straight into registers a chunk ahead (4-bit: 16 NT bytes a
 // lane and chunk) and are converted as their step begins. Tiles with K split among
 // gridDim.y slices leave their sums for mx4_slice_reduce_kernel.
-// Bound by the matrix cores: 2048 x 4096 x 4096 196 us with the planes' pass, 1051
+// Bound by the matrix cores: 2048 x 4096 x 4096 192 us with the planes' pass, 1073
 // TFLOP/s of bf16 products (three per weight), where a plain bf16 product of 8192^3
 // runs at 1198 through the library on the same card.
 constexpr int kGemmBlocks = 8;  // m-blocks of a tile, and waves
