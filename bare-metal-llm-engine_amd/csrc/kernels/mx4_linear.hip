@@ -733,10 +733,11 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
   }
 }
 
-// y[m][n] = s_m times the sum over the slices, in their order. blockIdx.y: a row, whose
-// sum of squares is in `parts` parts. The sums are read from L2 mostly; what it costs is a
-// launch and two round trips (16 x 11008, 8 slices, 6.3 MB: 4 us).
-template <bool RMS>
+// y[m][n] = s_m times the sum over the slices, in their order, C of them loaded
+// together (past the last one, the last one again) and the row's sums of squares, in
+// `parts` parts, beside them. blockIdx.y: a row. The sums are in L2 mostly; what it
+// costs is a launch and one round trip (16 x 11008, 8 slices, 6.3 MB: 3.9 us).
+template <int C, bool RMS>
 __global__ __launch_bounds__(256) void mx4_slice_reduce_kernel(const float* __restrict__ sums,
                                                                const float* __restrict__ squares,
                                                                float* __restrict__ y, long long M,
@@ -744,33 +745,39 @@ __global__ __launch_bounds__(256) void mx4_slice_reduce_kernel(const float* __re
                                                                int parts, float eps) {
   const long long row = blockIdx.y;
   const long long stride = M * N;
-  float sc = 1.0f;
-  if constexpr (RMS) {
-    float t = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < parts; ++s) t += squares[row * parts + s];
-    sc = 1.0f / sqrtf(t / static_cast<float>(K) + eps);
-  }
-  const long long n = 4 * (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x);
-  if (n >= N) return;
+  // four columns a thread; the last ones of a row whose N is no multiple of four overlap
+  // their neighbour's, and both write the same bits
+  const long long n4 = 4 * (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x);
+  const bool whole = n4 < N && N >= 4;
+  const long long n = whole ? std::min(n4, N - 4) : 0;
   const float* p = sums + row * N + n;
-  float* out = y + row * N + n;
-  if (n + 4 <= N) {
-    floatx4 v = *reinterpret_cast<const floatx4u*>(p);
-#pragma unroll 4
-    for (int s = 1; s < slices; ++s) {
-      const floatx4 a = *reinterpret_cast<const floatx4u*>(p + s * stride);
+  float t = 0.0f;
+  if constexpr (RMS)
+    for (int q = threadIdx.x & 63; q < parts; q += 64) t += squares[row * parts + q];
+  floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (whole) {
+    for (int s0 = 0; s0 < slices; s0 += C) {
+      floatx4 a[C];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += a[e];
+      for (int s = 0; s < C; ++s)
+        a[s] = *reinterpret_cast<const floatx4u*>(p + min(s0 + s, slices - 1) * stride);
+#pragma unroll
+      for (int s = 0; s < C; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = s0 + s < slices ? v[e] + a[s][e] : v[e];
     }
+  }
+  const float sc = RMS ? 1.0f / sqrtf(gemv::wave_sum(t) / static_cast<float>(K) + eps) : 1.0f;
+  float* out = y + row * N;
+  if (whole) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= sc;
-    *reinterpret_cast<floatx4u*>(out) = v;
-  } else {
-    for (int e = 0; e < N - n; ++e) {
-      float v = p[e];
-      for (int s = 1; s < slices; ++s) v += p[s * stride + e];
-      out[e] = v * sc;
+    *reinterpret_cast<floatx4u*>(out + n) = v;
+  } else if (n4 < N) {
+    for (int c = 0; c < N; ++c) {
+      float u = 0.0f;
+      for (int s = 0; s < slices; ++s) u += p[s * stride + c];
+      out[c] = u * sc;
     }
   }
 }
@@ -783,8 +790,13 @@ void launch_reduce(const Mx4Args& a, const float* sums, const float* squares, in
     kernel<<<grid, 256, 0, stream>>>(sums, squares, a.y, a.M, a.N, static_cast<int>(a.K), slices, parts,
                                      a.eps);
   };
-  if (a.rms) go(mx4_slice_reduce_kernel<true>);
-  else go(mx4_slice_reduce_kernel<false>);
+  if (slices <= 4) {
+    if (a.rms) go(mx4_slice_reduce_kernel<4, true>);
+    else go(mx4_slice_reduce_kernel<4, false>);
+  } else {
+    if (a.rms) go(mx4_slice_reduce_kernel<8, true>);
+    else go(mx4_slice_reduce_kernel<8, false>);
+  }
   ENG_LAUNCH_CHECK();
 }
 
