@@ -69,17 +69,31 @@ __device__ __forceinline__ void split3(float v, float (&t)[3]) {
   t[2] = r - m;
 }
 
+// v, loaded at K - 4 where its own place lies past it, as the values at k = K - 4 + past
+// on: zeros from K on.
+__device__ __forceinline__ floatx4 aligned4(const floatx4& v, int past) {
+  floatx4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float t = past <= 0 ? v[e] : 0.0f;
+#pragma unroll
+    for (int d = 1; e + d < 4; ++d) t = past == d ? v[e + d] : t;
+    r[e] = t;
+  }
+  return r;
+}
+
 // Four values of a row of K at k, zeros from K on.
 __device__ __forceinline__ floatx4 load4(const float* __restrict__ row, int k, int K) {
-  floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (k + 4 <= K) {
-    v = *reinterpret_cast<const floatx4u*>(row + k);
-  } else {
+  if (K < 4) {  // (uniform)
+    floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < 3; ++e)
       if (k + e < K) v[e] = row[k + e];
+    return v;
   }
-  return v;
+  const floatx4 v = *reinterpret_cast<const floatx4u*>(row + min(k, K - 4));
+  return k <= K - 4 ? v : aligned4(v, k - (K - 4));
 }
 
 // The eight bf16 weights of one code word.
@@ -570,8 +584,8 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
     }
 #endif
   };
-  // A first unit that is not whole: value by value (K may be below 4).
-  auto load_x_tail = [&](X& f, int u) __attribute__((always_inline)) {
+  // K below 4: value by value.
+  auto load_x_short = [&](X& f, int u) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = u * kUnit + k_thread + 4 * h;
@@ -588,19 +602,9 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int past = u * kUnit + k_thread + 4 * h - (K - 4);
-      auto move = [&](floatx4& v) __attribute__((always_inline)) {
-        const floatx4 w = v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float t = past <= 0 ? w[e] : 0.0f;
-#pragma unroll
-          for (int d = 1; e + d < 4; ++d) t = past == d ? w[e + d] : t;
-          v[e] = t;
-        }
-      };
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) move(f.v[mb][h]);
-      if constexpr (RMS) move(f.gm[h]);
+      for (int mb = 0; mb < MB; ++mb) f.v[mb][h] = aligned4(f.v[mb][h], past);
+      if constexpr (RMS) f.gm[h] = aligned4(f.gm[h], past);
     }
   };
   float ss[MB];
@@ -677,14 +681,14 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
   };
 
   X xv;
-  if ((u0 + 1) * kUnit <= K) load_x(xv, u0, true);  // (uniform)
-  else load_x_tail(xv, u0);
+  if (K >= 4) load_x(xv, u0, true);  // (uniform)
+  else load_x_short(xv, u0);
   __builtin_amdgcn_sched_barrier(0);
   load_w(u0, true);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll 1
   for (int u = u0; u < u1; ++u) {
-    if (u > u0 && (u + 1) * kUnit > K) align_x(xv, u);  // (uniform)
+    if ((u + 1) * kUnit > K && K >= 4) align_x(xv, u);  // (uniform)
     put_x(xv);
     lds_barrier();
     load_x(xv, u + 1, u + 1 < u1);

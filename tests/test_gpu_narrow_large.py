@@ -32,6 +32,35 @@ def test_linear_launch_shapes(gpu, M, N, K, rms):
     check_linear(gpu, np.random.default_rng(M + N + K), M, N, K, rms)
 
 
+@pytest.mark.parametrize("M", [1, 4, 5, 20, 50, 70])
+@pytest.mark.parametrize("K", [2, 3, 4, 5, 6, 7, 127, 255, 256, 257, 258, 259, 511, 513])
+def test_linear_ends_of_rows(gpu, M, K):
+    """The last values of a row of X, every way it can end inside four values and a
+    unit, with infinities behind the end (the next row's, and gamma's)."""
+    rng = np.random.default_rng(1000 * M + K)
+    N = 45
+    x = rng.standard_normal((M + 1, K)).astype(np.float32)
+    x[M] = np.inf
+    g = np.append(1 + 0.1 * rng.standard_normal(K), [np.inf] * 8).astype(np.float32)
+    codes, scales = weights(rng, N, K)
+    dx, dg, dc, ds = (gpu.upload(a) for a in (x, g, codes, scales))
+    for rms in (False, True):
+        y = gpu.empty((M, N), np.float32)
+        if rms:
+            gpu.call("eng_rmsnorm_linear_mx4w_nk", dx.ptr, dg.ptr, dc.ptr, ds.ptr, y.ptr, M, N, K, EPS, None)
+        else:
+            gpu.call("eng_linear_mx4w_nk", dx.ptr, dc.ptr, ds.ptr, y.ptr, M, N, K, None)
+        gpu.sync()
+        want, a = narrow.linear64(x[:M], narrow.mx4_decode(codes, scales, K), g[:K] if rms else None,
+                                  EPS if rms else None)
+        helpers.assert_within(y.download(), want, narrow.linear_bound(want, a, K, rms), f"{M} x {K}")
+
+
+@pytest.mark.parametrize("M,N,K", [(6, 33000, 257), (12, 33000, 259), (40, 50000, 258), (8, 90000, 515)])
+def test_linear_ends_of_rows_after_whole_units(gpu, M, N, K):
+    check_linear(gpu, np.random.default_rng(K), M, N, K, True)
+
+
 def test_linear_passes_of_rows_agree_with_single_calls(gpu):
     """Rows on both sides of a pass's end equal the same rows in a call of their own
     size class, within the bound (the order of the sums may differ)."""
