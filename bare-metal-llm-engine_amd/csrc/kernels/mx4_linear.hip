@@ -149,8 +149,10 @@ struct Unit {
 // ---------------------------------------------------------------- 1 to 4 rows
 //
 // One workgroup of 16 waves per CU. X is split into LDS once (MR rows x 3 terms x K);
-// then the workgroup goes through its tiles of 16 weight rows, p, p + G, ..., the
-// waves splitting K by units. A wave's weights come P units ahead, across the
+// then the workgroup goes through its share of the weight rows, equal to within one row, in
+// tiles of 16, the waves splitting K by units (whole tiles dealt out in turn left some CUs
+// half a tile more: 1 x 11008 x 4096 7.7 us, 1 x 6144 x 4096 6.0 against 5.5). A wave's
+// weights come P units ahead, across the
 // tiles, so the stream does not stop where a tile ends: there the waves leave their
 // sums in LDS (two buffers in turn, one barrier a tile that waits for no load) and
 // one wave, another for each tile, adds and writes them. Rows 4 m + p of the A
@@ -158,7 +160,7 @@ struct Unit {
 // output comes from them). Terms sit 16 bytes apart modulo the banks' 256, so the
 // reads of a step (3 MR rows x 4 groups) spread over the banks.
 // Bound by the weights' bytes once they are many (1 x 152064 x 4096, 331 MB: 59 us,
-// 5.6 TB/s; 1 x 11008 x 4096, 24 MB: 7.7 us), below that by the latencies of one pass
+// 5.6 TB/s; 1 x 11008 x 4096, 24 MB: 7.4 us), below that by the latencies of one pass
 // (X, its split, one unit of weights, the sum: 4.0 us at 1 x 2051 x 1023). Two units in
 // flight: with three or four the last ones, which nothing needs, cost more (1 x 4096 x
 // 4096, 4.4 us, 0.6 and 1.0 us).
@@ -176,7 +178,7 @@ template <int MR, bool RMS, bool SV>
 __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
     const float* __restrict__ x, const float* __restrict__ gamma,
     const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
-    float* __restrict__ y, long long N, int K, int nb, int tiles_each, unsigned more, float eps) {
+    float* __restrict__ y, long long N, int K, int nb, int rows_each, unsigned more, float eps) {
   constexpr int THREADS = 64 * kDecodeWaves;
   constexpr int PX = MR == 1 ? 3 : MR == 2 ? 2 : 1;  // X loads ahead of the weights'
   constexpr int P = 2;                               // units of weights in flight
@@ -195,8 +197,10 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
   const int staged = units * kUnit;  // whole units: zeros past K
   const int u0 = units * wave / kDecodeWaves;
   const int u1 = units * (wave + 1) / kDecodeWaves;
-  // its tiles: `tiles_each`, and one more for the first `more` workgroups
-  const int mine = tiles_each + (blockIdx.x < more ? 1 : 0);
+  // its rows of W: `rows_each`, and one more for the first `more` workgroups
+  const int rows = rows_each + (blockIdx.x < more ? 1 : 0);
+  const long long first = static_cast<long long>(blockIdx.x) * rows_each + std::min(blockIdx.x, more);
+  const int mine = (rows + 15) / 16;
 
   struct X {
     floatx4 v[MR];
@@ -247,8 +251,7 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
   const unsigned char* crow;
   const unsigned char* srow;
   auto seek = [&] {
-    const long long t = blockIdx.x + static_cast<long long>(ft) * gridDim.x;
-    const long long n = ft < mine ? std::min(16 * t + i, N - 1) : 0;
+    const long long n = ft < mine ? first + min(16 * ft + i, rows - 1) : 0;
     crow = codes + n * (16ll * nb);
     srow = scales + n * nb;
   };
@@ -343,8 +346,8 @@ __global__ __launch_bounds__(64 * kDecodeWaves) void mx4_decode_kernel(
   for (int q = tid; q < 16 * MR * mine; q += THREADS) {
     const int t = q / (16 * MR);
     const int m = q / 16 % MR;
-    const long long n = 16 * (blockIdx.x + static_cast<long long>(t) * gridDim.x) + q % 16;
-    if (n < N) y[m * N + n] = out[t][m][q % 16];
+    const int n = 16 * t + q % 16;
+    if (n < rows) y[m * N + first + n] = out[t][m][q % 16];
   }
 }
 
@@ -378,8 +381,8 @@ void run_decode(const Mx4Args& a, hipStream_t stream) {
     static std::atomic<bool> done[64];
     allow_staged_lds(reinterpret_cast<const void*>(mx4_decode_kernel<MR, R, SV>), done, lds);
     mx4_decode_kernel<MR, R, SV><<<grid, 64 * kDecodeWaves, lds, stream>>>(
-        a.x, a.gamma, a.codes, a.scales, a.y, a.N, K, nb, static_cast<int>(tiles / wgs),
-        static_cast<unsigned>(tiles % wgs), a.eps);
+        a.x, a.gamma, a.codes, a.scales, a.y, a.N, K, nb, static_cast<int>(a.N / wgs),
+        static_cast<unsigned>(a.N % wgs), a.eps);
   };
   with_flags(a.rms, scales_by_8(a), go);
   ENG_LAUNCH_CHECK();
