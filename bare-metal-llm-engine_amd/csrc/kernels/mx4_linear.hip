@@ -152,8 +152,7 @@ struct Unit {
 // then the workgroup goes through its share of the weight rows, equal to within one row, in
 // tiles of 16, the waves splitting K by units (whole tiles dealt out in turn left some CUs
 // half a tile more: 1 x 11008 x 4096 7.7 us, 1 x 6144 x 4096 6.0 against 5.5). A wave's
-// weights come P units ahead, across the
-// tiles, so the stream does not stop where a tile ends: there the waves leave their
+// weights come P units ahead, across the tiles, so the stream does not stop where a tile ends: there the waves leave their
 // sums in LDS (two buffers in turn, one barrier a tile that waits for no load) and
 // one wave, another for each tile, adds and writes them. Rows 4 m + p of the A
 // operand are term p of row m; rows that are no term's read some other term (no
@@ -505,11 +504,11 @@ __device__ __forceinline__ void row_scales(const float* __restrict__ part, long 
 // in three terms against 8 of a 16-row tile of weights, and with all of K in every
 // workgroup their way from L2 set the time (16 x 11008 x 4096: 114 MB, 15 us).
 // What bounds it: with a few units to a workgroup, the latencies of one pass and the
-// instructions' own way in (a third of the wave's time at 16 x 11008 x 4096, 15.1 us
+// instructions' own way in (a third of the wave's time at 16 x 11008 x 4096, 13.8 us
 // with the reduce); with many, the sum of a unit's parts, which barriers keep from
-// overlapping within a workgroup (16 x 57344 x 8192 86 us; its weights alone 48 at a
+// overlapping within a workgroup (16 x 57344 x 8192 83 us; its weights alone 48 at a
 // large copy's rate). Weights a unit ahead in a second set of registers cost more than
-// they hide: 16 x 152064 x 4096 107 us, 115 so.
+// they hide: 16 x 152064 x 4096 105 us, 115 so.
 constexpr int kSliceWaves = 8;
 
 // Where lane (i, g)'s 16 bytes of step j sit in their fragment. A read is served in
@@ -876,9 +875,10 @@ void launch_slices(const Mx4Args& a, hipStream_t stream) {
 // weights of a chunk come straight into registers a chunk ahead (4-bit: 16 NT bytes a
 // lane and chunk) and are converted as their step begins. Tiles with K split among
 // gridDim.y slices leave their sums for mx4_slice_reduce_kernel.
-// Bound by the matrix cores: 2048 x 4096 x 4096 192 us with the planes' pass, 1073
-// TFLOP/s of bf16 products (three per weight), where a plain bf16 product of 8192^3
-// runs at 1198 through the library on the same card.
+// Bound by the matrix cores and the LDS beside them: 2048 x 4096 x 4096 189 us with the
+// planes' pass, 1090 TFLOP/s of bf16 products (three per weight), where a plain bf16
+// product of 8192^3 runs at 1198 through the library on the same card. Waves of 32 rows by
+// 32 NT columns, with half the LDS reads and twice the conversions, take 226 us.
 constexpr int kGemmBlocks = 8;  // m-blocks of a tile, and waves
 
 template <int NT, bool RMS>
