@@ -545,11 +545,10 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
     floatx4 gm[2];
   };
   // Rows past M repeat the last one: nothing comes of them.
-  int row_at[MB];  // the row's first byte (x is at most 2^31 of them)
+  unsigned row_at[MB];  // the row's first byte (x is at most 2^31 of them)
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb)
-    row_at[mb] = static_cast<int>(4u * static_cast<unsigned>(min(16 * mb + r, M - 1)) *
-                                  static_cast<unsigned>(K));
+    row_at[mb] = 4u * static_cast<unsigned>(min(16 * mb + r, M - 1)) * static_cast<unsigned>(K);
   // The weight rows of this wave; those past N read as zeros.
   const long long nw = (static_cast<long long>(blockIdx.x) * kSliceWaves + wave) * (16 * NT);
   [[maybe_unused]] const long long rows_left = std::max(std::min<long long>(N - nw, 16 * NT), 0ll);
@@ -573,16 +572,17 @@ __global__ __launch_bounds__(64 * kSliceWaves, 2) void mx4_slice_kernel(
   const int k_thread = (tid >> 8) * kChunk + 8 * e8;
   auto load_x = [&](X& f, int u, bool live) __attribute__((always_inline)) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int dead = live ? -4 : 1 << 29;  // (uniform)
+    const int dead = live ? 0 : 1 << 29;  // (uniform) 2^31 bytes on
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int k = max(min(u * kUnit + k_thread + 4 * h, K - 4), dead);
+      const unsigned at = 4u * static_cast<unsigned>(max(min(u * kUnit + k_thread + 4 * h, K - 4), dead));
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb)
         f.v[mb][h] = __builtin_bit_cast(
-            floatx4, __builtin_amdgcn_raw_buffer_load_b128(rx, row_at[mb] + 4 * k, 0, 0));
+            floatx4, __builtin_amdgcn_raw_buffer_load_b128(rx, static_cast<int>(row_at[mb] + at), 0, 0));
       if constexpr (RMS)
-        f.gm[h] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rg, 4 * k, 0, 0));
+        f.gm[h] = __builtin_bit_cast(
+            floatx4, __builtin_amdgcn_raw_buffer_load_b128(rg, static_cast<int>(at), 0, 0));
     }
 #endif
   };
@@ -942,7 +942,7 @@ __global__ __launch_bounds__(64 * kGemmBlocks, 2) void mx4_gemm_kernel(
   [[maybe_unused]] const int steps = 4 * ce;
   auto fetch_a = [&](unsigned short* dst, int step) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int so = min(step, steps - 1) * 3072;
+    const int so = min(step, steps - 1) * (3 * 1024);
     unsigned short* d = dst + wave * (3 * 512);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, d, 16, lane * 16, so, 0, 0);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, d + 512, 16, lane * 16, so + 1024, 0, 0);

@@ -61,6 +61,11 @@ def test_linear_ends_of_rows_after_whole_units(gpu, M, N, K):
     check_linear(gpu, np.random.default_rng(K), M, N, K, True)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 5, 1 << 23), (6, 3, 1 << 23), (20, 2, (1 << 23) - 5)])
+def test_linear_longest_rows(gpu, M, N, K):
+    check_linear(gpu, np.random.default_rng(M), M, N, K, M > 1)
+
+
 def test_linear_passes_of_rows_agree_with_single_calls(gpu):
     """Rows on both sides of a pass's end equal the same rows in a call of their own
     size class, within the bound (the order of the sums may differ)."""
