@@ -22,6 +22,7 @@ typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
 typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
@@ -45,6 +46,20 @@ __device__ __forceinline__ unsigned fp8x4(float a, float b, float c, float d) {
   return static_cast<unsigned>(w);
 }
 
+// The largest of the wave's values, none negative, in every lane.
+template <int CTRL>
+__device__ __forceinline__ int dpp_max(int x) {
+  return max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ int wave_max(int x) {
+  x = dpp_max<0xB1>(x);   // quad_perm [1, 0, 3, 2]
+  x = dpp_max<0x4E>(x);   // quad_perm [2, 3, 0, 1]
+  x = dpp_max<0x141>(x);  // row_half_mirror
+  x = dpp_max<0x140>(x);  // row_mirror
+  return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+             max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+}
+
 // One wave per (K or V, sequence, head, block of 32 tokens). A lane holds 8
 // consecutive dims of a token (16 bytes of the new rows, 8 of the cache), so a
 // wave load covers 64 / (D / 8) tokens and the block's new rows are in flight
@@ -54,8 +69,8 @@ __device__ __forceinline__ unsigned fp8x4(float a, float b, float c, float d) {
 // the block; if it grows, their codes are brought to it. Tokens at or past
 // kv_max_seq_len are dropped. Blocks belong to one wave each: no atomics.
 // Bound by the bytes of the new rows and their codes, and for a token each by the round
-// trips of position, old codes and scale (4 prompts of up to 1000 tokens, 8 heads of 128:
-// 6.8 us; one token each of 32 sequences of 32 heads 4.6).
+// trips of position, then new rows, old codes and scale together (4 prompts of up to 1000
+// tokens, 8 heads of 128: 5.6 us; one token each of 32 sequences of 32 heads 4.0).
 template <int D>
 __global__ __launch_bounds__(kWriteThreads) void kv_write_q8_kernel(
     const _Float16* __restrict__ k_new, const _Float16* __restrict__ v_new,
@@ -91,27 +106,46 @@ __global__ __launch_bounds__(kWriteThreads) void kv_write_q8_kernel(
   unsigned char* dst = (is_v ? v_cache : k_cache) + ((b * n_kv_heads + h) * kv_max + first) * D + d0;
   float* sp = (is_v ? v_scale : k_scale) + (b * n_kv_heads + h) * ((kv_max + kKvBlock - 1) / kKvBlock) + blk;
 
+  // Lanes without a new token (or an old one) take the nearest: no branches between the
+  // loads, and the maximum does not change.
   halfx8 x[LOADS];
 #pragma unroll
-  for (int r = 0; r < LOADS; ++r) {
-    const long long t = first + r * TPL + sub;
-    x[r] = halfx8{};
-    if (t >= lo && t < hi) x[r] = *reinterpret_cast<const halfx8*>(src + t * n_kv_heads * D);
-  }
+  for (int r = 0; r < LOADS; ++r)
+    x[r] = *reinterpret_cast<const halfx8*>(
+        src + std::min(std::max(first + r * TPL + sub, lo), hi - 1) * n_kv_heads * D);
   const bool kept = lo > first;
-  const float s_old = kept ? *sp : 0.0f;
-  int top = 0;
+  float s_old = 0.0f;
+  uintx2 old[LOADS];
+  if (kept) {  // (uniform)
+    s_old = *sp;
+#pragma unroll
+    for (int r = 0; r < LOADS; ++r)
+      old[r] = *reinterpret_cast<const uintx2*>(dst + std::min<long long>(r * TPL + sub, lo - first - 1) * D);
+  }
+  ushortx2 top2 = {0, 0};
 #pragma unroll
   for (int r = 0; r < LOADS; ++r) {
+    const uintx4 w = __builtin_bit_cast(uintx4, x[r]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const _Float16 v = x[r][e];  // (bit-casting a vector's element in place reads element 0)
-      const int m = __builtin_bit_cast(unsigned short, v) & 0x7fff;
-      top = max(top, m < 0x7c00 ? m : 0);
+    for (int e = 0; e < 4; ++e) {
+      const unsigned m = w[e] & 0x7fff7fffu;
+      top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(ushortx2, m));
     }
   }
+  int top = wave_max(std::max<int>(top2[0], top2[1]));
+  if (top >= 0x7c00) {  // (uniform) infinities or NaN among them: the finite ones' maximum
+    top = 0;
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) top = max(top, __shfl_xor(top, off));
+    for (int r = 0; r < LOADS; ++r) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const _Float16 v = x[r][e];  // (bit-casting a vector's element in place reads element 0)
+        const int m = __builtin_bit_cast(unsigned short, v) & 0x7fff;
+        top = max(top, m < 0x7c00 ? m : 0);
+      }
+    }
+    top = wave_max(top);
+  }
   const float amax = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(top)));
   // amax = 1.m 2^E: 448 = 1.75 2^8 holds it at 2^(E - 8) up to m = 0.75
   const int bits = __float_as_int(amax);
@@ -136,7 +170,7 @@ __global__ __launch_bounds__(kWriteThreads) void kv_write_q8_kernel(
     for (int r = 0; r < LOADS; ++r) {
       const int t = r * TPL + sub;
       if (first + t < lo) {
-        [[maybe_unused]] const uintx2 c = *reinterpret_cast<const uintx2*>(dst + t * D);
+        [[maybe_unused]] const uintx2 c = old[r];
         uintx2 o = {0, 0};
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
