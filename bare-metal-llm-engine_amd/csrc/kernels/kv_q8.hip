@@ -28,6 +28,9 @@ typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kKvBlock = 32;  // tokens that share a scale
 constexpr float kNegInf = -__builtin_huge_valf();
+// V scales below this one, zero among them, count as it: their values are below 448
+// 2^-40 < 2^-31 either way, and an fp16 output's half step is 2^-25 at the least.
+constexpr float kLeastVScale = 0x1p-40f;
 constexpr float kLog2e = 1.4426950408889634f;
 [[maybe_unused]] constexpr int kRsrcWord3 = 0x00020000;  // buffer descriptor: raw, 32-bit elements
 [[maybe_unused]] constexpr int kNonTemporal = 2;  // a buffer load's cache policy
@@ -226,6 +229,10 @@ struct AttnArgs {
 // over s', is raised only when a score passes it by 8 or more, and the weights
 // carry 2^7 so that their fp16 high and low terms hold 22 bits down to 2^-10 of
 // the largest (as in the fp16 cache's kernel). Sums, m and l are fp32.
+// With V scales from 2^-40 (smaller ones count as it) to 2^24, m passes the largest
+// score s by 24 at the most, so l, in units of 2^-7, is 2^-17 or more. A weight below
+// 2^-126, lost, would have added less than 2^-86 to it, 2^31 of them 2^-55; a split's l,
+// 2^15 2^40 2^23 at the most, under a lost weight of the merge 2^-48. Neither shows.
 //
 // Bound by the cache's bytes: 131072 tokens of 32 / 8 heads, D = 128 (270 MB) in 46
 // us with the merge, 5.9 TB/s. Workgroups of 4 waves, three to a CU, cover the
@@ -385,11 +392,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 3 : 1) void decode_q8_kernel(Att
     }
     const int left = nkeys - (wave + NW * t) * kKvBlock;  // keys from the block's first one on
     const float f = scale2 * x.ks;
-    // a V scale of zero (a block of zeros in a cache written elsewhere): the keys
-    // count, their values are zero
-    const bool no_v = x.vs == 0.0f;  // (uniform)
-    const float lv = no_v ? 0.0f : __builtin_amdgcn_logf(x.vs);  // log2
-    const float ivs = no_v ? 1.0f : __builtin_amdgcn_rcpf(x.vs);
+    const float vs = fabsf(x.vs) < kLeastVScale ? kLeastVScale : x.vs;
+    const float lv = __builtin_amdgcn_logf(vs);  // log2
+    const float ivs = __builtin_amdgcn_rcpf(vs);
     float sv[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sv[e] = fmaf(sc[e >> 2][e & 3], f, lv);
@@ -427,7 +432,6 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 3 : 1) void decode_q8_kernel(Att
 #endif
     }
     lsum = fmaf(ls, ivs, lsum);
-    if (no_v) return;
 #pragma unroll
     for (int d = 0; d < VD; ++d) {
       halfx8 av[4];

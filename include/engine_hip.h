@@ -491,10 +491,11 @@ int eng_rmsnorm_linear_mx4w_nk(const float* in, const float* rms_weight, const u
  * [batch, n_kv_heads, kv_max_seq_len, head_dim], 16-byte aligned; every block of
  * ENG_KV_Q8_BLOCK tokens of a (sequence, KV head) has one fp32 scale for K and
  * one for V, [batch, n_kv_heads, ceil(kv_max_seq_len / ENG_KV_Q8_BLOCK)]. The
- * value of a code is its e4m3 value times its block's scale (a cache written by
- * other means may have any finite scales of zero or more). head_dim is 64 or
- * 128. Positions and lengths are read on the device (int32 arrays of `batch`), so
- * a captured decode step is replayed for every token.
+ * value of a code is its e4m3 value times its block's scale. A cache written by
+ * other means may have any scales from zero to 2^24; V scales below 2^-40 count as
+ * 2^-40, whose values an fp16 output cannot show. head_dim is 64 or 128. Positions
+ * and lengths are read on the device (int32 arrays of `batch`), so a captured decode
+ * step is replayed for every token.
  *
  * eng_kv_cache_write_q8: rows k_new / v_new [batch, s_new, n_kv_heads, head_dim]
  * (16-byte aligned) become tokens pos[b] .. of sequence b; the first n_new[b] of
