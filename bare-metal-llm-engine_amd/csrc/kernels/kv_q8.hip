@@ -49,6 +49,22 @@ __device__ __forceinline__ unsigned fp8x4(float a, float b, float c, float d) {
   return static_cast<unsigned>(w);
 }
 
+// p is the fp32 value nearest to an exact p + rest: p with its last bit set (of the value
+// next towards zero) where rest is not zero. Rounded to e4m3, it gives the code nearest to
+// the exact value, where p could have become the middle between two codes. (|p| outside
+// the range in which codes differ is left alone: infinities, NaN, and what becomes zero.)
+__device__ __forceinline__ float to_odd(float p, float rest) {
+  const unsigned u = __float_as_uint(p);
+  const unsigned below = ((__float_as_uint(rest) ^ u) >> 31);  // the exact value is nearer to zero
+  const bool inexact = rest != 0.0f && fabsf(p) >= 0x1p-12f && fabsf(p) < 0x1p16f;
+  return inexact ? __uint_as_float((u - below) | 1u) : p;
+}
+
+// Whether s (the same in every lane, positive or zero) is a power of two, or zero.
+__device__ __forceinline__ bool power_of_two(float s) {
+  return (__builtin_amdgcn_readfirstlane(__float_as_int(s)) & 0x7fffff) == 0;
+}
+
 // The largest of the wave's values, none negative, in every lane.
 template <int CTRL>
 __device__ __forceinline__ int dpp_max(int x) {
@@ -69,7 +85,9 @@ __device__ __forceinline__ int wave_max(int x) {
 // together. The block's scale is the least power of two in [2^-15, 2^8] that
 // brings its largest finite new magnitude to 448 or less (2^-15 already holds
 // fp16's smallest steps), and no less than the scale of earlier tokens kept in
-// the block; if it grows, their codes are brought to it. Tokens at or past
+// the block; if it grows, their codes are brought to it. (Both roundings are right for any
+// scale kept from a cache written elsewhere: past powers of two, division and a sticky bit,
+// in branches of their own.) Tokens at or past
 // kv_max_seq_len are dropped. Blocks belong to one wave each: no atomics.
 // Bound by the bytes of the new rows and their codes, and for a token each by the round
 // trips of position, then new rows, old codes and scale together (4 prompts of up to 1000
@@ -156,34 +174,69 @@ __global__ __launch_bounds__(kWriteThreads) void kv_write_q8_kernel(
   e = min(max(e, -15), 8);
   const float s = fmaxf(__int_as_float((e + 127) << 23), s_old);
   const float inv = 1.0f / s;
-#pragma unroll
-  for (int r = 0; r < LOADS; ++r) {
-    const int t = r * TPL + sub;
-    if (first + t >= lo && first + t < hi) {
-      float v[8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = static_cast<float>(x[r][q]) * inv;
-      *reinterpret_cast<uintx2*>(dst + t * D) =
-          uintx2{fp8x4(v[0], v[1], v[2], v[3]), fp8x4(v[4], v[5], v[6], v[7])};
-    }
-  }
-  if (kept && s > s_old) {
-    [[maybe_unused]] const float ratio = s_old * inv;
+  if (power_of_two(s)) {
 #pragma unroll
     for (int r = 0; r < LOADS; ++r) {
       const int t = r * TPL + sub;
-      if (first + t < lo) {
-        [[maybe_unused]] const uintx2 c = old[r];
-        uintx2 o = {0, 0};
+      if (first + t >= lo && first + t < hi) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = static_cast<float>(x[r][q]) * inv;
+        *reinterpret_cast<uintx2*>(dst + t * D) =
+            uintx2{fp8x4(v[0], v[1], v[2], v[3]), fp8x4(v[4], v[5], v[6], v[7])};
+      }
+    }
+  } else {  // a scale kept from elsewhere; its rows again, so that this stays a small loop
+#pragma unroll 1
+    for (int t = sub; t < kKvBlock; t += TPL) {
+      if (first + t >= lo && first + t < hi) {
+        const halfx8 w = *reinterpret_cast<const halfx8*>(src + (first + t) * n_kv_heads * D);
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float f = static_cast<float>(w[q]);
+          v[q] = f / s;
+          v[q] = to_odd(v[q], fmaf(-v[q], s, f));
+        }
+        *reinterpret_cast<uintx2*>(dst + t * D) =
+            uintx2{fp8x4(v[0], v[1], v[2], v[3]), fp8x4(v[4], v[5], v[6], v[7])};
+      }
+    }
+  }
+  if (kept && s > s_old) {  // (s is a power of two)
+    [[maybe_unused]] const float ratio = s_old * inv;
+    if (power_of_two(s_old)) {
+#pragma unroll
+      for (int r = 0; r < LOADS; ++r) {
+        const int t = r * TPL + sub;
+        if (first + t < lo) {
+          [[maybe_unused]] const uintx2 c = old[r];
+          uintx2 o = {0, 0};
 #if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[q]), false);
+            const floatx2 z = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[q]), true);
+            o[q] = fp8x4(a[0] * ratio, a[1] * ratio, z[0] * ratio, z[1] * ratio);
+          }
+#endif
+          *reinterpret_cast<uintx2*>(dst + t * D) = o;
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int t = sub; first + t < lo; t += TPL) {
+        uintx2 c = *reinterpret_cast<const uintx2*>(dst + t * D);
+#if defined(__HIP_DEVICE_COMPILE__)
+        auto scaled = [&](float f) { return to_odd(f * ratio, fmaf(f, ratio, -(f * ratio))); };
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[q]), false);
           const floatx2 z = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[q]), true);
-          o[q] = fp8x4(a[0] * ratio, a[1] * ratio, z[0] * ratio, z[1] * ratio);
+          c[q] = fp8x4(scaled(a[0]), scaled(a[1]), scaled(z[0]), scaled(z[1]));
         }
 #endif
-        *reinterpret_cast<uintx2*>(dst + t * D) = o;
+        *reinterpret_cast<uintx2*>(dst + t * D) = c;
       }
     }
   }
