@@ -1161,7 +1161,9 @@ void launch_pass(const Mx4Args& a, hipStream_t stream) {
   }
 }
 
-// Rows in passes whose planes take at most 256 MiB of the stream's arena.
+// Rows in passes whose planes take at most 256 MiB of the stream's arena, or of 128 rows,
+// a tile of the GEMM, where these take more (K past 349000; 6.4 GB at K = 2^23): fewer rows
+// a pass would read the weights more often.
 void linear_mx4w(const Mx4Args& a, hipStream_t stream) {
   const long long row_bytes = (a.K + kChunk - 1) / kChunk * kChunk * 6;
   const long long pass = std::clamp((256ll << 20) / row_bytes / 128 * 128, 128ll, 32768ll);

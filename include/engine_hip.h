@@ -464,10 +464,14 @@ int eng_transpose_f32(const float* src, float* dst, int64_t rows, int64_t cols,
  * eng_rmsnorm_linear_mx4w_nk: out = RMSNorm(in, rms_weight, eps) . W^T, rms_weight
  * may be NULL; as for eng_rmsnorm_linear_* any zero dimension is a no-op.
  * Products are exact and sums fp32, as for fp16 weights: every fp32 activation
- * enters the matrix cores as three bf16 terms that add up to it. K is at most
- * 2^23. The same call gives the same bits; the kernel, and with it the order of
- * the sums, depends on M, N and K. From 5 rows (below that, where X does not fit
- * the LDS: M K past 20000 or so) the stream's scratch arena is used.
+ * enters the matrix cores as three bf16 terms that add up to it (but for its bits
+ * below 2^-133, which are dropped). Weights of 2^128 and more, 4 and 6 under the
+ * scale bytes 253 and 254, are infinities: the sums they enter are infinite or NaN.
+ * K is at most 2^23. The same call gives the same bits; the kernel, and with it the
+ * order of the sums, depends on M, N and K. From 5 rows (below that, where X does
+ * not fit the LDS: M K past 20000 or so) the stream's scratch arena is used: at 5 to
+ * 64 rows up to 128 M N bytes, past them 6 bytes for each activation of a pass (as
+ * many rows as make 256 MiB, at least 128) and up to 64 M N bytes.
  * ---------------------------------------------------------------------- */
 int eng_mx4_quantize_f32(const float* src, uint8_t* codes, uint8_t* scales, int64_t rows,
                          int64_t cols, eng_stream stream);

@@ -121,6 +121,42 @@ def test_first_and_last_scale_bytes(gpu, M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 3, 6, 70])
+def test_weights_past_fp32(gpu, M):
+    """Values of 2^128 and more (bytes 253 and 254) are infinities: what they enter is
+    infinite or NaN, and nothing else is touched."""
+    rng = np.random.default_rng(M)
+    N, K = 40, 200
+    X = rng.integers(1, 4, (M, K)).astype(F)
+    codes, _ = mx4.weights(rng, N, K)
+    scales = np.full((N, -(-K // 32)), 127, np.uint8)
+    clean, _ = narrow.linear64(X, narrow.mx4_decode(codes, scales, K))
+    codes[[3, 20], 7] = [0x70, 0x06]  # 6 at place 15, 4 at place 14
+    scales[3, 0], scales[20, 0] = 254, 253
+    codes[20, :7], codes[20, 8:16] = 0, 0
+    codes[20, 7] = 0x06
+    got = mx4.linear(gpu, X, codes, scales, N)
+    rest = np.delete(np.arange(N), [3, 20])
+    assert np.array_equal(got[:, rest], clean[:, rest])
+    assert not np.isfinite(got[:, [3, 20]]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 3, 6, 20, 70])
+def test_activations_near_the_least_subnormal(gpu, M):
+    """Bits below 2^-133 are dropped, nothing above them: weights of 2^100 make both show."""
+    rng = np.random.default_rng(M)
+    N, K = 30, 200
+    X = np.ldexp(rng.integers(-(1 << 10), 1 << 10, (M, K)), -140).astype(F)
+    codes = np.full((N, -(-K // 32) * 16), 0x22, np.uint8)
+    codes[:, rng.integers(0, K // 2, 40)] = 0x0A  # some -1, some zeros
+    scales = np.full((N, -(-K // 32)), 227, np.uint8)
+    kept = np.trunc(np.ldexp(X.astype(np.float64), 133)) * 2.0**-133
+    y, _ = narrow.linear64(kept, narrow.mx4_decode(codes, scales, K))
+    assert np.array_equal(mx4.linear(gpu, X, codes, scales, N), y)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [65, 70, 129, 300])
 def test_special_values_in_the_gemm(gpu, M):
     mx4.test_linear_special_values(gpu, M)
