@@ -692,6 +692,8 @@ void launch_decode(const AttnArgs& a, float* part_o, float* part_ml, dim3 grid, 
 template <int D>
 void run_decode(AttnArgs a, long long batch, hipStream_t s) {
   const long long units = batch * a.n_kv_heads * a.tiles;
+  ENG_CHECK(threads_fit(units, 256) && (a.nsplit == 1 || threads_fit(batch * a.n_heads, 64)),
+            "attention_decode_q8: too many (sequence, head) pairs for one launch");
   const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(a.nsplit));
   if (a.nsplit == 1) {
     launch_decode<D, false>(a, nullptr, nullptr, grid, s);
@@ -743,10 +745,11 @@ int eng_kv_cache_write_q8(const eng_half* k_new, const eng_half* v_new, uint8_t*
               "kv_cache_write_q8: k_new, v_new and the caches must be 16-byte aligned");
     const int reach = static_cast<int>((s_new + eng::kKvBlock - 2) / eng::kKvBlock + 1);
     ENG_CHECK(batch <= 0x7fffffffLL && n_kv_heads <= 0x7fffffffLL &&
-                  batch * n_kv_heads <= 0x7fffffffLL / reach,
+                  batch * n_kv_heads <= 0x7fffffffLL / reach &&
+                  eng::threads_fit((batch * n_kv_heads * reach + 1) / 2, eng::kWriteThreads),
               "kv_cache_write_q8: too many (sequence, head, block) units for one launch");
     const unsigned units = 2u * static_cast<unsigned>(batch * n_kv_heads * reach);
-    const unsigned grid = static_cast<unsigned>((units + 3ull) / 4);
+    const unsigned grid = (units + 3) / 4;
     auto go = [&](auto kernel) {
       kernel<<<grid, eng::kWriteThreads, 0, eng::as_stream(stream)>>>(
           reinterpret_cast<const _Float16*>(k_new), reinterpret_cast<const _Float16*>(v_new),

@@ -213,4 +213,9 @@ void launch_swiglu_f32(const float* g, const float* u, float* out, long long n,
 // Number of compute units of the current device (cached per device).
 int device_cu_count();
 
+// Whether a launch's first dimension stays below HIP's limit of 2^32 threads.
+inline bool threads_fit(long long blocks, long long threads) {
+  return blocks <= 0xffffffffLL / threads;
+}
+
 }  // namespace eng

@@ -370,9 +370,9 @@ void run_decode(const Mx4Args& a, hipStream_t stream) {
   const int nb = (K + 31) / 32;
   const std::size_t lds = static_cast<std::size_t>(6) * MR * decode_pitch(K);
   const long long tiles = (a.N + 15) / 16;
-  const long long wgs = std::min<long long>(
-      tiles, std::max<long long>(device_cu_count(), (tiles + kDecodeTiles - 1) / kDecodeTiles));
-  ENG_CHECK(wgs <= 0x7fffffffLL, "linear_mx4w: grid too large for one launch");
+  const long long least = (tiles + kDecodeTiles - 1) / kDecodeTiles;
+  ENG_CHECK(threads_fit(least, 64 * kDecodeWaves), "linear_mx4w: N too large for one launch");
+  const long long wgs = std::min<long long>(tiles, std::max<long long>(device_cu_count(), least));
   const unsigned grid = static_cast<unsigned>(wgs);
   auto go = [&](auto rms, auto sv) {
     constexpr bool R = decltype(rms)::value;
@@ -821,6 +821,7 @@ void slice_shape(const Mx4Args& a, int mb, int& nt, int& slices) {
   nt = 0;
   for (int cand : {1, 2, 3}) {
     const long long groups = (a.N + 128 * cand - 1) / (128 * cand);
+    if (!threads_fit(groups, 64 * kSliceWaves)) continue;
     for (long long s = 1; s <= std::min(units, 32ll); ++s) {
       double time = static_cast<double>((groups * s + cus - 1) / cus) *
                     (static_cast<double>((units + s - 1) / s) * (mb + 1.7 * cand) + 1.25);
@@ -836,7 +837,6 @@ void run_slices(const Mx4Args& a, int slices, hipStream_t stream) {
   const int M = static_cast<int>(a.M);
   const int nb = (K + 31) / 32;
   const long long groups = (a.N + 128 * NT - 1) / (128 * NT);
-  ENG_CHECK(groups <= 0x7fffffffLL, "linear_mx4w: grid too large for one launch");
   const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(slices));
   auto launch = [&](float* sums, float* squares) {
     with_flags(a.rms, scales_by_8(a), [&](auto rms, auto sv) {
@@ -860,6 +860,7 @@ void run_slices(const Mx4Args& a, int slices, hipStream_t stream) {
 
 template <int MB>
 void launch_slices(const Mx4Args& a, hipStream_t stream) {
+  ENG_CHECK(threads_fit(a.N / 384 + 1, 64 * kSliceWaves), "linear_mx4w: N too large for one launch");
   int nt = 0, slices = 1;
   slice_shape(a, MB, nt, slices);
   if (nt == 1) run_slices<MB, 1>(a, slices, stream);
@@ -1090,7 +1091,7 @@ void run_gemm(const Mx4Args& a, const Mx4Planes& p, float* sums, int slices, hip
   const int mblocks = static_cast<int>((a.M + 15) / 16);
   const int tiles_m = (mblocks + BMB - 1) / BMB;
   const long long tiles = tiles_m * ((a.N + 64 * NT - 1) / (64 * NT));
-  ENG_CHECK(tiles <= 0x7fffffffLL, "linear_mx4w: too many tiles for one launch");
+  ENG_CHECK(threads_fit(tiles, 64 * BMB), "linear_mx4w: too many tiles for one launch");
   const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(slices));
   auto go = [&](auto rms) {
     mx4_gemm_kernel<NT, decltype(rms)::value><<<grid, 64 * BMB, 0, stream>>>(
