@@ -736,6 +736,95 @@ TEST(gpu_kernels, ffn_sub_block_through_cpp_api) {
   EXPECT_TRUE(got_out == got_sum);
 }
 
+TEST(cpu_contract, narrow_launchers_reject_bad_arguments) {
+  float* p = g_dummy_f;
+  engine::half* ph = g_dummy_h;
+  auto* pb = reinterpret_cast<std::uint8_t*>(std::uintptr_t{0x1000});
+  auto* pi = reinterpret_cast<std::int32_t*>(std::uintptr_t{0x1000});
+  EXPECT_THROWS_MSG(engine::cuda::mx4_quantize(p, pb, pb, -1, 4), "negative");
+  EXPECT_THROWS_MSG(engine::cuda::mx4_quantize(ph, pb, pb, -1, 4), "negative");
+  EXPECT_THROWS_MSG(engine::cuda::mx4_dequantize(pb, pb, p, 4, -1), "negative");
+  EXPECT_THROWS_MSG(engine::cuda::mx4_dequantize(pb, pb, ph, 4, -1), "negative");
+  EXPECT_THROWS_MSG(engine::cuda::linear_nk(p, pb + 1, pb, p, 1, 4, 4), "aligned");
+  EXPECT_THROWS_MSG(engine::cuda::rmsnorm_linear_nk(p, p, pb, pb, p, 1, 4, 4, -1.0f), "eps");
+  EXPECT_THROWS_MSG(engine::cuda::kv_cache_write_q8(reinterpret_cast<engine::half*>(pb),
+                                                    reinterpret_cast<engine::half*>(pb), pb, pb, p, p,
+                                                    nullptr, nullptr, 1, 1, 1, 64, 32), "pos");
+  EXPECT_THROWS_MSG(engine::cuda::attention_decode_q8(ph, pb, pb, p, p, ph, pi, 1, 3, 2, 64, 1, 1, 1.0f),
+                    "divisible");
+}
+
+// Values that the narrow formats hold, so every result is exact.
+TEST(gpu_kernels, narrow_weights_and_cache_through_cpp_api) {
+  require_gpu(ctx);
+  const std::int64_t M = 3, N = 20, K = 70, blocks = 3;
+  const float grid[] = {0.0f, 0.5f, -1.0f, 1.5f, 2.0f, -3.0f, 4.0f, 6.0f};
+  std::vector<float> W(N * K), x(M * K), g(K, 2.0f);
+  for (std::int64_t i = 0; i < N * K; ++i) W[i] = grid[(i * 7 + i / 13) % 8];
+  for (std::int64_t n = 0; n < N; ++n)  // every block's largest magnitude is 6
+    for (std::int64_t b = 0; b < blocks; ++b) W[n * K + 32 * b] = 6.0f;
+  for (std::int64_t i = 0; i < M * K; ++i) x[i] = static_cast<float>(i % 5 - 2);
+  std::vector<engine::half> Wh(W.size());
+  for (std::size_t i = 0; i < W.size(); ++i) Wh[i] = engine::float_to_half(W[i]);
+  engine::DeviceBuffer<float> dW(W), dx(x), dg(g), back(W.size()), y(M * N), z(M * N);
+  engine::DeviceBuffer<engine::half> dWh(Wh), back_h(W.size());
+  engine::DeviceBuffer<std::uint8_t> codes(N * blocks * 16), scales(N * blocks);
+  engine::DeviceBuffer<std::uint8_t> codes_h(N * blocks * 16), scales_h(N * blocks);
+  engine::cuda::mx4_quantize(dW.get(), codes.get(), scales.get(), N, K);
+  engine::cuda::mx4_quantize(dWh.get(), codes_h.get(), scales_h.get(), N, K);
+  engine::cuda::mx4_dequantize(codes.get(), scales.get(), back.get(), N, K);
+  engine::cuda::mx4_dequantize(codes.get(), scales.get(), back_h.get(), N, K);
+  engine::cuda::linear_nk(dx.get(), codes.get(), scales.get(), y.get(), M, N, K);
+  engine::cuda::rmsnorm_linear_nk(dx.get(), dg.get(), codes.get(), scales.get(), z.get(), M, N, K, 0.0f);
+  ENGINE_ABI_CHECK(eng_device_sync());
+  EXPECT_TRUE(codes.download() == codes_h.download());
+  EXPECT_TRUE(scales.download() == scales_h.download());
+  EXPECT_TRUE(back.download() == W);
+  const std::vector<engine::half> bh = back_h.download();
+  int bad = 0;
+  for (std::size_t i = 0; i < W.size(); ++i) bad += engine::half_to_float(bh[i]) != W[i];
+  const std::vector<float> gy = y.download(), gz = z.download();
+  for (std::int64_t m = 0; m < M; ++m) {
+    double ss = 0.0;
+    for (std::int64_t k = 0; k < K; ++k) ss += x[m * K + k] * x[m * K + k];
+    for (std::int64_t n = 0; n < N; ++n) {
+      double sum = 0.0;
+      for (std::int64_t k = 0; k < K; ++k) sum += x[m * K + k] * W[n * K + k];
+      bad += gy[m * N + n] != static_cast<float>(sum);
+      // the mean, the root, the quotient and the product: a rounding each
+      const double want = 2.0 * sum / std::sqrt(ss / K);
+      bad += !(std::fabs(gz[m * N + n] - want) <= 4 * 0x1p-24 * std::fabs(want));
+    }
+  }
+  EXPECT_EQ(bad, 0);
+
+  // one token of two sequences, the second one inactive: the attention returns its V row
+  const std::int64_t B = 2, H = 4, G = 2, D = 64, room = 40, nb = 2;
+  std::vector<engine::half> kn(B * G * D), vn(B * G * D), q(B * H * D, engine::float_to_half(1.0f));
+  for (std::size_t i = 0; i < kn.size(); ++i) {
+    kn[i] = engine::float_to_half(static_cast<float>(i % 3));
+    vn[i] = engine::float_to_half(static_cast<float>(static_cast<int>(i % 9) - 4));
+  }
+  engine::DeviceBuffer<engine::half> dkn(kn), dvn(vn), dq(q), out(q.size());
+  engine::DeviceBuffer<std::uint8_t> kc(B * G * room * D), vc(B * G * room * D);
+  engine::DeviceBuffer<float> ks(B * G * nb), vs(B * G * nb);
+  engine::DeviceBuffer<std::int32_t> pos(std::vector<std::int32_t>{0, -1}), len(std::vector<std::int32_t>{1, 0});
+  engine::cuda::kv_cache_write_q8(dkn.get(), dvn.get(), kc.get(), vc.get(), ks.get(), vs.get(), pos.get(),
+                                  nullptr, B, 1, G, D, room);
+  engine::cuda::attention_decode_q8(dq.get(), kc.get(), vc.get(), ks.get(), vs.get(), out.get(), len.get(),
+                                    B, H, G, D, room, room, 0.125f);
+  ENGINE_ABI_CHECK(eng_device_sync());
+  const std::vector<engine::half> o = out.download();
+  bad = 0;
+  for (std::int64_t h = 0; h < H; ++h) {
+    for (std::int64_t d = 0; d < D; ++d) {
+      bad += o[h * D + d].u != vn[h / (H / G) * D + d].u;
+      bad += engine::half_to_float(o[(H + h) * D + d]) != 0.0f;
+    }
+  }
+  EXPECT_EQ(bad, 0);
+}
+
 // --------------------------------------------------------------------- engref
 // Writes an ENGREF01 file (the reference's container, tools/gen_reference.py:
 // 64-83) with explicit dtype codes.
