@@ -1,5 +1,6 @@
 // mx4.hip -- microscaled 4-bit floating point (OCP Microscaling Formats v1.0,
-// MXFP4): quantisation of rows, and linear layers with such weights.
+// MXFP4): quantisation of rows, and the values back (mx4_linear.hip has the linear
+// layers on such weights).
 //
 // Format: 32 values along a row share a scale byte s (E8M0: 2^(s - 127), 255 a
 // NaN); each value is a 4-bit E2M1 code, sign and one of 0, 0.5, 1, 1.5, 2, 3,
@@ -14,12 +15,7 @@ namespace eng {
 namespace {
 
 typedef float floatx2 __attribute__((ext_vector_type(2)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
-typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 32;  // values that share a scale
@@ -52,7 +48,8 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, long long n, floa
 // scale, rounds to nearest even and saturates at 6. A block with a NaN or an
 // infinity gets the NaN scale and zero codes. Memory bound: each value is read
 // once, in 16-byte loads where the rows allow (VEC): 11008 x 4096 fp16, 114 MB, 21.7 us,
-// 5.3 TB/s (a copy of 1 GiB runs at 5.2).
+// 5.3 TB/s (a copy of 1 GiB runs at 5.2); fp32, 204 MB, 38.1 us, 5.4 TB/s. Other rows go
+// value by value: 11008 x 4095 fp16 54.5 us, fp32 80.0.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void mx4_quantize_kernel(
     const T* __restrict__ src, unsigned* __restrict__ codes, unsigned char* __restrict__ scales,
@@ -98,7 +95,9 @@ __global__ __launch_bounds__(kThreads) void mx4_quantize_kernel(
 }
 
 // The values back: one word of codes, eight values a thread. Memory bound: 11008 x 4096
-// to fp16, 114 MB, 18.1 us (the codes partly from the 256 MB cache), 6.3 TB/s.
+// to fp16, 114 MB, 18.1 us over three sets of buffers (the codes partly from the 256 MB
+// cache), 24.4 over five; to fp32, 204 MB, 48.9 us over five. Rows that are not whole 16
+// bytes go value by value: 11008 x 4095 to fp16 65.3 us, to fp32 116.5.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void mx4_dequantize_kernel(
     const unsigned* __restrict__ codes, const unsigned char* __restrict__ scales,

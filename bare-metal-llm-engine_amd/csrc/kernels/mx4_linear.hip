@@ -876,10 +876,14 @@ void launch_slices(const Mx4Args& a, hipStream_t stream) {
 // weights of a chunk come straight into registers a chunk ahead (4-bit: 16 NT bytes a
 // lane and chunk) and are converted as their step begins. Tiles with K split among
 // gridDim.y slices leave their sums for mx4_slice_reduce_kernel.
-// Bound by the matrix cores and the LDS beside them: 2048 x 4096 x 4096 189 us with the
-// planes' pass, 1090 TFLOP/s of bf16 products (three per weight), where a plain bf16
-// product of 8192^3 runs at 1198 through the library on the same card. Waves of 32 rows by
-// 32 NT columns, with half the LDS reads and twice the conversions, take 226 us.
+// 2048 x 4096 x 4096 takes 189 us with the planes' pass, 1090 TFLOP/s of bf16 products
+// (three per weight); a plain bf16 product of 8192^3 through the library runs at 1198 on the
+// same card. That is no bound of the hardware: the matrix cores are busy 52 % of the kernel
+// (46 % at 512 x 11008 x 4096, 232 tiles on 256 CUs). A wave spends 58 % of its
+// time waiting to issue (54 %), behind its SIMD's other wave and its own matrix
+// instructions, 2 % of it for the LDS, and 25 % (28 %) at the steps' waits and barriers,
+// which keep the two waves of a SIMD in step. Waves of 32 rows by 32 NT columns, with half the LDS
+// reads and twice the conversions, take 226 us.
 constexpr int kGemmBlocks = 8;  // m-blocks of a tile, and waves
 
 template <int NT, bool RMS>
@@ -1106,7 +1110,10 @@ void run_gemm(const Mx4Args& a, const Mx4Planes& p, float* sums, int slices, hip
 // one workgroup per CU (a chunk of a 128 x 64 NT tile: its 192 NT matrix
 // instructions on four SIMDs and about a quarter of a microsecond; the fill and the
 // end of a tile about 2) and, past one slice, the sums' way out and back and the
-// reduce launch.
+// reduce launch. Held against every width and 1 to 16 slices (3, 6 and 12 too) at 65 to
+// 2048 rows of five matrices, 2051 x 1023 to 28672 x 8192: what it picks takes 3 %
+// (geometric mean) more than the fastest of them, 21 % at most (512 x 2051 x 1023 30.3 us,
+// 25.1 in three slices, a count that it does not try; 256 x 11008 x 4096 92 against 79).
 void gemm_shape(const Mx4Args& a, int& nt, int& slices) {
   const long long cus = device_cu_count();
   const long long chunks = (a.K + kChunk - 1) / kChunk;
@@ -1140,7 +1147,11 @@ void launch_mx4_gemm(const Mx4Args& a, hipStream_t stream) {
     launch_reduce(a, sums, p.part, slices, static_cast<int>((a.K + kChunk - 1) / kChunk), stream);
 }
 
-// One pass of rows at a.x, a.y.
+// One pass of rows at a.x, a.y. The least m-blocks that hold the rows, and the GEMM past
+// four: 16 x 28672 x 8192 takes 41.6 us in one m-block and 60 in two, 17 rows 59.7 in two
+// and 90 in four, 64 rows 91.7 in four and 176 in the GEMM (at 4096 x 4096 9.3 and 11.2,
+// 11.5 and 14.5, 18.9 and 28.0). Past 64 rows the GEMM pays for 128: 65 rows take 27.5 us
+// at 4096 x 4096 and 169 at 28672 x 8192.
 void launch_pass(const Mx4Args& a, hipStream_t stream) {
   if (decode_applies(a.M, a.K)) {
     switch (a.M) {
