@@ -535,6 +535,65 @@ int eng_attention_decode_q8(const eng_half* q, const uint8_t* k_cache, const uin
                             int64_t kv_max_seq_len, float scale, int split_kv, eng_stream stream);
 
 /* ------------------------------------------------------------------------
+ * Attention over long contexts (additive, no reference counterpart): new tokens of
+ * a batch with a sliding window, and single tokens of sequences that share a prefix.
+ * Caches are head-major, [batch, n_kv_heads, kv_max_seq_len, head_dim], 16-byte
+ * aligned: fp16 (each sequence's as eng_kv_cache_write_f16 fills it) or 8-bit with
+ * scales (eng_kv_cache_write_q8's). head_dim is 64 or 128. Positions, counts and
+ * lengths are int32 arrays on the device. Scores, softmax and sums are fp32; the
+ * weights are rounded to fp16 for their products with V where many query rows share
+ * the keys. A row that sees no key gets zeros. What a query does not see does not
+ * reach its result, infinities and NaN included.
+ *
+ * eng_attention_window_*: q and out [batch, s_new, n_heads, head_dim]. Query i of
+ * sequence b stands at position p = pos[b] + i, and its K and V rows and all before
+ * them are in the caches (write them first). It sees the keys j <= p, of these with
+ * window > 0 those with j > p - window or j < sinks; window == 0 is no window. s_new
+ * is a prompt's length, a piece's or 1. The first n_new[b] of a sequence's s_new
+ * queries are computed (all of them where n_new is NULL, none where pos[b] < 0) and
+ * the rows of out behind them left as they were. Keys at or past max_kv_len, the
+ * caller's bound on pos + n_new, are not seen; it and s_new choose the launch.
+ *
+ * eng_attention_prefix_*: one query of each sequence, q and out [batch, n_heads,
+ * head_dim], over the first prefix_len[g] tokens of prefix g, shared by the batch /
+ * n_prefix sequences of group g = b / (batch / n_prefix), and then the first
+ * kv_len[b] of its own, in one softmax. The prefixes are caches of their own,
+ * [n_prefix, n_kv_heads, prefix_max_seq_len, head_dim], each read once for its
+ * group. Lengths past max_prefix_len / max_kv_len are taken as these, lengths
+ * below zero as zero.
+ *
+ * split_kv = 0 chooses the number of pieces that a row's keys are computed in; a
+ * positive value asks for as many (at most 256, prefix and own keys 128 each). More
+ * than one uses the stream's scratch arena (eng_attention_prefix_* always does).
+ * ---------------------------------------------------------------------- */
+int eng_attention_window_f16(const eng_half* q, const eng_half* k_cache, const eng_half* v_cache,
+                             eng_half* out, const int32_t* pos, const int32_t* n_new, int64_t batch,
+                             int64_t s_new, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                             int64_t window, int64_t sinks, int64_t max_kv_len,
+                             int64_t kv_max_seq_len, float scale, int split_kv, eng_stream stream);
+int eng_attention_window_q8(const eng_half* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                            const float* k_scale, const float* v_scale, eng_half* out,
+                            const int32_t* pos, const int32_t* n_new, int64_t batch, int64_t s_new,
+                            int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t window,
+                            int64_t sinks, int64_t max_kv_len, int64_t kv_max_seq_len, float scale,
+                            int split_kv, eng_stream stream);
+int eng_attention_prefix_f16(const eng_half* q, const eng_half* k_prefix, const eng_half* v_prefix,
+                             const int32_t* prefix_len, const eng_half* k_cache,
+                             const eng_half* v_cache, const int32_t* kv_len, eng_half* out,
+                             int64_t n_prefix, int64_t batch, int64_t n_heads, int64_t n_kv_heads,
+                             int64_t head_dim, int64_t max_prefix_len, int64_t prefix_max_seq_len,
+                             int64_t max_kv_len, int64_t kv_max_seq_len, float scale, int split_kv,
+                             eng_stream stream);
+int eng_attention_prefix_q8(const eng_half* q, const uint8_t* k_prefix, const uint8_t* v_prefix,
+                            const float* k_prefix_scale, const float* v_prefix_scale,
+                            const int32_t* prefix_len, const uint8_t* k_cache, const uint8_t* v_cache,
+                            const float* k_scale, const float* v_scale, const int32_t* kv_len,
+                            eng_half* out, int64_t n_prefix, int64_t batch, int64_t n_heads,
+                            int64_t n_kv_heads, int64_t head_dim, int64_t max_prefix_len,
+                            int64_t prefix_max_seq_len, int64_t max_kv_len, int64_t kv_max_seq_len,
+                            float scale, int split_kv, eng_stream stream);
+
+/* ------------------------------------------------------------------------
  * ENGREF01 tensor files and device weight slabs.
  *
  * The container is the reference's golden format (tools/gen_reference.py:
