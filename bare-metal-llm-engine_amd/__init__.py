@@ -143,6 +143,10 @@ SIGNATURES = {
     "eng_attention_window_q8": [_p] * 8 + [_i64] * 9 + [_f, ctypes.c_int, _p],
     "eng_attention_prefix_f16": [_p] * 8 + [_i64] * 9 + [_f, ctypes.c_int, _p],
     "eng_attention_prefix_q8": [_p] * 12 + [_i64] * 9 + [_f, ctypes.c_int, _p],
+    "eng_beam_select_f32": [_p, _i64] + [_p] * 6 + [_i64] * 5 + [_p],
+    "eng_beam_select_f16": [_p, _i64] + [_p] * 6 + [_i64] * 5 + [_p],
+    "eng_kv_cache_reorder_f16": [_p] * 6 + [_i64] * 6 + [_p],
+    "eng_kv_cache_reorder_q8": [_p] * 10 + [_i64] * 6 + [_p],
     "eng_engref_open": [ctypes.c_char_p, _pp],
     "eng_engref_close": [_p],
     "eng_engref_count": [_p, ctypes.POINTER(ctypes.c_int32)],

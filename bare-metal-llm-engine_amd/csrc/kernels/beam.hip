@@ -1,0 +1,567 @@
+// beam.hip -- beam search: the best continuations over the beams of a group and the
+// vocabulary, and the reordering of the beams' caches that follows from them.
+//
+// Selection: candidate (beam b, token t) has the score s_b + x_bt - L_b, with L_b =
+// log sum_t exp x_bt. Within a beam the order is the logits' own, so the logits are read
+// once: a pass over a piece of a row keeps the piece's best candidates by (logit, lowest
+// token) as 64-bit keys and its max and sum of exponentials; a second kernel joins the
+// pieces and compares candidates of unlike beams by their scores in 64 bits.
+#include "gemv_kernels.hpp"
+#include "launch.hpp"
+
+#include <algorithm>
+
+namespace eng {
+namespace beam {
+namespace {
+
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef unsigned long long u64;
+
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr int kMaxOut = 64;    // candidates that a call may ask for
+constexpr int kMaxBeams = 32;
+constexpr int kWaves = 4;
+constexpr int kVpt = 16;       // values of a lane in one step of a wave
+constexpr int kWaveList = 64 * kVpt + kMaxOut;
+
+// Key of a candidate: larger logits first, then lower tokens. 0 stands for none.
+__device__ __forceinline__ u64 key_of(float x, unsigned token) {
+  const unsigned u = __float_as_uint(x + 0.0f);  // (-0 as 0)
+  const unsigned v = u ^ ((u >> 31) != 0 ? 0xffffffffu : 0x80000000u);
+  return (static_cast<u64>(v) << 32) | (0xffffffffu - token);
+}
+__device__ __forceinline__ float logit_of(u64 key) {
+  const unsigned v = static_cast<unsigned>(key >> 32);
+  return __uint_as_float(v ^ ((v >> 31) != 0 ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ unsigned token_of(u64 key) { return 0xffffffffu - static_cast<unsigned>(key); }
+
+// The largest of the wave's values, in every lane.
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_max(unsigned x) {
+  return max(x, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xF, 0xF, false)));
+}
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+  x = dpp_max<0xB1>(x);   // quad_perm [1, 0, 3, 2]
+  x = dpp_max<0x4E>(x);   // quad_perm [2, 3, 0, 1]
+  x = dpp_max<0x141>(x);  // row_half_mirror
+  x = dpp_max<0x140>(x);  // row_mirror
+  const unsigned a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+  const unsigned c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+  return max(max(a, b), max(c, d));
+}
+__device__ __forceinline__ u64 wave_max(u64 x) {
+  const unsigned hi = static_cast<unsigned>(x >> 32);
+  const unsigned top = wave_max(hi);
+  const unsigned low = wave_max(hi == top ? static_cast<unsigned>(x) : 0u);
+  return (static_cast<u64>(top) << 32) | low;
+}
+
+// One wave's `k` best keys, in descending order in list[0 .. count).
+struct Best {
+  u64* list;  // LDS, kWaveList entries
+  int k;
+  int count;
+  u64 floor;  // a key at or below it is not among them: the k-th best where there are k
+
+  // Adds N keys of each lane (0: none; all others differ).
+  template <int N>
+  __device__ __forceinline__ void offer(const u64 (&key)[N], int lane) {
+    u64 top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = max(top, key[i]);
+    const int lanes = __builtin_popcountll(__ballot(top > floor));
+    if (lanes == 0) return;
+    u64 least = floor;  // keys above it are taken
+    if (lanes > k) {
+      // the k-th best of the lanes' best keys: at least k keys are that large, and they
+      // are in k lanes
+      u64 t = top;
+      for (int i = 0; i < k; ++i) {
+        least = wave_max(t);
+        if (t == least) t = 0;
+      }
+      least -= 1;
+    }
+    int n = count;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bool in = key[i] > least;
+      const u64 mask = __ballot(in);
+      if (mask != 0) {
+        const int at = n + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
+        if (in) list[at] = key[i];
+        n += __builtin_popcountll(mask);
+      }
+    }
+    sort(n, lane);
+  }
+
+  // Brings the k best of list[0 .. n) to its front, in order: each entry's place is the
+  // number of larger ones.
+  __device__ __forceinline__ void sort(int n, int lane) {
+    wave_sync();
+    const int keep = min(n, k);
+    u64 mine[(kWaveList + 63) / 64];
+    int place[(kWaveList + 63) / 64];
+    const int steps = (n + 63) / 64;
+    if (steps == 1) {
+      mine[0] = lane < n ? list[lane] : 0;
+      place[0] = 0;
+      for (int j = 0; j < n; ++j) place[0] += list[j] > mine[0];
+      wave_sync();
+      if (lane < n && place[0] < keep) list[place[0]] = mine[0];
+    } else {
+#pragma unroll
+      for (int s = 0; s < (kWaveList + 63) / 64; ++s) {
+        mine[s] = 64 * s + lane < n ? list[64 * s + lane] : 0;
+        place[s] = 0;
+      }
+      for (int j = 0; j < n; ++j) {
+        const u64 x = list[j];
+#pragma unroll
+        for (int s = 0; s < (kWaveList + 63) / 64; ++s) place[s] += x > mine[s];
+      }
+      wave_sync();
+#pragma unroll
+      for (int s = 0; s < (kWaveList + 63) / 64; ++s)
+        if (mine[s] != 0 && place[s] < keep) list[place[s]] = mine[s];
+    }
+    wave_sync();
+    count = keep;
+    floor = count == k ? list[k - 1] : 0;
+  }
+
+  // LDS accesses of this wave before it are done before those behind it.
+  __device__ static __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+};
+
+struct SelectArgs {
+  const void* logits;
+  long long ld;
+  const float* scores;
+  const unsigned char* finished;
+  float* out_scores;
+  int* out_parent;
+  int* out_token;
+  unsigned char* out_finished;
+  int beams, n_out, vocab, eos;
+  int pieces;      // of a row
+  int piece;       // values of one, a multiple of kStep
+  u64* keys;       // [rows][pieces][n_out], 0 behind the last one
+  floatx2* sums;   // [rows][pieces]: max, sum of exp(x - max)
+};
+
+constexpr int kStep = 64 * kWaves * kVpt;  // values of a workgroup's step
+
+// One workgroup per (row, piece). NaN in a row makes its sum NaN, +inf too.
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
+  constexpr int VEC = 16 / sizeof(T);
+  __shared__ u64 s_list[kWaves][kWaveList];
+  __shared__ float s_max[kWaves], s_sum[kWaves];
+  __shared__ int s_count[kWaves];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const unsigned row = blockIdx.x / static_cast<unsigned>(a.pieces);
+  const int piece = static_cast<int>(blockIdx.x - row * static_cast<unsigned>(a.pieces));
+  const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+  const int begin = piece * a.piece;
+  const int end = min(begin + a.piece, a.vocab);
+
+  Best best = {s_list[wave], a.n_out, 0, 0};
+  float m = kNegInf, sum = 0.0f;
+  for (int at = begin; at < end; at += kStep) {
+    float v[kVpt];
+    u64 key[kVpt];
+#pragma unroll
+    for (int i = 0; i < kVpt / VEC; ++i) {
+      const int t0 = at + (i * 64 * kWaves + tid) * VEC;
+      if (VECTOR && t0 + VEC <= end) {
+        const uintx4 w = *reinterpret_cast<const uintx4*>(x + t0);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          if constexpr (sizeof(T) == 4) {
+            const unsigned u = w[e];
+            v[i * VEC + e] = __uint_as_float(u);
+          } else {
+            const unsigned short h = static_cast<unsigned short>(w[e / 2] >> (16 * (e % 2)));
+            v[i * VEC + e] = static_cast<float>(__builtin_bit_cast(_Float16, h));
+          }
+          key[i * VEC + e] = key_of(v[i * VEC + e], static_cast<unsigned>(t0 + e));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const bool in = t0 + e < end;
+          v[i * VEC + e] = in ? static_cast<float>(x[t0 + e]) : kNegInf;
+          key[i * VEC + e] = in ? key_of(v[i * VEC + e], static_cast<unsigned>(t0 + e)) : 0;
+        }
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kVpt; ++i) top = fmaxf(top, v[i]);
+    // (all -inf so far: against 0, whose sum stays 0)
+    const float ref = top == kNegInf ? 0.0f : top;
+    sum *= expf(m - ref);
+    m = top;
+#pragma unroll
+    for (int i = 0; i < kVpt; ++i) sum += expf(v[i] - ref);
+    best.offer(key, lane);
+  }
+  // the wave's max and sum
+  float wm = m;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) wm = fmaxf(wm, __shfl_xor(wm, off));
+  const float ref = wm == kNegInf ? 0.0f : wm;
+  const float ws = gemv::wave_sum(sum * expf(m - ref));
+  if (lane == 0) {
+    s_max[wave] = wm;
+    s_sum[wave] = ws;
+    s_count[wave] = best.count;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  // the other waves' keys behind its own
+  int n = best.count;
+  for (int w = 1; w < kWaves; ++w) {
+    const int c = s_count[w];
+    if (lane < c) best.list[n + lane] = s_list[w][lane];
+    n += c;
+  }
+  best.sort(n, lane);
+  const long long out = static_cast<long long>(blockIdx.x);
+  for (int i = lane; i < a.n_out; i += 64) a.keys[out * a.n_out + i] = i < best.count ? best.list[i] : 0;
+  if (lane == 0) {
+    float top = kNegInf;
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_max[w]);
+    const float r = top == kNegInf ? 0.0f : top;
+    float s = 0.0f;
+    for (int w = 0; w < kWaves; ++w) s += s_sum[w] * expf(s_max[w] - r);
+    a.sums[out] = floatx2{top, s};
+  }
+}
+
+// One workgroup per group: each wave joins the pieces of beams wave, wave + 4, ..; then
+// the beams' candidates are put in order by (score, beam, token). A candidate whose score
+// is no number, or of a beam without a finite score, counts as -inf; such a beam's come
+// in the order of the tokens, so its first n_out stand for it.
+__global__ __launch_bounds__(64 * kWaves) void join_kernel(SelectArgs a) {
+  __shared__ u64 s_list[kWaves][kWaveList];
+  __shared__ double s_score[kMaxBeams * kMaxOut];
+  __shared__ int s_token[kMaxBeams * kMaxOut];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const long long group = blockIdx.x;
+  const int k = a.n_out;
+  const double ninf = -__builtin_huge_val();
+  for (int b = wave; b < a.beams; b += kWaves) {
+    const long long row = group * a.beams + b;
+    const float given = a.scores[row];
+    const bool done = a.finished != nullptr && a.finished[row] != 0;
+    float m = kNegInf;
+    for (int i = lane; i < a.pieces; i += 64) m = fmaxf(m, a.sums[row * a.pieces + i][0]);
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
+    double sum = 0.0;
+    for (int i = lane; i < a.pieces; i += 64) {
+      const floatx2 p = a.sums[row * a.pieces + i];
+      sum += static_cast<double>(p[1]) * (p[0] == kNegInf ? 1.0 : exp(static_cast<double>(p[0]) - m));
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
+    const double lse = static_cast<double>(m) + log(sum);
+    const bool finite = given > kNegInf && given < -kNegInf;
+    const bool plain = !done && finite && lse - lse == 0.0;
+    Best best = {s_list[wave], k, 0, 0};
+    if (plain) {
+      const long long n = static_cast<long long>(a.pieces) * k;
+      const u64* keys = a.keys + row * n;
+      for (long long i0 = 0; i0 < n; i0 += 64 * 4) {
+        u64 key[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) key[j] = i0 + 64 * j + lane < n ? keys[i0 + 64 * j + lane] : 0;
+        best.offer(key, lane);
+      }
+    }
+    for (int i = lane; i < k; i += 64) {
+      double score = ninf;
+      int token = i;
+      if (plain) {
+        // (fewer than k tokens in the vocabulary: none)
+        token = -1;
+        if (i < best.count) {
+          const u64 key = best.list[i];
+          token = static_cast<int>(token_of(key));
+          score = static_cast<double>(given) + (static_cast<double>(logit_of(key)) - lse);
+        }
+      } else if (done && finite) {
+        // its end token first, then the others
+        token = i == 0 ? a.eos : i - 1 < a.eos ? i - 1 : i;
+        if (i == 0) score = given;
+      }
+      if (token >= a.vocab) token = -1;
+      s_score[b * k + i] = score == score ? score : ninf;
+      s_token[b * k + i] = token;
+    }
+  }
+  __syncthreads();
+  const int n = a.beams * k;
+  for (int i = tid; i < n; i += 64 * kWaves) {
+    const double score = s_score[i];
+    const int token = s_token[i];
+    if (token < 0) continue;
+    const int b = i / k;
+    int place = 0;  // (a beam's own are in order)
+    for (int j = 0; j < n; ++j) place += s_token[j] >= 0 && (s_score[j] > score || (s_score[j] == score && j < i));
+    if (place < k) {
+      const long long out = group * k + place;
+      a.out_scores[out] = static_cast<float>(score);
+      a.out_parent[out] = b;
+      a.out_token[out] = token;
+      if (a.out_finished != nullptr)
+        a.out_finished[out] = (a.finished != nullptr && a.finished[group * a.beams + b] != 0) || token == a.eos;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------- reorder
+
+struct ReorderArgs {
+  const unsigned char* src[2];
+  unsigned char* dst[2];
+  const float* src_scale[2];
+  float* dst_scale[2];
+  const int* parent;
+  const int* lens;
+  int beams, heads;
+  long long max_len;
+  long long head_bytes;    // of a head's cache
+  long long scale_blocks;  // of a head
+  unsigned chunks;         // workgroups of a head
+  int row_bytes;           // of a token
+  bool in_place;
+};
+
+// One workgroup per (group, head, K or V, 256 16-byte columns of the head's cache): a
+// thread loads its column of every beam's parent, then stores to the beams, so the beams
+// of a group may change places in their own buffers. A parent that several beams share is
+// read once from memory and then from the caches. The thread of a 32-token block's first
+// column moves the block's scale.
+template <int MB>
+__global__ __launch_bounds__(256) void reorder_kernel(ReorderArgs a) {
+  const unsigned chunk = blockIdx.x % a.chunks;
+  const unsigned rest = blockIdx.x / a.chunks;
+  const int side = static_cast<int>(rest & 1);
+  const unsigned heads = static_cast<unsigned>(a.heads);
+  const unsigned gh = rest >> 1;
+  const long long group = gh / heads;
+  const long long head = gh - static_cast<unsigned>(group) * heads;
+  const long long at = (static_cast<long long>(chunk) * 256 + threadIdx.x) * 16;
+  const long long token = at / a.row_bytes;
+  const long long first = group * a.beams;
+  const long long beam_bytes = a.head_bytes * heads;
+  const long long base = (first * heads + head) * a.head_bytes + at;
+  const unsigned char* src = a.src[side] + base;
+  unsigned char* dst = a.dst[side] + base;
+  uintx4 v[MB];
+  bool go[MB];
+#pragma unroll
+  for (int j = 0; j < MB; ++j) {
+    go[j] = false;
+    if (j < a.beams) {
+      const int p = a.parent[first + j];
+      if (p >= 0 && p < a.beams && !(a.in_place && p == j)) {
+        go[j] = token < std::min<long long>(a.lens[first + p], a.max_len);
+        if (go[j]) v[j] = *reinterpret_cast<const uintx4*>(src + p * beam_bytes);
+      }
+    }
+  }
+  float s[MB];
+  const bool scales = a.src_scale[side] != nullptr && at % (32ll * a.row_bytes) == 0;
+  const long long beam_blocks = a.scale_blocks * heads;
+  const long long sbase = (first * heads + head) * a.scale_blocks + token / 32;
+  if (scales) {
+#pragma unroll
+    for (int j = 0; j < MB; ++j)
+      if (go[j]) s[j] = a.src_scale[side][sbase + a.parent[first + j] * beam_blocks];
+  }
+#pragma unroll
+  for (int j = 0; j < MB; ++j)
+    if (go[j]) *reinterpret_cast<uintx4*>(dst + j * beam_bytes) = v[j];
+  if (scales) {
+#pragma unroll
+    for (int j = 0; j < MB; ++j)
+      if (go[j]) a.dst_scale[side][sbase + j * beam_blocks] = s[j];
+  }
+}
+
+void select_entry(const void* logits, bool half, int64_t ld, const float* scores, const uint8_t* finished,
+                  float* out_scores, int32_t* out_parent, int32_t* out_token, uint8_t* out_finished,
+                  int64_t batch, int64_t beams, int64_t n_out, int64_t vocab, int64_t eos, hipStream_t s) {
+  ENG_CHECK(batch >= 0, "beam_select: batch must be non-negative");
+  ENG_CHECK(beams > 0 && beams <= kMaxBeams, "beam_select: beams must be 1 to 32");
+  ENG_CHECK(n_out > 0 && n_out <= kMaxOut, "beam_select: n_out must be 1 to 64");
+  ENG_CHECK(vocab > 0 && vocab < 0x7fffffffLL - kStep, "beam_select: vocab must be positive and below 2^31 - 4097");
+  ENG_CHECK(n_out <= beams * vocab, "beam_select: n_out > beams * vocab");
+  ENG_CHECK(ld >= vocab, "beam_select: ld < vocab");
+  ENG_CHECK(eos < vocab, "beam_select: eos >= vocab");
+  if (batch == 0) return;
+  ENG_CHECK(logits != nullptr, "beam_select: logits is null");
+  ENG_CHECK(scores != nullptr, "beam_select: scores is null");
+  ENG_CHECK(out_scores != nullptr && out_parent != nullptr && out_token != nullptr,
+            "beam_select: out_scores/out_parent/out_token is null");
+  ENG_CHECK(finished == nullptr || eos >= 0, "beam_select: finished beams need eos");
+  const long long elem = half ? 2 : 4;
+  ENG_CHECK(aligned_to(logits, elem), "beam_select: logits must be aligned to their type");
+  SelectArgs a = {};
+  a.logits = logits;
+  a.ld = ld;
+  a.scores = scores;
+  a.finished = finished;
+  a.out_scores = out_scores;
+  a.out_parent = out_parent;
+  a.out_token = out_token;
+  a.out_finished = out_finished;
+  a.beams = static_cast<int>(beams);
+  a.n_out = static_cast<int>(n_out);
+  a.vocab = static_cast<int>(vocab);
+  a.eos = eos < 0 ? -1 : static_cast<int>(eos);
+  // Pieces of a row: a workgroup's step each while that leaves fewer than four to a CU.
+  const long long steps = (vocab + kStep - 1) / kStep;
+  ENG_CHECK(batch <= 0xffffffffLL / (64 * kWaves) / (beams * steps),
+            "beam_select: too many logits for one launch");
+  const long long rows = batch * beams;
+  const long long want = std::max(1ll, 4ll * device_cu_count() / rows);
+  const long long per = (steps + std::min(steps, want) - 1) / std::min(steps, want);
+  a.piece = static_cast<int>(per * kStep);
+  a.pieces = static_cast<int>((steps + per - 1) / per);
+  const std::size_t lists = static_cast<std::size_t>(rows) * a.pieces;
+  StreamScratch scratch(s, lists * (n_out + 1) * 8);
+  a.keys = static_cast<u64*>(scratch.get());
+  a.sums = reinterpret_cast<floatx2*>(a.keys + lists * n_out);
+  const bool vector = aligned_to(logits, 16) && (ld * elem) % 16 == 0;
+  const unsigned grid = static_cast<unsigned>(lists);
+  auto go = [&](auto kernel) { kernel<<<grid, 64 * kWaves, 0, s>>>(a); };
+  if (half) vector ? go(piece_kernel<_Float16, true>) : go(piece_kernel<_Float16, false>);
+  else vector ? go(piece_kernel<float, true>) : go(piece_kernel<float, false>);
+  ENG_LAUNCH_CHECK();
+  join_kernel<<<static_cast<unsigned>(batch), 64 * kWaves, 0, s>>>(a);
+  ENG_LAUNCH_CHECK();
+}
+
+void reorder_entry(const void* k_src, const void* v_src, const float* ks_src, const float* vs_src, void* k_dst,
+                   void* v_dst, float* ks_dst, float* vs_dst, bool q8, const int32_t* parent,
+                   const int32_t* kv_len, int64_t batch, int64_t beams, int64_t n_kv_heads, int64_t head_dim,
+                   int64_t max_kv_len, int64_t kv_max_seq_len, hipStream_t s) {
+  ENG_CHECK(batch >= 0, "kv_cache_reorder: batch must be non-negative");
+  ENG_CHECK(beams > 0 && beams <= kMaxBeams, "kv_cache_reorder: beams must be 1 to 32");
+  ENG_CHECK(n_kv_heads > 0, "kv_cache_reorder: n_kv_heads must be positive");
+  ENG_CHECK(head_dim == 64 || head_dim == 128, "kv_cache_reorder: head_dim must be 64 or 128");
+  ENG_CHECK(max_kv_len >= 0, "kv_cache_reorder: max_kv_len must be non-negative");
+  ENG_CHECK(kv_max_seq_len >= max_kv_len, "kv_cache_reorder: kv_max_seq_len < max_kv_len");
+  ENG_CHECK(kv_max_seq_len <= 0x7fffffffLL - 32, "kv_cache_reorder: kv_max_seq_len must be below 2^31 - 32");
+  if (batch == 0 || max_kv_len == 0) return;
+  ENG_CHECK(k_src != nullptr && v_src != nullptr, "kv_cache_reorder: k_src/v_src is null");
+  ENG_CHECK(k_dst != nullptr && v_dst != nullptr, "kv_cache_reorder: k_dst/v_dst is null");
+  ENG_CHECK(!q8 || (ks_src != nullptr && vs_src != nullptr && ks_dst != nullptr && vs_dst != nullptr),
+            "kv_cache_reorder: a scale buffer is null");
+  ENG_CHECK(parent != nullptr, "kv_cache_reorder: parent is null");
+  ENG_CHECK(kv_len != nullptr, "kv_cache_reorder: kv_len is null");
+  ENG_CHECK(aligned_to(k_src, 16) && aligned_to(v_src, 16) && aligned_to(k_dst, 16) && aligned_to(v_dst, 16),
+            "kv_cache_reorder: the caches must be 16-byte aligned");
+  const bool in_place = k_src == k_dst;
+  ENG_CHECK(in_place == (v_src == v_dst) && (!q8 || (in_place == (ks_src == ks_dst) && in_place == (vs_src == vs_dst))),
+            "kv_cache_reorder: all buffers in place, or none");
+  ReorderArgs a = {};
+  a.src[0] = static_cast<const unsigned char*>(k_src);
+  a.src[1] = static_cast<const unsigned char*>(v_src);
+  a.dst[0] = static_cast<unsigned char*>(k_dst);
+  a.dst[1] = static_cast<unsigned char*>(v_dst);
+  a.src_scale[0] = ks_src;
+  a.src_scale[1] = vs_src;
+  a.dst_scale[0] = ks_dst;
+  a.dst_scale[1] = vs_dst;
+  a.parent = parent;
+  a.lens = kv_len;
+  a.beams = static_cast<int>(beams);
+  a.max_len = max_kv_len;
+  a.row_bytes = static_cast<int>(head_dim * (q8 ? 1 : 2));
+  a.head_bytes = kv_max_seq_len * a.row_bytes;
+  a.scale_blocks = (kv_max_seq_len + 31) / 32;
+  a.in_place = in_place;
+  const long long chunks = (max_kv_len * a.row_bytes / 16 + 255) / 256;
+  ENG_CHECK(n_kv_heads <= 0x7fffffffLL && batch <= 0xffffffffLL / 256 / 2 / chunks / n_kv_heads,
+            "kv_cache_reorder: too many (group, head, token) units for one launch");
+  a.heads = static_cast<int>(n_kv_heads);
+  a.chunks = static_cast<unsigned>(chunks);
+  const unsigned grid = static_cast<unsigned>(batch * n_kv_heads * 2 * chunks);
+  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(a); };
+  if (beams <= 4) go(reorder_kernel<4>);
+  else if (beams <= 8) go(reorder_kernel<8>);
+  else if (beams <= 16) go(reorder_kernel<16>);
+  else go(reorder_kernel<32>);
+  ENG_LAUNCH_CHECK();
+}
+
+}  // namespace
+}  // namespace beam
+}  // namespace eng
+
+using eng::guarded;
+
+extern "C" {
+
+int eng_beam_select_f32(const float* logits, int64_t ld, const float* scores, const uint8_t* finished,
+                        float* out_scores, int32_t* out_parent, int32_t* out_token,
+                        uint8_t* out_finished, int64_t batch, int64_t beams, int64_t n_out,
+                        int64_t vocab, int64_t eos, eng_stream stream) {
+  return guarded([&] {
+    eng::beam::select_entry(logits, false, ld, scores, finished, out_scores, out_parent, out_token, out_finished,
+                            batch, beams, n_out, vocab, eos, eng::as_stream(stream));
+  });
+}
+
+int eng_beam_select_f16(const eng_half* logits, int64_t ld, const float* scores, const uint8_t* finished,
+                        float* out_scores, int32_t* out_parent, int32_t* out_token,
+                        uint8_t* out_finished, int64_t batch, int64_t beams, int64_t n_out,
+                        int64_t vocab, int64_t eos, eng_stream stream) {
+  return guarded([&] {
+    eng::beam::select_entry(logits, true, ld, scores, finished, out_scores, out_parent, out_token, out_finished,
+                            batch, beams, n_out, vocab, eos, eng::as_stream(stream));
+  });
+}
+
+int eng_kv_cache_reorder_f16(const eng_half* k_src, const eng_half* v_src, eng_half* k_dst, eng_half* v_dst,
+                             const int32_t* parent, const int32_t* kv_len, int64_t batch, int64_t beams,
+                             int64_t n_kv_heads, int64_t head_dim, int64_t max_kv_len,
+                             int64_t kv_max_seq_len, eng_stream stream) {
+  return guarded([&] {
+    eng::beam::reorder_entry(k_src, v_src, nullptr, nullptr, k_dst, v_dst, nullptr, nullptr, false, parent, kv_len,
+                             batch, beams, n_kv_heads, head_dim, max_kv_len, kv_max_seq_len, eng::as_stream(stream));
+  });
+}
+
+int eng_kv_cache_reorder_q8(const uint8_t* k_src, const uint8_t* v_src, const float* k_scale_src,
+                            const float* v_scale_src, uint8_t* k_dst, uint8_t* v_dst, float* k_scale_dst,
+                            float* v_scale_dst, const int32_t* parent, const int32_t* kv_len,
+                            int64_t batch, int64_t beams, int64_t n_kv_heads, int64_t head_dim,
+                            int64_t max_kv_len, int64_t kv_max_seq_len, eng_stream stream) {
+  return guarded([&] {
+    eng::beam::reorder_entry(k_src, v_src, k_scale_src, v_scale_src, k_dst, v_dst, k_scale_dst, v_scale_dst, true,
+                             parent, kv_len, batch, beams, n_kv_heads, head_dim, max_kv_len, kv_max_seq_len,
+                             eng::as_stream(stream));
+  });
+}
+
+}  // extern "C"

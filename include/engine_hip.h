@@ -594,6 +594,54 @@ int eng_attention_prefix_q8(const eng_half* q, const uint8_t* k_prefix, const ui
                             float scale, int split_kv, eng_stream stream);
 
 /* ------------------------------------------------------------------------
+ * Beam search over a batch of groups of `beams` sequences (additive, no reference
+ * counterpart): the next candidates, and the caches brought in line with them.
+ *
+ * eng_beam_select_*: logits [batch * beams rows of ld], the first `vocab` of a row
+ * counting; scores [batch, beams], the beams' sums of log-probabilities so far.
+ * Candidate (b, t) scores scores[b] + logits[b][t] - log sum_u exp logits[b][u]. The
+ * n_out best of a group's beams * vocab candidates come out in descending order:
+ * out_scores, out_parent (the beam, 0 .. beams - 1) and out_token [batch, n_out].
+ * Candidates of one beam are compared by their logits, those of unlike beams by
+ * their scores in 64 bits; ties go to the lower beam, then the lower token. finished
+ * [batch, beams] (bytes; NULL: none) marks beams that have ended: such a beam has
+ * one candidate, token eos with its score unchanged, and needs no valid logits. out_finished
+ * [batch, n_out] (may be NULL) is 1 where the parent has ended or the token is eos
+ * (eos < 0: no token is). A candidate whose score is -inf or no number ranks last, as
+ * -inf: all of a beam's whose score is not finite or whose row holds a NaN, +inf or only
+ * -inf, and all but one of a finished beam's. beams is 1 to 32, n_out 1 to 64 and at most beams
+ * * vocab. Outputs must not overlap inputs. Uses the stream's scratch arena.
+ *
+ * eng_kv_cache_reorder_*: sequence (g, j) of the caches [batch * beams, n_kv_heads,
+ * kv_max_seq_len, head_dim] gets the first kv_len[g beams + p] tokens of sequence
+ * (g, p), p = parent[g][j] (out_parent with n_out == beams), into buffers of the
+ * same shape, or, with the same pointers as source and destination, in place: beams
+ * that keep their place (p == j) are then not touched. 8-bit caches move with the
+ * scales of the blocks that the tokens reach. Tokens behind the length stay as they
+ * were, and so does a sequence whose p is outside 0 .. beams - 1. Lengths are at
+ * most max_kv_len, beyond it they are taken as it. kv_len is not reordered. Source and destination
+ * buffers must be the same or not overlap; head_dim is 64 or 128, caches are 16-byte
+ * aligned.
+ * ---------------------------------------------------------------------- */
+int eng_beam_select_f32(const float* logits, int64_t ld, const float* scores, const uint8_t* finished,
+                        float* out_scores, int32_t* out_parent, int32_t* out_token,
+                        uint8_t* out_finished, int64_t batch, int64_t beams, int64_t n_out,
+                        int64_t vocab, int64_t eos, eng_stream stream);
+int eng_beam_select_f16(const eng_half* logits, int64_t ld, const float* scores, const uint8_t* finished,
+                        float* out_scores, int32_t* out_parent, int32_t* out_token,
+                        uint8_t* out_finished, int64_t batch, int64_t beams, int64_t n_out,
+                        int64_t vocab, int64_t eos, eng_stream stream);
+int eng_kv_cache_reorder_f16(const eng_half* k_src, const eng_half* v_src, eng_half* k_dst, eng_half* v_dst,
+                             const int32_t* parent, const int32_t* kv_len, int64_t batch, int64_t beams,
+                             int64_t n_kv_heads, int64_t head_dim, int64_t max_kv_len,
+                             int64_t kv_max_seq_len, eng_stream stream);
+int eng_kv_cache_reorder_q8(const uint8_t* k_src, const uint8_t* v_src, const float* k_scale_src,
+                            const float* v_scale_src, uint8_t* k_dst, uint8_t* v_dst, float* k_scale_dst,
+                            float* v_scale_dst, const int32_t* parent, const int32_t* kv_len,
+                            int64_t batch, int64_t beams, int64_t n_kv_heads, int64_t head_dim,
+                            int64_t max_kv_len, int64_t kv_max_seq_len, eng_stream stream);
+
+/* ------------------------------------------------------------------------
  * ENGREF01 tensor files and device weight slabs.
  *
  * The container is the reference's golden format (tools/gen_reference.py:

@@ -139,3 +139,30 @@ def check(got, want, what):
         bad = err > bound[fin]
         assert not bad.any(), (f"{what} {at}: error {err[bad].max():.3g} over a bound of "
                                f"{bound[fin][bad].min():.3g}, {bad.sum()} of {bad.size}")
+
+
+# ---------------------------------------------------------------- beam search
+def select64(logits, scores, finished, n_out, eos):
+    """(scores, parent, token, finished) of one group: logits [beams, V] float64."""
+    beams, V = logits.shape
+    cand = np.full((beams, V), -np.inf)
+    order = np.zeros((beams, V))  # candidates of a beam compare by their logits
+    for b in range(beams):
+        if not np.isfinite(scores[b]):
+            continue
+        if finished is not None and finished[b]:
+            cand[b, eos] = scores[b]
+            continue
+        x = logits[b]
+        if np.isnan(x).any() or x.max() in (np.inf, -np.inf):
+            continue
+        lse = x.max() + np.log(np.exp(x - x.max()).sum())
+        cand[b] = scores[b] + (x - lse)
+        order[b] = x
+    beam = np.repeat(np.arange(beams), V)
+    token = np.tile(np.arange(V), beams)
+    at = np.lexsort((token, -order.reshape(-1), beam, -cand.reshape(-1)))
+    at = at[:n_out]
+    s, p, t = cand.reshape(-1)[at], beam[at], token[at]
+    f = np.array([(finished is not None and bool(finished[b])) or u == eos for b, u in zip(p, t)])
+    return s, p, t, f
