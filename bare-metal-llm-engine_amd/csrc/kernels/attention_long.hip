@@ -2,7 +2,7 @@
 // one token each, with a sliding window and first tokens that stay visible, and single
 // tokens over a prefix that several sequences share. Caches are fp16 or e4m3 (kv_q8.hip
 // has the format).
-#include "attention_tiles.hpp"
+#include "attention_few.hpp"
 
 #include <cmath>
 
@@ -74,22 +74,31 @@ void merge(const Args& a, long long rows, int states, hipStream_t s) {
   ENG_LAUNCH_CHECK();
 }
 
+// Launches of a part: the tiles of 128 rows, or up to two parts of few rows together.
 template <int D>
-void tiles(const Args& a, long long units, bool q8, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(units * a.row_tiles), static_cast<unsigned>(a.nsplit));
+void tiles(const Args& a, bool q8, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(a.units * a.row_tiles), static_cast<unsigned>(a.nsplit));
   if (q8) tile_kernel<D, true><<<grid, 64 * kTileWaves, 0, s>>>(a);
   else tile_kernel<D, false><<<grid, 64 * kTileWaves, 0, s>>>(a);
   ENG_LAUNCH_CHECK();
 }
+template <int D>
+void few(const Args& a, const Args& b, bool q8, hipStream_t s) {
+  const long long wgs0 = a.units * a.row_tiles * a.nsplit;
+  const long long wgs = wgs0 + b.units * b.row_tiles * b.nsplit;
+  if (q8) few_kernel<D, true><<<static_cast<unsigned>(wgs), 64 * kFewWaves, 0, s>>>(a, b, static_cast<unsigned>(wgs0));
+  else few_kernel<D, false><<<static_cast<unsigned>(wgs), 64 * kFewWaves, 0, s>>>(a, b, static_cast<unsigned>(wgs0));
+  ENG_LAUNCH_CHECK();
+}
 
-int row_tiles_of(long long rows) { return static_cast<int>((rows + kTileRows - 1) / kTileRows); }
+int tiles_of(long long rows, int tile) { return static_cast<int>((rows + tile - 1) / tile); }
 
-// Splits of the keys for `wgs` workgroups that read up to `keys` keys each: two workgroups
-// per CU, at least four tiles a split.
-int auto_splits(long long wgs, long long keys) {
-  const long long tiles = (keys + kTileKeys - 1) / kTileKeys;
+// Splits of the keys of `wgs` workgroups that read up to `keys` keys each, in steps of
+// `step` keys.
+int auto_splits(long long wgs, long long keys, long long step) {
+  const long long steps = (keys + step - 1) / step;
   const long long want = 2ll * device_cu_count() / wgs;
-  return static_cast<int>(std::max(1ll, std::min({want, tiles / 4, static_cast<long long>(kMaxStates)})));
+  return static_cast<int>(std::max(1ll, std::min({want, steps / 4, static_cast<long long>(kMaxStates)})));
 }
 
 constexpr long long kMaxLen = 0x7fffffffLL - kKvBlock;  // positions are 32-bit on the device
@@ -100,54 +109,73 @@ std::size_t state_bytes(long long rows, int states, long long D) {
 }
 
 void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hipStream_t s) {
-  const long long units = batch * a.n_kv;
   const long long rows = batch * a.s_new * a.n_heads;
   const long long unit_rows = static_cast<long long>(a.s_new) * a.group;
+  const bool one = a.s_new == 1;  // a unit's rows see the same keys
+  const int tile = one ? kFewRows : kTileRows;
+  a.units = batch * a.n_kv;
   ENG_CHECK(unit_rows <= 0x3fffffffLL && rows <= 0xffffffffLL - 4 && threads_fit((rows + 3) / 4, 256) &&
-                threads_fit(units * row_tiles_of(unit_rows), 64 * kTileWaves),
+                threads_fit(a.units, 256) && threads_fit(a.units * tiles_of(unit_rows, tile), 256),
             "attention_window: too many query rows for one launch");
-  a.row_tiles = row_tiles_of(unit_rows);
+  a.row_tiles = tiles_of(unit_rows, tile);
   long long keys = a.max_len;  // what a tile of rows can see
   if (a.window != 0)
-    keys = std::min(keys, a.window + a.sinks + std::min<long long>(a.s_new, kTileRows / a.group + 2) + kKvBlock);
-  const long long most = std::max(1ll, (keys + kTileKeys - 1) / kTileKeys);
-  a.nsplit = split_kv == 0 ? auto_splits(units * a.row_tiles, keys)
+    keys = std::min(keys, a.window + a.sinks + std::min<long long>(a.s_new, tile / a.group + 2) + kKvBlock);
+  const long long step = one ? kKvBlock : kTileKeys;
+  const long long most = std::max(1ll, (keys + step - 1) / step);
+  a.nsplit = split_kv == 0 ? auto_splits(a.units * a.row_tiles, keys, step)
                            : static_cast<int>(std::min<long long>({split_kv, most, kMaxStates}));
+  if (one)
+    ENG_CHECK(threads_fit(a.units * a.row_tiles * a.nsplit, 256),
+              "attention_window: too many query rows and splits for one launch");
   a.part_stride = a.nsplit;
   auto go = [&](auto dim) {
     constexpr int kD = decltype(dim)::value;
+    auto launch = [&] {
+      if (one) few<kD>(a, Args{}, q8, s);
+      else tiles<kD>(a, q8, s);
+    };
     if (a.nsplit == 1) {
-      tiles<kD>(a, units, q8, s);
+      launch();
       return;
     }
     StreamScratch scratch(s, state_bytes(rows, a.nsplit, kD));
     a.part_o = static_cast<float*>(scratch.get());
     a.part_ml = a.part_o + rows * a.nsplit * kD;
-    tiles<kD>(a, units, q8, s);
+    launch();
     merge<kD>(a, rows, a.nsplit, s);
   };
   if (D == 64) go(std::integral_constant<int, 64>{});
   else go(std::integral_constant<int, 128>{});
 }
 
+// Shared rows of a KV head up to which the prefix is read in tiles of 16 of them.
+constexpr long long kFewShared = 32;
+
 void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, long long D, int split_kv,
                 bool q8, hipStream_t s) {
   const long long rows = batch * mine.n_heads;
   const long long unit_rows = static_cast<long long>(shared.s_new) * shared.group;
+  const bool few_shared = unit_rows <= kFewShared;
+  const int tile = few_shared ? kFewRows : kTileRows;
+  shared.units = n_prefix * shared.n_kv;
+  mine.units = batch * mine.n_kv;
   ENG_CHECK(unit_rows <= 0x3fffffffLL && rows <= 0xffffffffLL - 4 && threads_fit((rows + 3) / 4, 256) &&
-                threads_fit(n_prefix * shared.n_kv * row_tiles_of(unit_rows), 64 * kTileWaves) &&
-                threads_fit(batch * mine.n_kv * row_tiles_of(mine.group), 64 * kTileWaves),
+                threads_fit(shared.units, 256) && threads_fit(mine.units, 256),
             "attention_prefix: too many query rows for one launch");
-  shared.row_tiles = row_tiles_of(unit_rows);
-  mine.row_tiles = row_tiles_of(mine.group);
-  auto splits = [&](const Args& a, long long units) {
+  shared.row_tiles = tiles_of(unit_rows, tile);
+  mine.row_tiles = tiles_of(mine.group, kFewRows);
+  auto splits = [&](const Args& a, long long step) {
     if (a.max_len == 0) return 0;
-    const long long most = (a.max_len + kTileKeys - 1) / kTileKeys;
-    return split_kv == 0 ? std::min(auto_splits(units * a.row_tiles, a.max_len), kMaxStates / 2)
+    const long long most = (a.max_len + step - 1) / step;
+    return split_kv == 0 ? std::min(auto_splits(a.units * a.row_tiles, a.max_len, step), kMaxStates / 2)
                          : static_cast<int>(std::min<long long>({split_kv, most, kMaxStates / 2}));
   };
-  shared.nsplit = splits(shared, n_prefix * shared.n_kv);
-  mine.nsplit = splits(mine, batch * mine.n_kv);
+  shared.nsplit = splits(shared, few_shared ? kKvBlock : kTileKeys);
+  mine.nsplit = splits(mine, kKvBlock);
+  ENG_CHECK(threads_fit(shared.units * shared.row_tiles * std::max(1, few_shared ? shared.nsplit : 1) +
+                            mine.units * mine.row_tiles * std::max(1, mine.nsplit), 256),
+            "attention_prefix: too many query rows for one launch");
   const int states = shared.nsplit + mine.nsplit;
   shared.part_stride = mine.part_stride = states;
   mine.part0 = shared.nsplit;
@@ -156,8 +184,9 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
     StreamScratch scratch(s, state_bytes(rows, states, kD));
     shared.part_o = mine.part_o = static_cast<float*>(scratch.get());
     shared.part_ml = mine.part_ml = shared.part_o + rows * states * kD;
-    if (shared.nsplit > 0) tiles<kD>(shared, n_prefix * shared.n_kv, q8, s);
-    if (mine.nsplit > 0) tiles<kD>(mine, batch * mine.n_kv, q8, s);
+    if (!few_shared && shared.nsplit > 0) tiles<kD>(shared, q8, s);
+    if (few_shared) few<kD>(shared, mine, q8, s);
+    else if (mine.nsplit > 0) few<kD>(mine, Args{}, q8, s);
     merge<kD>(mine, rows, states, s);
   };
   if (D == 64) go(std::integral_constant<int, 64>{});

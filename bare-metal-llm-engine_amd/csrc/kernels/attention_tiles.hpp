@@ -103,6 +103,7 @@ struct Args {
   bool causal;
   long long window;   // 0: none
   int sinks;
+  long long units;    // (sequence or prefix, KV head) pairs
   int row_tiles, nsplit;
   // State of row r's split s (r counts the rows of out): r part_stride + part0 + s.
   int part_stride, part0;
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
   const int col = lane & 31;
   const int half = lane >> 5;
   // the rows with the most keys first
-  const unsigned units = gridDim.x / static_cast<unsigned>(a.row_tiles);
+  const unsigned units = static_cast<unsigned>(a.units);
   const unsigned rank = blockIdx.x / units;
   const unsigned unit = blockIdx.x - rank * units;
   const int rt = a.row_tiles - 1 - static_cast<int>(rank);
