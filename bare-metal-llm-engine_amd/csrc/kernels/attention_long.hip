@@ -74,13 +74,21 @@ void merge(const Args& a, long long rows, int states, hipStream_t s) {
   ENG_LAUNCH_CHECK();
 }
 
-// Launches of a part: the tiles of 128 rows, or up to two parts of few rows together.
-template <int D>
-void tiles(const Args& a, bool q8, hipStream_t s) {
+// Launches of a part: tiles of many rows, or up to two parts of few rows together.
+constexpr int tile_rows(int waves) { return 32 * waves; }
+template <int D, bool Q8, int NW>
+void tiles(const Args& a, hipStream_t s) {
+  constexpr std::size_t kLds = 2 * kTileBuffers * kTileKeys * D * sizeof(_Float16);
+  static std::atomic<bool> done[64];
+  allow_staged_lds(reinterpret_cast<const void*>(tile_kernel<D, Q8, NW, 1>), done, kLds);
   const dim3 grid(static_cast<unsigned>(a.units * a.row_tiles), static_cast<unsigned>(a.nsplit));
-  if (q8) tile_kernel<D, true><<<grid, 64 * kTileWaves, 0, s>>>(a);
-  else tile_kernel<D, false><<<grid, 64 * kTileWaves, 0, s>>>(a);
+  tile_kernel<D, Q8, NW, 1><<<grid, 64 * NW, kLds, s>>>(a);
   ENG_LAUNCH_CHECK();
+}
+template <int D>
+void tiles(const Args& a, bool q8, int waves, hipStream_t s) {
+  if (q8) waves == 8 ? tiles<D, true, 8>(a, s) : tiles<D, true, 4>(a, s);
+  else waves == 8 ? tiles<D, false, 8>(a, s) : tiles<D, false, 4>(a, s);
 }
 template <int D>
 void few(const Args& a, const Args& b, bool q8, hipStream_t s) {
@@ -89,6 +97,11 @@ void few(const Args& a, const Args& b, bool q8, hipStream_t s) {
   if (q8) few_kernel<D, true><<<static_cast<unsigned>(wgs), 64 * kFewWaves, 0, s>>>(a, b, static_cast<unsigned>(wgs0));
   else few_kernel<D, false><<<static_cast<unsigned>(wgs), 64 * kFewWaves, 0, s>>>(a, b, static_cast<unsigned>(wgs0));
   ENG_LAUNCH_CHECK();
+}
+
+// Waves of a tile: eight where that leaves a workgroup for every CU.
+int tile_waves(long long units, long long unit_rows) {
+  return units * ((unit_rows + tile_rows(8) - 1) / tile_rows(8)) >= device_cu_count() ? 8 : 4;
 }
 
 int tiles_of(long long rows, int tile) { return static_cast<int>((rows + tile - 1) / tile); }
@@ -112,10 +125,11 @@ void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hip
   const long long rows = batch * a.s_new * a.n_heads;
   const long long unit_rows = static_cast<long long>(a.s_new) * a.group;
   const bool one = a.s_new == 1;  // a unit's rows see the same keys
-  const int tile = one ? kFewRows : kTileRows;
   a.units = batch * a.n_kv;
+  const int waves = tile_waves(a.units, unit_rows);
+  const int tile = one ? kFewRows : tile_rows(waves);
   ENG_CHECK(unit_rows <= 0x3fffffffLL && rows <= 0xffffffffLL - 4 && threads_fit((rows + 3) / 4, 256) &&
-                threads_fit(a.units, 256) && threads_fit(a.units * tiles_of(unit_rows, tile), 256),
+                threads_fit(a.units, 256) && threads_fit(a.units * tiles_of(unit_rows, tile), 512),
             "attention_window: too many query rows for one launch");
   a.row_tiles = tiles_of(unit_rows, tile);
   long long keys = a.max_len;  // what a tile of rows can see
@@ -133,7 +147,7 @@ void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hip
     constexpr int kD = decltype(dim)::value;
     auto launch = [&] {
       if (one) few<kD>(a, Args{}, q8, s);
-      else tiles<kD>(a, q8, s);
+      else tiles<kD>(a, q8, waves, s);
     };
     if (a.nsplit == 1) {
       launch();
@@ -157,8 +171,9 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
   const long long rows = batch * mine.n_heads;
   const long long unit_rows = static_cast<long long>(shared.s_new) * shared.group;
   const bool few_shared = unit_rows <= kFewShared;
-  const int tile = few_shared ? kFewRows : kTileRows;
   shared.units = n_prefix * shared.n_kv;
+  const int waves = tile_waves(shared.units, unit_rows);
+  const int tile = few_shared ? kFewRows : tile_rows(waves);
   mine.units = batch * mine.n_kv;
   ENG_CHECK(unit_rows <= 0x3fffffffLL && rows <= 0xffffffffLL - 4 && threads_fit((rows + 3) / 4, 256) &&
                 threads_fit(shared.units, 256) && threads_fit(mine.units, 256),
@@ -174,7 +189,7 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
   shared.nsplit = splits(shared, few_shared ? kKvBlock : kTileKeys);
   mine.nsplit = splits(mine, kKvBlock);
   ENG_CHECK(threads_fit(shared.units * shared.row_tiles * std::max(1, few_shared ? shared.nsplit : 1) +
-                            mine.units * mine.row_tiles * std::max(1, mine.nsplit), 256),
+                            mine.units * mine.row_tiles * std::max(1, mine.nsplit), 512),
             "attention_prefix: too many query rows for one launch");
   const int states = shared.nsplit + mine.nsplit;
   shared.part_stride = mine.part_stride = states;
@@ -184,7 +199,7 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
     StreamScratch scratch(s, state_bytes(rows, states, kD));
     shared.part_o = mine.part_o = static_cast<float*>(scratch.get());
     shared.part_ml = mine.part_ml = shared.part_o + rows * states * kD;
-    if (!few_shared && shared.nsplit > 0) tiles<kD>(shared, q8, s);
+    if (!few_shared && shared.nsplit > 0) tiles<kD>(shared, q8, waves, s);
     if (few_shared) few<kD>(shared, mine, q8, s);
     else if (mine.nsplit > 0) few<kD>(mine, Args{}, q8, s);
     merge<kD>(mine, rows, states, s);

@@ -140,30 +140,42 @@ __device__ __forceinline__ Seen seen_by(const Args& a, const Unit& u, int t) {
   return s;
 }
 
-constexpr int kTileRows = 128;
 constexpr int kTileKeys = 64;
-constexpr int kTileWaves = 4;
+constexpr int kTileBuffers = 3;
 
-// One workgroup per (unit, 128 rows, split of their keys), 4 waves of 32 rows. K and V
-// tiles of 64 keys pass through LDS in two buffers as fp16 (e4m3 codes are converted on
-// the way, exact; a block's scale multiplies its scores, a V block's joins the weights as
-// in decode_q8_kernel). Products on v_mfma_f32_32x32x16_f16: S^T = K . Q^T with K as the
-// A operand leaves a row's scores in two lanes, O^T = V^T . P^T takes them in place as the
-// B operand: element r of half-wave g is key 8 (r / 4) + 4 g + r % 4 of its 32, and V is
-// read from LDS transposed (4 keys of a dim for each lane) in that order. A row of an LDS
-// tile is D fp16; its 16-byte pieces are permuted by the row so that neither read has
-// bank conflicts.
+// One workgroup per (unit, tile of rows, split of their keys), 4 waves of 32 RB rows. K
+// and V tiles of 64 keys pass through LDS as fp16 in three buffers, a tile's loads issued
+// two tiles ahead (8-bit codes are converted on the way, exact; a K block's scale
+// multiplies its scores, a V block's joins the weights as in few_kernel). Products on
+// v_mfma_f32_32x32x16_f16: S^T = K . Q^T with K as the A operand leaves a row's scores in
+// two lanes, O^T = V^T . P^T takes them in place as the B operand: element r of half-wave
+// g is key 8 (r / 4) + 4 g + r % 4 of its 32, and V is read from LDS transposed (4 keys
+// of a dim for each lane) in that order. A row of an LDS tile is D fp16; its 16-byte
+// pieces are permuted by the row so that neither read has bank conflicts.
+//
+// A wave takes 32 keys at a time, and issues the score products of the next 32 with the
+// exponentials of these, so that the matrix cores and the vector unit, which are busy for
+// about as long (RB = 2, D = 128: 32 products of 32 cycles; 32 exponentials of 16 and as
+// many each of a multiply-add, an addition, half a maximum and half a conversion), work
+// side by side. RB = 2 reads a K or V fragment from LDS once for 64 rows.
 // Weights are rounded to fp16 (2^-11 of each at the most, as the output is); m, l, O are
 // fp32 and l sums the weights before rounding.
-template <int D, bool Q8>
-__global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
+//
+// A NaN or an infinity in a V row would reach, as 0 times it, rows that do not see its
+// key. So where a workgroup's sums are not all finite it computes them again with such
+// values taken out and added for the rows that see them (careful_pass).
+template <int D, bool Q8, int NW, int RB>
+__global__ __launch_bounds__(64 * NW, 2) void tile_kernel(Args a) {
+  constexpr int kRows = 32 * RB * NW;
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");
   constexpr int CPR = D / 8;   // 16-byte pieces of an LDS row
   constexpr int KS = D / 16;   // k-steps of a score
   constexpr int DB = D / 32;   // 32-dim blocks of an output
   constexpr int TILE = kTileKeys * D;
-  __shared__ __attribute__((aligned(16))) _Float16 s_k[2][TILE];
-  __shared__ __attribute__((aligned(16))) _Float16 s_v[2][TILE];
+  extern __shared__ __attribute__((aligned(16))) _Float16 s_tiles[];  // K [3][TILE], V [3][TILE]
+  __shared__ __attribute__((aligned(16))) float s_scale[kTileBuffers][2][4];  // of 32 keys: f, lv, 1 / v scale
+  _Float16* const s_k = s_tiles;
+  _Float16* const s_v = s_tiles + kTileBuffers * TILE;
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -180,15 +192,14 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
   const int split = static_cast<int>(blockIdx.y);
   const Unit u = unit_of(a, b);
   const int rows = u.n * a.group;
-  const int row0 = rt * kTileRows;
+  const int row0 = rt * kRows;
   if (row0 >= rows) return;
 
   // the workgroup's keys, as tiles: sinks first, then from the window's start on
   const unsigned group = static_cast<unsigned>(a.group);
-  const int tok_first = static_cast<int>(static_cast<unsigned>(row0) / group);
-  const int tok_last = static_cast<int>(static_cast<unsigned>(min(row0 + kTileRows, rows) - 1) / group);
-  const int hi = seen_by(a, u, tok_last).hi;
-  const int lo = seen_by(a, u, tok_first).lo;
+  auto token_of = [&](int r) { return static_cast<int>(static_cast<unsigned>(r) / group); };
+  const int hi = seen_by(a, u, token_of(min(row0 + kRows, rows) - 1)).hi;
+  const int lo = seen_by(a, u, token_of(row0)).lo;
   const int sink_end = min(min(a.sinks, lo), hi);
   const int sink_tiles = (sink_end + kTileKeys - 1) / kTileKeys;
   const int start = max(lo / kKvBlock * kKvBlock, sink_tiles * kTileKeys);
@@ -199,30 +210,32 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
   auto base_of = [&](int t) { return t < sink_tiles ? t * kTileKeys : start + (t - sink_tiles) * kTileKeys; };
 
   // the wave's rows, and this lane's
-  const int wrow = row0 + 32 * wave;
-  const int r = min(wrow + col, rows - 1);
-  const int tok = static_cast<int>(static_cast<unsigned>(r) / group);
-  const Seen mine = seen_by(a, u, tok);
-  const Seen first = seen_by(a, u, static_cast<int>(static_cast<unsigned>(min(wrow, rows - 1)) / group));
-  const Seen last = seen_by(a, u, static_cast<int>(static_cast<unsigned>(min(wrow + 31, rows - 1)) / group));
-  const long long orow = (b * a.s_new + tok) * a.n_heads + kvh * a.group + (r - tok * a.group);
-
-  halfx8 qf[KS];
-  {
-    const _Float16* qp = a.q + orow * D + 8 * half;
+  const int wrow = row0 + 32 * RB * wave;
+  const Seen first = seen_by(a, u, token_of(min(wrow, rows - 1)));
+  const Seen last = seen_by(a, u, token_of(min(wrow + 32 * RB - 1, rows - 1)));
+  Seen mine[RB];
+  long long orow[RB];
+  halfx8 qf[RB][KS];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int r = min(wrow + 32 * rb + col, rows - 1);
+    const int tok = token_of(r);
+    mine[rb] = seen_by(a, u, tok);
+    orow[rb] = (b * a.s_new + tok) * a.n_heads + kvh * a.group + (r - tok * a.group);
+    const _Float16* qp = a.q + orow[rb] * D + 8 * half;
     if ((reinterpret_cast<std::uintptr_t>(a.q) & 15) == 0) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const halfx8*>(qp + 16 * s);
+      for (int s = 0; s < KS; ++s) qf[rb][s] = *reinterpret_cast<const halfx8*>(qp + 16 * s);
     } else {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) qf[s][j] = qp[16 * s + j];
+        for (int j = 0; j < 8; ++j) qf[rb][s][j] = qp[16 * s + j];
       }
     }
     if (a.scale < 0.0f) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) qf[s] = -qf[s];
+      for (int s = 0; s < KS; ++s) qf[rb][s] = -qf[rb][s];
     }
   }
   const float scale2 = fabsf(a.scale) * kLog2e;
@@ -234,57 +247,66 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
   [[maybe_unused]] const long long sb = bh * ((a.kv_max + kKvBlock - 1) / kKvBlock);
   auto swz = [](int row) { return D == 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1; };
 
-  // ---- global to LDS. Keys past the last one are taken as the last one: finite where it
-  // is, and masked.
-  constexpr int LOADS = Q8 ? TILE / 16 / 256 : 1;
-  [[maybe_unused]] uintx4 rk[LOADS], rv[LOADS];
-  float ks_at[2][2] = {}, vs_at[2][2] = {};  // scales of the tile in use and the next one's
-  auto stage = [&]([[maybe_unused]] int t, [[maybe_unused]] int buf) __attribute__((always_inline)) {
-    if constexpr (!Q8) {
-      const int base = base_of(t);
-      constexpr int RPI = 64 / CPR;  // rows of a wave load
+  // ---- global to LDS, by way of registers. Keys past the last one are taken as the last
+  // one, and masked.
+  constexpr int PIECES = TILE * static_cast<int>(sizeof(Elem)) / 16;
+  constexpr int LOADS = (PIECES + 64 * NW - 1) / (64 * NW);
+  const bool loads = PIECES >= 64 * NW || tid < PIECES;  // (uniform in a wave)
+  constexpr int LPR = D * static_cast<int>(sizeof(Elem)) / 16;  // loads of a row
+  uintx4 rk[LOADS], rv[LOADS];
+  [[maybe_unused]] float rks = 0.0f, rvs = 0.0f;
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    const int base = base_of(t);
 #pragma unroll
-      for (int i = 0; i < TILE / 512 / kTileWaves; ++i) {
-        const int ins = i * kTileWaves + wave;
-        const int row = ins * RPI + lane / CPR;
-        const int piece = (lane % CPR) ^ swz(row);
-        const long long at = static_cast<long long>(min(base + row, hi - 1)) * D + 8 * piece;
-        dma16(kg + at, &s_k[buf][ins * 512]);
-        dma16(vg + at, &s_v[buf][ins * 512]);
+    for (int i = 0; i < LOADS; ++i) {
+      const int n = i * 64 * NW + (PIECES >= 64 * NW ? tid : tid & (PIECES - 1));
+      const long long at = static_cast<long long>(min(base + n / LPR, hi - 1)) * D + (n % LPR) * (D / LPR);
+      rk[i] = *reinterpret_cast<const uintx4*>(kg + at);
+      rv[i] = *reinterpret_cast<const uintx4*>(vg + at);
+    }
+    if constexpr (Q8) {
+      const int blk = min(base / kKvBlock + (tid & 1), (hi - 1) / kKvBlock);
+      rks = a.ks[sb + blk];
+      rvs = a.vs[sb + blk];
+    }
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int n = i * 64 * NW + tid;
+      const int row = n / LPR;
+      if (!loads) continue;
+      if constexpr (Q8) {
+        const int at = buf * TILE + row * D + 8 * ((2 * (n % LPR)) ^ swz(row));
+        *reinterpret_cast<halfx8*>(s_k + at) = eight_fp8(rk[i][0], rk[i][1]);
+        *reinterpret_cast<halfx8*>(s_k + at + 8) = eight_fp8(rk[i][2], rk[i][3]);
+        *reinterpret_cast<halfx8*>(s_v + at) = eight_fp8(rv[i][0], rv[i][1]);
+        *reinterpret_cast<halfx8*>(s_v + at + 8) = eight_fp8(rv[i][2], rv[i][3]);
+      } else {
+        const int at = buf * TILE + row * D + 8 * ((n % LPR) ^ swz(row));
+        *reinterpret_cast<uintx4*>(s_k + at) = rk[i];
+        *reinterpret_cast<uintx4*>(s_v + at) = rv[i];
+      }
+    }
+    if constexpr (Q8) {
+      if (tid < 2) {
+        // (at least 1e-30, so that a mask's -inf stays -inf under a scale of zero)
+        const float vs = fmaxf(rvs, kLeastVScale);
+        *reinterpret_cast<floatx4*>(s_scale[buf][tid]) =
+            floatx4{fmaxf(scale2 * rks, 1e-30f), __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), 0.0f};
       }
     }
   };
-  auto fetch = [&]([[maybe_unused]] int t) __attribute__((always_inline)) {
-    if constexpr (Q8) {
-      const int base = base_of(t);
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int n = i * 256 + tid;
-        const int row = n / (D / 16);
-        const long long at = static_cast<long long>(min(base + row, hi - 1)) * D + 16 * (n % (D / 16));
-        rk[i] = *reinterpret_cast<const uintx4*>(kg + at);
-        rv[i] = *reinterpret_cast<const uintx4*>(vg + at);
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int blk = min(base / kKvBlock + s, (hi - 1) / kKvBlock);
-        ks_at[1][s] = a.ks[sb + blk];
-        vs_at[1][s] = a.vs[sb + blk];
-      }
-    }
+  // The factor of a 32-key block's scores, log2 and inverse of its V scale.
+  struct Scale {
+    float f, lv, ivs;
   };
-  auto put = [&]([[maybe_unused]] int buf) __attribute__((always_inline)) {
+  auto scale_of = [&](int buf, int sub) __attribute__((always_inline)) {
     if constexpr (Q8) {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int n = i * 256 + tid;
-        const int row = n / (D / 16);
-        const int at = row * D + 8 * ((2 * (n % (D / 16))) ^ swz(row));
-        *reinterpret_cast<halfx8*>(&s_k[buf][at]) = eight_fp8(rk[i][0], rk[i][1]);
-        *reinterpret_cast<halfx8*>(&s_k[buf][at + 8]) = eight_fp8(rk[i][2], rk[i][3]);
-        *reinterpret_cast<halfx8*>(&s_v[buf][at]) = eight_fp8(rv[i][0], rv[i][1]);
-        *reinterpret_cast<halfx8*>(&s_v[buf][at + 8]) = eight_fp8(rv[i][2], rv[i][3]);
-      }
+      const floatx4 x = *reinterpret_cast<const floatx4*>(s_scale[buf][sub]);
+      return Scale{x[0], x[1], x[2]};
+    } else {
+      return Scale{fmaxf(scale2, 1e-30f), 0.0f, 1.0f};
     }
   };
 
@@ -297,205 +319,293 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(Args a) {
   for (int d = 0; d < DB; ++d)
     vat[d] = vrow * D + 8 * ((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vswz) + 4 * (lane & 1);
 
-  // Sixteen keys of V from `key0` on (A operand): infinities and NaN taken out, and added
-  // to acc for the rows that see them, their number found by a product with 0 and 1.
-  auto apart = [&](halfx8 av, int key0, floatx16& acc) __attribute__((always_inline)) {
-    bool any = false;
+  float m[RB], l[RB];
+  floatx16 o[RB][DB];
+  auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) any |= !(fabsf(static_cast<float>(av[j])) < __builtin_huge_valf());
-    if (!__any(any)) return av;
-    halfx8 sees, kind[3], clean;
+    for (int rb = 0; rb < RB; ++rb) {
+      m[rb] = kNegInf;
+      l[rb] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int key = key0 + 8 * (j >> 2) + 4 * half + (j & 3);
-      sees[j] = static_cast<_Float16>(key < mine.hi && (key >= mine.lo || key < a.sinks) ? 1.0f : 0.0f);
-      const float x = static_cast<float>(av[j]);
-      kind[0][j] = static_cast<_Float16>(x == __builtin_huge_valf() ? 1.0f : 0.0f);
-      kind[1][j] = static_cast<_Float16>(x == kNegInf ? 1.0f : 0.0f);
-      kind[2][j] = static_cast<_Float16>(x != x ? 1.0f : 0.0f);
-      clean[j] = fabsf(x) < __builtin_huge_valf() ? av[j] : static_cast<_Float16>(0.0f);
+      for (int d = 0; d < DB; ++d) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[rb][d][e] = 0.0f;
+      }
     }
+  };
+  struct Scores {
+    floatx16 x[RB];
+  };
+  halfx8 kf[KS], vf[2][DB];
+  auto read_k = [&](int buf, int sub) __attribute__((always_inline)) {
 #pragma unroll
-    for (int n = 0; n < 3; ++n) {
-      floatx16 c = {};
+    for (int st = 0; st < KS; ++st)
+      kf[st] = *reinterpret_cast<const halfx8*>(s_k + buf * TILE + (32 * sub + col) * D +
+                                                8 * ((2 * st + half) ^ kswz));
+  };
+  auto read_v = [&](int buf, int sub) __attribute__((always_inline)) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const _Float16* vp = s_v + buf * TILE + vat[d] + (32 * sub + 16 * st) * D;
+        const halfx4 v0 = read_transposed(vp), v1 = read_transposed(vp + 8 * D);
+        vf[st][d] = halfx8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+      }
+    }
+  };
+  auto scores = [&](Scores& s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) s.x[rb] = floatx16{};
 #if defined(__HIP_DEVICE_COMPILE__)
-      c = __builtin_amdgcn_mfma_f32_32x32x16_f16(kind[n], sees, c, 0, 0, 0);
-#endif
-      const float x = n == 0 ? __builtin_huge_valf() : n == 1 ? kNegInf : __builtin_nanf("");
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[e] += c[e] > 0.0f ? x : 0.0f;
+    for (int st = 0; st < KS; ++st) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+        s.x[rb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[st], qf[rb][st], s.x[rb], 0, 0, 0);
     }
-    return clean;
+#endif
+  };
+  auto mask = [&](Scores& s, int key0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = key0 + 8 * (e >> 2) + 4 * half + (e & 3);
+        const bool hidden = (j >= mine[rb].hi) | ((j < mine[rb].lo) & (j >= a.sinks));
+        s.x[rb][e] = hidden ? kNegInf : s.x[rb][e];
+      }
+    }
+  };
+  auto whole = [&](int key0) {  // seen by all rows of the wave
+    return key0 + kKvBlock <= first.hi && (last.lo <= key0 || key0 + kKvBlock <= a.sinks);
+  };
+  auto seen = [&](int key0, int keys) {  // by any
+    return key0 < last.hi && (key0 + keys > first.lo || key0 < a.sinks);
+  };
+  // The largest score of a row, in units of log2.
+  auto largest = [&](const Scores& s, const Scale& c, float (&mx)[RB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      float x = s.x[rb][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) x = fmaxf(x, s.x[rb][e]);
+      mx[rb] = pair_max(fmaf(x, c.f, c.lv));
+    }
+  };
+  auto raise = [&](const float (&mx)[RB]) __attribute__((always_inline)) {
+    bool up = mx[0] > m[0] + kLazy;
+    if constexpr (RB == 2) up |= mx[RB - 1] > m[RB - 1] + kLazy;
+    if (!__any(up)) return;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const float mn = fmaxf(m[rb], mx[rb]);
+      const float alpha = weight2(m[rb], mn);
+      m[rb] = mn;
+      l[rb] *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[rb][d] *= alpha;
+    }
+  };
+  auto weights = [&](const Scores& s, const Scale& c, halfx8 (&pb)[RB][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const float add = c.lv - (m[rb] == kNegInf ? 0.0f : m[rb] - kWeightShift);
+      float ls = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s.x[rb][e], c.f, add));
+        ls += p;
+        pb[rb][e >> 3][e & 7] = static_cast<_Float16>(p);
+      }
+      l[rb] = fmaf(ls, c.ivs, l[rb]);
+    }
+  };
+  auto products = [&](const halfx8 (&pb)[RB][2]) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          o[rb][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[st][d], pb[rb][st], o[rb][d], 0, 0, 0);
+      }
+    }
+#endif
   };
 
-  float m, l;
-  floatx16 o[DB];
-  bool careful = false;  // the second time: V's infinities and NaN kept from rows that do not see them
-  for (;;) {
-    m = kNegInf;
-    l = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DB; ++d) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
-    }
-    if (t0 < t1) {
-      if constexpr (Q8) {
-        fetch(t0);
-        put(0);
-#pragma unroll
-        for (int s = 0; s < 2; ++s) ks_at[0][s] = ks_at[1][s], vs_at[0][s] = vs_at[1][s];
-        if (t0 + 1 < t1) fetch(t0 + 1);
-      } else {
-        stage(t0, 0);
+  clear();
+  // (tiles past the last one are taken as the last one, and not used)
+  auto fetch_at = [&](int t) __attribute__((always_inline)) { fetch(min(t, t1 - 1)); };
+  if (t0 < t1) {
+    fetch(t0);
+    put(0);
+    fetch_at(t0 + 1);
+    put(1);
+    fetch_at(t0 + 2);
+  }
+  Scores even, odd;  // of a tile's first and second 32 keys
+  float mx[RB];
+  bool primed = false;  // `even` holds the tile's scores, mx their maxima, kf the second keys
+  int buf = 0;
+  for (int t = t0; t < t1; ++t) {
+    // All waves are done with the tile before this one, whose buffer the tile after the
+    // next takes; this one and the next are in LDS.
+    const int next = buf + 1 == kTileBuffers ? 0 : buf + 1;
+    const int free = next + 1 == kTileBuffers ? 0 : next + 1;
+    lds_barrier();
+    const int base = base_of(t);
+    if (seen(base, kTileKeys)) {
+      halfx8 pb[RB][2];
+      Scale c = scale_of(buf, 0);
+      if (!primed) {
+        read_k(buf, 0);
+        scores(even);
+        read_k(buf, 1);
       }
-    }
-    for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
-      float f[2], lv[2], ivs[2];
-      if constexpr (Q8) {
-        lds_barrier();  // the tile is written, the other buffer read
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          // (at least 1e-30, so that a mask's -inf stays -inf under a scale of zero)
-          f[s] = fmaxf(scale2 * ks_at[0][s], 1e-30f);
-          const float vs = fmaxf(vs_at[0][s], kLeastVScale);
-          lv[s] = __builtin_amdgcn_logf(vs);
-          ivs[s] = __builtin_amdgcn_rcpf(vs);
-        }
-        if (t + 1 < t1) {
-          put(buf ^ 1);
-#pragma unroll
-          for (int s = 0; s < 2; ++s) ks_at[0][s] = ks_at[1][s], vs_at[0][s] = vs_at[1][s];
-          if (t + 2 < t1) fetch(t + 2);
-        }
-      } else {
-#if defined(__HIP_DEVICE_COMPILE__)
-        __builtin_amdgcn_s_waitcnt(vmcnt_le(0));
-#endif
-        lds_barrier();
-        if (t + 1 < t1) stage(t + 1, buf ^ 1);
-        f[0] = f[1] = fmaxf(scale2, 1e-30f);
-        lv[0] = lv[1] = 0.0f;
-        ivs[0] = ivs[1] = 1.0f;
+      if (!primed || !whole(base)) {
+        if (!whole(base)) mask(even, base);
+        largest(even, c, mx);
       }
-      const int base = base_of(t);
-      if (base >= last.hi || (base >= a.sinks && base + kTileKeys <= first.lo)) continue;  // (uniform) unseen
+      raise(mx);
+      read_v(buf, 0);
+      put(free);
+      fetch_at(t + 3);
+      scores(odd);
+      weights(even, c, pb);
+      read_k(next, 0);
+      products(pb);
+      c = scale_of(buf, 1);
+      largest(odd, c, mx);
+      if (!whole(base + kKvBlock)) {
+        mask(odd, base + kKvBlock);
+        largest(odd, c, mx);
+      }
+      raise(mx);
+      read_v(buf, 1);
+      scores(even);
+      weights(odd, c, pb);
+      read_k(next, 1);
+      products(pb);
+      largest(even, scale_of(next, 0), mx);
+      primed = t + 1 < t1;
+    } else {
+      put(free);
+      fetch_at(t + 3);
+      primed = false;
+    }
+    buf = next;
+  }
 
-      floatx16 sc[2];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sc[s][e] = 0.0f;
-#pragma unroll
-        for (int st = 0; st < KS; ++st) {
-          [[maybe_unused]] const halfx8 ka = *reinterpret_cast<const halfx8*>(
-              &s_k[buf][(32 * s + col) * D + 8 * ((2 * st + half) ^ kswz)]);
-#if defined(__HIP_DEVICE_COMPILE__)
-          sc[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qf[st], sc[s], 0, 0, 0);
-#endif
-        }
-      }
-      const bool whole = base + kTileKeys <= first.hi && (last.lo <= base || base + kTileKeys <= a.sinks);
-      if (!whole) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int j = base + 32 * s + 8 * (e >> 2) + 4 * half + (e & 3);
-            if (j >= mine.hi || (j < mine.lo && j >= a.sinks)) sc[s][e] = kNegInf;
-          }
-        }
-      }
-      float mx = kNegInf;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        float x = sc[s][0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) x = fmaxf(x, sc[s][e]);
-        mx = fmaxf(mx, fmaf(x, f[s], lv[s]));
-      }
-      mx = pair_max(mx);
-      if (__any(mx > m + kLazy)) {
-        const float mn = fmaxf(m, mx);
-        const float alpha = weight2(m, mn);
-        m = mn;
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) o[d] *= alpha;
-      }
-      const float ref = m == kNegInf ? 0.0f : m - kWeightShift;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const float add = lv[s] - ref;
-        float ls = 0.0f;
-        halfx8 pb[2];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(sc[s][e], f[s], add));
-          ls += p;
-          pb[e >> 3][e & 7] = static_cast<_Float16>(p);
-        }
-        l = fmaf(ls, ivs[s], l);
+  // Tile by tile as above, without any overlap, values that are not finite kept apart.
+  auto careful_pass = [&]() {
+    clear();
+    for (int t = t0; t < t1; ++t) {
+      __syncthreads();
+      fetch(t);
+      put(0);
+      __syncthreads();
+#pragma unroll 1
+      for (int sub = 0; sub < 2; ++sub) {
+        const int key0 = base_of(t) + kKvBlock * sub;
+        if (!seen(key0, kKvBlock)) continue;
+        const Scale c = scale_of(0, sub);
+        halfx8 pb[RB][2];
+        read_k(0, sub);
+        read_v(0, sub);
+        scores(even);
+        mask(even, key0);
+        largest(even, c, mx);
+        raise(mx);
+        weights(even, c, pb);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
-            halfx8 av = {};
+            const halfx8 av = vf[st][d];
+            halfx8 clean, kind[3];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float x = static_cast<float>(av[j]);
+              kind[0][j] = static_cast<_Float16>(x == __builtin_huge_valf() ? 1.0f : 0.0f);
+              kind[1][j] = static_cast<_Float16>(x == kNegInf ? 1.0f : 0.0f);
+              kind[2][j] = static_cast<_Float16>(x != x ? 1.0f : 0.0f);
+              clean[j] = fabsf(x) < __builtin_huge_valf() ? av[j] : static_cast<_Float16>(0.0f);
+            }
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+              halfx8 sees;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int key = key0 + 16 * st + 8 * (j >> 2) + 4 * half + (j & 3);
+                sees[j] = static_cast<_Float16>(
+                    key < mine[rb].hi && (key >= mine[rb].lo || key < a.sinks) ? 1.0f : 0.0f);
+              }
+              // how many infinities and NaN a row sees in a dim
+#pragma unroll
+              for (int n = 0; n < 3; ++n) {
+                floatx16 count = {};
 #if defined(__HIP_DEVICE_COMPILE__)
-            const _Float16* vp = &s_v[buf][vat[d] + (32 * s + 16 * st) * D];
-            const halfx4 v0 = read_transposed(vp), v1 = read_transposed(vp + 8 * D);
-            av = halfx8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                count = __builtin_amdgcn_mfma_f32_32x32x16_f16(kind[n], sees, count, 0, 0, 0);
 #endif
-            if (careful && !whole) av = apart(av, base + 32 * s + 16 * st, o[d]);
+                const float x = n == 0 ? __builtin_huge_valf() : n == 1 ? kNegInf : __builtin_nanf("");
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[rb][d][e] += count[e] > 0.0f ? x : 0.0f;
+              }
 #if defined(__HIP_DEVICE_COMPILE__)
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, pb[st], o[d], 0, 0, 0);
+              o[rb][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(clean, pb[rb][st], o[rb][d], 0, 0, 0);
 #endif
+            }
           }
         }
       }
     }
-    if (careful) break;
-    float sum = 0.0f;
+  };
+  float sum = 0.0f;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum = fmaf(o[d][e], 0.0f, sum);
+      for (int e = 0; e < 16; ++e) sum = fmaf(o[rb][d][e], 0.0f, sum);
     }
-    if (!__syncthreads_or(sum != sum)) break;
-    careful = true;
   }
+  if (__syncthreads_or(sum != sum)) careful_pass();
 
-  l += __shfl_xor(l, 32);
-  if (wrow + col >= rows) return;
-  if (a.part_o != nullptr) {
-    const long long slot = orow * a.part_stride + a.part0 + split;
-#pragma unroll
-    for (int d = 0; d < DB; ++d) {
-#pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<floatx4*>(a.part_o + slot * D + 32 * d + 2 * e + 4 * half) =
-            floatx4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
-    }
-    if (half == 0) *reinterpret_cast<floatx2*>(a.part_ml + 2 * slot) = floatx2{m, l};
-    return;
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros)
-  _Float16* op = a.out + orow * D + 4 * half;
   const bool aligned = (reinterpret_cast<std::uintptr_t>(a.out) & 7) == 0;
 #pragma unroll
-  for (int d = 0; d < DB; ++d) {
+  for (int rb = 0; rb < RB; ++rb) {
+    l[rb] += __shfl_xor(l[rb], 32);
+    if (wrow + 32 * rb + col >= rows) continue;
+    if (a.part_o != nullptr) {
+      const long long slot = orow[rb] * a.part_stride + a.part0 + split;
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      halfx4 y;
+      for (int d = 0; d < DB; ++d) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = static_cast<_Float16>(o[d][e + j] * inv);
-      _Float16* at = op + 32 * d + 2 * e;
-      if (aligned) {
-        *reinterpret_cast<halfx4*>(at) = y;
-      } else {
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<floatx4*>(a.part_o + slot * D + 32 * d + 2 * e + 4 * half) =
+              floatx4{o[rb][d][e], o[rb][d][e + 1], o[rb][d][e + 2], o[rb][d][e + 3]};
+      }
+      if (half == 0) *reinterpret_cast<floatx2*>(a.part_ml + 2 * slot) = floatx2{m[rb], l[rb]};
+      continue;
+    }
+    const float inv = l[rb] == 0.0f ? 0.0f : 1.0f / l[rb];  // (no key seen: zeros)
+    _Float16* op = a.out + orow[rb] * D + 4 * half;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) at[j] = y[j];
+    for (int d = 0; d < DB; ++d) {
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        halfx4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = static_cast<_Float16>(o[rb][d][e + j] * inv);
+        _Float16* at = op + 32 * d + 2 * e;
+        if (aligned) {
+          *reinterpret_cast<halfx4*>(at) = y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) at[j] = y[j];
+        }
       }
     }
   }
