@@ -78,11 +78,11 @@ void merge(const Args& a, long long rows, int states, hipStream_t s) {
 constexpr int tile_rows(int waves) { return 32 * waves; }
 template <int D, bool Q8, int NW>
 void tiles(const Args& a, hipStream_t s) {
-  constexpr std::size_t kLds = 2 * kTileBuffers * kTileKeys * D * sizeof(_Float16);
+  constexpr std::size_t kLds = 2 * tile_buffers(NW) * kTileKeys * D * sizeof(_Float16);
   static std::atomic<bool> done[64];
-  allow_staged_lds(reinterpret_cast<const void*>(tile_kernel<D, Q8, NW, 1>), done, kLds);
+  allow_staged_lds(reinterpret_cast<const void*>(tile_kernel<D, Q8, NW>), done, kLds);
   const dim3 grid(static_cast<unsigned>(a.units * a.row_tiles), static_cast<unsigned>(a.nsplit));
-  tile_kernel<D, Q8, NW, 1><<<grid, 64 * NW, kLds, s>>>(a);
+  tile_kernel<D, Q8, NW><<<grid, 64 * NW, kLds, s>>>(a);
   ENG_LAUNCH_CHECK();
 }
 template <int D>
@@ -107,10 +107,10 @@ int tile_waves(long long units, long long unit_rows) {
 int tiles_of(long long rows, int tile) { return static_cast<int>((rows + tile - 1) / tile); }
 
 // Splits of the keys of `wgs` workgroups that read up to `keys` keys each, in steps of
-// `step` keys.
-int auto_splits(long long wgs, long long keys, long long step) {
+// `step` keys, for `per_cu` workgroups to a CU.
+int auto_splits(long long wgs, long long keys, long long step, int per_cu) {
   const long long steps = (keys + step - 1) / step;
-  const long long want = 2ll * device_cu_count() / wgs;
+  const long long want = static_cast<long long>(per_cu) * device_cu_count() / wgs;
   return static_cast<int>(std::max(1ll, std::min({want, steps / 4, static_cast<long long>(kMaxStates)})));
 }
 
@@ -126,7 +126,7 @@ void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hip
   const long long unit_rows = static_cast<long long>(a.s_new) * a.group;
   const bool one = a.s_new == 1;  // a unit's rows see the same keys
   a.units = batch * a.n_kv;
-  const int waves = tile_waves(a.units, unit_rows);
+  const int waves = D == 64 ? 4 : tile_waves(a.units, unit_rows);
   const int tile = one ? kFewRows : tile_rows(waves);
   ENG_CHECK(unit_rows <= 0x3fffffffLL && rows <= 0xffffffffLL - 4 && threads_fit((rows + 3) / 4, 256) &&
                 threads_fit(a.units, 256) && threads_fit(a.units * tiles_of(unit_rows, tile), 512),
@@ -137,7 +137,7 @@ void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hip
     keys = std::min(keys, a.window + a.sinks + std::min<long long>(a.s_new, tile / a.group + 2) + kKvBlock);
   const long long step = one ? kKvBlock : kTileKeys;
   const long long most = std::max(1ll, (keys + step - 1) / step);
-  a.nsplit = split_kv == 0 ? auto_splits(a.units * a.row_tiles, keys, step)
+  a.nsplit = split_kv == 0 ? auto_splits(a.units * a.row_tiles, keys, step, one ? 2 : 8 / waves)
                            : static_cast<int>(std::min<long long>({split_kv, most, kMaxStates}));
   if (one)
     ENG_CHECK(threads_fit(a.units * a.row_tiles * a.nsplit, 256),
@@ -172,7 +172,7 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
   const long long unit_rows = static_cast<long long>(shared.s_new) * shared.group;
   const bool few_shared = unit_rows <= kFewShared;
   shared.units = n_prefix * shared.n_kv;
-  const int waves = tile_waves(shared.units, unit_rows);
+  const int waves = D == 64 ? 4 : tile_waves(shared.units, unit_rows);
   const int tile = few_shared ? kFewRows : tile_rows(waves);
   mine.units = batch * mine.n_kv;
   ENG_CHECK(unit_rows <= 0x3fffffffLL && rows <= 0xffffffffLL - 4 && threads_fit((rows + 3) / 4, 256) &&
@@ -180,14 +180,14 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
             "attention_prefix: too many query rows for one launch");
   shared.row_tiles = tiles_of(unit_rows, tile);
   mine.row_tiles = tiles_of(mine.group, kFewRows);
-  auto splits = [&](const Args& a, long long step) {
+  auto splits = [&](const Args& a, long long step, int per_cu) {
     if (a.max_len == 0) return 0;
     const long long most = (a.max_len + step - 1) / step;
-    return split_kv == 0 ? std::min(auto_splits(a.units * a.row_tiles, a.max_len, step), kMaxStates / 2)
+    return split_kv == 0 ? std::min(auto_splits(a.units * a.row_tiles, a.max_len, step, per_cu), kMaxStates / 2)
                          : static_cast<int>(std::min<long long>({split_kv, most, kMaxStates / 2}));
   };
-  shared.nsplit = splits(shared, few_shared ? kKvBlock : kTileKeys);
-  mine.nsplit = splits(mine, kKvBlock);
+  shared.nsplit = splits(shared, few_shared ? kKvBlock : kTileKeys, few_shared ? 2 : 8 / waves);
+  mine.nsplit = splits(mine, kKvBlock, 2);
   ENG_CHECK(threads_fit(shared.units * shared.row_tiles * std::max(1, few_shared ? shared.nsplit : 1) +
                             mine.units * mine.row_tiles * std::max(1, mine.nsplit), 512),
             "attention_prefix: too many query rows for one launch");

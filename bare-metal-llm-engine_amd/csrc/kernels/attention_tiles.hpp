@@ -141,41 +141,44 @@ __device__ __forceinline__ Seen seen_by(const Args& a, const Unit& u, int t) {
 }
 
 constexpr int kTileKeys = 64;
-constexpr int kTileBuffers = 3;
+// LDS buffers of a tile of NW waves.
+constexpr int tile_buffers(int NW) { return NW == 8 ? 3 : 2; }
 
-// One workgroup per (unit, tile of rows, split of their keys), 4 waves of 32 RB rows. K
-// and V tiles of 64 keys pass through LDS as fp16 in three buffers, a tile's loads issued
-// two tiles ahead (8-bit codes are converted on the way, exact; a K block's scale
-// multiplies its scores, a V block's joins the weights as in few_kernel). Products on
-// v_mfma_f32_32x32x16_f16: S^T = K . Q^T with K as the A operand leaves a row's scores in
-// two lanes, O^T = V^T . P^T takes them in place as the B operand: element r of half-wave
-// g is key 8 (r / 4) + 4 g + r % 4 of its 32, and V is read from LDS transposed (4 keys
-// of a dim for each lane) in that order. A row of an LDS tile is D fp16; its 16-byte
-// pieces are permuted by the row so that neither read has bank conflicts.
+// One workgroup per (unit, tile of 32 NW rows, split of their keys), NW waves of 32 rows.
+// K and V tiles of 64 keys pass through LDS as fp16 in two buffers, by way of registers
+// (8-bit codes are converted on the way, exact; a K block's scale multiplies its scores, a
+// V block's joins the weights as in few_kernel). Products on v_mfma_f32_32x32x16_f16: S^T =
+// K . Q^T with K as the A operand leaves a row's scores in two lanes, O^T = V^T . P^T takes
+// them in place as the B operand: element r of half-wave g is key 8 (r / 4) + 4 g + r % 4
+// of its 32, and V is read from LDS transposed (4 keys of a dim for each lane) in that
+// order. A row of an LDS tile is D fp16; its 16-byte pieces are permuted by the row so that
+// neither read has bank conflicts (256 and about 148 bytes a clock; 128 and 120 before).
 //
-// A wave takes 32 keys at a time, and issues the score products of the next 32 with the
-// exponentials of these, so that the matrix cores and the vector unit, which are busy for
-// about as long (RB = 2, D = 128: 32 products of 32 cycles; 32 exponentials of 16 and as
-// many each of a multiply-add, an addition, half a maximum and half a conversion), work
-// side by side. RB = 2 reads a K or V fragment from LDS once for 64 rows.
+// A wave takes 32 keys in two phases of about 500 cycles at D = 128: exponentials (16 of 16
+// cycles, and as many each of a multiply-add, an addition, half a maximum and half a
+// conversion), then matrix products (16 of 32 cycles: O of these keys, the scores of the
+// next 32). Eight waves put two on a SIMD, and the barriers between the phases keep waves
+// 4 to 7 one phase behind waves 0 to 3, so that one of the two has the vector unit and the
+// other the matrix cores.
 // Weights are rounded to fp16 (2^-11 of each at the most, as the output is); m, l, O are
 // fp32 and l sums the weights before rounding.
 //
 // A NaN or an infinity in a V row would reach, as 0 times it, rows that do not see its
 // key. So where a workgroup's sums are not all finite it computes them again with such
 // values taken out and added for the rows that see them (careful_pass).
-template <int D, bool Q8, int NW, int RB>
-__global__ __launch_bounds__(64 * NW, 2) void tile_kernel(Args a) {
-  constexpr int kRows = 32 * RB * NW;
+template <int D, bool Q8, int NW>
+__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) {
+  constexpr int kRows = 32 * NW;
+  constexpr int NB = tile_buffers(NW);
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");
   constexpr int CPR = D / 8;   // 16-byte pieces of an LDS row
   constexpr int KS = D / 16;   // k-steps of a score
   constexpr int DB = D / 32;   // 32-dim blocks of an output
   constexpr int TILE = kTileKeys * D;
-  extern __shared__ __attribute__((aligned(16))) _Float16 s_tiles[];  // K [3][TILE], V [3][TILE]
-  __shared__ __attribute__((aligned(16))) float s_scale[kTileBuffers][2][4];  // of 32 keys: f, lv, 1 / v scale
+  extern __shared__ __attribute__((aligned(16))) _Float16 s_tiles[];  // K [NB][TILE], V [NB][TILE]
+  __shared__ __attribute__((aligned(16))) float s_scale[NB][2][4];  // of 32 keys: f, lv, 1 / v scale
   _Float16* const s_k = s_tiles;
-  _Float16* const s_v = s_tiles + kTileBuffers * TILE;
+  _Float16* const s_v = s_tiles + NB * TILE;
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -210,32 +213,29 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_kernel(Args a) {
   auto base_of = [&](int t) { return t < sink_tiles ? t * kTileKeys : start + (t - sink_tiles) * kTileKeys; };
 
   // the wave's rows, and this lane's
-  const int wrow = row0 + 32 * RB * wave;
+  const int wrow = row0 + 32 * wave;
   const Seen first = seen_by(a, u, token_of(min(wrow, rows - 1)));
-  const Seen last = seen_by(a, u, token_of(min(wrow + 32 * RB - 1, rows - 1)));
-  Seen mine[RB];
-  long long orow[RB];
-  halfx8 qf[RB][KS];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int r = min(wrow + 32 * rb + col, rows - 1);
-    const int tok = token_of(r);
-    mine[rb] = seen_by(a, u, tok);
-    orow[rb] = (b * a.s_new + tok) * a.n_heads + kvh * a.group + (r - tok * a.group);
-    const _Float16* qp = a.q + orow[rb] * D + 8 * half;
+  const Seen last = seen_by(a, u, token_of(min(wrow + 31, rows - 1)));
+  const int r = min(wrow + col, rows - 1);
+  const int tok = token_of(r);
+  const Seen mine = seen_by(a, u, tok);
+  const long long orow = (b * a.s_new + tok) * a.n_heads + kvh * a.group + (r - tok * a.group);
+  halfx8 qf[KS];
+  {
+    const _Float16* qp = a.q + orow * D + 8 * half;
     if ((reinterpret_cast<std::uintptr_t>(a.q) & 15) == 0) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) qf[rb][s] = *reinterpret_cast<const halfx8*>(qp + 16 * s);
+      for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const halfx8*>(qp + 16 * s);
     } else {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) qf[rb][s][j] = qp[16 * s + j];
+        for (int j = 0; j < 8; ++j) qf[s][j] = qp[16 * s + j];
       }
     }
     if (a.scale < 0.0f) {
 #pragma unroll
-      for (int s = 0; s < KS; ++s) qf[rb][s] = -qf[rb][s];
+      for (int s = 0; s < KS; ++s) qf[s] = -qf[s];
     }
   }
   const float scale2 = fabsf(a.scale) * kLog2e;
@@ -245,7 +245,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_kernel(Args a) {
   const Elem* kg = static_cast<const Elem*>(a.k) + bh * a.kv_max * D;
   const Elem* vg = static_cast<const Elem*>(a.v) + bh * a.kv_max * D;
   [[maybe_unused]] const long long sb = bh * ((a.kv_max + kKvBlock - 1) / kKvBlock);
-  auto swz = [](int row) { return D == 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1; };
+  auto k_swz = [](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
+  auto v_swz = [](int row) { return D == 128 ? (row & 3) << 2 : (row & 3) << 1; };
 
   // ---- global to LDS, by way of registers. Keys past the last one are taken as the last
   // one, and masked.
@@ -276,16 +277,19 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_kernel(Args a) {
       const int n = i * 64 * NW + tid;
       const int row = n / LPR;
       if (!loads) continue;
+      const int at = buf * TILE + row * D;
+      const int piece = n % LPR;
       if constexpr (Q8) {
-        const int at = buf * TILE + row * D + 8 * ((2 * (n % LPR)) ^ swz(row));
-        *reinterpret_cast<halfx8*>(s_k + at) = eight_fp8(rk[i][0], rk[i][1]);
-        *reinterpret_cast<halfx8*>(s_k + at + 8) = eight_fp8(rk[i][2], rk[i][3]);
-        *reinterpret_cast<halfx8*>(s_v + at) = eight_fp8(rv[i][0], rv[i][1]);
-        *reinterpret_cast<halfx8*>(s_v + at + 8) = eight_fp8(rv[i][2], rv[i][3]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          *reinterpret_cast<halfx8*>(s_k + at + 8 * ((2 * piece + j) ^ k_swz(row))) =
+              eight_fp8(rk[i][2 * j], rk[i][2 * j + 1]);
+          *reinterpret_cast<halfx8*>(s_v + at + 8 * ((2 * piece + j) ^ v_swz(row))) =
+              eight_fp8(rv[i][2 * j], rv[i][2 * j + 1]);
+        }
       } else {
-        const int at = buf * TILE + row * D + 8 * ((n % LPR) ^ swz(row));
-        *reinterpret_cast<uintx4*>(s_k + at) = rk[i];
-        *reinterpret_cast<uintx4*>(s_v + at) = rv[i];
+        *reinterpret_cast<uintx4*>(s_k + at + 8 * (piece ^ k_swz(row))) = rk[i];
+        *reinterpret_cast<uintx4*>(s_v + at + 8 * (piece ^ v_swz(row))) = rv[i];
       }
     }
     if constexpr (Q8) {
@@ -311,32 +315,28 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_kernel(Args a) {
   };
 
   // ---- LDS addresses of the fragments
-  const int kswz = swz(col);
+  const int kswz = k_swz(col);
   const int vrow = 4 * half + ((lane & 15) >> 2);  // + 16 s + 8 j + 32 sub
-  const int vswz = swz(vrow);
+  const int vswz = v_swz(vrow);
   int vat[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d)
     vat[d] = vrow * D + 8 * ((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vswz) + 4 * (lane & 1);
 
-  float m[RB], l[RB];
-  floatx16 o[RB][DB];
+  float m, l;
+  floatx16 o[DB];
   auto clear = [&]() __attribute__((always_inline)) {
+    m = kNegInf;
+    l = 0.0f;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      m[rb] = kNegInf;
-      l[rb] = 0.0f;
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[rb][d][e] = 0.0f;
-      }
-    }
+    for (int d = 0; d < DB; ++d) o[d] = floatx16{};
   };
+  // What a phase of products takes: fragments of K and V, and the weights.
+  halfx8 kf[KS], vf[2][DB], pb[2];
   struct Scores {
-    floatx16 x[RB];
+    floatx16 x;
   };
-  halfx8 kf[KS], vf[2][DB];
+  Scores even, odd;  // of a tile's first and second 32 keys
   auto read_k = [&](int buf, int sub) __attribute__((always_inline)) {
 #pragma unroll
     for (int st = 0; st < KS; ++st)
@@ -355,150 +355,136 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_kernel(Args a) {
     }
   };
   auto scores = [&](Scores& s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) s.x[rb] = floatx16{};
+    floatx16 sc = {};
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
-    for (int st = 0; st < KS; ++st) {
+    for (int st = 0; st < KS; ++st) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[st], qf[st], sc, 0, 0, 0);
+#endif
+    s.x = sc;
+  };
+  auto products = [&]() __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-        s.x[rb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[st], qf[rb][st], s.x[rb], 0, 0, 0);
+    for (int st = 0; st < 2; ++st) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[st][d], pb[st], o[d], 0, 0, 0);
     }
 #endif
   };
-  auto mask = [&](Scores& s, int key0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int j = key0 + 8 * (e >> 2) + 4 * half + (e & 3);
-        const bool hidden = (j >= mine[rb].hi) | ((j < mine[rb].lo) & (j >= a.sinks));
-        s.x[rb][e] = hidden ? kNegInf : s.x[rb][e];
-      }
-    }
-  };
-  auto whole = [&](int key0) {  // seen by all rows of the wave
+  auto whole = [&](int key0) {  // 32 keys, seen by all rows of the wave
     return key0 + kKvBlock <= first.hi && (last.lo <= key0 || key0 + kKvBlock <= a.sinks);
   };
   auto seen = [&](int key0, int keys) {  // by any
     return key0 < last.hi && (key0 + keys > first.lo || key0 < a.sinks);
   };
-  // The largest score of a row, in units of log2.
-  auto largest = [&](const Scores& s, const Scale& c, float (&mx)[RB]) __attribute__((always_inline)) {
+  // 32 keys' scores: hidden ones to -inf, and the row's largest in units of log2.
+  auto mask = [&](Scores& s, int key0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      float x = s.x[rb][0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) x = fmaxf(x, s.x[rb][e]);
-      mx[rb] = pair_max(fmaf(x, c.f, c.lv));
+    for (int e = 0; e < 16; ++e) {
+      const int j = key0 + 8 * (e >> 2) + 4 * half + (e & 3);
+      const bool hidden = (j >= mine.hi) | ((j < mine.lo) & (j >= a.sinks));
+      s.x[e] = hidden ? kNegInf : s.x[e];
     }
   };
-  auto raise = [&](const float (&mx)[RB]) __attribute__((always_inline)) {
-    bool up = mx[0] > m[0] + kLazy;
-    if constexpr (RB == 2) up |= mx[RB - 1] > m[RB - 1] + kLazy;
-    if (!__any(up)) return;
+  auto largest = [&](const Scores& s, const Scale& c) __attribute__((always_inline)) {
+    float x[4];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const float mn = fmaxf(m[rb], mx[rb]);
-      const float alpha = weight2(m[rb], mn);
-      m[rb] = mn;
-      l[rb] *= alpha;
-#pragma unroll
-      for (int d = 0; d < DB; ++d) o[rb][d] *= alpha;
-    }
+    for (int e = 0; e < 4; ++e) x[e] = fmaxf(fmaxf(s.x[e], s.x[e + 4]), fmaxf(s.x[e + 8], s.x[e + 12]));
+    return pair_max(fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), c.f, c.lv));
   };
-  auto weights = [&](const Scores& s, const Scale& c, halfx8 (&pb)[RB][2]) __attribute__((always_inline)) {
+  auto raise = [&](float mx) __attribute__((always_inline)) {
+    if (!__any(mx > m + kLazy)) return;
+    const float mn = fmaxf(m, mx);
+    const float alpha = weight2(m, mn);
+    m = mn;
+    l *= alpha;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const float add = c.lv - (m[rb] == kNegInf ? 0.0f : m[rb] - kWeightShift);
-      float ls = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s.x[rb][e], c.f, add));
-        ls += p;
-        pb[rb][e >> 3][e & 7] = static_cast<_Float16>(p);
-      }
-      l[rb] = fmaf(ls, c.ivs, l[rb]);
-    }
+    for (int d = 0; d < DB; ++d) o[d] *= alpha;
   };
-  auto products = [&](const halfx8 (&pb)[RB][2]) __attribute__((always_inline)) {
-#if defined(__HIP_DEVICE_COMPILE__)
+  auto weigh = [&](const Scores& s, const Scale& c) __attribute__((always_inline)) {
+    const float add = c.lv - (m == kNegInf ? 0.0f : m - kWeightShift);
+    float ls[4] = {};
 #pragma unroll
-    for (int st = 0; st < 2; ++st) {
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-          o[rb][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[st][d], pb[rb][st], o[rb][d], 0, 0, 0);
-      }
+    for (int e = 0; e < 16; ++e) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(s.x[e], c.f, add));
+      ls[e & 3] += p;
+      pb[e >> 3][e & 7] = static_cast<_Float16>(p);
     }
-#endif
+    l = fmaf((ls[0] + ls[1]) + (ls[2] + ls[3]), c.ivs, l);
   };
 
   clear();
-  // (tiles past the last one are taken as the last one, and not used)
-  auto fetch_at = [&](int t) __attribute__((always_inline)) { fetch(min(t, t1 - 1)); };
   if (t0 < t1) {
+    // (tiles past the last one are taken as the last one, and not used)
+    auto fetch_at = [&](int t) __attribute__((always_inline)) { fetch(min(t, t1 - 1)); };
     fetch(t0);
     put(0);
     fetch_at(t0 + 1);
-    put(1);
-    fetch_at(t0 + 2);
-  }
-  Scores even, odd;  // of a tile's first and second 32 keys
-  float mx[RB];
-  bool primed = false;  // `even` holds the tile's scores, mx their maxima, kf the second keys
-  int buf = 0;
-  for (int t = t0; t < t1; ++t) {
-    // All waves are done with the tile before this one, whose buffer the tile after the
-    // next takes; this one and the next are in LDS.
-    const int next = buf + 1 == kTileBuffers ? 0 : buf + 1;
-    const int free = next + 1 == kTileBuffers ? 0 : next + 1;
-    lds_barrier();
-    const int base = base_of(t);
-    if (seen(base, kTileKeys)) {
-      halfx8 pb[RB][2];
-      Scale c = scale_of(buf, 0);
-      if (!primed) {
-        read_k(buf, 0);
-        scores(even);
-        read_k(buf, 1);
-      }
-      if (!primed || !whole(base)) {
-        if (!whole(base)) mask(even, base);
-        largest(even, c, mx);
-      }
-      raise(mx);
-      read_v(buf, 0);
-      put(free);
-      fetch_at(t + 3);
-      scores(odd);
-      weights(even, c, pb);
-      read_k(next, 0);
-      products(pb);
-      c = scale_of(buf, 1);
-      largest(odd, c, mx);
-      if (!whole(base + kKvBlock)) {
-        mask(odd, base + kKvBlock);
-        largest(odd, c, mx);
-      }
-      raise(mx);
-      read_v(buf, 1);
-      scores(even);
-      weights(odd, c, pb);
-      read_k(next, 1);
-      products(pb);
-      largest(even, scale_of(next, 0), mx);
-      primed = t + 1 < t1;
-    } else {
-      put(free);
-      fetch_at(t + 3);
-      primed = false;
+    if constexpr (NB == 3) {
+      put(1);
+      fetch_at(t0 + 2);
     }
-    buf = next;
+    float mx = 0.0f;
+    bool primed = false;  // `even` holds the tile's scores, mx their largest, kf the second keys
+    int buf = 0;
+    for (int t = t0; t < t1; ++t) {
+      // NB == 3: all waves are done with the tile before this one, whose buffer the tile
+      // after the next takes; this one and the next are in LDS. NB == 2: the next one takes
+      // it, and is there for the second 32 keys.
+      const int next = buf + 1 == NB ? 0 : buf + 1;
+      const int free = (buf + NB - 1) % NB;
+      lds_barrier();
+      const int base = base_of(t);
+      if (seen(base, kTileKeys)) {
+        Scale c = scale_of(buf, 0);
+        if (!primed) {
+          read_k(buf, 0);
+          scores(even);
+          read_k(buf, 1);
+        }
+        if (!primed || !whole(base)) {
+          if (!whole(base)) mask(even, base);
+          mx = largest(even, c);
+        }
+        raise(mx);
+        read_v(buf, 0);
+        put(free);
+        fetch_at(t + NB);
+        scores(odd);
+        weigh(even, c);
+        if constexpr (NB == 3) read_k(next, 0);
+        products();
+        c = scale_of(buf, 1);
+        mx = largest(odd, c);
+        if (!whole(base + kKvBlock)) {
+          mask(odd, base + kKvBlock);
+          mx = largest(odd, c);
+        }
+        raise(mx);
+        if constexpr (NB == 2) {
+          lds_barrier();
+          read_k(next, 0);
+        }
+        read_v(buf, 1);
+        if constexpr (NB == 3) scores(even);
+        weigh(odd, c);
+        if constexpr (NB == 2) scores(even);
+        read_k(next, 1);
+        products();
+        mx = largest(even, scale_of(next, 0));
+        primed = t + 1 < t1;
+      } else {
+        put(free);
+        fetch_at(t + NB);
+        if constexpr (NB == 2) lds_barrier();
+        primed = false;
+      }
+      buf = next;
+    }
   }
 
-  // Tile by tile as above, without any overlap, values that are not finite kept apart.
+  // Tile by tile as above, one phase after the other, values that are not finite kept apart.
   auto careful_pass = [&]() {
     clear();
     for (int t = t0; t < t1; ++t) {
@@ -510,53 +496,46 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_kernel(Args a) {
       for (int sub = 0; sub < 2; ++sub) {
         const int key0 = base_of(t) + kKvBlock * sub;
         if (!seen(key0, kKvBlock)) continue;
-        const Scale c = scale_of(0, sub);
-        halfx8 pb[RB][2];
         read_k(0, sub);
         read_v(0, sub);
         scores(even);
+        const Scale c = scale_of(0, sub);
         mask(even, key0);
-        largest(even, c, mx);
-        raise(mx);
-        weights(even, c, pb);
+        raise(largest(even, c));
+        weigh(even, c);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
+          halfx8 sees;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = key0 + 16 * st + 8 * (j >> 2) + 4 * half + (j & 3);
+            sees[j] = static_cast<_Float16>(key < mine.hi && (key >= mine.lo || key < a.sinks) ? 1.0f : 0.0f);
+          }
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
-            const halfx8 av = vf[st][d];
             halfx8 clean, kind[3];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float x = static_cast<float>(av[j]);
+              const float x = static_cast<float>(vf[st][d][j]);
               kind[0][j] = static_cast<_Float16>(x == __builtin_huge_valf() ? 1.0f : 0.0f);
               kind[1][j] = static_cast<_Float16>(x == kNegInf ? 1.0f : 0.0f);
               kind[2][j] = static_cast<_Float16>(x != x ? 1.0f : 0.0f);
-              clean[j] = fabsf(x) < __builtin_huge_valf() ? av[j] : static_cast<_Float16>(0.0f);
+              clean[j] = fabsf(x) < __builtin_huge_valf() ? vf[st][d][j] : static_cast<_Float16>(0.0f);
             }
+            // how many infinities and NaN a row sees in a dim
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-              halfx8 sees;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int key = key0 + 16 * st + 8 * (j >> 2) + 4 * half + (j & 3);
-                sees[j] = static_cast<_Float16>(
-                    key < mine[rb].hi && (key >= mine[rb].lo || key < a.sinks) ? 1.0f : 0.0f);
-              }
-              // how many infinities and NaN a row sees in a dim
-#pragma unroll
-              for (int n = 0; n < 3; ++n) {
-                floatx16 count = {};
+            for (int n = 0; n < 3; ++n) {
+              floatx16 count = {};
 #if defined(__HIP_DEVICE_COMPILE__)
-                count = __builtin_amdgcn_mfma_f32_32x32x16_f16(kind[n], sees, count, 0, 0, 0);
+              count = __builtin_amdgcn_mfma_f32_32x32x16_f16(kind[n], sees, count, 0, 0, 0);
 #endif
-                const float x = n == 0 ? __builtin_huge_valf() : n == 1 ? kNegInf : __builtin_nanf("");
+              const float x = n == 0 ? __builtin_huge_valf() : n == 1 ? kNegInf : __builtin_nanf("");
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[rb][d][e] += count[e] > 0.0f ? x : 0.0f;
-              }
-#if defined(__HIP_DEVICE_COMPILE__)
-              o[rb][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(clean, pb[rb][st], o[rb][d], 0, 0, 0);
-#endif
+              for (int e = 0; e < 16; ++e) o[d][e] += count[e] > 0.0f ? x : 0.0f;
             }
+#if defined(__HIP_DEVICE_COMPILE__)
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(clean, pb[st], o[d], 0, 0, 0);
+#endif
           }
         }
       }
@@ -564,48 +543,42 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_kernel(Args a) {
   };
   float sum = 0.0f;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
+  for (int d = 0; d < DB; ++d) {
 #pragma unroll
-    for (int d = 0; d < DB; ++d) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sum = fmaf(o[rb][d][e], 0.0f, sum);
-    }
+    for (int e = 0; e < 16; ++e) sum = fmaf(o[d][e], 0.0f, sum);
   }
   if (__syncthreads_or(sum != sum)) careful_pass();
 
-  const bool aligned = (reinterpret_cast<std::uintptr_t>(a.out) & 7) == 0;
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    l[rb] += __shfl_xor(l[rb], 32);
-    if (wrow + 32 * rb + col >= rows) continue;
-    if (a.part_o != nullptr) {
-      const long long slot = orow[rb] * a.part_stride + a.part0 + split;
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-#pragma unroll
-        for (int e = 0; e < 16; e += 4)
-          *reinterpret_cast<floatx4*>(a.part_o + slot * D + 32 * d + 2 * e + 4 * half) =
-              floatx4{o[rb][d][e], o[rb][d][e + 1], o[rb][d][e + 2], o[rb][d][e + 3]};
-      }
-      if (half == 0) *reinterpret_cast<floatx2*>(a.part_ml + 2 * slot) = floatx2{m[rb], l[rb]};
-      continue;
-    }
-    const float inv = l[rb] == 0.0f ? 0.0f : 1.0f / l[rb];  // (no key seen: zeros)
-    _Float16* op = a.out + orow[rb] * D + 4 * half;
+  l += __shfl_xor(l, 32);
+  if (wrow + col >= rows) return;
+  if (a.part_o != nullptr) {
+    const long long slot = orow * a.part_stride + a.part0 + split;
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        halfx4 y;
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<floatx4*>(a.part_o + slot * D + 32 * d + 2 * e + 4 * half) =
+            floatx4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+    }
+    if (half == 0) *reinterpret_cast<floatx2*>(a.part_ml + 2 * slot) = floatx2{m, l};
+    return;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros)
+  _Float16* op = a.out + orow * D + 4 * half;
+  const bool aligned = (reinterpret_cast<std::uintptr_t>(a.out) & 7) == 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = static_cast<_Float16>(o[rb][d][e + j] * inv);
-        _Float16* at = op + 32 * d + 2 * e;
-        if (aligned) {
-          *reinterpret_cast<halfx4*>(at) = y;
-        } else {
+  for (int d = 0; d < DB; ++d) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) at[j] = y[j];
-        }
+    for (int e = 0; e < 16; e += 4) {
+      halfx4 y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = static_cast<_Float16>(o[d][e + j] * inv);
+      _Float16* at = op + 32 * d + 2 * e;
+      if (aligned) {
+        *reinterpret_cast<halfx4*>(at) = y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) at[j] = y[j];
       }
     }
   }
