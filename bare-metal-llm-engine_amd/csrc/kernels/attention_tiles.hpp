@@ -378,13 +378,25 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
   auto seen = [&](int key0, int keys) {  // by any
     return key0 < last.hi && (key0 + keys > first.lo || key0 < a.sinks);
   };
-  // 32 keys' scores: hidden ones to -inf, and the row's largest in units of log2.
+  // 32 keys' scores: hidden ones to -inf. An element's key is a constant from the lane's
+  // first one on, so either end costs a comparison with it and a select.
   auto mask = [&](Scores& s, int key0) __attribute__((always_inline)) {
+    const int at = key0 + 4 * half;
+    if (key0 < a.sinks) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int j = key0 + 8 * (e >> 2) + 4 * half + (e & 3);
-      const bool hidden = (j >= mine.hi) | ((j < mine.lo) & (j >= a.sinks));
-      s.x[e] = hidden ? kNegInf : s.x[e];
+      for (int e = 0; e < 16; ++e) {
+        const int j = at + 8 * (e >> 2) + (e & 3);
+        s.x[e] = (j < mine.lo) & (j >= a.sinks) ? kNegInf : s.x[e];
+      }
+    } else if (last.lo > key0) {
+      const int lo = mine.lo - at;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s.x[e] = 8 * (e >> 2) + (e & 3) < lo ? kNegInf : s.x[e];
+    }
+    if (key0 + kKvBlock > first.hi) {
+      const int hi = mine.hi - at;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s.x[e] = 8 * (e >> 2) + (e & 3) >= hi ? kNegInf : s.x[e];
     }
   };
   auto largest = [&](const Scores& s, const Scale& c) __attribute__((always_inline)) {
@@ -437,24 +449,33 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
       lds_barrier();
       const int base = base_of(t);
       if (seen(base, kTileKeys)) {
+        const bool one = seen(base, kKvBlock), two = seen(base + kKvBlock, kKvBlock);
         Scale c = scale_of(buf, 0);
         if (!primed) {
           read_k(buf, 0);
           scores(even);
           read_k(buf, 1);
+          mx = largest(even, c);
         }
-        if (!primed || !whole(base)) {
-          if (!whole(base)) mask(even, base);
+        if (!whole(base)) {
+          mask(even, base);
           mx = largest(even, c);
         }
         raise(mx);
-        read_v(buf, 0);
-        put(free);
-        fetch_at(t + NB);
-        scores(odd);
-        weigh(even, c);
-        if constexpr (NB == 3) read_k(next, 0);
-        products();
+        if (one) {
+          read_v(buf, 0);
+          put(free);
+          fetch_at(t + NB);
+          scores(odd);
+          weigh(even, c);
+          if constexpr (NB == 3) read_k(next, 0);
+          products();
+        } else {
+          put(free);
+          fetch_at(t + NB);
+          scores(odd);
+          if constexpr (NB == 3) read_k(next, 0);
+        }
         c = scale_of(buf, 1);
         mx = largest(odd, c);
         if (!whole(base + kKvBlock)) {
@@ -466,12 +487,17 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
           lds_barrier();
           read_k(next, 0);
         }
-        read_v(buf, 1);
-        if constexpr (NB == 3) scores(even);
-        weigh(odd, c);
-        if constexpr (NB == 2) scores(even);
-        read_k(next, 1);
-        products();
+        if (two) {
+          read_v(buf, 1);
+          if constexpr (NB == 3) scores(even);
+          weigh(odd, c);
+          if constexpr (NB == 2) scores(even);
+          read_k(next, 1);
+          products();
+        } else {
+          scores(even);
+          read_k(next, 1);
+        }
         mx = largest(even, scale_of(next, 0));
         primed = t + 1 < t1;
       } else {
