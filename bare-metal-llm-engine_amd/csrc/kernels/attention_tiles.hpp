@@ -254,53 +254,55 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
   constexpr int LOADS = (PIECES + 64 * NW - 1) / (64 * NW);
   const bool loads = PIECES >= 64 * NW || tid < PIECES;  // (uniform in a wave)
   constexpr int LPR = D * static_cast<int>(sizeof(Elem)) / 16;  // loads of a row
-  uintx4 rk[LOADS], rv[LOADS];
-  [[maybe_unused]] float rks = 0.0f, rvs = 0.0f;
-  auto fetch = [&](int t) __attribute__((always_inline)) {
+  uintx4 raw[LOADS];  // of K or V
+  [[maybe_unused]] float raw_ks = 0.0f, raw_vs = 0.0f;
+  auto fetch = [&](int t, const Elem* g) __attribute__((always_inline)) {
     const int base = base_of(t);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int n = i * 64 * NW + (PIECES >= 64 * NW ? tid : tid & (PIECES - 1));
       const long long at = static_cast<long long>(min(base + n / LPR, hi - 1)) * D + (n % LPR) * (D / LPR);
-      rk[i] = *reinterpret_cast<const uintx4*>(kg + at);
-      rv[i] = *reinterpret_cast<const uintx4*>(vg + at);
-    }
-    if constexpr (Q8) {
-      const int blk = min(base / kKvBlock + (tid & 1), (hi - 1) / kKvBlock);
-      rks = a.ks[sb + blk];
-      rvs = a.vs[sb + blk];
+      raw[i] = *reinterpret_cast<const uintx4*>(g + at);
     }
   };
-  auto put = [&](int buf) __attribute__((always_inline)) {
+  auto put = [&](_Float16* tile, auto swz) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int n = i * 64 * NW + tid;
       const int row = n / LPR;
-      if (!loads) continue;
-      const int at = buf * TILE + row * D;
       const int piece = n % LPR;
+      if (!loads) continue;
       if constexpr (Q8) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          *reinterpret_cast<halfx8*>(s_k + at + 8 * ((2 * piece + j) ^ k_swz(row))) =
-              eight_fp8(rk[i][2 * j], rk[i][2 * j + 1]);
-          *reinterpret_cast<halfx8*>(s_v + at + 8 * ((2 * piece + j) ^ v_swz(row))) =
-              eight_fp8(rv[i][2 * j], rv[i][2 * j + 1]);
-        }
+        for (int j = 0; j < 2; ++j)
+          *reinterpret_cast<halfx8*>(tile + row * D + 8 * ((2 * piece + j) ^ swz(row))) =
+              eight_fp8(raw[i][2 * j], raw[i][2 * j + 1]);
       } else {
-        *reinterpret_cast<uintx4*>(s_k + at + 8 * (piece ^ k_swz(row))) = rk[i];
-        *reinterpret_cast<uintx4*>(s_v + at + 8 * (piece ^ v_swz(row))) = rv[i];
-      }
-    }
-    if constexpr (Q8) {
-      if (tid < 2) {
-        // (at least 1e-30, so that a mask's -inf stays -inf under a scale of zero)
-        const float vs = fmaxf(rvs, kLeastVScale);
-        *reinterpret_cast<floatx4*>(s_scale[buf][tid]) =
-            floatx4{fmaxf(scale2 * rks, 1e-30f), __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), 0.0f};
+        *reinterpret_cast<uintx4*>(tile + row * D + 8 * (piece ^ swz(row))) = raw[i];
       }
     }
   };
+  auto fetch_k = [&](int t) __attribute__((always_inline)) {  // and the scales of both
+    fetch(t, kg);
+    if constexpr (Q8) {
+      const long long blk = sb + min(base_of(t) / kKvBlock + (tid & 1), (hi - 1) / kKvBlock);
+      raw_ks = a.ks[blk];
+      raw_vs = a.vs[blk];
+    }
+  };
+  auto fetch_v = [&](int t) __attribute__((always_inline)) { fetch(t, vg); };
+  auto put_k = [&](int buf) __attribute__((always_inline)) {
+    put(s_k + buf * TILE, k_swz);
+    if constexpr (Q8) {
+      if (tid < 2) {
+        // (at least 1e-30, so that a mask's -inf stays -inf under a scale of zero)
+        const float vs = fmaxf(raw_vs, kLeastVScale);
+        *reinterpret_cast<floatx4*>(s_scale[buf][tid]) =
+            floatx4{fmaxf(scale2 * raw_ks, 1e-30f), __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), 0.0f};
+      }
+    }
+  };
+  auto put_v = [&](int buf) __attribute__((always_inline)) { put(s_v + buf * TILE, v_swz); };
   // The factor of a 32-key block's scores, log2 and inverse of its V scale.
   struct Scale {
     float f, lv, ivs;
@@ -429,14 +431,18 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
   clear();
   if (t0 < t1) {
     // (tiles past the last one are taken as the last one, and not used)
-    auto fetch_at = [&](int t) __attribute__((always_inline)) { fetch(min(t, t1 - 1)); };
-    fetch(t0);
-    put(0);
-    fetch_at(t0 + 1);
+    auto at_most = [&](int t) { return min(t, t1 - 1); };
+    fetch_k(t0);
+    put_k(0);
+    fetch_v(t0);
+    put_v(0);
     if constexpr (NB == 3) {
-      put(1);
-      fetch_at(t0 + 2);
+      fetch_k(at_most(t0 + 1));
+      put_k(1);
+      fetch_v(at_most(t0 + 1));
+      put_v(1);
     }
+    fetch_k(at_most(t0 + NB - 1));
     float mx = 0.0f;
     bool primed = false;  // `even` holds the tile's scores, mx their largest, kf the second keys
     int buf = 0;
@@ -464,15 +470,15 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
         raise(mx);
         if (one) {
           read_v(buf, 0);
-          put(free);
-          fetch_at(t + NB);
+          put_k(free);
+          fetch_v(at_most(t + NB - 1));
           scores(odd);
           weigh(even, c);
           if constexpr (NB == 3) read_k(next, 0);
           products();
         } else {
-          put(free);
-          fetch_at(t + NB);
+          put_k(free);
+          fetch_v(at_most(t + NB - 1));
           scores(odd);
           if constexpr (NB == 3) read_k(next, 0);
         }
@@ -489,21 +495,27 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
         }
         if (two) {
           read_v(buf, 1);
+          put_v(free);
+          fetch_k(at_most(t + NB));
           if constexpr (NB == 3) scores(even);
           weigh(odd, c);
           if constexpr (NB == 2) scores(even);
           read_k(next, 1);
           products();
         } else {
+          put_v(free);
+          fetch_k(at_most(t + NB));
           scores(even);
           read_k(next, 1);
         }
         mx = largest(even, scale_of(next, 0));
         primed = t + 1 < t1;
       } else {
-        put(free);
-        fetch_at(t + NB);
+        put_k(free);
+        fetch_v(at_most(t + NB - 1));
         if constexpr (NB == 2) lds_barrier();
+        put_v(free);
+        fetch_k(at_most(t + NB));
         primed = false;
       }
       buf = next;
@@ -515,8 +527,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
     clear();
     for (int t = t0; t < t1; ++t) {
       __syncthreads();
-      fetch(t);
-      put(0);
+      fetch_k(t);
+      put_k(0);
+      fetch_v(t);
+      put_v(0);
       __syncthreads();
 #pragma unroll 1
       for (int sub = 0; sub < 2; ++sub) {
