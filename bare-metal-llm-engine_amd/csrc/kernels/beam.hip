@@ -25,18 +25,25 @@ constexpr int kMaxBeams = 32;
 constexpr int kWaves = 4;
 constexpr int kVpt = 16;       // values of a lane in one step of a wave
 constexpr int kWaveList = 64 * kVpt + kMaxOut;
+constexpr int kWaveSteps = (kWaveList + 63) / 64;
 
-// Key of a candidate: larger logits first, then lower tokens. 0 stands for none.
-__device__ __forceinline__ u64 key_of(float x, unsigned token) {
+// A logit as a number that orders like it. 0 stands for none.
+__device__ __forceinline__ unsigned order_of(float x) {
   const unsigned u = __float_as_uint(x + 0.0f);  // (-0 as 0)
-  const unsigned v = u ^ ((u >> 31) != 0 ? 0xffffffffu : 0x80000000u);
-  return (static_cast<u64>(v) << 32) | (0xffffffffu - token);
+  return u ^ ((u >> 31) != 0 ? 0xffffffffu : 0x80000000u);
+}
+// Key of a candidate: larger logits first, then lower tokens.
+__device__ __forceinline__ u64 key_of(float x, unsigned token) {
+  return (static_cast<u64>(order_of(x)) << 32) | (0xffffffffu - token);
 }
 __device__ __forceinline__ float logit_of(u64 key) {
   const unsigned v = static_cast<unsigned>(key >> 32);
   return __uint_as_float(v ^ ((v >> 31) != 0 ? 0x80000000u : 0xffffffffu));
 }
 __device__ __forceinline__ unsigned token_of(u64 key) { return 0xffffffffu - static_cast<unsigned>(key); }
+
+// e^x to 2 units in the last place and the rounding of x log2 e.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
 // The largest of the wave's values, in every lane.
 template <int CTRL>
@@ -59,6 +66,12 @@ __device__ __forceinline__ u64 wave_max(u64 x) {
   return (static_cast<u64>(top) << 32) | low;
 }
 
+__device__ __forceinline__ u64 lane_value(u64 x, int lane) {
+  const unsigned lo = __builtin_amdgcn_readlane(static_cast<unsigned>(x), lane);
+  const unsigned hi = __builtin_amdgcn_readlane(static_cast<unsigned>(x >> 32), lane);
+  return (static_cast<u64>(hi) << 32) | lo;
+}
+
 // One wave's `k` best keys, in descending order in list[0 .. count).
 struct Best {
   u64* list;  // LDS, kWaveList entries
@@ -66,69 +79,67 @@ struct Best {
   int count;
   u64 floor;  // a key at or below it is not among them: the k-th best where there are k
 
-  // Adds N keys of each lane (0: none; all others differ).
-  template <int N>
-  __device__ __forceinline__ void offer(const u64 (&key)[N], int lane) {
-    u64 top = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) top = max(top, key[i]);
-    const int lanes = __builtin_popcountll(__ballot(top > floor));
-    if (lanes == 0) return;
-    u64 least = floor;  // keys above it are taken
-    if (lanes > k) {
-      // the k-th best of the lanes' best keys: at least k keys are that large, and they
-      // are in k lanes
-      u64 t = top;
-      for (int i = 0; i < k; ++i) {
-        least = wave_max(t);
-        if (t == least) t = 0;
-      }
-      least -= 1;
+  // A value that at least k lanes' `top` reach, few more where halving the interval 24
+  // times finds one (fewer lanes than k above `least`: least).
+  __device__ __forceinline__ unsigned reached(unsigned top, unsigned least) const {
+    unsigned hi = wave_max(top);
+    int n = __builtin_popcountll(__ballot(top > least));
+    for (int i = 0; i < 24 && n > k + 8 && hi > least + 1; ++i) {
+      const unsigned mid = least + (hi - least) / 2;
+      const int c = __builtin_popcountll(__ballot(top > mid));
+      if (c >= k) least = mid, n = c;
+      else hi = mid;
     }
+    return least + 1;
+  }
+
+  // Adds the keys above `floor` of key_at(0 .. N - 1), N of each lane, that may be among
+  // the best: those whose order value is `least` or more. top: the lane's largest.
+  template <int N, class F>
+  __device__ __forceinline__ void take(unsigned least, F&& order_at, int lane, unsigned (&token)[N]) {
     int n = count;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const bool in = key[i] > least;
+      const unsigned v = order_at(i);
+      const u64 key = (static_cast<u64>(v) << 32) | token[i];
+      const bool in = v >= least && key > floor;
       const u64 mask = __ballot(in);
       if (mask != 0) {
         const int at = n + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
                                                      __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
-        if (in) list[at] = key[i];
+        if (in) list[at] = key;
         n += __builtin_popcountll(mask);
       }
     }
     sort(n, lane);
   }
 
-  // Brings the k best of list[0 .. n) to its front, in order: each entry's place is the
+  // Brings the k best of list[0 .. n) to its front, in order: an entry's place is the
   // number of larger ones.
   __device__ __forceinline__ void sort(int n, int lane) {
     wave_sync();
     const int keep = min(n, k);
-    u64 mine[(kWaveList + 63) / 64];
-    int place[(kWaveList + 63) / 64];
-    const int steps = (n + 63) / 64;
-    if (steps == 1) {
-      mine[0] = lane < n ? list[lane] : 0;
-      place[0] = 0;
-      for (int j = 0; j < n; ++j) place[0] += list[j] > mine[0];
+    if (n <= 64) {
+      const u64 mine = lane < n ? list[lane] : 0;
+      int place = 0;
+      for (int j = 0; j < n; ++j) place += lane_value(mine, j) > mine;
       wave_sync();
-      if (lane < n && place[0] < keep) list[place[0]] = mine[0];
+      if (lane < n && place < keep) list[place] = mine;
     } else {
+      // Many equal logits, or k past 32. The k best by rounds, each the largest left.
+      u64 mine[kWaveSteps];
 #pragma unroll
-      for (int s = 0; s < (kWaveList + 63) / 64; ++s) {
-        mine[s] = 64 * s + lane < n ? list[64 * s + lane] : 0;
-        place[s] = 0;
-      }
-      for (int j = 0; j < n; ++j) {
-        const u64 x = list[j];
-#pragma unroll
-        for (int s = 0; s < (kWaveList + 63) / 64; ++s) place[s] += x > mine[s];
-      }
+      for (int s = 0; s < kWaveSteps; ++s) mine[s] = 64 * s + lane < n ? list[64 * s + lane] : 0;
       wave_sync();
+      for (int j = 0; j < keep; ++j) {
+        u64 top = 0;
 #pragma unroll
-      for (int s = 0; s < (kWaveList + 63) / 64; ++s)
-        if (mine[s] != 0 && place[s] < keep) list[place[s]] = mine[s];
+        for (int s = 0; s < kWaveSteps; ++s) top = max(top, mine[s]);
+        top = wave_max(top);
+#pragma unroll
+        for (int s = 0; s < kWaveSteps; ++s) mine[s] = mine[s] == top ? 0 : mine[s];
+        if (lane == 0) list[j] = top;
+      }
     }
     wave_sync();
     count = keep;
@@ -180,8 +191,7 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
   Best best = {s_list[wave], a.n_out, 0, 0};
   float m = kNegInf, sum = 0.0f;
   for (int at = begin; at < end; at += kStep) {
-    float v[kVpt];
-    u64 key[kVpt];
+    float v[kVpt];  // (-inf behind the row's end)
 #pragma unroll
     for (int i = 0; i < kVpt / VEC; ++i) {
       const int t0 = at + (i * 64 * kWaves + tid) * VEC;
@@ -196,34 +206,42 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
             const unsigned short h = static_cast<unsigned short>(w[e / 2] >> (16 * (e % 2)));
             v[i * VEC + e] = static_cast<float>(__builtin_bit_cast(_Float16, h));
           }
-          key[i * VEC + e] = key_of(v[i * VEC + e], static_cast<unsigned>(t0 + e));
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const bool in = t0 + e < end;
-          v[i * VEC + e] = in ? static_cast<float>(x[t0 + e]) : kNegInf;
-          key[i * VEC + e] = in ? key_of(v[i * VEC + e], static_cast<unsigned>(t0 + e)) : 0;
-        }
+        for (int e = 0; e < VEC; ++e) v[i * VEC + e] = t0 + e < end ? static_cast<float>(x[t0 + e]) : kNegInf;
       }
     }
-    float top = m;
+    float top = v[0];
 #pragma unroll
-    for (int i = 0; i < kVpt; ++i) top = fmaxf(top, v[i]);
+    for (int i = 1; i < kVpt; ++i) top = fmaxf(top, v[i]);
     // (all -inf so far: against 0, whose sum stays 0)
-    const float ref = top == kNegInf ? 0.0f : top;
-    sum *= expf(m - ref);
-    m = top;
+    const float mn = fmaxf(m, top);
+    const float ref = mn == kNegInf ? 0.0f : mn;
+    float part[4] = {};
 #pragma unroll
-    for (int i = 0; i < kVpt; ++i) sum += expf(v[i] - ref);
-    best.offer(key, lane);
+    for (int i = 0; i < kVpt; ++i) part[i & 3] += exp_of(v[i] - ref);
+    sum = fmaf(sum, exp_of(m - ref), (part[0] + part[1]) + (part[2] + part[3]));
+    m = mn;
+    // Later tokens lose a tie, so only larger logits than the k-th best get in.
+    const unsigned lane_top = order_of(top);
+    const unsigned least = static_cast<unsigned>(best.floor >> 32);
+    if (__any(lane_top > least)) {
+      unsigned token[kVpt];
+#pragma unroll
+      for (int i = 0; i < kVpt; ++i) token[i] = 0xffffffffu - (at + ((i / VEC) * 64 * kWaves + tid) * VEC + i % VEC);
+      best.take(best.reached(lane_top, least), [&](int i) {
+        const bool in = 0xffffffffu - token[i] < static_cast<unsigned>(end);
+        return in ? order_of(v[i]) : 0u;
+      }, lane, token);
+    }
   }
   // the wave's max and sum
   float wm = m;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) wm = fmaxf(wm, __shfl_xor(wm, off));
   const float ref = wm == kNegInf ? 0.0f : wm;
-  const float ws = gemv::wave_sum(sum * expf(m - ref));
+  const float ws = gemv::wave_sum(sum * exp_of(m - ref));
   if (lane == 0) {
     s_max[wave] = wm;
     s_sum[wave] = ws;
@@ -246,7 +264,7 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_max[w]);
     const float r = top == kNegInf ? 0.0f : top;
     float s = 0.0f;
-    for (int w = 0; w < kWaves; ++w) s += s_sum[w] * expf(s_max[w] - r);
+    for (int w = 0; w < kWaves; ++w) s += s_sum[w] * exp_of(s_max[w] - r);
     a.sums[out] = floatx2{top, s};
   }
 }
@@ -269,6 +287,16 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(SelectArgs a) {
     const long long row = group * a.beams + b;
     const float given = a.scores[row];
     const bool done = a.finished != nullptr && a.finished[row] != 0;
+    const long long n = static_cast<long long>(a.pieces) * k;
+    u64 key[4];
+    auto load_keys = [&](long long i0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const long long i = i0 + 64 * j + lane;
+        key[j] = i < n ? a.keys[row * n + i] : 0;
+      }
+    };
+    load_keys(0);
     float m = kNegInf;
     for (int i = lane; i < a.pieces; i += 64) m = fmaxf(m, a.sums[row * a.pieces + i][0]);
 #pragma unroll
@@ -285,13 +313,19 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(SelectArgs a) {
     const bool plain = !done && finite && lse - lse == 0.0;
     Best best = {s_list[wave], k, 0, 0};
     if (plain) {
-      const long long n = static_cast<long long>(a.pieces) * k;
-      const u64* keys = a.keys + row * n;
-      for (long long i0 = 0; i0 < n; i0 += 64 * 4) {
-        u64 key[4];
+      for (long long i0 = 0;; i0 += 64 * 4) {
+        unsigned top = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) key[j] = i0 + 64 * j + lane < n ? keys[i0 + 64 * j + lane] : 0;
-        best.offer(key, lane);
+        for (int j = 0; j < 4; ++j) top = max(top, static_cast<unsigned>(key[j] >> 32));
+        unsigned token[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) token[j] = static_cast<unsigned>(key[j]);
+        // (here a later key may win a tie)
+        const unsigned least = static_cast<unsigned>(best.floor >> 32);
+        best.take(best.reached(top, least == 0 ? 0 : least - 1),
+                  [&](int j) { return static_cast<unsigned>(key[j] >> 32); }, lane, token);
+        if (i0 + 64 * 4 >= n) break;
+        load_keys(i0 + 64 * 4);
       }
     }
     for (int i = lane; i < k; i += 64) {
