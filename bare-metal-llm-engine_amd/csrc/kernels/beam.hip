@@ -10,6 +10,7 @@
 #include "launch.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace eng {
 namespace beam {
@@ -27,19 +28,19 @@ constexpr int kVpt = 16;       // values of a lane in one step of a wave
 constexpr int kWaveList = 64 * kVpt + kMaxOut;
 constexpr int kWaveSteps = (kWaveList + 63) / 64;
 
-// A logit as a number that orders like it. 0 stands for none.
+// A logit as a number that orders like it.
 __device__ __forceinline__ unsigned order_of(float x) {
   const unsigned u = __float_as_uint(x + 0.0f);  // (-0 as 0)
   return u ^ ((u >> 31) != 0 ? 0xffffffffu : 0x80000000u);
 }
-// Key of a candidate: larger logits first, then lower tokens.
+// Key of a candidate: larger logits first, then lower tokens. 0 stands for none.
 __device__ __forceinline__ u64 key_of(float x, unsigned token) {
   return (static_cast<u64>(order_of(x)) << 32) | (0xffffffffu - token);
 }
-__device__ __forceinline__ float logit_of(u64 key) {
-  const unsigned v = static_cast<unsigned>(key >> 32);
+__device__ __forceinline__ float value_of(unsigned v) {
   return __uint_as_float(v ^ ((v >> 31) != 0 ? 0x80000000u : 0xffffffffu));
 }
+__device__ __forceinline__ float logit_of(u64 key) { return value_of(static_cast<unsigned>(key >> 32)); }
 __device__ __forceinline__ unsigned token_of(u64 key) { return 0xffffffffu - static_cast<unsigned>(key); }
 
 // e^x to 2 units in the last place and the rounding of x log2 e.
@@ -72,51 +73,46 @@ __device__ __forceinline__ u64 lane_value(u64 x, int lane) {
   return (static_cast<u64>(hi) << 32) | lo;
 }
 
-// One wave's `k` best keys, in descending order in list[0 .. count).
+// One wave's candidates, of which it keeps the `k` best.
 struct Best {
   u64* list;  // LDS, kWaveList entries
   int k;
-  int count;
-  u64 floor;  // a key at or below it is not among them: the k-th best where there are k
+  int n;
 
   // A value that at least k lanes' `top` reach, few more where halving the interval 24
-  // times finds one (fewer lanes than k above `least`: least).
-  __device__ __forceinline__ unsigned reached(unsigned top, unsigned least) const {
-    unsigned hi = wave_max(top);
-    int n = __builtin_popcountll(__ballot(top > least));
-    for (int i = 0; i < 24 && n > k + 8 && hi > least + 1; ++i) {
-      const unsigned mid = least + (hi - least) / 2;
-      const int c = __builtin_popcountll(__ballot(top > mid));
-      if (c >= k) least = mid, n = c;
+  // times finds one.
+  __device__ __forceinline__ unsigned reached(unsigned top) const {
+    unsigned hi = wave_max(top), lo = ~wave_max(~top);  // (all reach lo)
+    int c = 64;
+    for (int i = 0; i < 24 && c > k + 8 && hi - lo > 1; ++i) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      const int reach = __builtin_popcountll(__ballot(top >= mid));
+      if (reach >= k) lo = mid, c = reach;
       else hi = mid;
     }
-    return least + 1;
+    return lo;
   }
 
-  // Adds the keys above `floor` of key_at(0 .. N - 1), N of each lane, that may be among
-  // the best: those whose order value is `least` or more. top: the lane's largest.
-  template <int N, class F>
-  __device__ __forceinline__ void take(unsigned least, F&& order_at, int lane, unsigned (&token)[N]) {
-    int n = count;
+  // Adds those of N items of each lane that reach(i) says, item i being key_at(i) (0: none).
+  template <int N, class R, class K>
+  __device__ __forceinline__ void add(R&& reach, K&& key_at, int lane) {
+    static_assert(64 * N + kMaxOut <= kWaveList, "the list holds them all");
+    if (n > kMaxOut) sort(lane);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const unsigned v = order_at(i);
-      const u64 key = (static_cast<u64>(v) << 32) | token[i];
-      const bool in = v >= least && key > floor;
-      const u64 mask = __ballot(in);
-      if (mask != 0) {
-        const int at = n + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
-                                                     __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
-        if (in) list[at] = key;
-        n += __builtin_popcountll(mask);
-      }
+      if (__ballot(reach(i)) == 0) continue;
+      const u64 key = key_at(i);
+      const u64 mask = __ballot(reach(i) && key != 0);
+      const int at = n + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(mask >> 32),
+                                                   __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(mask), 0));
+      if (reach(i) && key != 0) list[at] = key;
+      n += __builtin_popcountll(mask);
     }
-    sort(n, lane);
   }
 
   // Brings the k best of list[0 .. n) to its front, in order: an entry's place is the
   // number of larger ones.
-  __device__ __forceinline__ void sort(int n, int lane) {
+  __device__ __forceinline__ void sort(int lane) {
     wave_sync();
     const int keep = min(n, k);
     if (n <= 64) {
@@ -142,8 +138,7 @@ struct Best {
       }
     }
     wave_sync();
-    count = keep;
-    floor = count == k ? list[k - 1] : 0;
+    n = keep;
   }
 
   // LDS accesses of this wave before it are done before those behind it.
@@ -165,17 +160,20 @@ struct SelectArgs {
   unsigned char* out_finished;
   int beams, n_out, vocab, eos;
   int pieces;      // of a row
-  int piece;       // values of one, a multiple of kStep
   u64* keys;       // [rows][pieces][n_out], 0 behind the last one
   floatx2* sums;   // [rows][pieces]: max, sum of exp(x - max)
 };
 
 constexpr int kStep = 64 * kWaves * kVpt;  // values of a workgroup's step
 
-// One workgroup per (row, piece). NaN in a row makes its sum NaN, +inf too.
-template <typename T, bool VECTOR>
+// One workgroup per (row, piece of STEPS steps), the whole piece in registers, 16 STEPS
+// values of a lane. The k-th largest of the lanes' largest values bounds the k best from
+// below, so few values are looked at one by one. NaN in a row makes its sum NaN, +inf too.
+// Bound by the logits' bytes.
+template <typename T, bool VECTOR, int STEPS>
 __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
   constexpr int VEC = 16 / sizeof(T);
+  constexpr int LOADS = kVpt / VEC;
   __shared__ u64 s_list[kWaves][kWaveList];
   __shared__ float s_max[kWaves], s_sum[kWaves];
   __shared__ int s_count[kWaves];
@@ -185,80 +183,75 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
   const unsigned row = blockIdx.x / static_cast<unsigned>(a.pieces);
   const int piece = static_cast<int>(blockIdx.x - row * static_cast<unsigned>(a.pieces));
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-  const int begin = piece * a.piece;
-  const int end = min(begin + a.piece, a.vocab);
+  const int begin = piece * (STEPS * kStep);
+  const int end = min(begin + STEPS * kStep, a.vocab);
 
-  Best best = {s_list[wave], a.n_out, 0, 0};
-  float m = kNegInf, sum = 0.0f;
-  for (int at = begin; at < end; at += kStep) {
-    float v[kVpt];  // (-inf behind the row's end)
+  uintx4 raw[STEPS][LOADS];  // as in memory; -inf behind the row's end
 #pragma unroll
-    for (int i = 0; i < kVpt / VEC; ++i) {
-      const int t0 = at + (i * 64 * kWaves + tid) * VEC;
+  for (int c = 0; c < STEPS; ++c) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int t0 = begin + c * kStep + (i * 64 * kWaves + tid) * VEC;
       if (VECTOR && t0 + VEC <= end) {
-        const uintx4 w = *reinterpret_cast<const uintx4*>(x + t0);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          if constexpr (sizeof(T) == 4) {
-            const unsigned u = w[e];
-            v[i * VEC + e] = __uint_as_float(u);
-          } else {
-            const unsigned short h = static_cast<unsigned short>(w[e / 2] >> (16 * (e % 2)));
-            v[i * VEC + e] = static_cast<float>(__builtin_bit_cast(_Float16, h));
-          }
-        }
+        raw[c][i] = *reinterpret_cast<const uintx4*>(x + t0);
       } else {
+        T some[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i * VEC + e] = t0 + e < end ? static_cast<float>(x[t0 + e]) : kNegInf;
+        for (int e = 0; e < VEC; ++e) some[e] = t0 + e < end ? x[t0 + e] : static_cast<T>(kNegInf);
+        raw[c][i] = __builtin_bit_cast(uintx4, some);
       }
     }
-    float top = v[0];
+  }
+  auto value = [&](int c, int i) __attribute__((always_inline)) {
+    const unsigned w = raw[c][i / VEC][i % VEC * sizeof(T) / 4];
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(w >> (16 * (i % 2)))));
+  };
+  float m = kNegInf;
 #pragma unroll
-    for (int i = 1; i < kVpt; ++i) top = fmaxf(top, v[i]);
-    // (all -inf so far: against 0, whose sum stays 0)
-    const float mn = fmaxf(m, top);
-    const float ref = mn == kNegInf ? 0.0f : mn;
-    float part[4] = {};
+  for (int c = 0; c < STEPS; ++c) {
 #pragma unroll
-    for (int i = 0; i < kVpt; ++i) part[i & 3] += exp_of(v[i] - ref);
-    sum = fmaf(sum, exp_of(m - ref), (part[0] + part[1]) + (part[2] + part[3]));
-    m = mn;
-    // Later tokens lose a tie, so only larger logits than the k-th best get in.
-    const unsigned lane_top = order_of(top);
-    const unsigned least = static_cast<unsigned>(best.floor >> 32);
-    if (__any(lane_top > least)) {
-      unsigned token[kVpt];
+    for (int i = 0; i < kVpt; ++i) m = fmaxf(m, value(c, i));
+  }
+  float part[4] = {};
+  {
+    const float ref = m == kNegInf ? 0.0f : m;  // (all -inf: against 0, a sum of 0)
 #pragma unroll
-      for (int i = 0; i < kVpt; ++i) token[i] = 0xffffffffu - (at + ((i / VEC) * 64 * kWaves + tid) * VEC + i % VEC);
-      best.take(best.reached(lane_top, least), [&](int i) {
-        const bool in = 0xffffffffu - token[i] < static_cast<unsigned>(end);
-        return in ? order_of(v[i]) : 0u;
-      }, lane, token);
+    for (int c = 0; c < STEPS; ++c) {
+#pragma unroll
+      for (int i = 0; i < kVpt; ++i) part[i & 3] += exp_of(value(c, i) - ref);
     }
   }
-  // the wave's max and sum
-  float wm = m;
+  const float sum = (part[0] + part[1]) + (part[2] + part[3]);
+  Best best = {s_list[wave], a.n_out, 0};
+  const float least = value_of(best.reached(order_of(m)));
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) wm = fmaxf(wm, __shfl_xor(wm, off));
+  for (int c = 0; c < STEPS; ++c)
+    best.add<kVpt>([&](int i) { return value(c, i) >= least; }, [&](int i) {
+      const int t = begin + c * kStep + (i / VEC * 64 * kWaves + tid) * VEC + i % VEC;
+      return t < end ? key_of(value(c, i), static_cast<unsigned>(t)) : 0;
+    }, lane);
+  best.sort(lane);
+  // the wave's max and sum
+  const float wm = value_of(wave_max(order_of(m)));
   const float ref = wm == kNegInf ? 0.0f : wm;
   const float ws = gemv::wave_sum(sum * exp_of(m - ref));
   if (lane == 0) {
     s_max[wave] = wm;
     s_sum[wave] = ws;
-    s_count[wave] = best.count;
+    s_count[wave] = best.n;
   }
   __syncthreads();
   if (wave != 0) return;
   // the other waves' keys behind its own
-  int n = best.count;
   for (int w = 1; w < kWaves; ++w) {
     const int c = s_count[w];
-    if (lane < c) best.list[n + lane] = s_list[w][lane];
-    n += c;
+    if (lane < c) best.list[best.n + lane] = s_list[w][lane];
+    best.n += c;
   }
-  best.sort(n, lane);
+  best.sort(lane);
   const long long out = static_cast<long long>(blockIdx.x);
-  for (int i = lane; i < a.n_out; i += 64) a.keys[out * a.n_out + i] = i < best.count ? best.list[i] : 0;
+  for (int i = lane; i < a.n_out; i += 64) a.keys[out * a.n_out + i] = i < best.n ? best.list[i] : 0;
   if (lane == 0) {
     float top = kNegInf;
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_max[w]);
@@ -299,34 +292,29 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(SelectArgs a) {
     load_keys(0);
     float m = kNegInf;
     for (int i = lane; i < a.pieces; i += 64) m = fmaxf(m, a.sums[row * a.pieces + i][0]);
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
-    double sum = 0.0;
+    m = value_of(wave_max(order_of(m)));
+    float part = 0.0f;
     for (int i = lane; i < a.pieces; i += 64) {
       const floatx2 p = a.sums[row * a.pieces + i];
-      sum += static_cast<double>(p[1]) * (p[0] == kNegInf ? 1.0 : exp(static_cast<double>(p[0]) - m));
+      part = fmaf(p[1], p[0] == kNegInf ? 1.0f : exp_of(p[0] - m), part);
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
+    const double sum = gemv::wave_sum(part);
     const double lse = static_cast<double>(m) + log(sum);
     const bool finite = given > kNegInf && given < -kNegInf;
     const bool plain = !done && finite && lse - lse == 0.0;
-    Best best = {s_list[wave], k, 0, 0};
+    Best best = {s_list[wave], k, 0};
     if (plain) {
       for (long long i0 = 0;; i0 += 64 * 4) {
         unsigned top = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) top = max(top, static_cast<unsigned>(key[j] >> 32));
-        unsigned token[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) token[j] = static_cast<unsigned>(key[j]);
-        // (here a later key may win a tie)
-        const unsigned least = static_cast<unsigned>(best.floor >> 32);
-        best.take(best.reached(top, least == 0 ? 0 : least - 1),
-                  [&](int j) { return static_cast<unsigned>(key[j] >> 32); }, lane, token);
+        const unsigned least = best.reached(top);
+        best.add<4>([&](int j) { return static_cast<unsigned>(key[j] >> 32) >= least; },
+                    [&](int j) { return key[j]; }, lane);
         if (i0 + 64 * 4 >= n) break;
         load_keys(i0 + 64 * 4);
       }
+      best.sort(lane);
     }
     for (int i = lane; i < k; i += 64) {
       double score = ninf;
@@ -334,7 +322,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(SelectArgs a) {
       if (plain) {
         // (fewer than k tokens in the vocabulary: none)
         token = -1;
-        if (i < best.count) {
+        if (i < best.n) {
           const u64 key = best.list[i];
           token = static_cast<int>(token_of(key));
           score = static_cast<double>(given) + (static_cast<double>(logit_of(key)) - lse);
@@ -357,6 +345,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(SelectArgs a) {
     if (token < 0) continue;
     const int b = i / k;
     int place = 0;  // (a beam's own are in order)
+#pragma unroll 8
     for (int j = 0; j < n; ++j) place += s_token[j] >= 0 && (s_score[j] > score || (s_score[j] == score && j < i));
     if (place < k) {
       const long long out = group * k + place;
@@ -471,14 +460,13 @@ void select_entry(const void* logits, bool half, int64_t ld, const float* scores
   a.n_out = static_cast<int>(n_out);
   a.vocab = static_cast<int>(vocab);
   a.eos = eos < 0 ? -1 : static_cast<int>(eos);
-  // Pieces of a row: a workgroup's step each while that leaves fewer than four to a CU.
+  // Steps of a piece: as many as leave two workgroups to a CU, up to four.
   const long long steps = (vocab + kStep - 1) / kStep;
   ENG_CHECK(batch <= 0xffffffffLL / (64 * kWaves) / (beams * steps),
             "beam_select: too many logits for one launch");
   const long long rows = batch * beams;
-  const long long want = std::max(1ll, 4ll * device_cu_count() / rows);
-  const long long per = (steps + std::min(steps, want) - 1) / std::min(steps, want);
-  a.piece = static_cast<int>(per * kStep);
+  int per = 4;
+  while (per > 1 && rows * ((steps + per - 1) / per) < 2ll * device_cu_count()) per /= 2;
   a.pieces = static_cast<int>((steps + per - 1) / per);
   const std::size_t lists = static_cast<std::size_t>(rows) * a.pieces;
   StreamScratch scratch(s, lists * (n_out + 1) * 8);
@@ -486,9 +474,15 @@ void select_entry(const void* logits, bool half, int64_t ld, const float* scores
   a.sums = reinterpret_cast<floatx2*>(a.keys + lists * n_out);
   const bool vector = aligned_to(logits, 16) && (ld * elem) % 16 == 0;
   const unsigned grid = static_cast<unsigned>(lists);
-  auto go = [&](auto kernel) { kernel<<<grid, 64 * kWaves, 0, s>>>(a); };
-  if (half) vector ? go(piece_kernel<_Float16, true>) : go(piece_kernel<_Float16, false>);
-  else vector ? go(piece_kernel<float, true>) : go(piece_kernel<float, false>);
+  auto go = [&](auto elem, auto vec) {
+    using T = decltype(elem);
+    constexpr bool kVector = decltype(vec)::value;
+    if (per == 4) piece_kernel<T, kVector, 4><<<grid, 64 * kWaves, 0, s>>>(a);
+    else if (per == 2) piece_kernel<T, kVector, 2><<<grid, 64 * kWaves, 0, s>>>(a);
+    else piece_kernel<T, kVector, 1><<<grid, 64 * kWaves, 0, s>>>(a);
+  };
+  if (half) vector ? go(_Float16{}, std::true_type{}) : go(_Float16{}, std::false_type{});
+  else vector ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
   ENG_LAUNCH_CHECK();
   join_kernel<<<static_cast<unsigned>(batch), 64 * kWaves, 0, s>>>(a);
   ENG_LAUNCH_CHECK();
