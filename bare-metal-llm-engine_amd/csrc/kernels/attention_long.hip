@@ -106,12 +106,22 @@ int tile_waves(long long units, long long unit_rows) {
 
 int tiles_of(long long rows, int tile) { return static_cast<int>((rows + tile - 1) / tile); }
 
-// Splits of the keys of `wgs` workgroups that read up to `keys` keys each, in steps of
-// `step` keys, for `per_cu` workgroups to a CU.
-int auto_splits(long long wgs, long long keys, long long step, int per_cu) {
-  const long long steps = (keys + step - 1) / step;
-  const long long want = static_cast<long long>(per_cu) * device_cu_count() / wgs;
-  return static_cast<int>(std::max(1ll, std::min({want, steps / 4, static_cast<long long>(kMaxStates)})));
+// Splits of the keys, up to `keys`, of `wgs` workgroups of many rows: as many as fill the
+// CUs, two workgroups of four waves to each, at least four tiles a split.
+int tile_splits(long long wgs, long long keys, int waves) {
+  const long long want = (8 / waves) * static_cast<long long>(device_cu_count()) / wgs;
+  return static_cast<int>(std::max(1ll, std::min({want, (keys + kTileKeys - 1) / kTileKeys / 4,
+                                                  static_cast<long long>(kMaxStates)})));
+}
+// And of few rows: one workgroup to a CU, at least two blocks a split, and one split,
+// without the merge's launch, up to 12 blocks at D = 128 or 24 at D = 64 (one token of 32
+// heads: 300 tokens 7.3 us, 8.2 in four splits; 8192 tokens of 32 / 8 heads 12.5-13.3 in 16
+// or 32 splits, 16.5 in 8 or 64; 16 sequences of 2048 30 in 1 to 4, 34 in 8).
+int few_splits(long long wgs, long long keys, long long D) {
+  const long long blocks = (keys + kKvBlock - 1) / kKvBlock;
+  if (blocks * D <= 12 * 128) return 1;
+  const long long want = device_cu_count() / wgs;
+  return static_cast<int>(std::max(1ll, std::min({want, blocks / 2, static_cast<long long>(kMaxStates)})));
 }
 
 constexpr long long kMaxLen = 0x7fffffffLL - kKvBlock;  // positions are 32-bit on the device
@@ -137,7 +147,8 @@ void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hip
     keys = std::min(keys, a.window + a.sinks + std::min<long long>(a.s_new, tile / a.group + 2) + kKvBlock);
   const long long step = one ? kKvBlock : kTileKeys;
   const long long most = std::max(1ll, (keys + step - 1) / step);
-  a.nsplit = split_kv == 0 ? auto_splits(a.units * a.row_tiles, keys, step, one ? 2 : 8 / waves)
+  a.nsplit = split_kv == 0 ? (one ? few_splits(a.units * a.row_tiles, keys, D)
+                                  : tile_splits(a.units * a.row_tiles, keys, waves))
                            : static_cast<int>(std::min<long long>({split_kv, most, kMaxStates}));
   if (one)
     ENG_CHECK(threads_fit(a.units * a.row_tiles * a.nsplit, 256),
@@ -180,14 +191,17 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
             "attention_prefix: too many query rows for one launch");
   shared.row_tiles = tiles_of(unit_rows, tile);
   mine.row_tiles = tiles_of(mine.group, kFewRows);
-  auto splits = [&](const Args& a, long long step, int per_cu) {
+  auto splits = [&](const Args& a, bool of_few) {
     if (a.max_len == 0) return 0;
-    const long long most = (a.max_len + step - 1) / step;
-    return split_kv == 0 ? std::min(auto_splits(a.units * a.row_tiles, a.max_len, step, per_cu), kMaxStates / 2)
-                         : static_cast<int>(std::min<long long>({split_kv, most, kMaxStates / 2}));
+    const long long step = of_few ? kKvBlock : kTileKeys;
+    const long long wgs = a.units * a.row_tiles;
+    const int chosen = split_kv != 0 ? static_cast<int>(std::min<long long>(split_kv, (a.max_len + step - 1) / step))
+                       : of_few      ? few_splits(wgs, a.max_len, D)
+                                     : tile_splits(wgs, a.max_len, waves);
+    return std::min(chosen, kMaxStates / 2);
   };
-  shared.nsplit = splits(shared, few_shared ? kKvBlock : kTileKeys, few_shared ? 2 : 8 / waves);
-  mine.nsplit = splits(mine, kKvBlock, 2);
+  shared.nsplit = splits(shared, few_shared);
+  mine.nsplit = splits(mine, true);
   ENG_CHECK(threads_fit(shared.units * shared.row_tiles * std::max(1, few_shared ? shared.nsplit : 1) +
                             mine.units * mine.row_tiles * std::max(1, mine.nsplit), 512),
             "attention_prefix: too many query rows for one launch");
