@@ -124,7 +124,7 @@ int few_splits(long long wgs, long long keys, long long D) {
   return static_cast<int>(std::max(1ll, std::min({want, blocks / 2, static_cast<long long>(kMaxStates)})));
 }
 
-constexpr long long kMaxLen = 0x7fffffffLL - kKvBlock;  // positions are 32-bit on the device
+constexpr long long kMaxLen = 0x7fffffffLL - 2 * kTileKeys;  // 32-bit positions, up to a tile past the end
 
 // State of a call in the stream's arena: o [rows][states][D], then (m, l) of each.
 std::size_t state_bytes(long long rows, int states, long long D) {
@@ -152,7 +152,7 @@ void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hip
                            : static_cast<int>(std::min<long long>({split_kv, most, kMaxStates}));
   if (one)
     ENG_CHECK(threads_fit(a.units * a.row_tiles * a.nsplit, 256),
-              "attention_window: too many query rows and splits for one launch");
+              "attention_window: too many query rows for one launch");
   a.part_stride = a.nsplit;
   auto go = [&](auto dim) {
     constexpr int kD = decltype(dim)::value;
@@ -243,7 +243,7 @@ void window_entry(const eng_half* q, const void* k, const void* v, const float* 
   ENG_CHECK(sinks >= 0, "attention_window: sinks must be non-negative");
   ENG_CHECK(max_kv_len >= 0, "attention_window: max_kv_len must be non-negative");
   ENG_CHECK(kv_max_seq_len >= max_kv_len, "attention_window: kv_max_seq_len < max_kv_len");
-  ENG_CHECK(kv_max_seq_len <= kMaxLen, "attention_window: kv_max_seq_len must be below 2^31 - 32");
+  ENG_CHECK(kv_max_seq_len <= kMaxLen, "attention_window: kv_max_seq_len must be below 2^31 - 128");
   ENG_CHECK(std::isfinite(scale), "attention_window: scale must be finite");
   ENG_CHECK(split_kv >= 0, "attention_window: split_kv must be non-negative");
   ENG_CHECK(aligned_to(k, 16) && aligned_to(v, 16), "attention_window: the caches must be 16-byte aligned");
@@ -268,7 +268,7 @@ void window_entry(const eng_half* q, const void* k, const void* v, const float* 
   a.s_new = static_cast<int>(s_new);
   a.max_len = static_cast<int>(max_kv_len);
   a.causal = true;
-  a.window = window;
+  a.window = std::min<int64_t>(window, 1ll << 40);
   a.sinks = window == 0 ? 0 : static_cast<int>(std::min(sinks, max_kv_len));
   a.scale = scale;
   run_window(a, batch, head_dim, split_kv, q8, s);
@@ -300,7 +300,7 @@ void prefix_entry(const eng_half* q, const void* kp, const void* vp, const float
   ENG_CHECK(prefix_max_seq_len >= max_prefix_len, "attention_prefix: prefix_max_seq_len < max_prefix_len");
   ENG_CHECK(kv_max_seq_len >= max_kv_len, "attention_prefix: kv_max_seq_len < max_kv_len");
   ENG_CHECK(prefix_max_seq_len <= kMaxLen && kv_max_seq_len <= kMaxLen,
-            "attention_prefix: prefix_max_seq_len and kv_max_seq_len must be below 2^31 - 32");
+            "attention_prefix: prefix_max_seq_len and kv_max_seq_len must be below 2^31 - 128");
   ENG_CHECK(std::isfinite(scale), "attention_prefix: scale must be finite");
   ENG_CHECK(split_kv >= 0, "attention_prefix: split_kv must be non-negative");
   ENG_CHECK(aligned_to(kp, 16) && aligned_to(vp, 16) && aligned_to(k, 16) && aligned_to(v, 16),

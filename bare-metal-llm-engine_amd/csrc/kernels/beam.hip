@@ -435,7 +435,7 @@ void select_entry(const void* logits, bool half, int64_t ld, const float* scores
   ENG_CHECK(batch >= 0, "beam_select: batch must be non-negative");
   ENG_CHECK(beams > 0 && beams <= kMaxBeams, "beam_select: beams must be 1 to 32");
   ENG_CHECK(n_out > 0 && n_out <= kMaxOut, "beam_select: n_out must be 1 to 64");
-  ENG_CHECK(vocab > 0 && vocab < 0x7fffffffLL - kStep, "beam_select: vocab must be positive and below 2^31 - 4097");
+  ENG_CHECK(vocab > 0 && vocab < 0x80000000LL - 65536, "beam_select: vocab must be positive and below 2^31 - 65536");
   ENG_CHECK(n_out <= beams * vocab, "beam_select: n_out > beams * vocab");
   ENG_CHECK(ld >= vocab, "beam_select: ld < vocab");
   ENG_CHECK(eos < vocab, "beam_select: eos >= vocab");

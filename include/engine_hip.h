@@ -564,7 +564,9 @@ int eng_attention_decode_q8(const eng_half* q, const uint8_t* k_cache, const uin
  *
  * split_kv = 0 chooses the number of pieces that a row's keys are computed in; a
  * positive value asks for as many (at most 256, prefix and own keys 128 each). More
- * than one uses the stream's scratch arena (eng_attention_prefix_* always does).
+ * than one uses the stream's scratch arena (eng_attention_prefix_* always does). The
+ * same call gives the same bits; the order of the sums, and with it the last bits,
+ * depends on the shape, on max_kv_len and on split_kv.
  * ---------------------------------------------------------------------- */
 int eng_attention_window_f16(const eng_half* q, const eng_half* k_cache, const eng_half* v_cache,
                              eng_half* out, const int32_t* pos, const int32_t* n_new, int64_t batch,
@@ -605,12 +607,13 @@ int eng_attention_prefix_q8(const eng_half* q, const uint8_t* k_prefix, const ui
  * Candidates of one beam are compared by their logits, those of unlike beams by
  * their scores in 64 bits; ties go to the lower beam, then the lower token. finished
  * [batch, beams] (bytes; NULL: none) marks beams that have ended: such a beam has
- * one candidate, token eos with its score unchanged, and needs no valid logits. out_finished
+ * one candidate, token eos with its score unchanged, whatever its logits are. out_finished
  * [batch, n_out] (may be NULL) is 1 where the parent has ended or the token is eos
  * (eos < 0: no token is). A candidate whose score is -inf or no number ranks last, as
- * -inf: all of a beam's whose score is not finite or whose row holds a NaN, +inf or only
- * -inf, and all but one of a finished beam's. beams is 1 to 32, n_out 1 to 64 and at most beams
- * * vocab. Outputs must not overlap inputs. Uses the stream's scratch arena.
+ * -inf: all of a beam's whose score is not finite or whose row holds a NaN, +inf or
+ * only -inf, and all but one of a finished beam's. beams is 1 to 32, n_out 1 to 64 and
+ * at most beams * vocab. Outputs must not overlap inputs. Uses the stream's scratch
+ * arena.
  *
  * eng_kv_cache_reorder_*: sequence (g, j) of the caches [batch * beams, n_kv_heads,
  * kv_max_seq_len, head_dim] gets the first kv_len[g beams + p] tokens of sequence
@@ -618,10 +621,10 @@ int eng_attention_prefix_q8(const eng_half* q, const uint8_t* k_prefix, const ui
  * same shape, or, with the same pointers as source and destination, in place: beams
  * that keep their place (p == j) are then not touched. 8-bit caches move with the
  * scales of the blocks that the tokens reach. Tokens behind the length stay as they
- * were, and so does a sequence whose p is outside 0 .. beams - 1. Lengths are at
- * most max_kv_len, beyond it they are taken as it. kv_len is not reordered. Source and destination
- * buffers must be the same or not overlap; head_dim is 64 or 128, caches are 16-byte
- * aligned.
+ * were, and so does a sequence whose p is outside 0 .. beams - 1. Lengths past
+ * max_kv_len are taken as it; kv_len itself is not reordered. Source and destination
+ * buffers are the same or do not overlap; beams is 1 to 32, head_dim 64 or 128, caches
+ * are 16-byte aligned.
  * ---------------------------------------------------------------------- */
 int eng_beam_select_f32(const float* logits, int64_t ld, const float* scores, const uint8_t* finished,
                         float* out_scores, int32_t* out_parent, int32_t* out_token,
