@@ -293,6 +293,118 @@ inline void attention_decode_q8(const half* q, const std::uint8_t* k_cache,
                                            stream));
 }
 
+/// Attention of s_new new tokens of each sequence, already in their fp16 caches, at device
+/// positions pos[b] on, with a sliding window (0: none) and first tokens that stay visible
+/// (additive; eng_attention_window_f16).
+inline void attention_window(const half* q, const half* k_cache, const half* v_cache, half* out,
+                             const std::int32_t* pos, const std::int32_t* n_new, std::int64_t batch,
+                             std::int64_t s_new, std::int64_t n_heads, std::int64_t n_kv_heads,
+                             std::int64_t head_dim, std::int64_t window, std::int64_t sinks,
+                             std::int64_t max_kv_len, std::int64_t kv_max_seq_len, float scale,
+                             int split_kv = 0, hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_attention_window_f16(detail::bits(q), detail::bits(k_cache), detail::bits(v_cache),
+                                            detail::bits(out), pos, n_new, batch, s_new, n_heads,
+                                            n_kv_heads, head_dim, window, sinks, max_kv_len,
+                                            kv_max_seq_len, scale, split_kv, stream));
+}
+/// The same over 8-bit caches.
+inline void attention_window_q8(const half* q, const std::uint8_t* k_cache,
+                                const std::uint8_t* v_cache, const float* k_scale,
+                                const float* v_scale, half* out, const std::int32_t* pos,
+                                const std::int32_t* n_new, std::int64_t batch, std::int64_t s_new,
+                                std::int64_t n_heads, std::int64_t n_kv_heads,
+                                std::int64_t head_dim, std::int64_t window, std::int64_t sinks,
+                                std::int64_t max_kv_len, std::int64_t kv_max_seq_len, float scale,
+                                int split_kv = 0, hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_attention_window_q8(detail::bits(q), k_cache, v_cache, k_scale, v_scale,
+                                           detail::bits(out), pos, n_new, batch, s_new, n_heads,
+                                           n_kv_heads, head_dim, window, sinks, max_kv_len,
+                                           kv_max_seq_len, scale, split_kv, stream));
+}
+
+/// Single-token attention of each sequence over the prefix that its group shares and then its
+/// own fp16 cache (additive; eng_attention_prefix_f16).
+inline void attention_prefix(const half* q, const half* k_prefix, const half* v_prefix,
+                             const std::int32_t* prefix_len, const half* k_cache,
+                             const half* v_cache, const std::int32_t* kv_len, half* out,
+                             std::int64_t n_prefix, std::int64_t batch, std::int64_t n_heads,
+                             std::int64_t n_kv_heads, std::int64_t head_dim,
+                             std::int64_t max_prefix_len, std::int64_t prefix_max_seq_len,
+                             std::int64_t max_kv_len, std::int64_t kv_max_seq_len, float scale,
+                             int split_kv = 0, hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_attention_prefix_f16(
+      detail::bits(q), detail::bits(k_prefix), detail::bits(v_prefix), prefix_len,
+      detail::bits(k_cache), detail::bits(v_cache), kv_len, detail::bits(out), n_prefix, batch,
+      n_heads, n_kv_heads, head_dim, max_prefix_len, prefix_max_seq_len, max_kv_len,
+      kv_max_seq_len, scale, split_kv, stream));
+}
+/// The same over 8-bit caches.
+inline void attention_prefix_q8(const half* q, const std::uint8_t* k_prefix,
+                                const std::uint8_t* v_prefix, const float* k_prefix_scale,
+                                const float* v_prefix_scale, const std::int32_t* prefix_len,
+                                const std::uint8_t* k_cache, const std::uint8_t* v_cache,
+                                const float* k_scale, const float* v_scale,
+                                const std::int32_t* kv_len, half* out, std::int64_t n_prefix,
+                                std::int64_t batch, std::int64_t n_heads, std::int64_t n_kv_heads,
+                                std::int64_t head_dim, std::int64_t max_prefix_len,
+                                std::int64_t prefix_max_seq_len, std::int64_t max_kv_len,
+                                std::int64_t kv_max_seq_len, float scale, int split_kv = 0,
+                                hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_attention_prefix_q8(
+      detail::bits(q), k_prefix, v_prefix, k_prefix_scale, v_prefix_scale, prefix_len, k_cache,
+      v_cache, k_scale, v_scale, kv_len, detail::bits(out), n_prefix, batch, n_heads, n_kv_heads,
+      head_dim, max_prefix_len, prefix_max_seq_len, max_kv_len, kv_max_seq_len, scale, split_kv,
+      stream));
+}
+
+/// The n_out best continuations of each group of beams: logits [batch * beams rows of ld],
+/// the beams' scores and (optionally) which have ended; out_finished may be nullptr (additive;
+/// eng_beam_select_f32 / _f16).
+inline void beam_select(const float* logits, std::int64_t ld, const float* scores,
+                        const std::uint8_t* finished, float* out_scores, std::int32_t* out_parent,
+                        std::int32_t* out_token, std::uint8_t* out_finished, std::int64_t batch,
+                        std::int64_t beams, std::int64_t n_out, std::int64_t vocab,
+                        std::int64_t eos, hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_beam_select_f32(logits, ld, scores, finished, out_scores, out_parent,
+                                       out_token, out_finished, batch, beams, n_out, vocab, eos,
+                                       stream));
+}
+inline void beam_select(const half* logits, std::int64_t ld, const float* scores,
+                        const std::uint8_t* finished, float* out_scores, std::int32_t* out_parent,
+                        std::int32_t* out_token, std::uint8_t* out_finished, std::int64_t batch,
+                        std::int64_t beams, std::int64_t n_out, std::int64_t vocab,
+                        std::int64_t eos, hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_beam_select_f16(detail::bits(logits), ld, scores, finished, out_scores,
+                                       out_parent, out_token, out_finished, batch, beams, n_out,
+                                       vocab, eos, stream));
+}
+
+/// The caches of each group's beams brought in line with `parent`, in place where source and
+/// destination are the same (additive; eng_kv_cache_reorder_f16 / _q8).
+inline void kv_cache_reorder(const half* k_src, const half* v_src, half* k_dst, half* v_dst,
+                             const std::int32_t* parent, const std::int32_t* kv_len,
+                             std::int64_t batch, std::int64_t beams, std::int64_t n_kv_heads,
+                             std::int64_t head_dim, std::int64_t max_kv_len,
+                             std::int64_t kv_max_seq_len, hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_kv_cache_reorder_f16(detail::bits(k_src), detail::bits(v_src),
+                                            detail::bits(k_dst), detail::bits(v_dst), parent,
+                                            kv_len, batch, beams, n_kv_heads, head_dim, max_kv_len,
+                                            kv_max_seq_len, stream));
+}
+inline void kv_cache_reorder_q8(const std::uint8_t* k_src, const std::uint8_t* v_src,
+                                const float* k_scale_src, const float* v_scale_src,
+                                std::uint8_t* k_dst, std::uint8_t* v_dst, float* k_scale_dst,
+                                float* v_scale_dst, const std::int32_t* parent,
+                                const std::int32_t* kv_len, std::int64_t batch, std::int64_t beams,
+                                std::int64_t n_kv_heads, std::int64_t head_dim,
+                                std::int64_t max_kv_len, std::int64_t kv_max_seq_len,
+                                hipStream_t stream = nullptr) {
+  ENGINE_ABI_CHECK(eng_kv_cache_reorder_q8(k_src, v_src, k_scale_src, v_scale_src, k_dst, v_dst,
+                                           k_scale_dst, v_scale_dst, parent, kv_len, batch, beams,
+                                           n_kv_heads, head_dim, max_kv_len, kv_max_seq_len,
+                                           stream));
+}
+
 }  // namespace hip
 
 // Call sites written against the reference use engine::cuda::...

@@ -825,6 +825,121 @@ TEST(gpu_kernels, narrow_weights_and_cache_through_cpp_api) {
   EXPECT_EQ(bad, 0);
 }
 
+// -------------------------------------------------------- long contexts, beams
+TEST(cpu_kernels, long_context_launchers_refuse_through_cpp_api) {
+  (void)ctx;
+  auto* ph = reinterpret_cast<engine::half*>(0x1000);
+  auto* pb = reinterpret_cast<std::uint8_t*>(0x1000);
+  auto* pf = reinterpret_cast<float*>(0x1000);
+  auto* pi = reinterpret_cast<std::int32_t*>(0x1000);
+  EXPECT_THROWS_MSG(engine::cuda::attention_window(ph, ph, ph, ph, pi, nullptr, 1, 1, 3, 2, 64, 0, 0, 1, 1, 1.0f),
+                    "divisible");
+  EXPECT_THROWS_MSG(engine::cuda::attention_window_q8(ph, pb, pb, nullptr, pf, ph, pi, nullptr, 1, 1, 2, 2, 64, 0,
+                                                      0, 1, 1, 1.0f), "k_scale/v_scale is null");
+  EXPECT_THROWS_MSG(engine::cuda::attention_prefix(ph, ph, ph, pi, ph, ph, pi, ph, 2, 3, 2, 2, 64, 1, 1, 1, 1, 1.0f),
+                    "divisible by n_prefix");
+  EXPECT_THROWS_MSG(engine::cuda::attention_prefix_q8(ph, pb, pb, pf, pf, pi, pb, pb, pf, pf, pi, ph, 1, 1, 2, 2, 96,
+                                                      1, 1, 1, 1, 1.0f), "head_dim");
+  EXPECT_THROWS_MSG(engine::cuda::beam_select(pf, 8, pf, nullptr, pf, pi, pi, nullptr, 1, 1, 9, 8, -1), "n_out > beams");
+  EXPECT_THROWS_MSG(engine::cuda::beam_select(ph, 7, pf, nullptr, pf, pi, pi, nullptr, 1, 1, 1, 8, -1), "ld < vocab");
+  EXPECT_THROWS_MSG(engine::cuda::kv_cache_reorder(ph, ph, ph, ph, nullptr, pi, 1, 2, 1, 64, 4, 4), "parent is null");
+  EXPECT_THROWS_MSG(engine::cuda::kv_cache_reorder_q8(pb, pb, pf, pf, pb, pb, nullptr, pf, pi, pi, 1, 2, 1, 64, 4, 4),
+                    "scale buffer is null");
+}
+
+// A query that sees one key returns that key's value, so every result is exact.
+TEST(gpu_kernels, long_context_through_cpp_api) {
+  require_gpu(ctx);
+  const std::int64_t B = 2, S = 5, H = 4, G = 2, D = 64, room = 32;
+  std::vector<engine::half> q(B * S * H * D), kv(B * G * room * D);
+  for (std::size_t i = 0; i < q.size(); ++i) q[i] = engine::float_to_half(static_cast<float>(i % 7) - 3.0f);
+  for (std::size_t i = 0; i < kv.size(); ++i) kv[i] = engine::float_to_half(static_cast<float>(i % 15) - 7.0f);
+  std::vector<std::uint8_t> kv8(kv.size());
+  for (std::size_t i = 0; i < kv8.size(); ++i) kv8[i] = static_cast<std::uint8_t>(i % 100);  // e4m3 codes
+  engine::DeviceBuffer<engine::half> dq(q), dkv(kv), out(q.size()), out8(q.size());
+  engine::DeviceBuffer<std::uint8_t> dkv8(kv8);
+  engine::DeviceBuffer<float> ones(std::vector<float>(B * G, 1.0f));
+  engine::DeviceBuffer<std::int32_t> pos(std::vector<std::int32_t>{0, 9}), none(std::vector<std::int32_t>{0, 0}),
+      one(std::vector<std::int32_t>{1, 1});
+  engine::cuda::attention_window(dq.get(), dkv.get(), dkv.get(), out.get(), pos.get(), nullptr, B, S, H, G, D, 1, 0,
+                                 room, room, 0.125f);
+  engine::cuda::attention_window_q8(dq.get(), dkv8.get(), dkv8.get(), ones.get(), ones.get(), out8.get(), pos.get(),
+                                    nullptr, B, S, H, G, D, 1, 0, room, room, 0.125f);
+  ENGINE_ABI_CHECK(eng_device_sync());
+  std::vector<engine::half> o = out.download(), o8 = out8.download();
+  auto e4m3 = [](int c) {
+    return (c >> 3) == 0 ? (c & 7) * 0.001953125f : (1.0f + (c & 7) / 8.0f) * static_cast<float>(1u << (c >> 3)) / 128.0f;
+  };
+  int bad = 0;
+  for (std::int64_t b = 0; b < B; ++b)
+    for (std::int64_t i = 0; i < S; ++i)
+      for (std::int64_t h = 0; h < H; ++h)
+        for (std::int64_t d = 0; d < D; ++d) {
+          const std::int64_t at = ((b * S + i) * H + h) * D + d;
+          const std::int64_t src = ((b * G + h / (H / G)) * room + (b == 0 ? 0 : 9) + i) * D + d;
+          bad += engine::half_to_float(o[at]) != engine::half_to_float(kv[src]);
+          bad += engine::half_to_float(o8[at]) != e4m3(kv8[src]);
+        }
+  EXPECT_EQ(bad, 0);
+
+  // a prefix of one token and no token of their own; then none and one
+  engine::cuda::attention_prefix(dq.get(), dkv.get(), dkv.get(), one.get(), dkv.get(), dkv.get(), none.get(), out.get(),
+                                 1, B, H, G, D, room, room, room, room, 0.125f);
+  engine::cuda::attention_prefix_q8(dq.get(), dkv8.get(), dkv8.get(), ones.get(), ones.get(), none.get(), dkv8.get(),
+                                    dkv8.get(), ones.get(), ones.get(), one.get(), out8.get(), 1, B, H, G, D, room,
+                                    room, room, room, 0.125f);
+  ENGINE_ABI_CHECK(eng_device_sync());
+  o = out.download(), o8 = out8.download();
+  for (std::int64_t b = 0; b < B; ++b)
+    for (std::int64_t h = 0; h < H; ++h)
+      for (std::int64_t d = 0; d < D; ++d) {
+        const std::int64_t at = (b * H + h) * D + d, g = h / (H / G);
+        bad += engine::half_to_float(o[at]) != engine::half_to_float(kv[g * room * D + d]);
+        bad += engine::half_to_float(o8[at]) != e4m3(kv8[(b * G + g) * room * D + d]);
+      }
+  EXPECT_EQ(bad, 0);
+
+  // two beams over ten words: the second's word 3, the first's 7, then its 2
+  std::vector<float> x(2 * 10, 0.0f);
+  x[7] = 3.0f, x[2] = 2.0f, x[10 + 3] = 9.0f;
+  std::vector<engine::half> xh(x.size());
+  for (std::size_t i = 0; i < x.size(); ++i) xh[i] = engine::float_to_half(x[i]);
+  engine::DeviceBuffer<float> dx(x), scores(std::vector<float>{-1.0f, -1.0f}), s(3);
+  engine::DeviceBuffer<engine::half> dxh(xh);
+  engine::DeviceBuffer<std::int32_t> parent(3), token(3);
+  engine::DeviceBuffer<std::uint8_t> ended(3);
+  for (int half = 0; half < 2; ++half) {
+    if (half) engine::cuda::beam_select(dxh.get(), 10, scores.get(), nullptr, s.get(), parent.get(), token.get(),
+                                        ended.get(), 1, 2, 3, 10, 7);
+    else engine::cuda::beam_select(dx.get(), 10, scores.get(), nullptr, s.get(), parent.get(), token.get(), ended.get(),
+                                   1, 2, 3, 10, 7);
+    ENGINE_ABI_CHECK(eng_device_sync());
+    EXPECT_TRUE(parent.download() == (std::vector<std::int32_t>{1, 0, 0}));
+    EXPECT_TRUE(token.download() == (std::vector<std::int32_t>{3, 7, 2}));
+    EXPECT_TRUE(ended.download() == (std::vector<std::uint8_t>{0, 1, 0}));
+  }
+
+  // the two sequences change places in their own buffers
+  engine::DeviceBuffer<std::int32_t> swap(std::vector<std::int32_t>{1, 0}), all(std::vector<std::int32_t>{32, 32});
+  engine::DeviceBuffer<engine::half> k2(kv), v2(kv);
+  engine::DeviceBuffer<std::uint8_t> k3(kv8), v3(kv8);
+  std::vector<float> sc{1.0f, 2.0f, 3.0f, 4.0f};
+  engine::DeviceBuffer<float> ks(sc), vs(sc);
+  engine::cuda::kv_cache_reorder(k2.get(), v2.get(), k2.get(), v2.get(), swap.get(), all.get(), 1, 2, G, D, room, room);
+  engine::cuda::kv_cache_reorder_q8(k3.get(), v3.get(), ks.get(), vs.get(), k3.get(), v3.get(), ks.get(), vs.get(),
+                                    swap.get(), all.get(), 1, 2, G, D, room, room);
+  ENGINE_ABI_CHECK(eng_device_sync());
+  const std::vector<engine::half> g2 = k2.download();
+  const std::vector<std::uint8_t> g3 = v3.download();
+  const std::size_t n = kv.size() / 2;
+  for (std::size_t i = 0; i < n; ++i) {
+    bad += g2[i].u != kv[n + i].u || g2[n + i].u != kv[i].u;
+    bad += g3[i] != kv8[n + i] || g3[n + i] != kv8[i];
+  }
+  EXPECT_EQ(bad, 0);
+  EXPECT_TRUE(vs.download() == (std::vector<float>{3.0f, 4.0f, 1.0f, 2.0f}));
+}
+
 // --------------------------------------------------------------------- engref
 // Writes an ENGREF01 file (the reference's container, tools/gen_reference.py:
 // 64-83) with explicit dtype codes.
