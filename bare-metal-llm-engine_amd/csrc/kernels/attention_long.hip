@@ -87,8 +87,13 @@ void tiles(const Args& a, hipStream_t s) {
 }
 template <int D>
 void tiles(const Args& a, bool q8, int waves, hipStream_t s) {
-  if (q8) waves == 8 ? tiles<D, true, 8>(a, s) : tiles<D, true, 4>(a, s);
-  else waves == 8 ? tiles<D, false, 8>(a, s) : tiles<D, false, 4>(a, s);
+  if constexpr (D == 128) {
+    if (waves == 8) {
+      q8 ? tiles<D, true, 8>(a, s) : tiles<D, false, 8>(a, s);
+      return;
+    }
+  }
+  q8 ? tiles<D, true, 4>(a, s) : tiles<D, false, 4>(a, s);
 }
 template <int D>
 void few(const Args& a, const Args& b, bool q8, hipStream_t s) {
@@ -99,8 +104,9 @@ void few(const Args& a, const Args& b, bool q8, hipStream_t s) {
   ENG_LAUNCH_CHECK();
 }
 
-// Waves of a tile: eight where that leaves a workgroup for every CU.
-int tile_waves(long long units, long long unit_rows) {
+// Waves of a tile: at D = 128 eight where that leaves a workgroup for every CU, else four.
+int tile_waves(long long units, long long unit_rows, long long D) {
+  if (D == 64) return 4;
   return units * ((unit_rows + tile_rows(8) - 1) / tile_rows(8)) >= device_cu_count() ? 8 : 4;
 }
 
@@ -136,7 +142,7 @@ void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hip
   const long long unit_rows = static_cast<long long>(a.s_new) * a.group;
   const bool one = a.s_new == 1;  // a unit's rows see the same keys
   a.units = batch * a.n_kv;
-  const int waves = D == 64 ? 4 : tile_waves(a.units, unit_rows);
+  const int waves = tile_waves(a.units, unit_rows, D);
   const int tile = one ? kFewRows : tile_rows(waves);
   ENG_CHECK(unit_rows <= 0x3fffffffLL && rows <= 0xffffffffLL - 4 && threads_fit((rows + 3) / 4, 256) &&
                 threads_fit(a.units, 256) && threads_fit(a.units * tiles_of(unit_rows, tile), 512),
@@ -174,8 +180,12 @@ void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hip
   else go(std::integral_constant<int, 128>{});
 }
 
-// Shared rows of a KV head up to which the prefix is read in tiles of 16 of them.
-constexpr long long kFewShared = 32;
+// Shared rows of a KV head up to which the prefix is read in tiles of 16 of them, all in the
+// launch that reads the sequences' own tokens, though each tile reads it (the L2 holds it):
+// 64 rows, 2000 tokens, 4 heads of 64: 10.4 us, 16.4 in one tile of 128 rows; 128 rows, 8192
+// tokens, 8 heads of 128 27-33 (30-35); eight such groups of 2000 tokens 47-68 (48-62); 256
+// rows 38 (38).
+constexpr long long kFewShared = 128;
 
 void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, long long D, int split_kv,
                 bool q8, hipStream_t s) {
@@ -183,7 +193,7 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
   const long long unit_rows = static_cast<long long>(shared.s_new) * shared.group;
   const bool few_shared = unit_rows <= kFewShared;
   shared.units = n_prefix * shared.n_kv;
-  const int waves = D == 64 ? 4 : tile_waves(shared.units, unit_rows);
+  const int waves = tile_waves(shared.units, unit_rows, D);
   const int tile = few_shared ? kFewRows : tile_rows(waves);
   mine.units = batch * mine.n_kv;
   ENG_CHECK(unit_rows <= 0x3fffffffLL && rows <= 0xffffffffLL - 4 && threads_fit((rows + 3) / 4, 256) &&

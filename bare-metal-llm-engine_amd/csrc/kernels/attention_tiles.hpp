@@ -1,6 +1,6 @@
 // attention_tiles.hpp -- attention of many query rows over a KV cache on the matrix
-// cores: tiles of 128 rows by 64 keys, for prompts (causal, sliding window, sinks) and
-// for the sequences of a batch that share a prefix (every row sees every key).
+// cores: tiles of 128 or 256 rows by 64 keys, for prompts (causal, sliding window, sinks)
+// and for the sequences of a batch that share a prefix (every row sees every key).
 //
 // Rows: the query heads of a KV head's group share its keys, so the rows of a unit (a
 // sequence or a shared prefix, and a KV head) are its (token, head of the group) pairs,
@@ -145,27 +145,36 @@ constexpr int kTileKeys = 64;
 constexpr int tile_buffers(int NW) { return NW == 8 ? 3 : 2; }
 
 // One workgroup per (unit, tile of 32 NW rows, split of their keys), NW waves of 32 rows.
-// K and V tiles of 64 keys pass through LDS as fp16 in two buffers, by way of registers
+// K and V tiles of 64 keys pass through LDS as fp16, by way of registers, K and V in turn
 // (8-bit codes are converted on the way, exact; a K block's scale multiplies its scores, a
 // V block's joins the weights as in few_kernel). Products on v_mfma_f32_32x32x16_f16: S^T =
 // K . Q^T with K as the A operand leaves a row's scores in two lanes, O^T = V^T . P^T takes
 // them in place as the B operand: element r of half-wave g is key 8 (r / 4) + 4 g + r % 4
 // of its 32, and V is read from LDS transposed (4 keys of a dim for each lane) in that
 // order. A row of an LDS tile is D fp16; its 16-byte pieces are permuted by the row so that
-// neither read has bank conflicts (256 and about 148 bytes a clock; 128 and 120 before).
+// neither read has bank conflicts: 235 bytes a clock and CU for K, 148 for V, against 123
+// and 122 for one permutation that suits V's rows only.
 //
-// A wave takes 32 keys in two phases of about 500 cycles at D = 128: exponentials (16 of 16
-// cycles, and as many each of a multiply-add, an addition, half a maximum and half a
-// conversion), then matrix products (16 of 32 cycles: O of these keys, the scores of the
-// next 32). Eight waves put two on a SIMD, and the barriers between the phases keep waves
-// 4 to 7 one phase behind waves 0 to 3, so that one of the two has the vector unit and the
-// other the matrix cores.
+// A wave takes 32 keys at a time. The exponentials of 32 keys' scores (16 of 12 cycles, as
+// many multiply-adds, additions and halves of maxima and conversions) are issued among the
+// matrix products of the next 32 keys' scores, then come the products with V; two waves on
+// a SIMD fill each other's gaps. K fragments are read one such step ahead. Eight waves share
+// a tile where that leaves a workgroup for every CU; else four, two workgroups to a CU, and
+// at D = 64, with three to a CU, always (prompts of 777 tokens, window 256: 36 us, 49 with
+// eight waves).
+// Bound by the matrix cores and power together: 2048 tokens after 6144, 32 / 8 heads of
+// 128: 277 us, 870 TFLOP/s, at 1.8 to 2.1 GHz (a large fp16 product of the library's 1175).
+// Slower: the two waves of a SIMD one phase apart, exponentials against products, by
+// barriers (309; a phase then waits for its own latencies); 64 rows to a wave, half the LDS
+// reads (376 to 442; the compiler moves values between the register files); direct loads
+// to LDS (their wait covers the next tile's: 638 TFLOP/s).
 // Weights are rounded to fp16 (2^-11 of each at the most, as the output is); m, l, O are
 // fp32 and l sums the weights before rounding.
 //
 // A NaN or an infinity in a V row would reach, as 0 times it, rows that do not see its
 // key. So where a workgroup's sums are not all finite it computes them again with such
-// values taken out and added for the rows that see them (careful_pass).
+// values taken out and added for the rows that see them (careful_pass, about six times the
+// time).
 template <int D, bool Q8, int NW>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) {
   constexpr int kRows = 32 * NW;
@@ -251,8 +260,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
   // ---- global to LDS, by way of registers. Keys past the last one are taken as the last
   // one, and masked.
   constexpr int PIECES = TILE * static_cast<int>(sizeof(Elem)) / 16;
-  constexpr int LOADS = (PIECES + 64 * NW - 1) / (64 * NW);
-  const bool loads = PIECES >= 64 * NW || tid < PIECES;  // (uniform in a wave)
+  constexpr int LOADS = PIECES / (64 * NW);
+  static_assert(LOADS * 64 * NW == PIECES, "whole loads");
   constexpr int LPR = D * static_cast<int>(sizeof(Elem)) / 16;  // loads of a row
   uintx4 raw[LOADS];  // of K or V
   [[maybe_unused]] float raw_ks = 0.0f, raw_vs = 0.0f;
@@ -260,7 +269,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
     const int base = base_of(t);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int n = i * 64 * NW + (PIECES >= 64 * NW ? tid : tid & (PIECES - 1));
+      const int n = i * 64 * NW + tid;
       const long long at = static_cast<long long>(min(base + n / LPR, hi - 1)) * D + (n % LPR) * (D / LPR);
       raw[i] = *reinterpret_cast<const uintx4*>(g + at);
     }
@@ -271,7 +280,6 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
       const int n = i * 64 * NW + tid;
       const int row = n / LPR;
       const int piece = n % LPR;
-      if (!loads) continue;
       if constexpr (Q8) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
