@@ -10,8 +10,6 @@ namespace attn {
 constexpr int kFewRows = 16;   // rows of a tile
 constexpr int kFewWaves = 4;
 
-typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
-
 // One workgroup per (unit, tile of 16 rows, split of the unit's keys), 4 waves; a wave
 // takes every fourth block of 32 keys straight from memory into registers, two blocks in
 // flight. Both products are on v_mfma_f32_16x16x32_f16: S^T = K . Q^T with K as the A
@@ -25,6 +23,12 @@ typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
 // The keys are [0, hi) without [sinks, lo) and a block's loads go through a descriptor
 // that ends with its last key, so rows past it read as zeros; values of hidden keys before
 // the window are set to zero, so nothing of either reaches a sum.
+//
+// Bound by the caches' bytes: one token of 16 sequences of up to 8192, window 4096, 32 / 8
+// heads of 128, 8-bit: 135 MB in 25 us, 5.4 TB/s; eight groups of four beams over 4096
+// tokens of 32 heads 252 MB in 51 us. (On tile_kernel, whose tiles a few rows leave empty, 77
+// and 164.) Up to 128 rows over one prefix the L2 serves the tiles after the first: 32
+// sequences, 8 heads of 128, 8192 tokens 31 us, 63 MB.
 template <int D, bool Q8>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(Args a0, Args a1, unsigned wgs0) {
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");

