@@ -26,7 +26,6 @@ constexpr int kMaxBeams = 32;
 constexpr int kWaves = 4;
 constexpr int kVpt = 16;       // values of a lane in one step of a wave
 constexpr int kWaveList = 64 * kVpt + kMaxOut;
-constexpr int kWaveSteps = (kWaveList + 63) / 64;
 
 // A logit as a number that orders like it.
 __device__ __forceinline__ unsigned order_of(float x) {
@@ -73,9 +72,11 @@ __device__ __forceinline__ u64 lane_value(u64 x, int lane) {
   return (static_cast<u64>(hi) << 32) | lo;
 }
 
-// One wave's candidates, of which it keeps the `k` best.
+// One wave's candidates, of which it keeps the `k` best. CAP: room in its list, in LDS.
+template <int CAP>
 struct Best {
-  u64* list;  // LDS, kWaveList entries
+  static constexpr int kSteps = (CAP + 63) / 64;
+  u64* list;
   int k;
   int n;
 
@@ -96,7 +97,7 @@ struct Best {
   // Adds those of N items of each lane that reach(i) says, item i being key_at(i) (0: none).
   template <int N, class R, class K>
   __device__ __forceinline__ void add(R&& reach, K&& key_at, int lane) {
-    static_assert(64 * N + kMaxOut <= kWaveList, "the list holds them all");
+    static_assert(64 * N + kMaxOut <= CAP, "the list holds them all");
     if (n > kMaxOut) sort(lane);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -123,17 +124,17 @@ struct Best {
       if (lane < n && place < keep) list[place] = mine;
     } else {
       // Many equal logits, or k past 32. The k best by rounds, each the largest left.
-      u64 mine[kWaveSteps];
+      u64 mine[kSteps];
 #pragma unroll
-      for (int s = 0; s < kWaveSteps; ++s) mine[s] = 64 * s + lane < n ? list[64 * s + lane] : 0;
+      for (int s = 0; s < kSteps; ++s) mine[s] = 64 * s + lane < n ? list[64 * s + lane] : 0;
       wave_sync();
       for (int j = 0; j < keep; ++j) {
         u64 top = 0;
 #pragma unroll
-        for (int s = 0; s < kWaveSteps; ++s) top = max(top, mine[s]);
+        for (int s = 0; s < kSteps; ++s) top = max(top, mine[s]);
         top = wave_max(top);
 #pragma unroll
-        for (int s = 0; s < kWaveSteps; ++s) mine[s] = mine[s] == top ? 0 : mine[s];
+        for (int s = 0; s < kSteps; ++s) mine[s] = mine[s] == top ? 0 : mine[s];
         if (lane == 0) list[j] = top;
       }
     }
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
     }
   }
   const float sum = (part[0] + part[1]) + (part[2] + part[3]);
-  Best best = {s_list[wave], a.n_out, 0};
+  Best<kWaveList> best = {s_list[wave], a.n_out, 0};
   const float least = value_of(best.reached(order_of(m)));
 #pragma unroll
   for (int c = 0; c < STEPS; ++c)
@@ -264,22 +265,27 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
   }
 }
 
-// One workgroup per group: each wave joins the pieces of beams wave, wave + 4, ..; then
-// the beams' candidates are put in order by (score, beam, token). A candidate whose score
-// is no number, or of a beam without a finite score, counts as -inf; such a beam's come
-// in the order of the tokens, so its first n_out stand for it. Bound by a chain of round
-// trips (pieces, logarithm, sort, ranks): 7-8 us whatever the size.
-__global__ __launch_bounds__(64 * kWaves) void join_kernel(SelectArgs a) {
-  __shared__ u64 s_list[kWaves][kWaveList];
+constexpr int kJoinWaves = 16;  // at the most: one for each beam
+constexpr int kJoinList = 64 * 4 + kMaxOut;
+
+// One workgroup per group, a wave for each beam up to kJoinWaves: a wave joins its beam's
+// pieces; then the beams' candidates are put in order by (score, beam, token). A candidate
+// whose score is no number, or of a beam without a finite score, counts as -inf; such a
+// beam's come in the order of the tokens, so its first n_out stand for it. Bound by a chain
+// of round trips (pieces, logarithm, sort, ranks): 4 beams 6-7 us, 10 beams of 10
+// candidates 10, 32 of 32 56 (compared each with each, by four waves, 18 and 560).
+__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
+  __shared__ u64 s_list[kJoinWaves][kJoinList];
   __shared__ double s_score[kMaxBeams * kMaxOut];
   __shared__ int s_token[kMaxBeams * kMaxOut];
+  const int threads = static_cast<int>(blockDim.x);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const long long group = blockIdx.x;
   const int k = a.n_out;
   const double ninf = -__builtin_huge_val();
-  for (int b = wave; b < a.beams; b += kWaves) {
+  for (int b = wave; b < a.beams; b += threads / 64) {
     const long long row = group * a.beams + b;
     const float given = a.scores[row];
     const bool done = a.finished != nullptr && a.finished[row] != 0;
@@ -305,7 +311,7 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(SelectArgs a) {
     const double lse = static_cast<double>(m) + log(sum);
     const bool finite = given > kNegInf && given < -kNegInf;
     const bool plain = !done && finite && lse - lse == 0.0;
-    Best best = {s_list[wave], k, 0};
+    Best<kJoinList> best = {s_list[wave], k, 0};
     if (plain) {
       for (long long i0 = 0;; i0 += 64 * 4) {
         unsigned top = 0;
@@ -342,14 +348,21 @@ __global__ __launch_bounds__(64 * kWaves) void join_kernel(SelectArgs a) {
   }
   __syncthreads();
   const int n = a.beams * k;
-  for (int i = tid; i < n; i += 64 * kWaves) {
+  for (int i = tid; i < n; i += threads) {
     const double score = s_score[i];
     const int token = s_token[i];
     if (token < 0) continue;
     const int b = i / k;
-    int place = 0;  // (a beam's own are in order)
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) place += s_token[j] >= 0 && (s_score[j] > score || (s_score[j] == score && j < i));
+    // Each beam's own are in order, those without a token last: counted up to the first that
+    // comes behind this one. A place past the k-th is none.
+    int place = i - b * k;
+    for (int c = 0; c < a.beams && place < k; ++c) {
+      if (c == b) continue;
+      for (int j = c * k; j < c * k + k && place < k; ++j) {
+        if (s_token[j] < 0 || !(s_score[j] > score || (s_score[j] == score && c < b))) break;
+        ++place;
+      }
+    }
     if (place < k) {
       const long long out = group * k + place;
       a.out_scores[out] = static_cast<float>(score);
@@ -384,7 +397,9 @@ struct ReorderArgs {
 // of a group may change places in their own buffers. A parent that several beams share is
 // read once from memory and then from the caches. The thread of a 32-token block's first
 // column moves the block's scale. Bound by memory: 64 beams of 1000 tokens, 32 heads of 128,
-// 8-bit, into other buffers 161 us, 5.5 TB/s.
+// 8-bit, into other buffers 162 us, 5.5 TB/s; 14 beams in two groups of 1724 tokens, 40 heads
+// of 128, fp16, 170 us, 5.2 TB/s (271 with a branch around each load, which a wave then
+// waits for one by one).
 template <int MB>
 __global__ __launch_bounds__(256) void reorder_kernel(ReorderArgs a) {
   const unsigned chunk = blockIdx.x % a.chunks;
@@ -398,38 +413,46 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderArgs a) {
   const long long token = at / a.row_bytes;
   const long long first = group * a.beams;
   const long long beam_bytes = a.head_bytes * heads;
-  const long long base = (first * heads + head) * a.head_bytes + at;
-  const unsigned char* src = a.src[side] + base;
-  unsigned char* dst = a.dst[side] + base;
-  uintx4 v[MB];
-  bool go[MB];
+  const long long base = (first * heads + head) * a.head_bytes;
+  // What each beam takes, the same in all threads: its parent's tokens, 0 of them where it
+  // stays as it is. Such a beam loads what another one takes and does not store it: no
+  // branches between the loads.
+  const long long chunk_token = static_cast<long long>(chunk) * 4096 / a.row_bytes;
+  int p[MB];
+  long long n[MB];
+  int some = -1;
 #pragma unroll
   for (int j = 0; j < MB; ++j) {
-    go[j] = false;
-    if (j < a.beams) {
-      const int p = a.parent[first + j];
-      if (p >= 0 && p < a.beams && !(a.in_place && p == j)) {
-        go[j] = token < std::min<long long>(a.lens[first + p], a.max_len);
-        if (go[j]) v[j] = *reinterpret_cast<const uintx4*>(src + p * beam_bytes);
-      }
-    }
+    p[j] = __builtin_amdgcn_readfirstlane(a.parent[first + std::min(j, a.beams - 1)]);
+    if (j >= a.beams || p[j] < 0 || p[j] >= a.beams || (a.in_place && p[j] == j)) p[j] = -1;
   }
-  float s[MB];
-  const bool scales = a.src_scale[side] != nullptr && at % (32ll * a.row_bytes) == 0;
-  const long long beam_blocks = a.scale_blocks * heads;
-  const long long sbase = (first * heads + head) * a.scale_blocks + token / 32;
-  if (scales) {
 #pragma unroll
-    for (int j = 0; j < MB; ++j)
-      if (go[j]) s[j] = a.src_scale[side][sbase + a.parent[first + j] * beam_blocks];
+  for (int j = 0; j < MB; ++j) {
+    const int len = __builtin_amdgcn_readfirstlane(a.lens[first + std::max(p[j], 0)]);
+    n[j] = p[j] < 0 ? 0 : std::min<long long>(len, a.max_len);
+    some = n[j] > chunk_token ? p[j] : some;
   }
+  if (some < 0) return;
+  // (a thread past the last token loads the last one)
+  const unsigned char* from = a.src[side] + base + std::min(at, a.max_len * a.row_bytes - 16);
+  uintx4 v[MB];
 #pragma unroll
   for (int j = 0; j < MB; ++j)
-    if (go[j]) *reinterpret_cast<uintx4*>(dst + j * beam_bytes) = v[j];
+    v[j] = *reinterpret_cast<const uintx4*>(from + (n[j] > chunk_token ? p[j] : some) * beam_bytes);
+  const long long beam_blocks = a.scale_blocks * heads;
+  const long long sbase = (first * heads + head) * a.scale_blocks + token / 32;
+  float s[MB] = {};
+  const bool scales = a.src_scale[side] != nullptr && at % (32ll * a.row_bytes) == 0 && token < a.max_len;
   if (scales) {
 #pragma unroll
-    for (int j = 0; j < MB; ++j)
-      if (go[j]) a.dst_scale[side][sbase + j * beam_blocks] = s[j];
+    for (int j = 0; j < MB; ++j) s[j] = a.src_scale[side][sbase + (n[j] > chunk_token ? p[j] : some) * beam_blocks];
+  }
+#pragma unroll
+  for (int j = 0; j < MB; ++j) {
+    if (token < n[j]) {
+      *reinterpret_cast<uintx4*>(a.dst[side] + base + at + j * beam_bytes) = v[j];
+      if (scales) a.dst_scale[side][sbase + j * beam_blocks] = s[j];
+    }
   }
 }
 
@@ -488,7 +511,7 @@ void select_entry(const void* logits, bool half, int64_t ld, const float* scores
   if (half) vector ? go(_Float16{}, std::true_type{}) : go(_Float16{}, std::false_type{});
   else vector ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
   ENG_LAUNCH_CHECK();
-  join_kernel<<<static_cast<unsigned>(batch), 64 * kWaves, 0, s>>>(a);
+  join_kernel<<<static_cast<unsigned>(batch), 64 * std::min(a.beams, kJoinWaves), 0, s>>>(a);
   ENG_LAUNCH_CHECK();
 }
 
