@@ -8,10 +8,9 @@ namespace eng {
 namespace attn {
 
 constexpr int kFewRows = 16;   // rows of a tile
-constexpr int kFewWaves = 4;
 
-// One workgroup per (unit, tile of 16 rows, split of the unit's keys), 4 waves; a wave
-// takes every fourth block of 32 keys straight from memory into registers, two blocks in
+// One workgroup per (unit, tile of 16 rows, split of the unit's keys), NW waves; a wave
+// takes every NW-th block of 32 keys straight from memory into registers, two blocks in
 // flight. Both products are on v_mfma_f32_16x16x32_f16: S^T = K . Q^T with K as the A
 // operand, whose row i is key (i / 4) + 4 (i % 4) of 16, so that accumulator element r of
 // lane group g is key g + 4 r; O^T = V^T . P^T takes the scores in place as the B operand,
@@ -29,8 +28,8 @@ constexpr int kFewWaves = 4;
 // tokens of 32 heads 252 MB in 51 us. (On tile_kernel, whose tiles a few rows leave empty, 77
 // and 164.) Up to 128 rows over one prefix the L2 serves the tiles after the first: 32
 // sequences, 8 heads of 128, 8192 tokens 31 us, 63 MB.
-template <int D, bool Q8>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(Args a0, Args a1, unsigned wgs0) {
+template <int D, bool Q8, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void few_kernel(Args a0, Args a1, unsigned wgs0) {
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");
   constexpr int KS = D / 32;            // 32-dim steps of a score
   constexpr int ES = Q8 ? 1 : 2;        // bytes of a value
@@ -39,7 +38,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(Args a0, Args a1
   constexpr int VD = VW * ES / 4;       // in 32-bit words
   constexpr int kBlockBytes = kKvBlock * D * ES;
   constexpr int WS = kFewRows * (D + 2);  // a wave's state in LDS: o, m, l
-  __shared__ __attribute__((aligned(16))) float s_state[kFewWaves * WS];
+  __shared__ __attribute__((aligned(16))) float s_state[NW * WS];
 
   const bool second = blockIdx.x >= wgs0;
   const Args& a = second ? a1 : a0;
@@ -76,9 +75,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(Args a0, Args a1
   const int per = (blocks + a.nsplit - 1) / a.nsplit;
   const int t0 = min(split * per, blocks);
   const int n = min(per, blocks - t0);                                // of this split
-  const int nb = wave < n ? (n - wave + kFewWaves - 1) / kFewWaves : 0;  // of this wave
+  const int nb = wave < n ? (n - wave + NW - 1) / NW : 0;  // of this wave
   auto block_of = [&](int i) {  // the wave's i-th
-    const int t = t0 + wave + kFewWaves * i;
+    const int t = t0 + wave + NW * i;
     return t < sink_blocks ? t : start + (t - sink_blocks);
   };
 
@@ -292,8 +291,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(Args a0, Args a1
     }
   }
   __syncthreads();
-  const int live = min(kFewWaves, n);  // waves with a block
-  for (int idx = tid; idx < gq * D; idx += 64 * kFewWaves) {
+  const int live = min(NW, n);  // waves with a block
+  for (int idx = tid; idx < gq * D; idx += 64 * NW) {
     const int r = idx / D;
     const int d = idx - r * D;
     float mb = kNegInf;

@@ -96,13 +96,18 @@ void tiles(const Args& a, bool q8, int waves, hipStream_t s) {
   }
   q8 ? tiles<D, true, 4>(a, s) : tiles<D, false, 4>(a, s);
 }
-template <int D>
-void few(const Args& a, const Args& b, bool q8, hipStream_t s) {
+template <int D, bool Q8>
+void few(const Args& a, const Args& b, int waves, hipStream_t s) {
   const long long wgs0 = a.units * a.row_tiles * a.nsplit;
-  const long long wgs = wgs0 + b.units * b.row_tiles * b.nsplit;
-  if (q8) few_kernel<D, true><<<static_cast<unsigned>(wgs), 64 * kFewWaves, 0, s>>>(a, b, static_cast<unsigned>(wgs0));
-  else few_kernel<D, false><<<static_cast<unsigned>(wgs), 64 * kFewWaves, 0, s>>>(a, b, static_cast<unsigned>(wgs0));
+  const auto wgs = static_cast<unsigned>(wgs0 + b.units * b.row_tiles * b.nsplit);
+  const auto first = static_cast<unsigned>(wgs0);
+  if (waves == 1) few_kernel<D, Q8, 1><<<wgs, 64, 0, s>>>(a, b, first);
+  else few_kernel<D, Q8, 4><<<wgs, 64 * 4, 0, s>>>(a, b, first);
   ENG_LAUNCH_CHECK();
+}
+template <int D>
+void few(const Args& a, const Args& b, bool q8, int waves, hipStream_t s) {
+  q8 ? few<D, true>(a, b, waves, s) : few<D, false>(a, b, waves, s);
 }
 
 // Waves of a tile: at D = 128 eight where that leaves a workgroup for every CU, else four.
@@ -129,6 +134,15 @@ int few_splits(long long wgs, long long keys, long long D) {
   if (blocks * D <= 12 * 128) return 1;
   const long long want = device_cu_count() / wgs;
   return static_cast<int>(std::max(1ll, std::min({want, blocks / 2, static_cast<long long>(kMaxStates)})));
+}
+
+// Waves of a workgroup of few rows. One, without three that find nothing to do, where a split
+// is one block, and up to four blocks where four workgroups for each CU hide the chain of
+// loads: one token of 64 sequences of 32 heads of 128, fp16, 20 tokens 8.2 us (18.2 with
+// four waves), 100 tokens 19.7 (27.2), 200 34 (36); of 16 sequences of 8 KV heads, 100 tokens
+// 7.4 (6.2).
+int few_waves(long long wgs, long long blocks) {
+  return blocks <= 1 || (blocks <= 4 && wgs >= 4 * static_cast<long long>(device_cu_count())) ? 1 : 4;
 }
 
 constexpr long long kMaxLen = 0x7fffffffLL - 2 * kTileKeys;  // 32-bit positions, up to a tile past the end
@@ -164,7 +178,8 @@ void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hip
   auto go = [&](auto dim) {
     constexpr int kD = decltype(dim)::value;
     auto launch = [&] {
-      if (one) few<kD>(a, Args{}, q8, s);
+      const long long wgs = a.units * a.row_tiles * a.nsplit;
+      if (one) few<kD>(a, Args{}, q8, few_waves(wgs, (most + a.nsplit - 1) / a.nsplit), s);
       else tiles<kD>(a, q8, waves, s);
     };
     if (a.nsplit == 1) {
@@ -216,6 +231,17 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
   ENG_CHECK(threads_fit(shared.units * shared.row_tiles * std::max(1, few_shared ? shared.nsplit : 1) +
                             mine.units * mine.row_tiles * std::max(1, mine.nsplit), 512),
             "attention_prefix: too many query rows for one launch");
+  // of the launch of few rows: workgroups, and the blocks of a split at the most
+  auto blocks_of = [](const Args& a) {
+    const long long blocks = (a.max_len + kKvBlock - 1) / kKvBlock;
+    return a.nsplit > 0 ? (blocks + a.nsplit - 1) / a.nsplit : 0;
+  };
+  long long wgs = mine.units * mine.row_tiles * mine.nsplit;
+  long long blocks = blocks_of(mine);
+  if (few_shared) {
+    wgs += shared.units * shared.row_tiles * shared.nsplit;
+    blocks = std::max(blocks, blocks_of(shared));
+  }
   const int states = shared.nsplit + mine.nsplit;
   shared.part_stride = mine.part_stride = states;
   mine.part0 = shared.nsplit;
@@ -225,8 +251,8 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
     shared.part_o = mine.part_o = static_cast<float*>(scratch.get());
     shared.part_ml = mine.part_ml = shared.part_o + rows * states * kD;
     if (!few_shared && shared.nsplit > 0) tiles<kD>(shared, q8, waves, s);
-    if (few_shared) few<kD>(shared, mine, q8, s);
-    else if (mine.nsplit > 0) few<kD>(mine, Args{}, q8, s);
+    if (few_shared) few<kD>(shared, mine, q8, few_waves(wgs, blocks), s);
+    else if (mine.nsplit > 0) few<kD>(mine, Args{}, q8, few_waves(wgs, blocks), s);
     merge<kD>(mine, rows, states, s);
   };
   if (D == 64) go(std::integral_constant<int, 64>{});

@@ -148,3 +148,12 @@ def test_replayed_with_lengths_that_grow(gpu, kind):
             s.sync()
             assert np.array_equal(do.download(), want)
         graph.destroy()
+
+
+@KINDS
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("prefix,longest", [(15, 5), (32, 32), (33, 128), (129, 40)])
+def test_many_short_sequences(gpu, kind, D, prefix, longest):
+    # enough of them for a workgroup of one wave each, up to four blocks of keys
+    run(gpu, kind, 10, 8, 8, D, [(5 * g) % (prefix + 1) for g in range(12)] + [prefix],
+        [(37 * b) % (longest + 1) for b in range(130)], max_prefix=prefix, max_len=longest)

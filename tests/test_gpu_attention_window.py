@@ -325,3 +325,13 @@ def test_keys_of_minus_infinity(gpu, S):
             want[0, i, h] = lc.attend_rows(q[0, i, h], cache.values[0][0, 0, j], cache.values[1][0, 0, j],
                                            cache.vmax[0, 0], 0.125)
     lc.check(got, want, "-inf")
+
+
+@KINDS
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("longest,window,sinks", [(32, 0, 0), (64, 0, 0), (128, 0, 0),
+                                                  (129, 0, 0), (300, 50, 3), (300, 20, 0)])
+def test_many_short_sequences(gpu, kind, D, longest, window, sinks):
+    # enough of them for a workgroup of one wave each, up to four blocks of keys
+    pos = [(37 * b) % (longest + 1) - 1 for b in range(130)]
+    run(gpu, kind, 130, 1, 8, 8, D, pos, None, window, sinks, max_len=longest)
