@@ -272,7 +272,7 @@ constexpr int kJoinList = 64 * 4 + kMaxOut;
 // pieces; then the beams' candidates are put in order by (score, beam, token). A candidate
 // whose score is no number, or of a beam without a finite score, counts as -inf; such a
 // beam's come in the order of the tokens, so its first n_out stand for it. Bound by a chain
-// of round trips (pieces, logarithm, sort, ranks): 4 beams 6-7 us, 10 beams of 10
+// of round trips (pieces, logarithm, sort, ranks): 4 beams 5.5-7 us, 10 beams of 10
 // candidates 10, 32 of 32 56 (compared each with each, by four waves, 18 and 560).
 __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
   __shared__ u64 s_list[kJoinWaves][kJoinList];
