@@ -266,7 +266,8 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
 }
 
 constexpr int kJoinWaves = 16;  // at the most: one for each beam
-constexpr int kJoinList = 64 * 4 + kMaxOut;
+constexpr int kJoinKeys = 4;    // of a lane in one go
+constexpr int kJoinList = 64 * kJoinKeys + kMaxOut;
 
 // One workgroup per group, a wave for each beam up to kJoinWaves: a wave joins its beam's
 // pieces; then the beams' candidates are put in order by (score, beam, token). A candidate
@@ -290,10 +291,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
     const float given = a.scores[row];
     const bool done = a.finished != nullptr && a.finished[row] != 0;
     const long long n = static_cast<long long>(a.pieces) * k;
-    u64 key[4];
+    u64 key[kJoinKeys];
     auto load_keys = [&](long long i0) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < kJoinKeys; ++j) {
         const long long i = i0 + 64 * j + lane;
         key[j] = i < n ? a.keys[row * n + i] : 0;
       }
@@ -313,15 +314,15 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
     const bool plain = !done && finite && lse - lse == 0.0;
     Best<kJoinList> best = {s_list[wave], k, 0};
     if (plain) {
-      for (long long i0 = 0;; i0 += 64 * 4) {
+      for (long long i0 = 0;; i0 += 64 * kJoinKeys) {
         unsigned top = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = max(top, static_cast<unsigned>(key[j] >> 32));
+        for (int j = 0; j < kJoinKeys; ++j) top = max(top, static_cast<unsigned>(key[j] >> 32));
         const unsigned least = best.reached(top);
-        best.add<4>([&](int j) { return static_cast<unsigned>(key[j] >> 32) >= least; },
+        best.add<kJoinKeys>([&](int j) { return static_cast<unsigned>(key[j] >> 32) >= least; },
                     [&](int j) { return key[j]; }, lane);
-        if (i0 + 64 * 4 >= n) break;
-        load_keys(i0 + 64 * 4);
+        if (i0 + 64 * kJoinKeys >= n) break;
+        load_keys(i0 + 64 * kJoinKeys);
       }
       best.sort(lane);
     }
@@ -487,14 +488,18 @@ void select_entry(const void* logits, bool half, int64_t ld, const float* scores
   a.n_out = static_cast<int>(n_out);
   a.vocab = static_cast<int>(vocab);
   a.eos = eos < 0 ? -1 : static_cast<int>(eos);
-  // Steps of a piece: as many as leave two workgroups to a CU, up to four.
+  // Steps of a piece: as many as leave two workgroups to a CU, up to four; one to a CU, where
+  // the join would load a beam's candidates in more than one go (16 rows of 152064, 8 of
+  // them: 15.3 us with 304 workgroups, 17.0 with 608; 48 rows of 50257 18.7 and 16.9).
   const long long steps = (vocab + kStep - 1) / kStep;
   ENG_CHECK(batch <= 0xffffffffLL / (64 * kWaves) / (beams * steps),
             "beam_select: too many logits for one launch");
   const long long rows = batch * beams;
   int per = 4;
-  while (per > 1 && rows * ((steps + per - 1) / per) < 2ll * device_cu_count()) per /= 2;
-  a.pieces = static_cast<int>((steps + per - 1) / per);
+  auto pieces = [&](int n) { return (steps + n - 1) / n; };
+  while (per > 1 && rows * pieces(per) < 2ll * device_cu_count()) per /= 2;
+  while (per < 4 && pieces(per) * n_out > 64 * kJoinKeys && rows * pieces(2 * per) >= device_cu_count()) per *= 2;
+  a.pieces = static_cast<int>(pieces(per));
   const std::size_t lists = static_cast<std::size_t>(rows) * a.pieces;
   StreamScratch scratch(s, lists * (n_out + 1) * 8);
   a.keys = static_cast<u64*>(scratch.get());
