@@ -125,14 +125,18 @@ int tile_splits(long long wgs, long long keys, int waves) {
   return static_cast<int>(std::max(1ll, std::min({want, (keys + kTileKeys - 1) / kTileKeys / 4,
                                                   static_cast<long long>(kMaxStates)})));
 }
-// And of few rows: one workgroup to a CU, at least two blocks a split, and one split,
-// without the merge's launch, up to 12 blocks at D = 128 or 24 at D = 64 (one token of 32
-// heads: 300 tokens 7.3 us, 8.2 in four splits; 8192 tokens of 32 / 8 heads 12.5-13.3 in 16
-// or 32 splits, 16.5 in 8 or 64; 16 sequences of 2048 30 in 1 to 4, 34 in 8).
-int few_splits(long long wgs, long long keys, long long D) {
+// And of few rows: one workgroup to a CU, at least two blocks a split, and one split up to
+// 12 blocks at D = 128 or 24 at D = 64 (one token of 32 heads: 300 tokens 7.3 us, 8.2 in
+// four splits; 8192 tokens of 32 / 8 heads 12.5-13.3 in 16 or 32 splits, 16.5 in 8 or 64; 16
+// sequences of 2048 30 in 1 to 4, 34 in 8). Where one split needs no merge, up to more
+// blocks the fewer the splits that it stands for: 128 units of 600 tokens 10.3 us in one
+// and 13.0 in two, of 1500 22.2 and 21.5; 64 units of 400 8.5 and 9.1 in four, of 1000 13.3
+// and 12.1.
+int few_splits(long long wgs, long long keys, long long D, bool merged) {
   const long long blocks = (keys + kKvBlock - 1) / kKvBlock;
-  if (blocks * D <= 12 * 128) return 1;
   const long long want = device_cu_count() / wgs;
+  const long long single = merged ? 12 : std::max(12ll, 72 / std::max(want, 1ll));
+  if (blocks * D <= single * 128) return 1;
   return static_cast<int>(std::max(1ll, std::min({want, blocks / 2, static_cast<long long>(kMaxStates)})));
 }
 
@@ -168,7 +172,7 @@ void run_window(Args a, long long batch, long long D, int split_kv, bool q8, hip
     keys = std::min(keys, a.window + a.sinks + std::min<long long>(a.s_new, tile / a.group + 2) + kKvBlock);
   const long long step = one ? kKvBlock : kTileKeys;
   const long long most = std::max(1ll, (keys + step - 1) / step);
-  a.nsplit = split_kv == 0 ? (one ? few_splits(a.units * a.row_tiles, keys, D)
+  a.nsplit = split_kv == 0 ? (one ? few_splits(a.units * a.row_tiles, keys, D, false)
                                   : tile_splits(a.units * a.row_tiles, keys, waves))
                            : static_cast<int>(std::min<long long>({split_kv, most, kMaxStates}));
   if (one)
@@ -222,7 +226,7 @@ void run_prefix(Args shared, Args mine, long long n_prefix, long long batch, lon
     const long long step = of_few ? kKvBlock : kTileKeys;
     const long long wgs = a.units * a.row_tiles;
     const int chosen = split_kv != 0 ? static_cast<int>(std::min<long long>(split_kv, (a.max_len + step - 1) / step))
-                       : of_few      ? few_splits(wgs, a.max_len, D)
+                       : of_few      ? few_splits(wgs, a.max_len, D, true)
                                      : tile_splits(wgs, a.max_len, waves);
     return std::min(chosen, kMaxStates / 2);
   };
