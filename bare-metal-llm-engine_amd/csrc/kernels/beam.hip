@@ -5,17 +5,20 @@
 // log sum_t exp x_bt. Within a beam the order is the logits' own, so the logits are read
 // once: a pass over a piece of a row keeps the piece's best candidates by (logit, lowest
 // token) as 64-bit keys and its max and sum of exponentials; a second kernel joins the
-// pieces and compares candidates of unlike beams by their scores in 64 bits.
+// pieces and compares candidates of unlike beams by their scores in 64 bits, with sums of
+// fp32 exponentials where these tell the candidates apart and 64-bit ones where not.
 #include "gemv_kernels.hpp"
 #include "launch.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace eng {
 namespace beam {
 namespace {
 
+typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef unsigned long long u64;
@@ -44,6 +47,33 @@ __device__ __forceinline__ unsigned token_of(u64 key) { return 0xffffffffu - sta
 
 // e^x to 2 units in the last place and the rounding of x log2 e.
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+// e^d in 64 bits, d < 700 and no NaN, to 2e-14: 2^k 2^f, t = k + f, |f| <= 1/2, 2^f by the
+// polynomial of degree 9 that meets it in Chebyshev's points. Less than e^-700 counts as it.
+__device__ __forceinline__ double exp64(double d) {
+  constexpr double kLog2e = 1.4426950408889634, kRound = 0x1.8p52;
+  d = fmax(d, -700.0);
+  const double t = fma(d, kLog2e, kRound);  // (k in the lowest bits)
+  const double f = fma(d, kLog2e, kRound - t);
+  double p = 0x1.b69b333333333p-24;
+  p = fma(p, f, 0x1.63f1a66666666p-20);
+  p = fma(p, f, 0x1.ffcb2e3333335p-17);
+  p = fma(p, f, 0x1.43088c34ccccbp-13);
+  p = fma(p, f, 0x1.5d87fea9ba666p-10);
+  p = fma(p, f, 0x1.3b2ab72c33333p-7);
+  p = fma(p, f, 0x1.c6b08d70374acp-5);
+  p = fma(p, f, 0x1.ebfbdff813d86p-3);
+  p = fma(p, f, 0x1.62e42fefa3a31p-1);
+  p = fma(p, f, 0x1.000000000003fp+0);
+  uintx2 w = __builtin_bit_cast(uintx2, p);
+  w[1] += __builtin_bit_cast(uintx2, t)[0] << 20;
+  return __builtin_bit_cast(double, w);
+}
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off);
+  return x;
+}
 
 // The largest of the wave's values, in every lane.
 template <int CTRL>
@@ -163,6 +193,8 @@ struct SelectArgs {
   int pieces;      // of a row
   u64* keys;       // [rows][pieces][n_out], 0 behind the last one
   floatx2* sums;   // [rows][pieces]: max, sum of exp(x - max)
+  double* lse;     // [rows][2]: L as the largest logit and what is to be added; NaN: none
+  double near;     // scores of unlike beams this close may be in the wrong order
 };
 
 constexpr int kStep = 64 * kWaves * kVpt;  // values of a workgroup's step
@@ -275,6 +307,14 @@ constexpr int kJoinList = 64 * kJoinKeys + kMaxOut;
 // beam's come in the order of the tokens, so its first n_out stand for it. Bound by a chain
 // of round trips (pieces, logarithm, sort, ranks): 4 beams 5.5-7 us, 10 beams of 10
 // candidates 10, 32 of 32 56 (compared each with each, by four waves, 18 and 560).
+//
+// The sum of fp32 exponentials leaves L off by up to `near` / 2 (select_entry has the bound).
+// Where a chosen candidate and one of another beam are closer than `near`, both beams' sums
+// are formed again, from the logits, in 64 bits, and the candidates put in order again: of
+// groups with gaps of 0.1 in score about one in a thousand, 85 us for two beams of 152064.
+// The question itself costs 0.3 us. (All exponentials in 64 bits: 16 x 4 beams of 152064 in
+// 29 us in place of 22.)
+template <typename T>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
   __shared__ u64 s_list[kJoinWaves][kJoinList];
   __shared__ double s_score[kMaxBeams * kMaxOut];
@@ -309,9 +349,13 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
       part = fmaf(p[1], p[0] == kNegInf ? 1.0f : exp_of(p[0] - m), part);
     }
     const double sum = gemv::wave_sum(part);
-    const double lse = static_cast<double>(m) + log(sum);
+    const double peak = m, more = log(sum);  // L = peak + more, kept apart: rows far from zero lose nothing
     const bool finite = given > kNegInf && given < -kNegInf;
-    const bool plain = !done && finite && lse - lse == 0.0;
+    const bool plain = !done && finite && (peak + more) - (peak + more) == 0.0;
+    if (lane == 0) {
+      a.lse[2 * row] = plain ? peak : __builtin_nan("");
+      a.lse[2 * row + 1] = more;
+    }
     Best<kJoinList> best = {s_list[wave], k, 0};
     if (plain) {
       for (long long i0 = 0;; i0 += 64 * kJoinKeys) {
@@ -335,7 +379,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
         if (i < best.n) {
           const u64 key = best.list[i];
           token = static_cast<int>(token_of(key));
-          score = static_cast<double>(given) + (static_cast<double>(logit_of(key)) - lse);
+          score = static_cast<double>(given) + ((static_cast<double>(logit_of(key)) - peak) - more);
         }
       } else if (done && finite) {
         // its end token first, then the others
@@ -347,31 +391,88 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
       s_token[b * k + i] = token;
     }
   }
+  // beams whose order is open, in wave 0's list, which it is done with; a wave's sum in the next
+  unsigned* const s_open = reinterpret_cast<unsigned*>(s_list[0]);
+  double* const s_part = reinterpret_cast<double*>(s_list[1]);
+  if (tid == 0) *s_open = 0;
   __syncthreads();
   const int n = a.beams * k;
-  for (int i = tid; i < n; i += threads) {
-    const double score = s_score[i];
-    const int token = s_token[i];
-    if (token < 0) continue;
-    const int b = i / k;
-    // Each beam's own are in order, those without a token last: counted up to the first that
-    // comes behind this one. A place past the k-th is none.
-    int place = i - b * k;
-    for (int c = 0; c < a.beams && place < k; ++c) {
-      if (c == b) continue;
-      for (int j = c * k; j < c * k + k && place < k; ++j) {
-        if (s_token[j] < 0 || !(s_score[j] > score || (s_score[j] == score && c < b))) break;
-        ++place;
+  // Places of a thread's candidates, k and more for none; the beams whose order is open.
+  constexpr int kMine = (kMaxBeams * kMaxOut + 64 * kJoinWaves - 1) / (64 * kJoinWaves);
+  int place[kMine];
+  auto rank = [&] {
+    unsigned open = 0;
+#pragma unroll
+    for (int q = 0; q < kMine; ++q) {
+      const int i = tid + q * threads;
+      place[q] = k;
+      if (i >= n || s_token[i] < 0) continue;
+      const double score = s_score[i];
+      const int b = i / k;
+      // Each beam's own are in order, those without a token last: counted up to the first that
+      // comes behind this one. A place past the k-th is none.
+      int at = i - b * k;
+      unsigned close = 0;
+      for (int c = 0; c < a.beams && at < k; ++c) {
+        if (c == b) continue;
+        double behind = ninf;
+        for (int j = c * k; j < c * k + k && at < k; ++j) {
+          behind = s_token[j] < 0 ? ninf : s_score[j];
+          if (s_token[j] < 0 || !(behind > score || (behind == score && c < b))) break;
+          ++at;
+        }
+        if (score - behind <= a.near) close |= (1u << b) | (1u << c);
+      }
+      place[q] = at;
+      if (at < k) open |= close;
+    }
+    return open;
+  };
+  const unsigned open = rank();
+  if (open != 0) atomicOr(s_open, open);
+  __syncthreads();
+  for (unsigned again = *s_open; again != 0; again &= again - 1) {
+    const int b = __builtin_ctz(again);
+    const long long row = group * a.beams + b;
+    const double peak = a.lse[2 * row], more = a.lse[2 * row + 1];
+    if (peak != peak) continue;
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+    double part[4] = {};
+    for (int t0 = tid; t0 < a.vocab; t0 += 4 * threads) {
+      T v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = x[min(t0 + j * threads, a.vocab - 1)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double e = exp64((static_cast<double>(v[j]) - peak) - more);
+        part[j] += t0 + j * threads < a.vocab ? e : 0.0;
       }
     }
-    if (place < k) {
-      const long long out = group * k + place;
-      a.out_scores[out] = static_cast<float>(score);
-      a.out_parent[out] = b;
-      a.out_token[out] = token;
-      if (a.out_finished != nullptr)
-        a.out_finished[out] = (a.finished != nullptr && a.finished[group * a.beams + b] != 0) || token == a.eos;
-    }
+    const double mine = wave_sum((part[0] + part[1]) + (part[2] + part[3]));
+    __syncthreads();  // (s_part is read for the beam before)
+    if (lane == 0) s_part[wave] = mine;
+    __syncthreads();
+    double sum = 0.0;
+    for (int w = 0; w < threads / 64; ++w) sum += s_part[w];
+    const double change = log(sum);  // of L: terms against the old one add up to e^change
+    for (int i = b * k + tid; i < b * k + k; i += threads) s_score[i] -= change;
+  }
+  if (*s_open != 0) {
+    __syncthreads();
+    rank();
+  }
+#pragma unroll
+  for (int q = 0; q < kMine; ++q) {
+    if (place[q] >= k) continue;
+    const int i = tid + q * threads;
+    const int b = i / k;
+    const int token = s_token[i];
+    const long long out = group * k + place[q];
+    a.out_scores[out] = static_cast<float>(s_score[i]);
+    a.out_parent[out] = b;
+    a.out_token[out] = token;
+    if (a.out_finished != nullptr)
+      a.out_finished[out] = (a.finished != nullptr && a.finished[group * a.beams + b] != 0) || token == a.eos;
   }
 }
 
@@ -501,9 +602,10 @@ void select_entry(const void* logits, bool half, int64_t ld, const float* scores
   while (per < 4 && pieces(per) * n_out > 64 * kJoinKeys && rows * pieces(2 * per) >= device_cu_count()) per *= 2;
   a.pieces = static_cast<int>(pieces(per));
   const std::size_t lists = static_cast<std::size_t>(rows) * a.pieces;
-  StreamScratch scratch(s, lists * (n_out + 1) * 8);
+  StreamScratch scratch(s, (lists * (n_out + 1) + 2 * static_cast<std::size_t>(rows)) * 8);
   a.keys = static_cast<u64*>(scratch.get());
   a.sums = reinterpret_cast<floatx2*>(a.keys + lists * n_out);
+  a.lse = reinterpret_cast<double*>(a.sums + lists);
   const bool vector = aligned_to(logits, 16) && (ld * elem) % 16 == 0;
   const unsigned grid = static_cast<unsigned>(lists);
   auto go = [&](auto elem, auto vec) {
@@ -516,7 +618,17 @@ void select_entry(const void* logits, bool half, int64_t ld, const float* scores
   if (half) vector ? go(_Float16{}, std::true_type{}) : go(_Float16{}, std::false_type{});
   else vector ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
   ENG_LAUNCH_CHECK();
-  join_kernel<<<static_cast<unsigned>(batch), 64 * std::min(a.beams, kJoinWaves), 0, s>>>(a);
+  // How far L may be off, u = 2^-24: a term's argument a = x - max by 2.22 |a| u (difference,
+  // product, log2 e as an fp32 number), over a row in the mean 2.22 u log vocab at the most
+  // (the mean of -log w_i under w_i / S is an entropy less log S, and S >= 1); four
+  // exponentials of 2 u on a term's way into the row's sum and the products of three, 11 u;
+  // additions of a lane 18 u, a wave 6 u, a workgroup 4 u, and of the pieces in the join
+  // pieces / 64 + 6. Twice that for two beams.
+  a.near = 2.0 * 0x1p-24 * (2.22 * std::log(static_cast<double>(vocab)) + 45.0 + static_cast<double>(a.pieces) / 64.0 + 1.0);
+  // At least four waves, for the sums in 64 bits; a thread has up to two candidates.
+  const int join_threads = 64 * std::max(4, std::min(a.beams, kJoinWaves));
+  if (half) join_kernel<_Float16><<<static_cast<unsigned>(batch), join_threads, 0, s>>>(a);
+  else join_kernel<float><<<static_cast<unsigned>(batch), join_threads, 0, s>>>(a);
   ENG_LAUNCH_CHECK();
 }
 

@@ -1,0 +1,108 @@
+"""GPU tests of eng_beam_select_* where beams' candidates lie closer than fp32 sums tell
+apart: their order is that of the scores in 64 bits.
+
+Bounds of L = log sum exp, u = 2^-24. Of the sum of fp32 exponentials, relative: a term's
+argument a = x - max by 2.22 |a| u (difference, product, log2 e as an fp32 number), whose mean
+over the row's weights is log V at the most (an entropy less log of the sum, and that is 1
+at least); four exponentials of 2 u each on its way into the row's sum, 3 u of products;
+additions of a lane 18 u, a wave 6 u, a workgroup 4 u, the pieces V / 262144 + 6 u: WIDE(V).
+Candidates of unlike beams closer than twice that are compared by sums in 64 bits, v =
+2^-53: an exponential to 2e-14 and its argument's rounding, |x - L| log2 e v, under 2e-14
+for |x - L| < 100 and times its weight beyond; V / 256 + 20 additions of v: 6e-14 for V <
+60000, and the few roundings of scores under 1000 another 4e-13. EPS = 1e-12."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import long_context as lc
+from helpers import U32
+from test_gpu_beam import select
+
+pytestmark = pytest.mark.gpu
+KINDS = pytest.mark.parametrize("kind", ["f32", "f16"])
+EPS = 1e-12
+
+
+def wide(V):
+    return (2.22 * np.log(V) + 46 + V / 262144) * U32
+
+
+def lse64(x):
+    return x.max(-1) + np.log(np.exp(x - x.max(-1, keepdims=True)).sum(-1))
+
+
+@KINDS
+@pytest.mark.parametrize("V", [300, 4096, 9001, 50257])
+@pytest.mark.parametrize("spread", [0.5, 3.0, 20.0])
+def test_beams_a_hair_apart(gpu, kind, V, spread):
+    """Beam 1's score is set so that its best candidate meets beam 0's as nearly as an fp32
+    score can: the gaps are roundings of it, 1e-6 to nothing."""
+    rng = np.random.default_rng(V + int(10 * spread))
+    groups = 40
+    x = (spread * rng.standard_normal((groups, 2, V))).astype(np.float16 if kind == "f16" else np.float32)
+    lse = lse64(x.astype(np.float64))
+    top = x.astype(np.float64).max(2)
+    scores = np.zeros((groups, 2), np.float32)
+    scores[:, 0] = -rng.random(groups)
+    scores[:, 1] = (scores[:, 0].astype(np.float64) + (top[:, 0] - lse[:, 0])) - (top[:, 1] - lse[:, 1])
+    best = scores.astype(np.float64) + (top - lse)
+    apart = np.abs(best[:, 0] - best[:, 1]) > 2 * EPS
+    assert apart.sum() > 30 and (np.abs(best[:, 0] - best[:, 1]) < 1e-5).all()
+    got = select(gpu, kind, x, scores, None, 2, -1)
+    first = np.where(best[:, 0] > best[:, 1], 0, 1)
+    wrong = np.flatnonzero(apart & (got[1][:, 0] != first))
+    assert not len(wrong), f"groups {wrong}: gaps {(best[wrong, 0] - best[wrong, 1])}"
+
+
+@KINDS
+@pytest.mark.parametrize("V", [1, 63, 5000, 33000])
+@pytest.mark.parametrize("spread", [0.0, 2.0, 12.0])
+def test_scores_and_their_order(gpu, kind, V, spread):
+    rng = np.random.default_rng(V + 7)
+    x = (spread * rng.standard_normal((6, 3, V))).astype(np.float16 if kind == "f16" else np.float32)
+    scores = (-2 * rng.random((6, 3))).astype(np.float32)
+    n_out = min(6, 3 * V)
+    got = select(gpu, kind, x, scores, None, n_out, -1)
+    for g in range(6):
+        s = scores[g].astype(np.float64)[:, None] + (x[g].astype(np.float64) - lse64(x[g].astype(np.float64))[:, None])
+        at = s[got[1][g], got[2][g]]
+        assert (np.abs(got[0][g] - at) <= U32 * np.abs(at) + wide(V)).all()
+        assert (at >= np.sort(s.reshape(-1))[::-1][:n_out] - 2 * EPS).all()
+
+
+@KINDS
+def test_equal_rows_of_all_beams_tie_to_the_lower(gpu, kind):
+    """The same logits and scores in every beam: every token ties, in beams' order, however
+    the sums come out."""
+    rng = np.random.default_rng(0)
+    row = (2 * rng.standard_normal(20011)).astype(np.float16 if kind == "f16" else np.float32)
+    x = np.broadcast_to(row, (3, 5, 20011)).copy()
+    scores = np.full((3, 5), -1.25, np.float32)
+    got = select(gpu, kind, x, scores, None, 15, -1)
+    for g in range(3):
+        _, p, t, _ = lc.select64(x[g].astype(np.float64), scores[g].astype(np.float64), None, 15, -1)
+        assert np.array_equal(got[1][g], p) and np.array_equal(got[2][g], t)
+
+
+@KINDS
+def test_large_and_far_apart_logits(gpu, kind):
+    """Terms that vanish beside the largest, and rows far from zero, where exponents of x
+    itself would leave every range."""
+    rng = np.random.default_rng(2)
+    dt = np.float16 if kind == "f16" else np.float32
+    x = (3 * rng.standard_normal((4, 2, 3000))).astype(dt)
+    x[0] = (x[0] + (60000 if kind == "f16" else 1e30)).astype(dt)
+    x[1] = (x[1] - (60000 if kind == "f16" else 1e6)).astype(dt)
+    x[2, :, ::2] = -np.inf
+    x[2, :, 1::4] = np.finfo(dt).min
+    x[3] *= 100
+    scores = np.array([[-1, -1.5]] * 4, np.float32)
+    got = select(gpu, kind, x, scores, None, 4, -1)
+    for g in range(4):
+        s, p, t, _ = lc.select64(x[g].astype(np.float64), scores[g].astype(np.float64), None, 4, -1)
+        assert np.array_equal(got[1][g], p) and np.array_equal(got[2][g], t)
+        # (a score is formed from x and L, half a step of 64 bits of either each)
+        far = 4 * 2.0**-53 * np.abs(x[g].astype(np.float64)[np.isfinite(x[g])]).max()
+        assert (np.abs(got[0][g] - s) <= U32 * np.abs(s) + wide(3000) + far).all()
