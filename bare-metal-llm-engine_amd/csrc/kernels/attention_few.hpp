@@ -21,7 +21,10 @@ constexpr int kFewRows = 16;   // rows of a tile
 //
 // The keys are [0, hi) without [sinks, lo) and a block's loads go through a descriptor
 // that ends with its last key, so rows past it read as zeros; values of hidden keys before
-// the window are set to zero, so nothing of either reaches a sum.
+// the window are set to zero, so nothing of either reaches a sum. An infinity that is seen
+// would meet weights' second terms of 0. So a wave whose sums are not all finite computes
+// them again with V's infinities and NaN taken out, and adds these: its rows all see them.
+// (Of 8-bit values only NaN is not finite, and stays it. The question costs 0.2 us.)
 //
 // Bound by the caches' bytes: one token of 16 sequences of up to 8192, window 4096, 32 / 8
 // heads of 128, 8-bit: 135 MB in 25 us, 5.4 TB/s; eight groups of four beams over 4096
@@ -159,7 +162,8 @@ __global__ __launch_bounds__(64 * NW, 2) void few_kernel(Args a0, Args a1, unsig
 #pragma unroll
   for (int d = 0; d < VW; ++d) o[d] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  auto compute = [&](Block& x, int i) __attribute__((always_inline)) {
+  [[maybe_unused]] float apart[VW] = {};  // of dims VW col + c: what is not finite, taken out
+  auto compute = [&](Block& x, int i, auto careful) __attribute__((always_inline)) {
     const int first = block_of(i) * kKvBlock;
     floatx4 sc[2];
 #pragma unroll
@@ -193,6 +197,19 @@ __global__ __launch_bounds__(64 * NW, 2) void few_kernel(Args a0, Args a1, unsig
           sv[e] = kNegInf;
 #pragma unroll
           for (int w = 0; w < VD; ++w) x.v[e][w] = 0;
+        }
+      }
+    }
+    if constexpr (decltype(careful)::value) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int c = 0; c < VW; ++c) {
+          const unsigned word = x.v[e][c / 2];
+          const float y = static_cast<float>(__builtin_bit_cast(halfx2, word)[c % 2]);
+          if (fabsf(y) < __builtin_huge_valf()) continue;
+          apart[c] += y;
+          x.v[e][c / 2] = word & (c % 2 == 0 ? 0xffff0000u : 0x0000ffffu);
         }
       }
     }
@@ -265,7 +282,7 @@ __global__ __launch_bounds__(64 * NW, 2) void few_kernel(Args a0, Args a1, unsig
   for (int t = 0; t < nb; t += P) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      if (t + i < nb) compute(buf[i], t + i);
+      if (t + i < nb) compute(buf[i], t + i, std::false_type{});
       __builtin_amdgcn_sched_barrier(0);
       load(buf[i], t + i + P);
       __builtin_amdgcn_sched_barrier(0);
@@ -273,6 +290,31 @@ __global__ __launch_bounds__(64 * NW, 2) void few_kernel(Args a0, Args a1, unsig
   }
 
   // Lane (col, grp) holds dims VW (4 grp + r) + d of row col in o[d][r].
+  if constexpr (!Q8) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int d = 0; d < VW; ++d) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum = fmaf(o[d][r], 0.0f, sum);
+    }
+    if (__any(sum != sum)) {
+      m = kNegInf;
+      lsum = 0.0f;
+#pragma unroll
+      for (int d = 0; d < VW; ++d) o[d] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int t = 0; t < nb; ++t) {
+        load(buf[0], t);
+        compute(buf[0], t, std::true_type{});
+      }
+#pragma unroll
+      for (int d = 0; d < VW; ++d) {
+        apart[d] += __shfl_xor(apart[d], 16);
+        apart[d] += __shfl_xor(apart[d], 32);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[d][r] += __shfl(apart[d], 4 * grp + r);
+      }
+    }
+  }
   float lt = lsum + __shfl_xor(lsum, 16);
   lt += __shfl_xor(lt, 32);
   const int gq = min(rows - kFewRows * tile, kFewRows);

@@ -40,10 +40,11 @@ constexpr float kLeastVScale = 0x1p-40f;
 constexpr float kLazy = 8.0f;
 constexpr float kWeightShift = 7.0f;
 
-// 2^(a - b), 0 for a == -inf whatever b is; NaN stays NaN.
+// 2^(a - b), 0 for a == -inf whatever b is, else at least 2^-126, so that a state's
+// infinity stays one; NaN stays NaN.
 __device__ __forceinline__ float weight2(float a, float b) {
   const float w = __builtin_amdgcn_exp2f(a - b);
-  return a == kNegInf ? 0.0f : w;
+  return a == kNegInf ? 0.0f : w < 0x1p-126f ? 0x1p-126f : w;
 }
 
 // The largest of x over a lane and the lane 32 away.

@@ -543,7 +543,8 @@ int eng_attention_decode_q8(const eng_half* q, const uint8_t* k_cache, const uin
  * lengths are int32 arrays on the device. Scores, softmax and sums are fp32; the
  * weights are rounded to fp16 for their products with V where many query rows share
  * the keys. A row that sees no key, or none whose score is above -inf, gets zeros. What
- * a query does not see does not reach its result, infinities and NaN included.
+ * a query does not see does not reach its result, infinities and NaN included; what it
+ * sees of them in V does: an infinity stays one, two of unlike signs give NaN.
  *
  * eng_attention_window_*: q and out [batch, s_new, n_heads, head_dim]. Query i of
  * sequence b stands at position p = pos[b] + i, and its K and V rows and all before

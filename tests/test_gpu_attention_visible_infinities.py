@@ -76,3 +76,21 @@ def test_shared_prefixes(gpu, kind, D, per, H, G, plen, split):
     got = prefix.run(gpu, kind, per, H, G, D, plen, lens, split=split, edit=edit)
     assert np.isfinite(got[per:].astype(np.float64)).all()
     assert np.isfinite(got[:per, :, 7:].astype(np.float64)).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,split", [(1, 0), (1, 1), (1, 5), (40, 1), (40, 5)])
+def test_weights_far_below_the_largest(gpu, D, S, split):
+    """Keys whose weights no fp32 number holds (2^-150 of the largest and less) still count."""
+    def edit(k, v):
+        k[0, :, :, 0] = np.where(np.arange(k.shape[2]) % 97 == 5, 100, -100)
+        special(v, 0, np.arange(600), "f16")
+
+    rng = np.random.default_rng(4)
+    cache = lc.Cache(gpu, rng, "f16", 1, 2, 640, D, [640], edit=edit)
+    q = rng.standard_normal((1, S, 4, D)).astype(np.float16)
+    q[..., 0] = 8
+    q = q.astype(np.float64)
+    got = window.call(gpu, "f16", q, cache, [640 - S], None, 0, 0, 640, 0.125, split)
+    lc.check(got, lc.window64(q, cache, [640 - S], None, 0, 0, 640, 0.125), "far below")
+    assert np.isinf(got[0, 0, 0, 1:5].astype(np.float64)).all()
