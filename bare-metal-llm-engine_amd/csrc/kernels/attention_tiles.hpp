@@ -123,7 +123,8 @@ __device__ __forceinline__ Unit unit_of(const Args& a, long long b) {
   u.p0 = a.pos[b];
   u.n = a.s_new;
   if (a.causal) {
-    if (a.n_new != nullptr) u.n = min(u.n, a.n_new[b]);
+    // (below zero none: times the group it could come out above it)
+    if (a.n_new != nullptr) u.n = max(min(u.n, a.n_new[b]), 0);
     if (u.p0 < 0) u.n = 0;
   }
   return u;

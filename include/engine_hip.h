@@ -551,8 +551,8 @@ int eng_attention_decode_q8(const eng_half* q, const uint8_t* k_cache, const uin
  * them are in the caches (write them first). It sees the keys j <= p, of these with
  * window > 0 those with j > p - window or j < sinks; window == 0 is no window. s_new
  * is a prompt's length, a piece's or 1. The first n_new[b] of a sequence's s_new
- * queries are computed (all of them where n_new is NULL, none where pos[b] < 0) and
- * the rows of out behind them left as they were. Keys at or past max_kv_len, the
+ * queries are computed (all of them where n_new is NULL, none where n_new[b] or pos[b]
+ * is below zero) and the rows of out behind them left as they were. Keys at or past max_kv_len, the
  * caller's bound on pos + n_new, are not seen; it and s_new choose the launch.
  *
  * eng_attention_prefix_*: one query of each sequence, q and out [batch, n_heads,
