@@ -624,9 +624,12 @@ int eng_attention_prefix_q8(const eng_half* q, const uint8_t* k_prefix, const ui
  * (g, p), p = parent[g][j] (out_parent with n_out == beams), into buffers of the
  * same shape, or, with the same pointers as source and destination, in place: beams
  * that keep their place (p == j) are then not touched. 8-bit caches move with the
- * scales of the blocks that the tokens reach. Tokens behind the length stay as they
- * were, and so does a sequence whose p is outside 0 .. beams - 1. Lengths past
- * max_kv_len are taken as it; kv_len itself is not reordered. Source and destination
+ * scales of the blocks that the tokens reach. What lies behind the length stays as it
+ * was, fp16 values or 8-bit codes, and so does a sequence whose p is outside 0 ..
+ * beams - 1; codes in the last block that is reached are under the new scale then, so
+ * what they stood for is lost. Lengths past max_kv_len are taken as it. kv_len itself
+ * is not reordered: where a group's lengths differ, the next step needs it gathered by
+ * parent. Source and destination
  * buffers are the same or do not overlap; beams is 1 to 32, head_dim 64 or 128, caches
  * are 16-byte aligned.
  * ---------------------------------------------------------------------- */
