@@ -20,7 +20,6 @@ namespace {
 
 typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
 typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
-typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef unsigned long long u64;
 
 constexpr float kNegInf = -__builtin_huge_valf();
@@ -45,9 +44,6 @@ __device__ __forceinline__ float value_of(unsigned v) {
 __device__ __forceinline__ float logit_of(u64 key) { return value_of(static_cast<unsigned>(key >> 32)); }
 __device__ __forceinline__ unsigned token_of(u64 key) { return 0xffffffffu - static_cast<unsigned>(key); }
 
-// e^x to 2 units in the last place and the rounding of x log2 e.
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
-
 // e^d in 64 bits, d < 700 and no NaN, to 2e-14: 2^k 2^f, t = k + f, |f| <= 1/2, 2^f by the
 // polynomial of degree 9 that meets it in Chebyshev's points. Less than e^-700 counts as it.
 __device__ __forceinline__ double exp64(double d) {
@@ -69,10 +65,38 @@ __device__ __forceinline__ double exp64(double d) {
   w[1] += __builtin_bit_cast(uintx2, t)[0] << 20;
   return __builtin_bit_cast(double, w);
 }
-__device__ __forceinline__ double wave_sum(double x) {
+// Sums of exponentials are kept as sums of 2^(x log2 e - n), n the whole number that belongs
+// to the largest x, so that sums of unlike n are joined by shifts of exponents: exact.
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFar = 0x1p22f;  // past it n is not to be had in fp32
+__device__ __forceinline__ float exponent_of(float m) {
+  return fminf(fmaxf(rintf(m * kLog2e), -2.0f * kFar), 2.0f * kFar);
+}
+// A sum against m as one against top >= m.
+__device__ __forceinline__ double against(double sum, float m, float top) {
+  return __builtin_ldexp(sum, static_cast<int>(exponent_of(m) - exponent_of(top)));
+}
+// The sum over the wave, in every lane.
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double x) {
+  uintx2 w = __builtin_bit_cast(uintx2, x);
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off);
-  return x;
+  for (int i = 0; i < 2; ++i)
+    w[i] = static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w[i]), CTRL, 0xF, 0xF, false));
+  return x + __builtin_bit_cast(double, w);
+}
+__device__ __forceinline__ double wave_sum(double x) {
+  x = dpp_add<0xB1>(x);   // quad_perm [1, 0, 3, 2]
+  x = dpp_add<0x4E>(x);   // quad_perm [2, 3, 0, 1]
+  x = dpp_add<0x141>(x);  // row_half_mirror
+  x = dpp_add<0x140>(x);  // row_mirror
+  const uintx2 w = __builtin_bit_cast(uintx2, x);
+  double r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = __builtin_bit_cast(double, uintx2{static_cast<unsigned>(__builtin_amdgcn_readlane(w[0], 16 * i)),
+                                             static_cast<unsigned>(__builtin_amdgcn_readlane(w[1], 16 * i))});
+  return (r[0] + r[1]) + (r[2] + r[3]);
 }
 
 // The largest of the wave's values, in every lane.
@@ -192,7 +216,8 @@ struct SelectArgs {
   int beams, n_out, vocab, eos;
   int pieces;      // of a row
   u64* keys;       // [rows][pieces][n_out], 0 behind the last one
-  floatx2* sums;   // [rows][pieces]: max, sum of exp(x - max)
+  double* sums;    // [rows][pieces]: of 2^(x log2 e - n), n the largest logit's exponent_of
+  float* maxes;    // [rows][pieces]
   double* lse;     // [rows][2]: L as the largest logit and what is to be added; NaN: none
   double near;     // scores of unlike beams this close may be in the wrong order
 };
@@ -201,8 +226,8 @@ constexpr int kStep = 64 * kWaves * kVpt;  // values of a workgroup's step
 
 // One workgroup per (row, piece of STEPS steps), the whole piece in registers, 16 STEPS
 // values of a lane. The k-th largest of the lanes' largest values bounds the k best from
-// below, so few values are looked at one by one. NaN in a row makes its sum NaN, +inf too.
-// 64 rows of 152064 fp32 (39 MB) take 14.6 us: their loads, issued together, about 7, the
+// below, so few values are looked at one by one. A NaN in a row makes its sum NaN.
+// 64 rows of 152064 fp32 (39 MB) take 15.3 us: their loads, issued together, about 7, the
 // exponentials and the search behind them the rest (19 with a list kept over the steps, 17
 // in pieces of two steps). 4 rows of 32000: 6.6 us, latencies.
 template <typename T, bool VECTOR, int STEPS>
@@ -210,7 +235,8 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
   constexpr int VEC = 16 / sizeof(T);
   constexpr int LOADS = kVpt / VEC;
   __shared__ u64 s_list[kWaves][kWaveList];
-  __shared__ float s_max[kWaves], s_sum[kWaves];
+  __shared__ float s_max[kWaves];
+  __shared__ double s_sum[kWaves];
   __shared__ int s_count[kWaves];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -248,16 +274,25 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
 #pragma unroll
     for (int i = 0; i < kVpt; ++i) m = fmaxf(m, value(c, i));
   }
-  float part[4] = {};
-  {
-    const float ref = m == kNegInf ? 0.0f : m;  // (all -inf: against 0, a sum of 0)
+  const float shift = exponent_of(m);
+  float part[STEPS];
 #pragma unroll
-    for (int c = 0; c < STEPS; ++c) {
+  for (int c = 0; c < STEPS; ++c) {
+    float e[kVpt];
 #pragma unroll
-      for (int i = 0; i < kVpt; ++i) part[i & 3] += exp_of(value(c, i) - ref);
+    for (int i = 0; i < kVpt; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(value(c, i), kLog2e, -shift));
+#pragma unroll
+    for (int w = kVpt / 2; w > 0; w /= 2) {
+#pragma unroll
+      for (int i = 0; i < w; ++i) e[i] += e[i + w];
     }
+    part[c] = e[0];
   }
-  const float sum = (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+  for (int w = STEPS / 2; w > 0; w /= 2) {
+#pragma unroll
+    for (int c = 0; c < w; ++c) part[c] += part[c + w];
+  }
   Best<kWaveList> best = {s_list[wave], a.n_out, 0};
   const float least = value_of(best.reached(order_of(m)));
 #pragma unroll
@@ -269,8 +304,7 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
   best.sort(lane);
   // the wave's max and sum
   const float wm = value_of(wave_max(order_of(m)));
-  const float ref = wm == kNegInf ? 0.0f : wm;
-  const float ws = gemv::wave_sum(sum * exp_of(m - ref));
+  const double ws = wave_sum(against(part[0], m, wm));
   if (lane == 0) {
     s_max[wave] = wm;
     s_sum[wave] = ws;
@@ -290,10 +324,10 @@ __global__ __launch_bounds__(64 * kWaves) void piece_kernel(SelectArgs a) {
   if (lane == 0) {
     float top = kNegInf;
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_max[w]);
-    const float r = top == kNegInf ? 0.0f : top;
-    float s = 0.0f;
-    for (int w = 0; w < kWaves; ++w) s += s_sum[w] * exp_of(s_max[w] - r);
-    a.sums[out] = floatx2{top, s};
+    double s = 0.0;
+    for (int w = 0; w < kWaves; ++w) s += against(s_sum[w], s_max[w], top);
+    a.sums[out] = s;
+    a.maxes[out] = top;
   }
 }
 
@@ -305,15 +339,15 @@ constexpr int kJoinList = 64 * kJoinKeys + kMaxOut;
 // pieces; then the beams' candidates are put in order by (score, beam, token). A candidate
 // whose score is no number, or of a beam without a finite score, counts as -inf; such a
 // beam's come in the order of the tokens, so its first n_out stand for it. Bound by a chain
-// of round trips (pieces, logarithm, sort, ranks): 4 beams 5.5-7 us, 10 beams of 10
+// of round trips (pieces, logarithm, sort, ranks): 4 beams 5.6-7.5 us, 10 beams of 10
 // candidates 10, 32 of 32 56 (compared each with each, by four waves, 18 and 560).
 //
 // The sum of fp32 exponentials leaves L off by up to `near` / 2 (select_entry has the bound).
 // Where a chosen candidate and one of another beam are closer than `near`, both beams' sums
 // are formed again, from the logits, in 64 bits, and the candidates put in order again: of
-// groups with gaps of 0.1 in score about one in a thousand, 85 us for two beams of 152064.
-// The question itself costs 0.3 us. (All exponentials in 64 bits: 16 x 4 beams of 152064 in
-// 29 us in place of 22.)
+// groups with gaps of 0.1 in score about one in three thousand, 90-140 us for two beams
+// of 152064 (equal beams always: a workgroup's CU is all it has). The question costs 0.3 us. (All exponentials in 64 bits: 16 x 4 beams of
+// 152064 in 29 us in place of 22.)
 template <typename T>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
   __shared__ u64 s_list[kJoinWaves][kJoinList];
@@ -340,17 +374,27 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
       }
     };
     load_keys(0);
-    float m = kNegInf;
-    for (int i = lane; i < a.pieces; i += 64) m = fmaxf(m, a.sums[row * a.pieces + i][0]);
+    // a lane's first piece is loaded with the keys
+    const float* maxes = a.maxes + row * a.pieces;
+    const double* sums = a.sums + row * a.pieces;
+    const float max0 = lane < a.pieces ? maxes[lane] : kNegInf;
+    const double sum0 = lane < a.pieces ? sums[lane] : 0.0;
+    float m = max0;
+    for (int i = lane + 64; i < a.pieces; i += 64) m = fmaxf(m, maxes[i]);
     m = value_of(wave_max(order_of(m)));
-    float part = 0.0f;
-    for (int i = lane; i < a.pieces; i += 64) {
-      const floatx2 p = a.sums[row * a.pieces + i];
-      part = fmaf(p[1], p[0] == kNegInf ? 1.0f : exp_of(p[0] - m), part);
-    }
-    const double sum = gemv::wave_sum(part);
-    const double peak = m, more = log(sum);  // L = peak + more, kept apart: rows far from zero lose nothing
+    double part = against(sum0, max0, m);
+    for (int i = lane + 64; i < a.pieces; i += 64) part += against(sums[i], maxes[i], m);
+    const double sum = wave_sum(part);
     const bool finite = given > kNegInf && given < -kNegInf;
+    // L = peak + more, kept apart: rows far from zero lose nothing
+    const double peak = m;
+    double more = log(sum) - 0.6931471805599453 * (peak * kLog2e - exponent_of(m));
+    if (!done && finite && fabsf(m) > kFar && fabsf(m) < -kNegInf && sum == sum) {
+      const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+      double slow = 0.0;
+      for (int t = lane; t < a.vocab; t += 64) slow += exp64(static_cast<double>(x[t]) - peak);
+      more = log(wave_sum(slow));
+    }
     const bool plain = !done && finite && (peak + more) - (peak + more) == 0.0;
     if (lane == 0) {
       a.lse[2 * row] = plain ? peak : __builtin_nan("");
@@ -602,10 +646,12 @@ void select_entry(const void* logits, bool half, int64_t ld, const float* scores
   while (per < 4 && pieces(per) * n_out > 64 * kJoinKeys && rows * pieces(2 * per) >= device_cu_count()) per *= 2;
   a.pieces = static_cast<int>(pieces(per));
   const std::size_t lists = static_cast<std::size_t>(rows) * a.pieces;
-  StreamScratch scratch(s, (lists * (n_out + 1) + 2 * static_cast<std::size_t>(rows)) * 8);
+  StreamScratch scratch(s, lists * (n_out * sizeof(u64) + sizeof(double) + sizeof(float)) +
+                               static_cast<std::size_t>(rows) * 2 * sizeof(double));
   a.keys = static_cast<u64*>(scratch.get());
-  a.sums = reinterpret_cast<floatx2*>(a.keys + lists * n_out);
-  a.lse = reinterpret_cast<double*>(a.sums + lists);
+  a.sums = reinterpret_cast<double*>(a.keys + lists * n_out);
+  a.lse = a.sums + lists;
+  a.maxes = reinterpret_cast<float*>(a.lse + 2 * rows);
   const bool vector = aligned_to(logits, 16) && (ld * elem) % 16 == 0;
   const unsigned grid = static_cast<unsigned>(lists);
   auto go = [&](auto elem, auto vec) {
@@ -618,13 +664,12 @@ void select_entry(const void* logits, bool half, int64_t ld, const float* scores
   if (half) vector ? go(_Float16{}, std::true_type{}) : go(_Float16{}, std::false_type{});
   else vector ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
   ENG_LAUNCH_CHECK();
-  // How far L may be off, u = 2^-24: a term's argument a = x - max by 2.22 |a| u (difference,
-  // product, log2 e as an fp32 number), over a row in the mean 2.22 u log vocab at the most
-  // (the mean of -log w_i under w_i / S is an entropy less log S, and S >= 1); four
-  // exponentials of 2 u on a term's way into the row's sum and the products of three, 11 u;
-  // additions of a lane 18 u, a wave 6 u, a workgroup 4 u, and of the pieces in the join
-  // pieces / 64 + 6. Twice that for two beams.
-  a.near = 2.0 * 0x1p-24 * (2.22 * std::log(static_cast<double>(vocab)) + 45.0 + static_cast<double>(a.pieces) / 64.0 + 1.0);
+  // How far L may be off, u = 2^-24: a term by 1.22 |x - max| u (its argument's rounding, log2 e
+  // as an fp32 number; the part of it that all terms share is known), over a row in the mean
+  // 1.22 u log vocab at the most (the mean of -log w_i under w_i / S is an entropy less log
+  // S, and S >= 1), 2 u of the exponential, and a lane's additions 6 u; what follows is in 64
+  // bits. Twice that, and one u, for two beams.
+  a.near = 2.0 * 0x1p-24 * (1.22 * std::log(static_cast<double>(vocab)) + 10.0);
   // At least four waves, for the sums in 64 bits; a thread has up to two candidates.
   const int join_threads = 64 * std::max(4, std::min(a.beams, kJoinWaves));
   if (half) join_kernel<_Float16><<<static_cast<unsigned>(batch), join_threads, 0, s>>>(a);

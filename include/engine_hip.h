@@ -607,7 +607,7 @@ int eng_attention_prefix_q8(const eng_half* q, const uint8_t* k_prefix, const ui
  * out_scores, out_parent (the beam, 0 .. beams - 1) and out_token [batch, n_out].
  * Candidates of one beam are compared by their logits, those of unlike beams by
  * their scores in 64 bits; ties go to the lower beam, then the lower token. The sums
- * of exponentials are fp32, and out_scores with them good to 5e-6 and their own
+ * of exponentials are fp32, and out_scores with them good to 2e-6 and their own
  * rounding; a group in which that leaves an order open has them formed again in 64
  * bits, which takes it longer. finished
  * [batch, beams] (bytes; NULL: none) marks beams that have ended: such a beam has

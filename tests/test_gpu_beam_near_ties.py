@@ -2,11 +2,10 @@
 apart: their order is that of the scores in 64 bits.
 
 Bounds of L = log sum exp, u = 2^-24. Of the sum of fp32 exponentials, relative: a term's
-argument a = x - max by 2.22 |a| u (difference, product, log2 e as an fp32 number), whose mean
-over the row's weights is log V at the most (an entropy less log of the sum, and that is 1
-at least); four exponentials of 2 u each on its way into the row's sum, 3 u of products;
-additions of a lane 18 u, a wave 6 u, a workgroup 4 u, the pieces V / 262144 + 6 u: WIDE(V).
-Candidates of unlike beams closer than twice that are compared by sums in 64 bits, v =
+argument, x - max in the end, by 1.22 |x - max| u (one rounding, log2 e as an fp32 number) and
+half a u, whose mean over the row's weights is 1.22 log V u at the most (an entropy less log
+of the sum, and that is 1 at least); an exponential 2 u, a lane's additions 6 u, the rest in
+64 bits: wide(V). Candidates of unlike beams closer than twice that are compared by sums in 64 bits, v =
 2^-53: an exponential to 2e-14 and its argument's rounding, |x - L| log2 e v, under 2e-14
 for |x - L| < 100 and times its weight beyond; V / 256 + 20 additions of v: 6e-14 for V <
 60000, and the few roundings of scores under 1000 another 4e-13. EPS = 1e-12."""
@@ -26,7 +25,7 @@ EPS = 1e-12
 
 
 def wide(V):
-    return (2.22 * np.log(V) + 46 + V / 262144) * U32
+    return (1.22 * np.log(V) + 10) * U32
 
 
 def lse64(x):
@@ -106,3 +105,46 @@ def test_large_and_far_apart_logits(gpu, kind):
         # (a score is formed from x and L, half a step of 64 bits of either each)
         far = 4 * 2.0**-53 * np.abs(x[g].astype(np.float64)[np.isfinite(x[g])]).max()
         assert (np.abs(got[0][g] - s) <= U32 * np.abs(s) + wide(3000) + far).all()
+
+
+@pytest.mark.parametrize("base", [300.0, -5000.0, 2.0**21, 1e7, -3e7, 3e8, -1e30])
+def test_rows_far_from_zero(gpu, base):
+    """Logits whose differences count though the numbers are large: L less the row's largest
+    logit is compared, in which nothing is lost; and NaN, infinities and masks among them."""
+    rng = np.random.default_rng(3)
+    V, step = 5000, float(np.spacing(np.float32(abs(base))))
+    x = (base + step * rng.integers(0, 4, (5, 2, V))).astype(np.float32)
+    x[1, 0, 4321] = np.nan
+    x[1, 1, 17] = np.inf
+    x[2, 0, 1::2] = -np.inf
+    x[2, 1] = -np.inf
+    x[3, 0, 5] = np.finfo(np.float32).min
+    scores = (-rng.random((5, 2))).astype(np.float32)
+    got = select(gpu, "f32", x, scores, None, 3, -1)
+    for g in range(5):
+        want = []
+        for b in range(2):
+            row = x[g, b].astype(np.float64)
+            top = row.max()
+            if not np.isfinite(top):
+                want += [(-np.inf, -b, -t) for t in range(3)]
+                continue
+            more = np.log(np.exp(row - top).sum())
+            want += [(float(scores[g, b]) - more + (row[t] - top), -b, -t)
+                     for t in np.lexsort((np.arange(V), -row))[:3]]
+        want = sorted(want, reverse=True)[:3]
+        assert [(-b, -t) for _, b, t in want] == list(zip(got[1][g], got[2][g]))
+        for s, y in zip(want, got[0][g]):
+            assert y == s[0] or abs(y - s[0]) <= U32 * abs(s[0]) + wide(V)
+
+
+@KINDS
+def test_masked_rows(gpu, kind):
+    """Rows of -inf alone, in all beams but one: the others' order is the live beam's."""
+    rng = np.random.default_rng(4)
+    x = (3 * rng.standard_normal((3, 4, 9000))).astype(np.float16 if kind == "f16" else np.float32)
+    x[:, 1:] = -np.inf
+    got = select(gpu, kind, x, np.full((3, 4), -1, np.float32), None, 8, -1)
+    for g in range(3):
+        assert (got[1][g] == 0).all()
+        assert np.array_equal(got[2][g], np.lexsort((np.arange(9000), -x[g, 0].astype(np.float64)))[:8])

@@ -52,7 +52,7 @@ def check(gpu, kind, per, groups, beams, n_out, V, x=None, scores=None, ld=None,
     scores = (-10 - 4 * rng.random((groups, beams))).astype(np.float32) if scores is None else scores
     got = select(gpu, kind, x, scores, None, n_out, -1, ld, shift)
     # fp32 sums, as derived in test_gpu_beam_near_ties
-    wide = (2.22 * np.log(V) + 46 + V / 262144) * U32
+    wide = (1.22 * np.log(V) + 10) * U32
     for g in range(groups):
         s, p, t = expected(x[g], scores[g], n_out)
         assert np.array_equal(got[1][g], p), f"group {g}: parents"
