@@ -311,7 +311,10 @@ __global__ __launch_bounds__(64 * NW, 2) void few_kernel(Args a0, Args a1, unsig
         apart[d] += __shfl_xor(apart[d], 16);
         apart[d] += __shfl_xor(apart[d], 32);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[d][r] += __shfl(apart[d], 4 * grp + r);
+        for (int r = 0; r < 4; ++r) {
+          const float seen = __shfl(apart[d], 4 * grp + r);
+          o[d][r] += m == kNegInf ? 0.0f : seen;  // (no score above -inf: none of them)
+        }
       }
     }
   }

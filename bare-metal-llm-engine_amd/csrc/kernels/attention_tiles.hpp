@@ -590,6 +590,11 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void tile_kernel(Args a) 
         }
       }
     }
+    // (a row without a score above -inf: none of them)
+    if (m == kNegInf && l + __shfl_xor(l, 32) == 0.0f) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] = floatx16{};
+    }
   };
   float sum = 0.0f;
 #pragma unroll

@@ -94,3 +94,30 @@ def test_weights_far_below_the_largest(gpu, D, S, split):
     got = window.call(gpu, "f16", q, cache, [640 - S], None, 0, 0, 640, 0.125, split)
     lc.check(got, lc.window64(q, cache, [640 - S], None, 0, 0, 640, 0.125), "far below")
     assert np.isinf(got[0, 0, 0, 1:5].astype(np.float64)).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,split", [(1, 1), (1, 4), (40, 1), (40, 4)])
+def test_rows_without_a_score(gpu, D, S, split):
+    """Where all scores that a row sees are -inf it gets zeros, infinities in V or not, and such
+    keys in one of several splits leave the others' result as it is."""
+    def edit(k, v):
+        k[0, 0, :, 0] = -np.inf       # the first KV head: no score at all
+        k[0, 1, :128, 0] = -np.inf    # the second: from the 129th key on
+        v[0, :, 5, 3], v[0, :, 70, 4] = np.inf, -np.inf
+
+    rng = np.random.default_rng(12)
+    cache = lc.Cache(gpu, rng, "f16", 1, 2, 400, D, [400], edit=edit)
+    q = rng.standard_normal((1, S, 4, D)).astype(np.float16)
+    q[..., 0] = np.abs(q[..., 0]) + np.float16(0.5)
+    q = q.astype(np.float64)
+    got = window.call(gpu, "f16", q, cache, [400 - S], None, 0, 0, 400, 0.125, split)
+    assert (got[0, :, :2] == 0).all()
+    want = {}
+    for i in range(S):
+        j = np.arange(128, 400 - S + i + 1)
+        for h in (2, 3):
+            y, bound = lc.attend_rows(q[0, i, h], cache.values[0][0, 1, j], cache.values[1][0, 1, j],
+                                      cache.vmax[0, 1], 0.125)
+            rest = np.delete(np.arange(D), (3, 4))  # (weights of 0 times an infinity: left open)
+            assert (np.abs(got[0, i, h].astype(np.float64) - y) <= bound)[rest].all()
