@@ -163,9 +163,11 @@ constexpr int tile_buffers(int NW) { return NW == 8 ? 3 : 2; }
 // a SIMD fill each other's gaps. K fragments are read one such step ahead. Eight waves share
 // a tile where that leaves a workgroup for every CU; else four, two workgroups to a CU, and
 // at D = 64, with three to a CU, always (prompts of 777 tokens, window 256: 36 us, 49 with
-// eight waves).
-// Bound by the matrix cores and power together: 2048 tokens after 6144, 32 / 8 heads of
-// 128: 277 us, 870 TFLOP/s, at 1.8 to 2.1 GHz (a large fp16 product of the library's 1175).
+// eight waves). The four-wave forms at D = 128 fill their 256 registers and spill 16 (8-bit)
+// and 40 bytes (fp16) a lane.
+// Bound by the matrix cores and power together, and by the longest of one workgroup to a
+// CU: 2048 tokens after 6144, 32 / 8 heads of 128: 277-282 us, 870 TFLOP/s, at 1.8 to 2.1
+// GHz (a large fp16 product of the library's 1175).
 // Slower: the two waves of a SIMD one phase apart, exponentials against products, by
 // barriers (309; a phase then waits for its own latencies); 64 rows to a wave, half the LDS
 // reads (376 to 442; the compiler moves values between the register files); direct loads

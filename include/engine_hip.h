@@ -540,9 +540,11 @@ int eng_attention_decode_q8(const eng_half* q, const uint8_t* k_cache, const uin
  * Caches are head-major, [batch, n_kv_heads, kv_max_seq_len, head_dim], 16-byte
  * aligned: fp16 (each sequence's as eng_kv_cache_write_f16 fills it) or 8-bit with
  * scales (eng_kv_cache_write_q8's). head_dim is 64 or 128. Positions, counts and
- * lengths are int32 arrays on the device. Scores, softmax and sums are fp32; the
- * weights are rounded to fp16 for their products with V where many query rows share
- * the keys. A row that sees no key, or none whose score is above -inf, gets zeros. What
+ * lengths are int32 arrays on the device. Scores, softmax and sums are fp32. Weights
+ * enter their products with V as two fp16 terms (22 bits) for single tokens (s_new ==
+ * 1), and over a prefix for up to 128 query rows of a KV head (sequences of a group
+ * times n_heads / n_kv_heads), and rounded to fp16 once past that and for more new
+ * tokens. A row that sees no key, or none whose score is above -inf, gets zeros. What
  * a query does not see does not reach its result, infinities and NaN included; what it
  * sees of them in V does: an infinity stays one, two of unlike signs give NaN.
  *
@@ -552,16 +554,19 @@ int eng_attention_decode_q8(const eng_half* q, const uint8_t* k_cache, const uin
  * window > 0 those with j > p - window or j < sinks; window == 0 is no window. s_new
  * is a prompt's length, a piece's or 1. The first n_new[b] of a sequence's s_new
  * queries are computed (all of them where n_new is NULL, none where n_new[b] or pos[b]
- * is below zero) and the rows of out behind them left as they were. Keys at or past max_kv_len, the
- * caller's bound on pos + n_new, are not seen; it and s_new choose the launch.
+ * is below zero) and the rows of out behind them left as they were. Keys at or past
+ * max_kv_len, the caller's bound on pos + n_new, are not seen; it and s_new choose the
+ * launch. Single tokens over 8-bit caches without a window are eng_attention_decode_q8's
+ * too: that one is the faster where lengths come near their bound, this one where they
+ * are far below.
  *
  * eng_attention_prefix_*: one query of each sequence, q and out [batch, n_heads,
  * head_dim], over the first prefix_len[g] tokens of prefix g, shared by the batch /
  * n_prefix sequences of group g = b / (batch / n_prefix), and then the first
  * kv_len[b] of its own, in one softmax. The prefixes are caches of their own,
- * [n_prefix, n_kv_heads, prefix_max_seq_len, head_dim], each read once for its
- * group. Lengths past max_prefix_len / max_kv_len are taken as these, lengths
- * below zero as zero.
+ * [n_prefix, n_kv_heads, prefix_max_seq_len, head_dim], each read from memory once
+ * for its group (past 16 query rows of a KV head again from the L2). Lengths past
+ * max_prefix_len / max_kv_len are taken as these, lengths below zero as zero.
  *
  * split_kv = 0 chooses the number of pieces that a row's keys are computed in; a
  * positive value asks for as many (at most 256, prefix and own keys 128 each). More
