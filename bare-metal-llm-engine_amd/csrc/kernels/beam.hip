@@ -346,7 +346,7 @@ constexpr int kJoinList = 64 * kJoinKeys + kMaxOut;
 // Where a chosen candidate and one of another beam are closer than `near`, both beams' sums
 // are formed again, from the logits, in 64 bits, and the candidates put in order again: of
 // groups with gaps of 0.1 in score about one in three thousand, 90-140 us for two beams
-// of 152064 (equal beams always: a workgroup's CU is all it has). The question costs 0.3 us. (All exponentials in 64 bits: 16 x 4 beams of
+// of 152064 (a workgroup's CU is all it has). The question costs 0.3 us. (All exponentials in 64 bits: 16 x 4 beams of
 // 152064 in 29 us in place of 22.)
 template <typename T>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
@@ -475,10 +475,20 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
   const unsigned open = rank();
   if (open != 0) atomicOr(s_open, open);
   __syncthreads();
-  for (unsigned again = *s_open; again != 0; again &= again - 1) {
+  // Open beams whose sums agree in every bit have equal rows, whose order is that of the
+  // logits and scores (others' agree by chance only, with L closer than a term's last bit).
+  // Where all do, the order stands; sums in 64 bits otherwise.
+  const double* const first = a.lse + 2 * group * a.beams;
+  bool alike = true;
+  for (unsigned rest = *s_open; rest != 0; rest &= rest - 1) {
+    const int b = __builtin_ctz(rest), c = __builtin_ctz(*s_open);
+    alike = alike && first[2 * b] == first[2 * c] && first[2 * b + 1] == first[2 * c + 1];
+  }
+  const unsigned settle = alike ? 0 : *s_open;
+  for (unsigned again = settle; again != 0; again &= again - 1) {
     const int b = __builtin_ctz(again);
     const long long row = group * a.beams + b;
-    const double peak = a.lse[2 * row], more = a.lse[2 * row + 1];
+    const double peak = first[2 * b], more = first[2 * b + 1];
     if (peak != peak) continue;
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
     double part[4] = {};
@@ -501,7 +511,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(SelectArgs a) {
     const double change = log(sum);  // of L: terms against the old one add up to e^change
     for (int i = b * k + tid; i < b * k + k; i += threads) s_score[i] -= change;
   }
-  if (*s_open != 0) {
+  if (settle != 0) {
     __syncthreads();
     rank();
   }

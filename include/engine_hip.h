@@ -614,7 +614,8 @@ int eng_attention_prefix_q8(const eng_half* q, const uint8_t* k_prefix, const ui
  * their scores in 64 bits; ties go to the lower beam, then the lower token. The sums
  * of exponentials are fp32, and out_scores with them good to 2e-6 and their own
  * rounding; a group in which that leaves an order open has them formed again in 64
- * bits, which takes it longer. finished
+ * bits, which takes it longer (not for beams of equal logits: sums that agree in every
+ * bit count as equal). finished
  * [batch, beams] (bytes; NULL: none) marks beams that have ended: such a beam has
  * one candidate, token eos with its score unchanged, whatever its logits are. out_finished
  * [batch, n_out] (may be NULL) is 1 where the parent has ended or the token is eos

@@ -148,3 +148,26 @@ def test_masked_rows(gpu, kind):
     for g in range(3):
         assert (got[1][g] == 0).all()
         assert np.array_equal(got[2][g], np.lexsort((np.arange(9000), -x[g, 0].astype(np.float64)))[:8])
+
+
+@KINDS
+@pytest.mark.parametrize("V", [700, 20011])
+def test_equal_beams_beside_one_a_hair_apart(gpu, kind, V):
+    """Beams 1 and 3 are equal, beam 0 or 2 comes as near to them as an fp32 score can."""
+    rng = np.random.default_rng(V)
+    groups, dt = 30, np.float16 if kind == "f16" else np.float32
+    x = (3 * rng.standard_normal((groups, 4, V))).astype(dt)
+    x[:, 3] = x[:, 1]
+    lse, top = lse64(x.astype(np.float64)), x.astype(np.float64).max(2)
+    scores = np.full((groups, 4), -40, np.float32)
+    scores[:, 1] = scores[:, 3] = -rng.random(groups)
+    near = 2 * (np.arange(groups) % 2)
+    g = np.arange(groups)
+    scores[g, near] = (scores[:, 1].astype(np.float64) + (top[:, 1] - lse[:, 1])) - (top[g, near] - lse[g, near])
+    best = scores.astype(np.float64) + (top - lse)
+    got = select(gpu, kind, x, scores, None, 3, -1)
+    for i in range(groups):
+        if abs(best[i, near[i]] - best[i, 1]) <= 2 * EPS:
+            continue
+        _, p, t, _ = lc.select64(x[i].astype(np.float64), scores[i].astype(np.float64), None, 3, -1)
+        assert np.array_equal(got[1][i], p) and np.array_equal(got[2][i], t), f"group {i}: {got[1][i]} for {p}"
